@@ -507,6 +507,84 @@ int spr_project_rows_ex(const float* x, const float* factor, const float* div, i
                         int32_t r, int32_t precision, int32_t row_rms, float eps, float weight, float* out,
                         int32_t out_ld, int32_t out_col, hipStream_t stream);
 
+/* ---------------------------------------------------------------- 4-bit K/V cache
+ * (no counterpart in the reference: it keeps no K/V between calls)
+ *
+ * pages uint8 [num_pages, kv_heads, spr_kv4_page_bytes(1, page_size, d)], 16-byte aligned; one head's
+ * part of a page of page_size (32, 64, 128 or 256) tokens is the K codes [page_size, d / 2], the V
+ * codes, the K scales [page_size, d / 32] and the V scales; d is 64 or 128.  A code is a 4-bit float
+ * (sign, then 0, 0.5, 1, 1.5, 2, 3, 4, 6), the even dim in the low half of a byte; scale byte s is
+ * 2^(s - 127) for 32 dims of a token, 255 a NaN.  block_table int32 [sequences, wide] names a
+ * sequence's pages (-1: none), lengths int32 [sequences] its tokens, ref_count int32 [num_pages] how
+ * many sequences hold a page (0: free); wide * page_size <= 2^31 - 1.  seq_ids int32 [batch]
+ * (nullable: 0, 1, ..) names the sequences of a call. */
+int64_t spr_kv4_page_bytes(int32_t kv_heads, int32_t page_size, int32_t d);
+/* K and V rows into the cache: row t < counts[b] (nullable: rows) of entry b becomes token
+ * starts[b] + t of its sequence.  k, v [batch, kv_heads, rows, d] by strides in elements (rows of d
+ * packed, 16-byte aligned), dtype 0 / 1 / 2.  The scale's exponent is that of the group's largest
+ * magnitude rounded to two significant bits (half up), less two, its byte kept in [2, 252]; values
+ * round to the nearest code, ties to even, past 6 to 6; a group with an infinity or a NaN becomes
+ * NaN.  Rows with no page (a negative start, a place past the table, an entry outside the pool) are
+ * not written.  No two rows of a call may name one token. */
+int spr_kv4_store(uint8_t* pages, int32_t num_pages, int32_t kv_heads, int32_t page_size, int32_t d,
+                  const int32_t* block_table, int32_t sequences, int32_t wide, const int32_t* seq_ids,
+                  const int32_t* starts, const int32_t* counts, const void* k, const void* v, int32_t dtype,
+                  int32_t batch, int32_t rows, int64_t k_b, int64_t k_h, int64_t k_t, int64_t v_b, int64_t v_h,
+                  int64_t v_t, hipStream_t stream);
+/* The other way: k, v [batch, kv_heads, rows, d] (packed) from tokens starts[b] + t, t < counts[b];
+ * rows past the count are 0, rows with no page NaN. */
+int spr_kv4_load(const uint8_t* pages, int32_t num_pages, int32_t kv_heads, int32_t page_size, int32_t d,
+                 const int32_t* block_table, int32_t sequences, int32_t wide, const int32_t* seq_ids,
+                 const int32_t* starts, const int32_t* counts, void* k, void* v, int32_t dtype, int32_t batch,
+                 int32_t rows, hipStream_t stream);
+/* Page calls.  Each checks on the device all it is asked for and then happens whole or not at all;
+ * new pages are the lowest free ones, ascending, in the order of the named sequences (at most 2048 a
+ * call).  status int32 [1] (nullable) gets, unless it holds one already, 1 a sequence outside the
+ * table, 2 a sequence named twice, 3 a negative count or a range outside the sequence's pages, 4 more
+ * tokens than the table's row holds, 5 not enough free pages, 6 a fork onto a sequence that holds
+ * tokens, 7 a length outside the table or a table entry outside the pool. */
+size_t spr_kv4_pages_workspace(int32_t num_pages);
+/* Room for counts[i] more tokens of sequence seq_ids[i]; starts[i] (out) is the first one's place, -1
+ * for all if the call did not happen. */
+int spr_kv4_reserve(int32_t* block_table, int32_t* lengths, int32_t* ref_count, const int32_t* counts,
+                    const int32_t* seq_ids, int32_t n, int32_t sequences, int32_t wide, int32_t page_size,
+                    int32_t num_pages, int32_t* starts, int32_t* status, void* workspace, size_t workspace_bytes,
+                    hipStream_t stream);
+/* Pages [first_pages[i], first_pages[i] + page_counts[i]) of sequence seq_ids[i] are given back
+ * (nullable: 0, and all from there on, as any negative count says), the pages behind close up, the
+ * length loses their tokens. */
+int spr_kv4_free(int32_t* block_table, int32_t* lengths, int32_t* ref_count, const int32_t* seq_ids,
+                 const int32_t* first_pages, const int32_t* page_counts, int32_t n, int32_t sequences, int32_t wide,
+                 int32_t page_size, int32_t num_pages, int32_t* status, void* workspace, size_t workspace_bytes,
+                 hipStream_t stream);
+/* Sequence dst[i] (empty) continues as src[i] does: share != 0 on the same full pages and a copy of
+ * the last one where it is not full, share 0 on copies of all.  pages: `layers` pools, layer_bytes
+ * apart, of num_pages pages of page_bytes. */
+int spr_kv4_fork(uint8_t* pages, int64_t page_bytes, int64_t layer_bytes, int32_t layers, int32_t* block_table,
+                 int32_t* lengths, int32_t* ref_count, const int32_t* src, const int32_t* dst, int32_t n,
+                 int32_t sequences, int32_t wide, int32_t page_size, int32_t num_pages, int32_t share,
+                 int32_t* status, void* workspace, size_t workspace_bytes, hipStream_t stream);
+/* The held pages become pages 0 .. live - 1: the i-th lowest held page from live on moves to the i-th
+ * lowest free one below it, in every layer, table and ref_count.  live int32 [1] out. */
+int spr_kv4_compact(uint8_t* pages, int64_t page_bytes, int64_t layer_bytes, int32_t layers, int32_t* block_table,
+                    int32_t* ref_count, int32_t sequences, int32_t wide, int32_t num_pages, int32_t* live,
+                    void* workspace, size_t workspace_bytes, hipStream_t stream);
+/* out [batch, heads, rows, d] = softmax(scale q K^T) V over the sequence's tokens, lse fp32 [batch,
+ * heads, rows] (nullable) the natural log of the scaled sum.  q by strides in elements, dtype 0 bf16
+ * or 1 fp16, as out; query head h reads kv head h / (heads / kv_heads).  causal: of the counts[b]
+ * (nullable: rows) rows in use the last is the sequence's last token, and a row sees the tokens up to
+ * its own.  Rows that see nothing, and rows past the count, are 0 with lse -inf; a page outside the
+ * pool, a sequence outside the table or a length it cannot hold gives NaN.  max_length (a bound on
+ * the lengths, which may be exceeded) only sizes the launch. */
+size_t spr_kv4_attention_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t rows, int32_t d,
+                                   int64_t max_length);
+int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_t q_t, int32_t dtype, int32_t batch,
+                      int32_t heads, int32_t kv_heads, int32_t rows, int32_t d, const uint8_t* pages,
+                      int32_t num_pages, int32_t page_size, const int32_t* block_table, int32_t sequences,
+                      int32_t wide, const int32_t* lengths, const int32_t* counts, const int32_t* seq_ids,
+                      int32_t causal, float scale, int64_t max_length, void* out, float* lse, void* workspace,
+                      size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

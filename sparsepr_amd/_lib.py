@@ -128,6 +128,22 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                                 _i32, _i32, _i32, _i32, _vp, _vp]),
     "spr_svg_ear_scores": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _f32, _vp, _i64, _i32, _i32, _i64, _i64,
                                           _i32, _i32, _i32, _vp, _vp]),
+    # kv4.hip
+    "spr_kv4_page_bytes": (_i64, [_i32, _i32, _i32]),
+    "spr_kv4_pages_workspace": (_sz, [_i32]),
+    "spr_kv4_store": (ctypes.c_int, [_vp, _i32, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32,
+                                     _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "spr_kv4_load": (ctypes.c_int, [_vp, _i32, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32,
+                                    _i32, _vp]),
+    "spr_kv4_reserve": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _sz, _vp]),
+    "spr_kv4_free": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _sz, _vp]),
+    "spr_kv4_fork": (ctypes.c_int, [_vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32,
+                                    _vp, _vp, _sz, _vp]),
+    "spr_kv4_compact": (ctypes.c_int, [_vp, _i64, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _sz, _vp]),
+    # kv4_attention.hip
+    "spr_kv4_attention_workspace": (_sz, [_i32, _i32, _i32, _i32, _i32, _i64]),
+    "spr_kv4_attention": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _i32, _i32,
+                                         _vp, _i32, _i32, _vp, _vp, _vp, _i32, _f32, _i64, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _LIB: ctypes.CDLL | None = None

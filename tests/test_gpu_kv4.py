@@ -1,0 +1,560 @@
+"""The 4-bit paged K/V cache on the GPU against its definitions in 64 bits."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests import _kv4_model as model
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _gpu(a, dev, dtype=torch.int32):
+    return torch.from_numpy(np.ascontiguousarray(a)).to(dtype).to(dev)
+
+
+def _pool(rng, num_pages, heads, size, d, amp=1.0):
+    """Pages of rows as the encoder makes them, uint8 numpy, and every byte of them in use."""
+    pages = np.zeros((num_pages, heads, size * (d + d // 16)), np.uint8)
+    kc, vc, ks, vs = model.parts(pages, size, d)
+    for c, s, a in ((kc, ks, amp), (vc, vs, 1.0)):
+        codes, scales = model.encode(rng.standard_normal((num_pages, heads, size, d)) * a)
+        c[...], s[...] = codes, scales
+    return pages
+
+
+def _table(rng, lengths, size, num_pages, wide):
+    order, at = rng.permutation(num_pages), 0
+    table = np.full((len(lengths), wide), -1, np.int32)
+    for i, n in enumerate(lengths):
+        k = -(-n // size)
+        table[i, :k] = order[at:at + k]
+        at += k
+    return table
+
+
+def _same_nan(got, want):
+    return np.array_equal(np.isnan(got), np.isnan(want))
+
+
+# ------------------------------------------------------------------ rows in and out
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("d,size", [(64, 32), (128, 64), (128, 256)])
+def test_store_bytes_are_the_encoders_and_load_gives_their_values(dev, dtype, d, size):
+    from sparsepr_amd.kernels.kv4 import kv4_load, kv4_store
+
+    rng = np.random.default_rng(d + size)
+    b, h, t = 3, 2, 77
+    x = rng.standard_normal((2, b, h, t, d)) * np.exp(2.5 * rng.standard_normal((2, b, h, t, 1)))
+    x[0, 0, 0, 0] = 0.0
+    x[0, 0, 0, 1, :32] = -0.0
+    # values on the borders between codes, of every sign, at three scales
+    edge = np.array([0.25, 0.5, 0.75, 1.0, 1.25, 1.5, 1.75, 2.0, 2.5, 3.0, 3.5, 4.0, 5.0, 6.0, 6.96875, 7.0, 7.5])
+    for i, s in enumerate((1.0, 2.0**-9, 2.0**6)):
+        x[0, 0, 1, i, :34] = np.concatenate([edge, -edge]) * s
+        x[1, 0, 1, i, :34] = np.concatenate([-edge, edge]) * s * 0.5
+    # largest and smallest magnitudes of the type, and a group that passes the scale's range
+    big = float(torch.finfo(DT[dtype]).max)
+    x[0, 1, 0, 0, 0], x[0, 1, 0, 1, 3], x[0, 1, 0, 2, :] = big, -big, float(torch.finfo(DT[dtype]).tiny)
+    x[1, 1, 0, 0, 5] = float(torch.finfo(DT[dtype]).tiny) * 2.0**-6
+    x[1, 1, 1, 0, 7], x[1, 1, 1, 1, 40], x[1, 1, 1, 2, 1] = np.inf, -np.inf, np.nan
+    k, v = (torch.from_numpy(y).to(DT[dtype]).to(dev) for y in x)
+    lengths = [200, 0, 130]
+    starts, counts = np.array([123, 0, 53]), np.array([t, 0, t])
+    wide = 300 // size + 1
+    num_pages = 2 * wide + 3
+    table = _table(rng, [wide * size, 0, wide * size], size, num_pages, wide)
+    table[1] = -1
+    pages = rng.integers(0, 256, (num_pages, h, size * (d + d // 16)), np.uint8)
+    want = pages.copy()
+    for s in (0, 2):
+        for name, y, (ci, si) in (("k", k, (0, 2)), ("v", v, (1, 3))):
+            codes, scales = model.encode(y[s].double().cpu().numpy())
+            for i in range(t):
+                page, slot = table[s, (starts[s] + i) // size], (starts[s] + i) % size
+                model.parts(want[page], size, d)[ci][:, slot] = codes[:, i]
+                model.parts(want[page], size, d)[si][:, slot] = scales[:, i]
+    gp, gt = _gpu(pages, dev, torch.uint8), _gpu(table, dev)
+    kv4_store(gp, gt, k, v, _gpu(starts, dev), counts=_gpu(counts, dev))
+    assert np.array_equal(gp.cpu().numpy(), want)  # its own rows, and no other byte
+    for out in (torch.bfloat16, torch.float32, torch.float16):
+        gk, gv = kv4_load(gp, gt, _gpu(starts, dev), _gpu(counts, dev), t, d, dtype=out)
+        for got, y in ((gk, k), (gv, v)):
+            ref = model.decode(*model.encode(y.double().cpu().numpy()))
+            ref[1] = 0.0
+            want_t = torch.from_numpy(ref).to(out)  # exact in bf16 and fp32; fp16 rounds and overflows as torch does
+            assert _same_nan(got.double().cpu().numpy(), want_t.double().numpy())
+            assert torch.equal(torch.nan_to_num(got.cpu(), nan=0.0, posinf=9e4, neginf=-9e4),
+                               torch.nan_to_num(want_t, nan=0.0, posinf=9e4, neginf=-9e4))
+
+
+def test_store_reads_strided_rows_in_place_and_odd_ones_by_copy(dev):
+    from sparsepr_amd.kernels.kv4 import kv4_load, kv4_store
+
+    rng = np.random.default_rng(5)
+    b, h, t, d, size = 2, 3, 40, 64, 32
+    table = _table(rng, [64, 64], size, 5, 2)
+    zero, cnt = torch.zeros(b, dtype=torch.int32, device=dev), torch.full((b,), t, dtype=torch.int32, device=dev)
+    base = torch.randn((b, t, h, d), device=dev).to(torch.bfloat16)
+    odd = torch.randn((b, h, t, d + 1), device=dev).to(torch.bfloat16)[..., 1:]  # rows off 16 bytes
+    flipped = torch.randn((b, h, d, t), device=dev).to(torch.bfloat16).transpose(2, 3)  # rows not packed
+    one = torch.randn((b, 1, t, d), device=dev).to(torch.bfloat16).expand(b, h, t, d)  # one head for all
+    for k, v in ((base.transpose(1, 2), odd), (flipped, one)):
+        pages = torch.zeros((5, h, size * (d + d // 16)), dtype=torch.uint8, device=dev)
+        kv4_store(pages, _gpu(table, dev), k, v, zero)
+        gk, gv = kv4_load(pages, _gpu(table, dev), zero, cnt, t, d)
+        for got, x in ((gk, k), (gv, v)):
+            ref = model.decode(*model.encode(x.double().cpu().numpy()))
+            assert np.array_equal(got.double().cpu().numpy(), ref)
+
+
+def test_rows_without_a_page_are_not_written_and_read_as_nan(dev):
+    from sparsepr_amd.kernels.kv4 import kv4_load, kv4_store
+
+    rng = np.random.default_rng(6)
+    b, h, t, d, size, wide, num = 6, 2, 5, 128, 32, 2, 4
+    # 0: fine; 1: start -1 (a reserve that did not happen); 2: past the table; 3: no page; 4: a page
+    # number past the pool; 5: a sequence outside the table
+    table = np.array([[2, 0], [1, 3], [1, 3], [-1, 3], [num, 3], [1, 1]], np.int32)
+    starts, ids = np.array([30, -1, 62, 28, 0, 0]), np.array([0, 1, 2, 3, 4, 6])
+    k = torch.randn((b, h, t, d), device=dev).to(torch.bfloat16)
+    pages = rng.integers(0, 200, (num, h, size * (d + d // 16)), np.uint8)
+    gp, gt = _gpu(pages, dev, torch.uint8), _gpu(table, dev)
+    kv4_store(gp, gt, k, k, _gpu(starts, dev), seq_ids=_gpu(ids, dev))
+    live = np.zeros((b, t), bool)
+    live[0], live[2, :2], live[3, 4:] = True, True, True
+    want = pages.copy()
+    codes, scales = model.encode(k.double().cpu().numpy())
+    for i, j in zip(*np.nonzero(live)):
+        page, slot = table[i, (starts[i] + j) // size], (starts[i] + j) % size
+        kc, vc, ks, vs = model.parts(want[page], size, d)
+        kc[:, slot] = vc[:, slot] = codes[i, :, j]
+        ks[:, slot] = vs[:, slot] = scales[i, :, j]
+    assert np.array_equal(gp.cpu().numpy(), want)
+    gk, gv = kv4_load(gp, gt, _gpu(starts, dev), torch.full((b,), t, dtype=torch.int32, device=dev), t, d,
+                      seq_ids=_gpu(ids, dev))
+    for got in (gk, gv):
+        got = got.float().cpu().numpy()
+        assert np.array_equal(np.isnan(got).all((1, 3)), ~live) and np.array_equal(np.isnan(got).any((1, 3)), ~live)
+
+
+# ------------------------------------------------------------------ attention
+
+
+def _check_attention(got, lse, q, pages, table, lengths, counts, size, causal, scale, dtype, ids=None):
+    """Error bounds, element by element, u = 2^-24:
+    - a score is a sum of D exact products in fp32, D u sum|q k| at most, times the scale (2 u more);
+      with the subtraction and the argument of exp2 in fp32 and exp2 good to 2^-22, a probability is off
+      by e = (D + 6) u L + 2^-21 of itself, L the row's largest sum |q k| scale;
+    - bf16 calls round it once more, 2^-8; fp16 calls hold it in two terms, 2^-16;
+    - sums of n terms in fp32, n u of softmax |v| = A; numerator and denominator: twice e and n u;
+    - the output is rounded once, half a step of its type."""
+    b, hq, t, d = q.shape
+    u = 2.0**-24
+    rounds, last = (2.0**-8, 2.0**-8) if dtype == "bf16" else (2.0**-16, 2.0**-11)
+    for i in range(b):
+        s = i if ids is None else ids[i]
+        n = int(lengths[s])
+        k, v = model.tokens(pages, table[s], n, size, d)
+        out, ref_lse, spread, logit = model.attend(q[i].double().cpu().numpy(), k, v, int(counts[i]), causal, scale)
+        e = ((d + 6) * u * logit + 2.0**-21)[..., None]
+        tol = spread * (rounds + 2 * e + 2 * n * u) + last * np.abs(out) + 1e-30
+        if dtype == "fp16":
+            tol = tol + 2.0**-25  # half a step of the smallest fp16
+        o = got[i].double().cpu().numpy()
+        assert _same_nan(o, out), f"entry {i}"
+        bad = np.nan_to_num(np.abs(o - out)) > np.nan_to_num(tol, nan=np.inf)
+        assert not bad.any(), f"entry {i}: {np.argwhere(bad)[:4].tolist()} off by {np.abs(o - out)[bad][:4]}, {tol[bad][:4]}"
+        got_l = lse[i].double().cpu().numpy()
+        assert np.array_equal(np.isneginf(got_l), np.isneginf(ref_lse)) and _same_nan(got_l, ref_lse)
+        fin = np.isfinite(ref_lse) & (ref_lse > -1e30)
+        # the maximum and log2 of the sum, joined in fp32
+        tol_l = e[..., 0] + n * u + 2.0**-21 + 4 * u * np.abs(ref_lse)
+        assert (np.abs(got_l[fin] - ref_lse[fin]) <= tol_l[fin]).all(), f"entry {i}: lse"
+
+
+CASES = [
+    # hq, hk, d, rows, page, lengths, counts, causal, dtype
+    (1, 1, 128, 1, 32, [1], None, False, "bf16"),
+    (3, 1, 64, 1, 32, [0, 1, 31, 32, 33], None, False, "bf16"),
+    (4, 4, 128, 1, 64, [64, 63, 65, 128, 700], None, True, "bf16"),
+    (8, 2, 128, 1, 128, [129, 2500], None, True, "fp16"),
+    (5, 1, 64, 3, 64, [2, 3, 4, 100, 0], None, True, "fp16"),
+    (6, 2, 128, 5, 32, [3, 40, 333], [5, 2, 0], True, "bf16"),
+    (2, 2, 64, 16, 256, [16, 17, 300], [16, 16, 9], True, "bf16"),
+    (2, 1, 128, 16, 64, [100, 65], None, False, "bf16"),
+    (12, 4, 64, 11, 32, [44, 45], [11, 7], True, "bf16"),
+    (2, 2, 128, 33, 64, [33, 20, 150], None, True, "bf16"),
+    (4, 2, 128, 70, 64, [64, 200], [70, 64], True, "fp16"),
+    (3, 3, 64, 129, 128, [129, 400, 1], [129, 100, 129], True, "bf16"),
+    (2, 1, 128, 150, 32, [500, 31], [150, 1], False, "bf16"),
+    (2, 2, 128, 257, 64, [1000], None, True, "bf16"),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_attention_matches_the_formula(dev, case):
+    from sparsepr_amd.kernels.kv4 import kv4_attention
+
+    hq, hk, d, rows, size, lengths, counts, causal, dtype = case
+    rng = np.random.default_rng(hash((hq, d, rows)) % 1000)
+    b, wide = len(lengths), max(1, max(-(-n // size) for n in lengths)) + 1
+    num = sum(-(-n // size) for n in lengths) + 2
+    pages = _pool(rng, num, hk, size, d)
+    table = _table(rng, lengths, size, num, wide)
+    # what lies past a sequence's end, in its last page and in pages of nobody, is NaN
+    used = np.zeros((num, size), bool)
+    for i, n in enumerate(lengths):
+        for j in range(n):
+            used[table[i, j // size], j % size] = True
+    for part in model.parts(pages, size, d)[2:]:
+        part[np.broadcast_to(~used[:, None], (num, hk, size))] = 255
+    q = (torch.randn((b, hq, rows, d), generator=torch.Generator().manual_seed(3)) * 0.9).to(DT[dtype]).to(dev)
+    cnt = np.array(counts if counts is not None else [rows] * b)
+    scale = 1.0 / math.sqrt(d)
+    out, lse = kv4_attention(q, _gpu(pages, dev, torch.uint8), _gpu(table, dev), _gpu(lengths, dev),
+                             counts=None if counts is None else _gpu(cnt, dev), causal=causal, return_lse=True)
+    _check_attention(out, lse, q, pages, table, lengths, cnt, size, causal, scale, dtype)
+
+
+def test_seq_ids_share_scale_and_strides(dev):
+    """Two entries on one sequence, a scale of the caller's, q by its strides and q off 16 bytes."""
+    from sparsepr_amd.kernels.kv4 import kv4_attention
+
+    rng = np.random.default_rng(8)
+    hq, hk, d, size, rows = 6, 3, 64, 32, 4
+    lengths, ids = [70, 5, 33], [2, 0, 2, 1]
+    num = sum(-(-n // size) for n in lengths)
+    pages, table = _pool(rng, num, hk, size, d), _table(rng, lengths, size, num, 3)
+    args = (_gpu(pages, dev, torch.uint8), _gpu(table, dev), _gpu(lengths, dev))
+    base = torch.randn((4, rows, hq, d), device=dev).to(torch.bfloat16)
+    odd = torch.randn((4, hq, rows, d + 3), device=dev).to(torch.bfloat16)[..., 3:]
+    for q in (base.transpose(1, 2), odd, base.transpose(1, 2)[:, :, :1]):
+        out, lse = kv4_attention(q, *args, seq_ids=_gpu(ids, dev), causal=True, scale=0.3, return_lse=True)
+        _check_attention(out, lse, q, pages, table, lengths, [q.shape[2]] * 4, size, True, 0.3, "bf16", ids)
+
+
+@pytest.mark.parametrize("rows,hq", [(1, 2), (40, 2), (130, 2)])
+def test_nan_groups_reach_the_rows_that_see_them_and_no_others(dev, rows, hq):
+    from sparsepr_amd.kernels.kv4 import kv4_attention
+
+    rng = np.random.default_rng(9)
+    hk, d, size, n = 2, 128, 64, 200
+    for where in (0, n - rows // 2 - 1, n - 1):
+        for part, group in ((2, 1), (3, 2), (3, 0)):  # a K scale, V scales
+            pages, table = _pool(rng, 4, hk, size, d), _table(rng, [n], size, 4, 4)
+            model.parts(pages[table[0, where // size]], size, d)[part][1, where % size, group] = 255
+            q = torch.randn((1, hq, rows, d), device=dev).to(torch.bfloat16)
+            out, lse = kv4_attention(q, _gpu(pages, dev, torch.uint8), _gpu(table, dev), _gpu([n], dev), causal=True,
+                                     return_lse=True)
+            _check_attention(out, lse, q, pages, table, [n], [rows], size, True, d**-0.5, "bf16")
+
+
+@pytest.mark.parametrize("rows", [1, 50, 200])
+def test_broken_tables_give_nan_and_leave_the_others_alone(dev, rows):
+    from sparsepr_amd.kernels.kv4 import kv4_attention
+
+    rng = np.random.default_rng(10)
+    hk, d, size, wide = 1, 64, 32, 4
+    lengths = [100, 100, 129, -3, 100]  # 1: a page past the pool; 2: longer than the table; 3: negative
+    pages, table = _pool(rng, 12, hk, size, d), _table(rng, [100, 100, 128, 0, 0], size, 12, wide)
+    table[1, 2] = 99
+    table[4] = [0, -1, 1, 2]
+    ids = [0, 1, 2, 3, 4, 7, -1]
+    q = torch.randn((len(ids), 2, rows, d), device=dev).to(torch.bfloat16)
+    out, lse = kv4_attention(q, _gpu(pages, dev, torch.uint8), _gpu(table, dev), _gpu(lengths, dev),
+                             seq_ids=_gpu(ids, dev), return_lse=True)
+    _check_attention(out[:1], lse[:1], q[:1], pages, table, lengths, [rows], size, False, d**-0.5, "bf16")
+    assert torch.isnan(out[1:]).all() and torch.isnan(lse[1:]).all()
+
+
+def test_sharp_scores_and_long_sequences(dev):
+    """Scores far apart (one key takes all, the maximum moves late) and 40,000 keys in many shares."""
+    from sparsepr_amd.kernels.kv4 import kv4_attention
+
+    rng = np.random.default_rng(11)
+    for rows, n, amp in ((1, 40001, 1.0), (20, 3000, 25.0), (70, 3000, 25.0), (130, 9000, 4.0)):
+        hk, d, size = 1, 128, 64
+        num = -(-n // size)
+        pages, table = _pool(rng, num, hk, size, d, amp), _table(rng, [n], size, num, num)
+        q = torch.randn((1, 2, rows, d), device=dev).to(torch.bfloat16)
+        for longest in (None, 64, n):  # a wrong bound sizes the launch and nothing else
+            out, lse = kv4_attention(q, _gpu(pages, dev, torch.uint8), _gpu(table, dev), _gpu([n], dev),
+                                     max_length=longest, return_lse=True)
+            _check_attention(out, lse, q, pages, table, [n], [rows], size, False, d**-0.5, "bf16")
+
+
+def test_pages_past_two_gigabytes(dev):
+    from sparsepr_amd.kernels.kv4 import kv4_attention, kv4_compact, kv4_fork, kv4_load, kv4_store
+
+    rng = np.random.default_rng(12)
+    h, d, size = 16, 128, 256
+    each = h * size * (d + d // 16)
+    num = (5 << 29) // each + 1  # 2.5 GiB
+    pages = torch.zeros((num, h, each // h), dtype=torch.uint8, device=dev)
+    table = np.array([[num - 1, num - 3, num // 2, 1], [-1] * 4], np.int32)
+    refs = np.zeros(num, np.int32)
+    refs[table[0]] = 1
+    gt, gl, gr = _gpu(table, dev), _gpu([900, 0], dev), _gpu(refs, dev)
+    k, v = torch.randn((2, 1, h, 900, d), device=dev).to(torch.bfloat16)
+    zero, cnt = _gpu([0], dev), _gpu([900], dev)
+    kv4_store(pages, gt, k, v, zero)
+    want = [torch.from_numpy(model.decode(*model.encode(x.double().cpu().numpy()))) for x in (k, v)]
+
+    def check(seq):
+        got = kv4_load(pages, gt, zero, cnt, 900, d, seq_ids=_gpu([seq], dev))
+        assert all(torch.equal(a.double().cpu(), b) for a, b in zip(got, want))
+
+    check(0)
+    q = torch.randn((1, h, 3, d), device=dev).to(torch.bfloat16)
+    before = kv4_attention(q, pages, gt, gl, seq_ids=zero, causal=True)
+    kv4_fork(pages, gt, gl, gr, size, _gpu([0], dev), _gpu([1], dev), share=False)
+    check(1)
+    live = kv4_compact(pages, gt, gr)
+    assert int(live) == 8 and int(gt.max()) == 7 and int(gr.sum()) == 8
+    check(0), check(1)
+    for seq in (0, 1):
+        assert torch.equal(before, kv4_attention(q, pages, gt, gl, seq_ids=_gpu([seq], dev), causal=True))
+
+
+# ------------------------------------------------------------------ pages
+
+
+def _assert_same(cache, m):
+    assert np.array_equal(cache.block_table.cpu().numpy(), m.table)
+    assert np.array_equal(cache.lengths.cpu().numpy(), m.lengths)
+    assert np.array_equal(cache.ref_count.cpu().numpy(), m.refs)
+
+
+def _status(cache):
+    got = int(cache.status.item())
+    cache.status.zero_()
+    return got
+
+
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("size,num,wide", [(32, 40, 9), (64, 5000, 3)])
+def test_a_run_of_page_calls_follows_the_lists(dev, seed, size, num, wide):
+    """Random reserves, stores, frees of ranges, forks, copies and compactions, good ones and refused
+    ones: tables, lengths, holders and status after each call, the tokens of every sequence, and
+    attention over them, now and then."""
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    rng = np.random.default_rng(100 * seed + size)
+    seqs, h, d, layers = 7, 2, 64, 2
+    cache = KV4Cache(num, h, d, seqs, page_size=size, max_pages=wide, layers=layers, device=dev)
+    m = model.Pages(num, seqs, wide, size)
+    text = [[np.zeros((2, h, 0, d)) for _ in range(seqs)] for _ in range(layers)]  # K, V values of each sequence
+    seen = set()
+    for step in range(60):
+        op = rng.choice(["append", "append", "append", "free", "range", "fork", "copy", "compact"])
+        n = int(rng.integers(1, 4))
+        ids = [int(i) for i in rng.integers(-1 if rng.random() < 0.1 else 0, seqs + (rng.random() < 0.1), n)]
+        if rng.random() < 0.85:
+            ids = list(dict.fromkeys(ids))
+        if op == "append":
+            counts = [int(c) for c in rng.integers(-1 if rng.random() < 0.1 else 0, size * 2, len(ids))]
+            code, starts = m.reserve(ids, counts)
+            got = cache.reserve(counts, ids)
+            assert got.cpu().tolist() == starts
+            t = max(max(counts), 1)
+            for layer in range(layers):
+                k, v = torch.randn((2, len(ids), h, t, d), device=dev).to(torch.bfloat16)
+                cache.store(k, v, got, counts=counts, seq_ids=ids, layer=layer)
+                if code == 0:
+                    for x, (i, c) in enumerate(zip(ids, counts)):
+                        new = np.stack([model.decode(*model.encode(y[x, :, :c].double().cpu().numpy())) for y in (k, v)])
+                        text[layer][i] = np.concatenate([text[layer][i], new], 2)
+        elif op == "free":
+            code = m.free(ids)
+            cache.free(ids)
+            if code == 0:
+                for layer in range(layers):
+                    for i in ids:
+                        text[layer][i] = text[layer][i][:, :, :0]
+        elif op == "range":
+            firsts, counts = ([int(c) for c in rng.integers(0, 3, len(ids))] for _ in range(2))
+            counts = [c if rng.random() < 0.8 else -1 for c in counts]
+            before = m.lengths.copy()
+            code = m.free(ids, firsts, counts)
+            cache.free(ids, first_pages=firsts, page_counts=counts)
+            if code == 0:
+                for layer in range(layers):
+                    for i, f, c in zip(ids, firsts, counts):
+                        end = min((f + c) * size, before[i]) if c >= 0 else before[i]
+                        text[layer][i] = np.delete(text[layer][i], np.s_[f * size:end], 2)
+        elif op == "compact":
+            code, live = 0, m.compact()[0]
+            assert int(cache.compact()) == live
+        else:
+            to = [int(i) for i in rng.integers(0, seqs, len(ids))]
+            if rng.random() < 0.8:  # mostly onto empty ones
+                empty = [i for i in range(seqs) if m.lengths[i] == 0]
+                to = empty[:len(ids)]
+                ids = ids[:len(to)]
+            if not ids:
+                continue
+            code, _ = m.fork(ids, to, op == "fork")
+            cache.fork(ids, to, share=op == "fork")
+            if code == 0:
+                for layer in range(layers):
+                    for s, t in zip(ids, to):
+                        text[layer][t] = text[layer][s]
+        assert _status(cache) == code, (step, op, ids)
+        seen.add((op, code))
+        _assert_same(cache, m)
+        if step % 6 == 5:
+            longest = max(int(m.lengths.max()), 1)
+            for layer in range(layers):
+                got = cache.load([0] * seqs, m.lengths, longest, layer=layer)
+                for i in range(seqs):
+                    for g, want in zip(got, text[layer][i]):
+                        assert np.array_equal(g[i, :, :m.lengths[i]].double().cpu().numpy(), want), (step, i)
+            q = torch.randn((seqs, 4, 2, d), device=dev).to(torch.bfloat16)
+            out, lse = cache.attend(q, layer=1, causal=True, return_lse=True)
+            _check_attention(out, lse, q, cache.pages[1].cpu().numpy(), m.table, m.lengths, [2] * seqs, size, True,
+                             d**-0.5, "bf16")
+    assert len({op for op, code in seen if code == 0}) >= 4  # kinds of call, of six
+
+
+def test_every_refusal_is_named_and_changes_nothing(dev):
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    cache = KV4Cache(6, 1, 64, 4, page_size=32, max_pages=4, device=dev)
+    m = model.Pages(6, 4, 4, 32)
+    cache.reserve([70, 40], [0, 1])
+    m.reserve([0, 1], [70, 40])
+    cache.check()
+    for code, call, text in [
+        (1, lambda: cache.reserve([1], [4]), "outside the table"),
+        (1, lambda: cache.free([-1]), "outside the table"),
+        (1, lambda: cache.fork([0], [9]), "outside the table"),
+        (2, lambda: cache.reserve([1, 1], [2, 2]), "named twice"),
+        (2, lambda: cache.free([0, 1, 0]), "named twice"),
+        (2, lambda: cache.fork([0, 1], [2, 2]), "named twice"),
+        (2, lambda: cache.fork([0, 2], [3, 2]), "named twice"),
+        (3, lambda: cache.reserve([-1], [2]), "negative count"),
+        (3, lambda: cache.free([0], first_pages=[2], page_counts=[2]), "range outside"),
+        (3, lambda: cache.free([1], first_pages=[3]), "range outside"),
+        (4, lambda: cache.reserve([1, 129], [0, 2]), "more tokens than a row"),
+        (4, lambda: cache.reserve([2**31 - 1], [0]), "more tokens than a row"),
+        (5, lambda: cache.reserve([58, 10], [0, 2]), "not enough free pages"),
+        (5, lambda: cache.fork([0], [2], share=False), "not enough free pages"),
+        (5, lambda: cache.fork([0, 1], [2, 3]), "not enough free pages"),
+        (6, lambda: cache.fork([0], [1]), "holds tokens"),
+    ]:
+        got = call()
+        if got is not None:
+            assert (got == -1).all()
+        _assert_same(cache, m)
+        with pytest.raises(RuntimeError, match=text):
+            cache.check()
+        cache.check()
+    # the first one stays until it is read
+    cache.free([7])
+    cache.reserve([1, 1], [2, 2])
+    with pytest.raises(RuntimeError, match="outside the table"):
+        cache.check()
+    # tables that cannot be
+    cache.block_table[0, 1] = 6
+    for call in (lambda: cache.free([0]), lambda: cache.fork([0], [2])):
+        call()
+        with pytest.raises(RuntimeError, match="entry outside the pool"):
+            cache.check()
+    cache.lengths[1] = 129
+    for call in (lambda: cache.free([1]), lambda: cache.reserve([1], [1]), lambda: cache.fork([1], [2])):
+        call()
+        with pytest.raises(RuntimeError, match="length outside the table"):
+            cache.check()
+
+
+def test_as_many_sequences_as_a_call_may_name(dev):
+    from sparsepr_amd.kernels.kv4 import MAX_NAMED
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    rng = np.random.default_rng(13)
+    n = MAX_NAMED
+    cache = KV4Cache(9000, 1, 64, n, page_size=32, max_pages=3, device=dev)
+    m = model.Pages(9000, n, 3, 32)
+    ids = rng.permutation(n).tolist()
+    counts = rng.integers(0, 96, n).tolist()
+    code, starts = m.reserve(ids, counts)
+    assert cache.reserve(counts, ids).tolist() == starts and code == 0
+    _assert_same(cache, m)
+    m.free(ids[::2])
+    cache.free(ids[::2])
+    half = n // 2
+    assert m.fork(ids[1::2], ids[::2], True)[0] == 0
+    cache.fork(ids[1::2], ids[::2])
+    _assert_same(cache, m)
+    assert int(cache.compact()) == m.compact()[0] and half > 0
+    _assert_same(cache, m)
+    cache.check()
+    with pytest.raises(RuntimeError, match="at most"):
+        cache.free([0] * (n + 1))
+
+
+# ------------------------------------------------------------------ streams, graphs, repeats
+
+
+def _decode_step(cache, q, k, v):
+    cache.append(k, v)
+    return cache.attend(q, causal=True, max_length=300)
+
+
+def _filled(dev, seqs, h, d, tokens, seed):
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    g = torch.Generator(device=dev).manual_seed(seed)
+    cache = KV4Cache(60, h, d, seqs, page_size=32, max_pages=12, device=dev)
+    k, v = torch.randn((2, seqs, h, max(tokens), d), generator=g, device=dev).to(torch.bfloat16)
+    cache.append(k, v, counts=tokens)
+    return cache
+
+
+def test_a_captured_step_replays_as_eager_calls_do(dev):
+    seqs, h, d = 3, 2, 128
+    g = torch.Generator(device=dev).manual_seed(2)
+    steps = [[torch.randn((seqs, n, 1, d), generator=g, device=dev).to(torch.bfloat16) for n in (4, h, h)] for _ in range(70)]
+    eager, graphed = (_filled(dev, seqs, h, d, [200, 31, 0], 1) for _ in range(2))
+    ins = [x.clone() for x in steps[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _decode_step(_filled(dev, seqs, h, d, [5, 5, 5], 4), *ins)  # warm
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _decode_step(graphed, *ins)
+    for x in steps:  # two graphs' worth of steps, eager work and a synchronisation between replays
+        want = _decode_step(eager, *x)
+        for a, b in zip(ins, x):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert torch.equal(eager.block_table, graphed.block_table) and torch.equal(eager.lengths, graphed.lengths)
+    assert torch.equal(eager.pages, graphed.pages)
+    eager.check(), graphed.check()
+
+
+def test_calls_on_two_streams_and_repeats_give_the_same_bits(dev):
+    seqs, h, d = 4, 2, 64
+    caches = [_filled(dev, seqs, h, d, [300, 7, 128, 33], 5 + i) for i in range(2)]
+    q = [torch.randn((seqs, 8, t, d), device=dev).to(torch.float16) for t in (1, 60)]
+    want = [[c.attend(x, causal=True) for x in q] for c in caches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in caches]
+    for _ in range(5):
+        got = []
+        for c, s in zip(caches, streams):
+            with torch.cuda.stream(s):
+                got.append([c.attend(x, causal=True) for x in q])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
