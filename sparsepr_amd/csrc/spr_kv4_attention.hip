@@ -99,6 +99,10 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(spr::as_bf16x8(a), spr::as_bf16x8(b), c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(spr::as_bf16x8(a), spr::as_bf16x8(b), c, 0, 0, 0);
+}
+
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short v4i16;
 typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
 // ds_read_b64_tr_b16: in each group of 16 lanes, output lane 4A + B gets element B of the reads of
@@ -147,8 +151,8 @@ struct Held {
   uint32_t ks[2], vs[2];
 };
 
-// Up to 16 * NT query rows of one kv head against a share of its keys.  Grid (nsplit, kv_heads * row
-// tiles, batch); each wave walks 32-key blocks of its own with its own softmax, and the four are merged
+// Up to 16 * NT query rows of one kv head against a share of its keys.  Grid (nsplit, kv_heads,
+// batch); each wave walks 32-key blocks of its own with its own softmax, and the four are merged
 // at the end.
 //
 // Scores: S^T[key, row] = K Q^T by 16x16x32 MFMA.  A lane holds a quarter of one key's dims (16 bytes
@@ -171,8 +175,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kv4_few_kernel(AttnArgs a) {
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4;
-  const int tiles = gridDim.y / a.kv_heads;
-  const int hk = blockIdx.y / tiles, tile = blockIdx.y % tiles, b = blockIdx.z, split = blockIdx.x;
+  const int hk = blockIdx.y, b = blockIdx.z, split = blockIdx.x;
   const int total_rows = a.rows * a.group;
   const Span sp = span_of(a, b);
   const int32_t* row_table = a.table + static_cast<int64_t>(sp.seq) * a.wide;
@@ -182,7 +185,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kv4_few_kernel(AttnArgs a) {
   int32_t least = sp.length, most = 0;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int rho = tile * 16 * NT + n * 16 + m;
+    const int rho = n * 16 + m;
     const bool in = rho < total_rows;
     const int t = in ? rho / a.group : 0, h = hk * a.group + (in ? rho % a.group : 0);
     seen[n] = in ? visible_of(a, sp, t) : 0;
@@ -386,7 +389,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kv4_few_kernel(AttnArgs a) {
     constexpr int PIECES = D / 4;  // 16-byte pieces of a row
     for (int i = threadIdx.x; i < 16 * PIECES; i += 64 * FEW_WAVES) {
       const int r = i / PIECES, p = i % PIECES;
-      const int rho = tile * 16 * NT + n * 16 + r;
+      const int rho = n * 16 + r;
       if (rho >= total_rows) continue;
       float top = lds_ml[0][0][r];
 #pragma unroll
@@ -424,18 +427,371 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kv4_few_kernel(AttnArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------- many rows
+
+constexpr int MANY_WAVES = 8;
+constexpr int MANY_KEYS = 64;  // keys of a chunk
+
+__device__ __forceinline__ float max_xor32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_xor32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// 256 query rows (HALVES false: a wave has 32 rows and all keys) or 128 (true: waves w and w + 4 have
+// the same 32 rows, w the first 32 keys of every chunk and w + 4 the second, merged at the end) of one
+// kv head against a share of its keys.  One workgroup per CU, two waves per SIMD.
+//
+// A chunk of 64 keys is brought from its codes to bf16 once for all eight waves: a thread turns 32
+// values of one row (16 bytes of codes, one scale) into 64 bytes of a row-major LDS tile, 16 conversions
+// and 4 writes.  The codes of chunk x + 3 are loaded and those of x + 2 written at the end of chunk x.
+// Scores and output are S^T = K Q^T and O^T += V^T P^T by 32x32x16 MFMA with a lane owning one query
+// row; V^T comes from the transposing read, P from the accumulator in the same order of keys.  S of the
+// next 32 keys is computed beside the exponentials of the current ones.
+//
+// Tiles: 16-byte piece p of row r lies at p ^ (r & 15) in K and at p ^ (4 (r & 3) + (r >> 2 & 3)) in V
+// (D = 128; within the eight pieces of a row for D = 64, p ^ (r >> 1 & 7) and p ^ (4 (r >> 1 & 1) +
+// (r >> 2 & 3))): the conversion's writes of 16 rows, K's reads of 16 rows and V's transposing reads of
+// four rows by 64 bytes each meet every bank once.
+// K: two tiles (the chunk's second half is read before its barrier, the tile written behind it); V:
+// three (the second half is read behind the barrier).
+template <int D, bool F16, bool HALVES>
+__global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a) {
+  using Part = spr::Kv4Part<D>;
+  constexpr int ROW = 2 * D;
+  constexpr int TILE = MANY_KEYS * ROW;
+  constexpr int KSTEPS = D / 16, DBLK = D / 32;
+  constexpr int TROWS = HALVES ? 128 : 256;
+  constexpr int GROUPS = D / spr::KV4_GROUP;        // scales of a row
+  constexpr int CONV = MANY_KEYS * GROUPS;          // threads that convert K (and as many V)
+  __shared__ __align__(1024) uint8_t k_tiles[2][TILE];
+  __shared__ __align__(1024) uint8_t v_tiles[3][TILE];
+  __shared__ uint32_t v_bytes[3][MANY_KEYS];  // the V scale bytes of every key
+  __shared__ float merge_ml[4][64][2];
+
+  // consecutive tiles of one head and share on one XCD: they read the same codes
+  const int total_rows = a.rows * a.group;
+  const int tiles = (total_rows + TROWS - 1) / TROWS;
+  const int64_t total = static_cast<int64_t>(tiles) * a.nsplit * a.kv_heads * a.batch;
+  const int64_t id = (blockIdx.x & 7) * ((total + 7) / 8) + (blockIdx.x >> 3);
+  if (id >= total || (blockIdx.x >> 3) >= (total + 7) / 8) return;
+  const int tile = static_cast<int>(id % tiles);
+  const int split = static_cast<int>(id / tiles % a.nsplit);
+  const int64_t bh = id / tiles / a.nsplit;
+  const int hk = static_cast<int>(bh % a.kv_heads), b = static_cast<int>(bh / a.kv_heads);
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int blk = HALVES ? (wave & 3) : wave;
+  const int only = HALVES ? (wave >> 2) : 0;  // HALVES: which half of a chunk
+  const Span sp = span_of(a, b);
+  const int32_t* row_table = a.table + static_cast<int64_t>(sp.seq) * a.wide;
+
+  const int rho = tile * TROWS + blk * 32 + col;
+  const bool in = rho < total_rows;
+  const int t = in ? rho / a.group : 0, h = hk * a.group + (in ? rho % a.group : 0);
+  const bool used = in && t < sp.count;
+  const int32_t seen = used ? visible_of(a, sp, t) : 0;
+  // rows are token-major, so the last row of a list sees most and the first one in use least
+  const int row0 = tile * TROWS, row1 = min(row0 + TROWS, total_rows) - 1;
+  const int32_t t_last = min(row1 / a.group, sp.count - 1);
+  const int32_t most = t_last < row0 / a.group ? 0 : visible_of(a, sp, t_last);
+  const int32_t least = visible_of(a, sp, min(row0 / a.group, max(sp.count - 1, 0)));
+  const int w0 = row0 + blk * 32;
+  const bool wave_live = w0 < total_rows && w0 / a.group < sp.count;
+  const int32_t wave_least = visible_of(a, sp, min(w0 / a.group, max(sp.count - 1, 0)));
+
+  const int chunks = (most + MANY_KEYS - 1) / MANY_KEYS;
+  const int per = (chunks + a.nsplit - 1) / a.nsplit;
+  const int c0 = split * per, nch = min(chunks, c0 + per) - c0;
+
+  u32x4 qh[KSTEPS], ql[F16 ? KSTEPS : 1];
+  const uint16_t* qp = a.q + b * a.q_b + h * a.q_h + t * a.q_t + half * 8;
+#pragma unroll
+  for (int s = 0; s < KSTEPS; ++s) {
+    u32x4 lo;
+    split8<F16>(used ? *reinterpret_cast<const u32x4*>(qp + 16 * s) : u32x4{0, 0, 0, 0}, qh[s], lo);
+    if constexpr (F16) ql[s] = lo;
+  }
+  f32x16 o_acc[DBLK];
+#pragma unroll
+  for (int i = 0; i < DBLK; ++i) o_acc[i] = f32x16{};
+  float m_run = NEG_INF, l_run = 0.0f, neg_m = 0.0f, m_thr = NEG_INF;
+
+  // ---- codes to tiles
+  const int64_t head = static_cast<int64_t>(hk) * spr::kv4_head_bytes(1 << a.log_s, D);
+  const bool conv = threadIdx.x < 2 * CONV, conv_v = threadIdx.x >= CONV;
+  const int ci = threadIdx.x & (CONV - 1);
+  const int cr = (ci & 15) + 16 * (ci / (16 * GROUPS)), cg = (ci >> 4) & (GROUPS - 1);
+  u32x4 code = {0, 0, 0, 0};
+  uint32_t byte = 127;
+  int32_t next_page = -1;
+  auto look = [&](int c) {  // the page of this thread's row of chunk c
+    const int32_t key = (c0 + c) * MANY_KEYS + cr;
+    next_page = key < most ? row_table[key >> a.log_s] : -1;
+  };
+  auto fetch = [&](int c) {
+    const int32_t key = (c0 + c) * MANY_KEYS + cr;
+    const bool ok = next_page >= 0 && next_page < a.num_pages;
+    code = u32x4{0, 0, 0, 0};
+    byte = key < most ? 255 : 127;  // a page outside the pool is NaN; past the end nothing is read
+    if (ok && conv) {
+      const uint8_t* part = a.pages + next_page * a.page_stride + head;
+      const int32_t r = key & ((1 << a.log_s) - 1);
+      code = *reinterpret_cast<const u32x4*>(part + (conv_v ? Part::v_codes(a.log_s) : 0) + r * Part::CODE_ROW + cg * 16);
+      byte = part[(conv_v ? Part::v_scales(a.log_s) : Part::k_scales(a.log_s)) + r * Part::SCALE_ROW + cg];
+    }
+  };
+  const int swz_k = D == 128 ? (cr & 15) : ((cr >> 1) & 7);
+  const int swz_v = D == 128 ? 4 * (cr & 3) + ((cr >> 2) & 3) : 4 * ((cr >> 1) & 1) + ((cr >> 2) & 3);
+  auto stash = [&](int c) {
+    if (!conv) return;
+    const int32_t end = (c0 + c + 1) * MANY_KEYS;
+    uint8_t* to = (conv_v ? v_tiles[c % 3] : k_tiles[c & 1]) + cr * ROW;
+    const int x = conv_v ? swz_v : swz_k;
+    // a chunk that some row does not see whole keeps NaN V scales out of the products (0 * NaN); they
+    // are put in row by row
+    const float sc = spr::kv4_scale(conv_v && byte == 255 && end > least ? 127 : byte);
+    const uint32_t w[4] = {code.x, code.y, code.z, code.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(to + (((4 * cg + i) ^ x) << 4)) = spr::kv4_eight(w[i], sc);
+    if (conv_v) reinterpret_cast<uint8_t*>(&v_bytes[c % 3][cr])[cg] = static_cast<uint8_t>(byte);
+  };
+
+  // ---- products
+  const int k_x = D == 128 ? (half ^ (col & 15)) : (half ^ ((col >> 1) & 7));
+  const int tr_a = lane & 3, tr_i = (lane >> 2) & 3, tr_g = (lane >> 4) & 1;
+  const int v_lane = (4 * half + tr_i) * ROW + (tr_a & 1) * 8;
+  const int v_piece = 2 * tr_g + (tr_a >> 1);
+  const int v_x = (D == 128 ? 4 * tr_i : 4 * (tr_i >> 1)) + half;
+  auto kfrag = [&](const uint8_t* kt, int hf, int s) {
+    return *reinterpret_cast<const u32x4*>(kt + (hf * 32 + col) * ROW + (((2 * s) ^ k_x) << 4));
+  };
+  auto vfrag = [&](const uint8_t* vt, int hf, int f) {  // f = DBLK * key step + dim block
+    const uint8_t* at = vt + 16 * (2 * hf + f / DBLK) * ROW + v_lane;
+    const int p = 4 * (f % DBLK) + v_piece;
+    const u32x2 r0 = lds_read_tr16(at + ((p ^ v_x) << 4));
+    const u32x2 r1 = lds_read_tr16(at + 8 * ROW + ((p ^ v_x ^ 2) << 4));
+    return u32x4{r0[0], r0[1], r1[0], r1[1]};
+  };
+  auto s_mma = [&](f32x16& acc, const uint8_t* kt, int hf) {
+    acc = f32x16{};
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) {
+      const u32x4 k = kfrag(kt, hf, s);
+      acc = mfma32(k, qh[s], acc);
+      if constexpr (F16) acc = mfma32(k, ql[s], acc);
+    }
+  };
+  // mask, row maximum and lazy rescale of the 32 keys from `key` on
+  auto row_max = [&](f32x16& acc, int32_t key) {
+    if (key + 32 > wave_least) {
+      const int lim = seen - key - 4 * half;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (8 * (e / 4) + (e % 4) >= lim) acc[e] = NEG_INF;
+      }
+    }
+    float mx = NEG_INF;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[e]);
+    const float mloc = max_xor32(mx) * a.scale_log2;
+    const bool up = mloc > m_thr;
+    if (__ballot(up) != 0) {
+      // only the rows whose maximum grew move theirs: a row's result does not depend on its wave's
+      const float m_new = up ? mloc : m_run;
+      const float f = up ? exp2_hw(m_run - m_new) : 1.0f;
+      l_run *= f;
+#pragma unroll
+      for (int i = 0; i < DBLK; ++i) o_acc[i] *= f;
+      m_run = m_new;
+      m_thr = m_new + RESCALE_SLACK;
+      neg_m = m_new == NEG_INF ? 0.0f : -m_new;
+    }
+  };
+  // S of 32 keys (kt_n, hf_n) into acc_next beside the exponentials of acc, then O += P V (vt, hf)
+  auto step = [&](f32x16& acc_next, const uint8_t* kt_n, int hf_n, const f32x16& acc, const uint8_t* vt, int hf) {
+    uint32_t ph[2][4], pl[2][4];
+    float sum0 = 0.0f, sum1 = 0.0f;
+    acc_next = f32x16{};
+    constexpr int EACH = 16 / KSTEPS;  // elements of P beside each step of S
+    u32x4 ka[3];
+    ka[0] = kfrag(kt_n, hf_n, 0);
+    ka[1] = kfrag(kt_n, hf_n, 1);
+#pragma unroll
+    for (int st = 0; st < KSTEPS; ++st) {
+      if (st + 2 < KSTEPS) ka[(st + 2) % 3] = kfrag(kt_n, hf_n, st + 2);
+      acc_next = mfma32(ka[st % 3], qh[st], acc_next);
+      if constexpr (F16) acc_next = mfma32(ka[st % 3], ql[st], acc_next);
+#pragma unroll
+      for (int e = EACH * st; e < EACH * (st + 1); e += 2) {
+        const float p0 = exp2_hw(__builtin_fmaf(acc[e], a.scale_log2, neg_m));
+        const float p1 = exp2_hw(__builtin_fmaf(acc[e + 1], a.scale_log2, neg_m));
+        sum0 += p0;
+        sum1 += p1;
+        const uint32_t w = spr::pack_bf16x2(p0, p1);
+        ph[e / 8][(e % 8) / 2] = w;
+        if constexpr (F16) pl[e / 8][(e % 8) / 2] = spr::pack_bf16x2(p0 - spr::bf16_lo(w), p1 - spr::bf16_hi(w));
+      }
+    }
+    l_run += sum0 + sum1;
+    u32x4 va[3];
+    va[0] = vfrag(vt, hf, 0);
+    va[1] = vfrag(vt, hf, 1);
+#pragma unroll
+    for (int f = 0; f < 2 * DBLK; ++f) {
+      if (f + 2 < 2 * DBLK) va[(f + 2) % 3] = vfrag(vt, hf, f + 2);
+      const int k = f / DBLK;
+      o_acc[f % DBLK] = mfma32(va[f % 3], u32x4{ph[k][0], ph[k][1], ph[k][2], ph[k][3]}, o_acc[f % DBLK]);
+      if constexpr (F16) o_acc[f % DBLK] = mfma32(va[f % 3], u32x4{pl[k][0], pl[k][1], pl[k][2], pl[k][3]}, o_acc[f % DBLK]);
+    }
+  };
+  // NaN V scales of a chunk that some row does not see whole: their dims of the rows that see the key
+  auto put_nan = [&](int c) {
+    const int32_t first = (c0 + c) * MANY_KEYS;
+    if (first + MANY_KEYS <= least) return;
+    const uint32_t w = v_bytes[c % 3][lane];
+    uint32_t mine = 0;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) mine |= ((w >> (8 * g)) & 255) == 255 ? 1u << g : 0;
+    uint64_t keys = __ballot(mine != 0);
+    while (keys != 0) {
+      const int k = __builtin_ctzll(keys);
+      keys &= keys - 1;
+      const uint32_t groups = __builtin_amdgcn_readlane(mine, k);
+      if (HALVES && (k >> 5) != only) continue;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        if (((groups >> g) & 1) != 0 && first + k < seen) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o_acc[g][e] = __builtin_nanf("");
+        }
+      }
+    }
+  };
+
+  if (nch > 0) {
+    look(0), fetch(0), look(1), stash(0);
+    if (nch > 1) {
+      fetch(1), look(2), stash(1);
+    }
+    fetch(2), look(3);
+    __syncthreads();
+    f32x16 s_a, s_b;
+    if (wave_live) s_mma(s_a, k_tiles[0], only);
+    for (int x = 0; x < nch; ++x) {
+      const int32_t key = (c0 + x) * MANY_KEYS;
+      const uint8_t *kt = k_tiles[x & 1], *kt1 = k_tiles[(x + 1) & 1], *vt = v_tiles[x % 3];
+      // the last chunk computes a next S from an old tile, unused: the same straight code
+      if constexpr (HALVES) {
+        if (wave_live) row_max(s_a, key + 32 * only);
+        __syncthreads();
+        if (wave_live) {
+          step(s_b, kt1, only, s_a, vt, only);
+          s_a = s_b;
+          put_nan(x);
+        }
+      } else {
+        if (wave_live) {
+          row_max(s_a, key);
+          step(s_b, kt, 1, s_a, vt, 0);
+          row_max(s_b, key + 32);
+        }
+        __syncthreads();
+        if (wave_live) {
+          step(s_a, kt1, 0, s_b, vt, 1);
+          put_nan(x);
+        }
+      }
+      if (x + 2 < nch) {
+        stash(x + 2);
+        fetch(x + 3);
+        look(x + 4);
+      }
+    }
+  }
+
+  float l_tot = sum_xor32(l_run);
+  if constexpr (HALVES) {
+    // waves 4 .. 7 hand (m, l, O) to waves 0 .. 3 through the tiles: 32 rows of D floats each
+    float* po = reinterpret_cast<float*>(blk < 2 ? k_tiles[blk] : v_tiles[blk - 2]);
+    __syncthreads();
+    if (only == 1) {
+#pragma unroll
+      for (int i = 0; i < DBLK; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) po[(i * 16 + e) * 64 + lane] = o_acc[i][e];
+      }
+      merge_ml[blk][lane][0] = m_run;
+      merge_ml[blk][lane][1] = l_tot;
+    }
+    __syncthreads();
+    if (only == 1) return;
+    const float m1 = merge_ml[blk][lane][0], l1 = merge_ml[blk][lane][1];
+    const float top = fmaxf(m_run, m1);
+    // one without a maximum has no sum (or NaN)
+    const float f0 = m_run == NEG_INF ? 1.0f : exp2_hw(m_run - top), f1 = m1 == NEG_INF ? 1.0f : exp2_hw(m1 - top);
+#pragma unroll
+    for (int i = 0; i < DBLK; ++i) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o_acc[i][e] = o_acc[i][e] * f0 + po[(i * 16 + e) * 64 + lane] * f1;
+    }
+    l_tot = l_tot * f0 + l1 * f1;
+    m_run = top;
+  }
+  if (!in) return;
+  if (a.nsplit > 1) {
+    const int64_t at = (bh * a.nsplit + split) * total_rows + rho;
+#pragma unroll
+    for (int i = 0; i < DBLK; ++i) {
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        *reinterpret_cast<f32x4*>(a.part_o + at * D + i * 32 + 2 * e + 4 * half) =
+            f32x4{o_acc[i][e], o_acc[i][e + 1], o_acc[i][e + 2], o_acc[i][e + 3]};
+      }
+    }
+    if (half == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = float2{m_run, l_tot};
+    return;
+  }
+  // rows out of use were computed beside the others: nothing of that is kept
+  if (!used) l_tot = 0.0f;
+  else if (sp.broken) l_tot = __builtin_nanf("");
+  const float inv = 1.0f / l_tot;
+  const int64_t at = (static_cast<int64_t>(b) * a.kv_heads * a.group + h) * a.rows + t;
+#pragma unroll
+  for (int i = 0; i < DBLK; ++i) {
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      u32x2 w = {0, 0};
+      if (l_tot != 0.0f) {
+        w = u32x2{pack_out<F16>(o_acc[i][e] * inv, o_acc[i][e + 1] * inv),
+                  pack_out<F16>(o_acc[i][e + 2] * inv, o_acc[i][e + 3] * inv)};
+      }
+      *reinterpret_cast<u32x2*>(a.out + at * D + i * 32 + 2 * e + 4 * half) = w;
+    }
+  }
+  if (half == 0 && a.lse != nullptr) {
+    a.lse[at] = l_tot == 0.0f ? NEG_INF : (m_run + __builtin_amdgcn_logf(l_tot)) * LN2;
+  }
+}
+
 // ---------------------------------------------------------------------------- merge of key shares
 
-// One workgroup a row: its waves take the shares in turn, each lane D / 64 dims.
-template <int D, bool F16>
-__global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a) {
+// W waves a row take its shares in turn, each lane D / 64 dims; 4 / W rows a workgroup.
+template <int D, bool F16, int W>
+__global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, int64_t all_rows) {
   constexpr int E = D / 64;
   __shared__ float lds[4][D];
   __shared__ float lds_l[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / W) + wave / W;
   const int total_rows = a.rows * a.group;
-  const int64_t bh = blockIdx.x / total_rows;
-  const int rho = blockIdx.x % total_rows;
+  const bool in = row < all_rows;
+  const int64_t bh = in ? row / total_rows : 0;
+  const int rho = static_cast<int>(in ? row % total_rows : 0);
   const int b = static_cast<int>(bh / a.kv_heads), hk = static_cast<int>(bh % a.kv_heads);
   const Span sp = span_of(a, b);
   const int64_t first = bh * a.nsplit * total_rows + rho;
@@ -444,63 +800,98 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   float l = 0.0f, acc[E] = {};
-  for (int s = wave; s < a.nsplit; s += 4) {
+#pragma unroll 4
+  for (int s = wave % W; s < a.nsplit; s += W) {
     const int64_t at = first + static_cast<int64_t>(s) * total_rows;
-    const float ms = a.part_ml[at * 2], ls = a.part_ml[at * 2 + 1];
-    if (ms == NEG_INF && ls == ls) continue;  // saw nothing
+    const float ms = a.part_ml[at * 2];
+    // a share without a maximum saw nothing (or only NaN): its sums count as they are, zeros (or NaN)
     const float f = ms == NEG_INF ? 1.0f : exp2_hw(ms - top);
-    l += f * ls;
+    l += f * a.part_ml[at * 2 + 1];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] += f * a.part_o[at * D + lane * E + e];
   }
+  if constexpr (W > 1) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) lds[wave][lane * E + e] = acc[e];
-  if (lane == 0) lds_l[wave] = l;
-  __syncthreads();
-  if (wave != 0) return;
-  l = lds_l[0] + lds_l[1] + lds_l[2] + lds_l[3];
+    for (int e = 0; e < E; ++e) lds[wave][lane * E + e] = acc[e];
+    if (lane == 0) lds_l[wave] = l;
+    __syncthreads();
+    if (wave % W != 0) return;
+    for (int w = wave + 1; w < wave + W; ++w) {
+      l += lds_l[w];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += lds[w][lane * E + e];
+    }
+  }
+  if (!in) return;
   const int t = rho / a.group, h = hk * a.group + rho % a.group;
   if (t >= sp.count) l = 0.0f;
   else if (sp.broken) l = __builtin_nanf("");
   const int64_t at = (static_cast<int64_t>(b) * a.kv_heads * a.group + h) * a.rows + t;
+  const float inv = 1.0f / l;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int d = lane * E + e;
-    const float o = l == 0.0f ? 0.0f : (lds[0][d] + lds[1][d] + lds[2][d] + lds[3][d]) * (1.0f / l);
-    a.out[at * D + d] = F16 ? spr::f32_to_f16(o) : spr::f32_to_bf16(o);
+    const float o = l == 0.0f ? 0.0f : acc[e] * inv;
+    a.out[at * D + lane * E + e] = F16 ? spr::f32_to_f16(o) : spr::f32_to_bf16(o);
   }
   if (lane == 0 && a.lse != nullptr) a.lse[at] = l == 0.0f ? NEG_INF : (top + __builtin_amdgcn_logf(l)) * LN2;
 }
 
 // ---------------------------------------------------------------------------- host
 
-// Key shares of the few-row kernel: about four workgroups for every CU, none of less than four blocks
-// a wave.
-int32_t few_splits(int64_t groups, int64_t max_length) {
-  const int64_t fill = spr::ceil_div(1024, std::max<int64_t>(groups, 1));
-  const int64_t most = std::max<int64_t>(1, max_length / (4 * FEW_WAVES * FEW_KEYS));
-  return static_cast<int32_t>(std::min({fill, most, int64_t{256}}));
+// How a call is cut up: by the few-row kernel in 16 * nt rows, or by the many-row one in 128 (halves)
+// or 256 rows, and the keys in nsplit shares.
+struct Shape {
+  int32_t nt;  // 0: the many-row kernel
+  bool halves;
+  int32_t nsplit;
+  int64_t groups;  // workgroups to a share
+};
+
+Shape shape_of(int32_t batch, int32_t kv_heads, int32_t group, int32_t rows, int32_t d, int64_t max_length) {
+  const int64_t total = static_cast<int64_t>(rows) * group, heads = static_cast<int64_t>(batch) * kv_heads;
+  Shape s = {};
+  if (total <= 32) {
+    s.nt = total <= 16 ? 1 : 2;
+    s.groups = heads;
+    // about four workgroups for every CU, none of less than four blocks a wave
+    const int64_t fill = spr::ceil_div(1024, s.groups);
+    const int64_t most = std::max<int64_t>(1, max_length / (4 * FEW_WAVES * FEW_KEYS));
+    s.nsplit = static_cast<int32_t>(std::min({fill, most, int64_t{256}}));
+    return s;
+  }
+  s.halves = total <= 128;
+  s.groups = heads * spr::ceil_div(total, s.halves ? 128 : 256);
+  // one workgroup a CU, so a call takes whole rounds of 256: the shares that come out fastest, at about
+  // 1 us a chunk (half that with two waves to a row) and 4 TB/s for the partial results
+  const double chunks = static_cast<double>(spr::ceil_div(std::max<int64_t>(max_length, 1), MANY_KEYS));
+  double best = 0.0;
+  for (int32_t n = 1; n <= 64 && (n == 1 || chunks >= 8.0 * n); ++n) {
+    const double rounds = static_cast<double>(spr::ceil_div(s.groups * n, 256));
+    const double each = (s.halves ? 0.6 : 1.0) * (chunks / n + 3.0);
+    const double merge = n == 1 ? 0.0 : 6.0 + 8e-6 / 4.0 * d * static_cast<double>(heads * total) * n;
+    const double us = rounds * each + merge;
+    if (n == 1 || us < best) best = us, s.nsplit = n;
+  }
+  return s;
 }
 
 template <int D, bool F16>
-void launch_few(const AttnArgs& a, int nt, hipStream_t stream) {
-  const int tiles = static_cast<int>(spr::ceil_div(static_cast<int64_t>(a.rows) * a.group, 16 * nt));
-  const dim3 grid(a.nsplit, a.kv_heads * tiles, a.batch);
-  if (nt == 1) kv4_few_kernel<D, 1, F16><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
-  else kv4_few_kernel<D, 2, F16><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
-}
-
-struct Shape {
-  int32_t nt;      // 16-row tiles a workgroup
-  int32_t nsplit;  // key shares
-};
-
-Shape shape_of(int32_t batch, int32_t kv_heads, int32_t group, int32_t rows, int64_t max_length) {
-  const int64_t total = static_cast<int64_t>(rows) * group;
-  Shape s;
-  s.nt = total <= 16 ? 1 : 2;
-  s.nsplit = few_splits(batch * kv_heads * spr::ceil_div(total, 16 * s.nt), max_length);
-  return s;
+void launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
+  if (s.nt != 0) {
+    const dim3 grid(a.nsplit, a.kv_heads, a.batch);
+    if (s.nt == 1) kv4_few_kernel<D, 1, F16><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
+    else kv4_few_kernel<D, 2, F16><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
+  } else {
+    const unsigned grid = static_cast<unsigned>(spr::ceil_div(s.groups * s.nsplit, 8) * 8);
+    if (s.halves) kv4_many_kernel<D, F16, true><<<grid, 64 * MANY_WAVES, 0, stream>>>(a);
+    else kv4_many_kernel<D, F16, false><<<grid, 64 * MANY_WAVES, 0, stream>>>(a);
+  }
+  if (s.nsplit > 1) {
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.group * a.rows;
+    // four waves a row where there are many shares, one where there are many rows
+    if (s.nsplit >= 8) kv4_merge_kernel<D, F16, 4><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a, rows);
+    else kv4_merge_kernel<D, F16, 1><<<static_cast<unsigned>(spr::ceil_div(rows, 4)), 256, 0, stream>>>(a, rows);
+  }
 }
 
 }  // namespace
@@ -508,7 +899,7 @@ Shape shape_of(int32_t batch, int32_t kv_heads, int32_t group, int32_t rows, int
 extern "C" size_t spr_kv4_attention_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t rows, int32_t d,
                                               int64_t max_length) {
   if (batch <= 0 || kv_heads <= 0 || rows <= 0 || heads % kv_heads != 0) return 0;
-  const Shape s = shape_of(batch, kv_heads, heads / kv_heads, rows, max_length);
+  const Shape s = shape_of(batch, kv_heads, heads / kv_heads, rows, d, max_length);
   if (s.nsplit <= 1) return 0;
   return static_cast<size_t>(batch) * heads * rows * s.nsplit * (d + 2) * sizeof(float);
 }
@@ -537,7 +928,7 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
               "%s: %d rows of %d heads in %d sequences are too many for one call", what, rows, heads, batch);
   if (batch == 0 || rows == 0) return SPR_OK;
   const int32_t group = heads / kv_heads;
-  const Shape s = shape_of(batch, kv_heads, group, rows, std::min<int64_t>(max_length, static_cast<int64_t>(wide) * page_size));
+  const Shape s = shape_of(batch, kv_heads, group, rows, d, std::min<int64_t>(max_length, static_cast<int64_t>(wide) * page_size));
   const size_t part = static_cast<size_t>(batch) * heads * rows * s.nsplit;
   if (s.nsplit > 1 && (workspace == nullptr || workspace_bytes < part * (d + 2) * sizeof(float))) {
     spr_set_error("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, part * (d + 2) * sizeof(float));
@@ -557,25 +948,13 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
   a.log_s = 31 - __builtin_clz(static_cast<unsigned>(page_size));
   a.num_pages = num_pages, a.nsplit = s.nsplit, a.causal = causal;
   a.scale_log2 = scale * LOG2E;
-  const bool f16 = dtype == 1;
   if (d == 128) {
-    if (f16) launch_few<128, true>(a, s.nt, stream);
-    else launch_few<128, false>(a, s.nt, stream);
+    if (dtype == 1) launch<128, true>(a, s, stream);
+    else launch<128, false>(a, s, stream);
   } else {
-    if (f16) launch_few<64, true>(a, s.nt, stream);
-    else launch_few<64, false>(a, s.nt, stream);
+    if (dtype == 1) launch<64, true>(a, s, stream);
+    else launch<64, false>(a, s, stream);
   }
   SPR_LAUNCHED(what);
-  if (s.nsplit > 1) {
-    const unsigned rows_all = static_cast<unsigned>(static_cast<int64_t>(batch) * heads * rows);
-    if (d == 128) {
-      if (f16) kv4_merge_kernel<128, true><<<rows_all, 256, 0, stream>>>(a);
-      else kv4_merge_kernel<128, false><<<rows_all, 256, 0, stream>>>(a);
-    } else {
-      if (f16) kv4_merge_kernel<64, true><<<rows_all, 256, 0, stream>>>(a);
-      else kv4_merge_kernel<64, false><<<rows_all, 256, 0, stream>>>(a);
-    }
-    SPR_LAUNCHED(what);
-  }
   return SPR_OK;
 }
