@@ -187,6 +187,17 @@ def call(name: str, *args) -> int:
     return status
 
 
+def launch(name: str, device: torch.device, *args) -> int:
+    """`call` with the tensors' device as the current one and its current stream as the last argument.
+    What a call of a few microseconds spends on the host counts: the raw stream takes 0.1 us where
+    torch.cuda.current_stream takes 2, and the device is entered only where it is not the current one."""
+    index = device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
 def query(name: str, *args):
     return getattr(load(), name)(*args)
 

@@ -41,7 +41,9 @@ struct AttnArgs {
   float* part_ml;        // the same rows' (maximum, sum)
   int64_t q_b, q_h, q_t;  // strides in elements
   int64_t page_stride;    // bytes
-  int32_t batch, kv_heads, group, rows, sequences, wide, log_s, num_pages, nsplit, causal;
+  int32_t batch, kv_heads, group, rows, sequences, wide, log_s, num_pages, causal;
+  int32_t nsplit, share;          // shares of the keys, blocks of one
+  int32_t tile_rows, block_keys;  // query rows of a workgroup, keys of a block
   float scale_log2;  // softmax scale * log2(e)
 };
 
@@ -70,6 +72,30 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
 __device__ __forceinline__ int32_t visible_of(const AttnArgs& a, const Span& s, int t) {
   if (t >= s.count) return 0;
   return a.causal != 0 ? min(max(s.length - s.count + t + 1, 0), s.length) : s.length;
+}
+
+// Keys that the rows [row0, row0 + tile_rows) see at most.  Rows are token-major: the last one in use
+// sees most, the first one least.
+__device__ __forceinline__ int32_t most_of(const AttnArgs& a, const Span& s, int row0) {
+  const int32_t last = min((min(row0 + a.tile_rows, a.rows * a.group) - 1) / a.group, s.count - 1);
+  return last < row0 / a.group ? 0 : visible_of(a, s, last);
+}
+__device__ __forceinline__ int32_t least_of(const AttnArgs& a, const Span& s, int row0) {
+  return visible_of(a, s, min(row0 / a.group, max(s.count - 1, 0)));
+}
+
+// The keys of a tile are dealt in shares of `share` blocks, for every sequence alike: a short one takes
+// one share, and that writes its rows straight to the output; more than nsplit shares (a length past
+// the caller's bound) make them longer.
+struct Deal {
+  int32_t blocks, per, shares;
+};
+__device__ __forceinline__ Deal deal_of(const AttnArgs& a, int32_t keys) {
+  Deal d;
+  d.blocks = (keys + a.block_keys - 1) / a.block_keys;
+  d.per = max(a.share, (d.blocks + a.nsplit - 1) / a.nsplit);
+  d.shares = max(1, (d.blocks + d.per - 1) / d.per);
+  return d;
 }
 
 // Offset of a token block's page, and whether the table names one in the pool.
@@ -164,7 +190,7 @@ struct Held {
 // at u ^ (r & 7) (D = 128; u ^ ((r >> 1) & 3) for D = 64), its halves swapped in rows 8 .. 15: the
 // transposing read of eight rows meets every bank once, and so does the write of sixteen.
 template <int D, int NT, bool F16>
-__global__ __launch_bounds__(64 * FEW_WAVES) void kv4_few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kernel(AttnArgs a) {
   using Part = spr::Kv4Part<D>;
   constexpr int KS = D / 32;   // MFMA steps over the dims
   constexpr int VT = D / 16;   // 16-dim tiles of the output
@@ -178,19 +204,18 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kv4_few_kernel(AttnArgs a) {
   const int hk = blockIdx.y, b = blockIdx.z, split = blockIdx.x;
   const int total_rows = a.rows * a.group;
   const Span sp = span_of(a, b);
+  const Deal deal = deal_of(a, most_of(a, sp, 0));
+  if (split >= deal.shares) return;
   const int32_t* row_table = a.table + static_cast<int64_t>(sp.seq) * a.wide;
 
   u32x4 qh[NT][KS], ql[NT][F16 ? KS : 1];
   int32_t seen[NT];  // keys this lane's query row sees
-  int32_t least = sp.length, most = 0;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int rho = n * 16 + m;
     const bool in = rho < total_rows;
     const int t = in ? rho / a.group : 0, h = hk * a.group + (in ? rho % a.group : 0);
     seen[n] = in ? visible_of(a, sp, t) : 0;
-    if (in && t < sp.count) least = min(least, seen[n]);
-    most = max(most, seen[n]);
     const uint16_t* qp = a.q + b * a.q_b + h * a.q_h + t * a.q_t + g * (D / 4);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -200,17 +225,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kv4_few_kernel(AttnArgs a) {
       if constexpr (F16) ql[n][s] = lo;
     }
   }
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    least = min(least, __shfl_xor(least, o, 64));
-    most = max(most, __shfl_xor(most, o, 64));
-  }
-  least = __builtin_amdgcn_readfirstlane(least);
-  most = __builtin_amdgcn_readfirstlane(most);
-
-  const int blocks = (most + FEW_KEYS - 1) / FEW_KEYS;
-  const int per = (blocks + a.nsplit - 1) / a.nsplit;
-  const int last = min(blocks, (split + 1) * per);
+  const int32_t least = least_of(a, sp, 0);
+  const int32_t last = min(deal.blocks, (split + 1) * deal.per);
 
   f32x4 acc[NT][VT];
   float mx[NT], sum[NT];
@@ -355,20 +371,24 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kv4_few_kernel(AttnArgs a) {
     }
   };
 
-  int blk = split * per + wave;
+  // blocks that every row sees whole, then the others: two loops, since one that takes either step holds
+  // half as many registers again (181 against 126)
+  const int whole = min(last, least / FEW_KEYS);
+  int blk = split * deal.per + wave;
   if (blk < last) {
     Held<D> now, next;
     fetch(blk, now);
-    while (true) {
-      const int after = blk + FEW_WAVES;
-      if (after < last) fetch(after, next);
-      const int32_t key = blk * FEW_KEYS;
-      if (key + FEW_KEYS <= least) step(now, key, std::false_type{});
-      else step(now, key, std::true_type{});
-      if (after >= last) break;
-      now = next;
-      blk = after;
-    }
+    auto walk = [&](int end, auto masked) {
+      while (blk < end) {
+        const int after = blk + FEW_WAVES;
+        if (after < last) fetch(after, next);
+        step(now, blk * FEW_KEYS, masked);
+        now = next;
+        blk = after;
+      }
+    };
+    walk(whole, std::false_type{});
+    walk(last, std::true_type{});
   }
 
   // merge the waves, one 16-row tile at a time, through the V rows
@@ -407,7 +427,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kv4_few_kernel(AttnArgs a) {
         o += mw == NEG_INF && lw == lw ? f32x4{0, 0, 0, 0} : (mw == NEG_INF ? ow : f * ow);
       }
       const int t = rho / a.group, h = hk * a.group + rho % a.group;
-      if (a.nsplit > 1) {
+      if (deal.shares > 1) {
         const int64_t at = ((static_cast<int64_t>(b) * a.kv_heads + hk) * a.nsplit + split) * total_rows + rho;
         reinterpret_cast<f32x4*>(a.part_o + at * D)[p] = o;
         if (p == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = float2{top, l};
@@ -431,6 +451,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void kv4_few_kernel(AttnArgs a) {
 
 constexpr int MANY_WAVES = 8;
 constexpr int MANY_KEYS = 64;  // keys of a chunk
+constexpr int RUN = 4;
 
 __device__ __forceinline__ float max_xor32(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -472,12 +493,13 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
   __shared__ uint32_t v_bytes[3][MANY_KEYS];  // the V scale bytes of every key
   __shared__ float merge_ml[4][64][2];
 
-  // consecutive tiles of one head and share on one XCD: they read the same codes
+  // runs of RUN consecutive tiles of one head and share on one XCD (workgroup b runs on XCD b mod 8):
+  // they read the same codes, and shares of unlike length still spread over all XCDs
   const int total_rows = a.rows * a.group;
   const int tiles = (total_rows + TROWS - 1) / TROWS;
   const int64_t total = static_cast<int64_t>(tiles) * a.nsplit * a.kv_heads * a.batch;
-  const int64_t id = (blockIdx.x & 7) * ((total + 7) / 8) + (blockIdx.x >> 3);
-  if (id >= total || (blockIdx.x >> 3) >= (total + 7) / 8) return;
+  const int64_t id = static_cast<int64_t>(blockIdx.x / (8 * RUN)) * (8 * RUN) + (blockIdx.x & 7) * RUN + (blockIdx.x >> 3) % RUN;
+  if (id >= total) return;
   const int tile = static_cast<int>(id % tiles);
   const int split = static_cast<int>(id / tiles % a.nsplit);
   const int64_t bh = id / tiles / a.nsplit;
@@ -488,25 +510,21 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
   const int blk = HALVES ? (wave & 3) : wave;
   const int only = HALVES ? (wave >> 2) : 0;  // HALVES: which half of a chunk
   const Span sp = span_of(a, b);
+  const int row0 = tile * TROWS;
+  const int32_t most = most_of(a, sp, row0), least = least_of(a, sp, row0);
+  const Deal deal = deal_of(a, most);
+  if (split >= deal.shares) return;
   const int32_t* row_table = a.table + static_cast<int64_t>(sp.seq) * a.wide;
 
-  const int rho = tile * TROWS + blk * 32 + col;
+  const int rho = row0 + blk * 32 + col;
   const bool in = rho < total_rows;
   const int t = in ? rho / a.group : 0, h = hk * a.group + (in ? rho % a.group : 0);
   const bool used = in && t < sp.count;
   const int32_t seen = used ? visible_of(a, sp, t) : 0;
-  // rows are token-major, so the last row of a list sees most and the first one in use least
-  const int row0 = tile * TROWS, row1 = min(row0 + TROWS, total_rows) - 1;
-  const int32_t t_last = min(row1 / a.group, sp.count - 1);
-  const int32_t most = t_last < row0 / a.group ? 0 : visible_of(a, sp, t_last);
-  const int32_t least = visible_of(a, sp, min(row0 / a.group, max(sp.count - 1, 0)));
   const int w0 = row0 + blk * 32;
   const bool wave_live = w0 < total_rows && w0 / a.group < sp.count;
-  const int32_t wave_least = visible_of(a, sp, min(w0 / a.group, max(sp.count - 1, 0)));
-
-  const int chunks = (most + MANY_KEYS - 1) / MANY_KEYS;
-  const int per = (chunks + a.nsplit - 1) / a.nsplit;
-  const int c0 = split * per, nch = min(chunks, c0 + per) - c0;
+  const int32_t wave_least = least_of(a, sp, w0);
+  const int c0 = split * deal.per, nch = min(deal.blocks, c0 + deal.per) - c0;
 
   u32x4 qh[KSTEPS], ql[F16 ? KSTEPS : 1];
   const uint16_t* qp = a.q + b * a.q_b + h * a.q_h + t * a.q_t + half * 8;
@@ -743,7 +761,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
     m_run = top;
   }
   if (!in) return;
-  if (a.nsplit > 1) {
+  if (deal.shares > 1) {
     const int64_t at = (bh * a.nsplit + split) * total_rows + rho;
 #pragma unroll
     for (int i = 0; i < DBLK; ++i) {
@@ -794,14 +812,17 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, int64_t all_
   const int rho = static_cast<int>(in ? row % total_rows : 0);
   const int b = static_cast<int>(bh / a.kv_heads), hk = static_cast<int>(bh % a.kv_heads);
   const Span sp = span_of(a, b);
+  const int32_t shares = in ? deal_of(a, most_of(a, sp, rho / a.tile_rows * a.tile_rows)).shares : 1;
+  static_assert(W == 1 || W == 4, "waves of a workgroup leave together or wait for nobody");
+  if (shares == 1) return;  // written already, or no row
   const int64_t first = bh * a.nsplit * total_rows + rho;
   float top = NEG_INF;
-  for (int s = lane; s < a.nsplit; s += 64) top = fmaxf(top, a.part_ml[(first + static_cast<int64_t>(s) * total_rows) * 2]);
+  for (int s = lane; s < shares; s += 64) top = fmaxf(top, a.part_ml[(first + static_cast<int64_t>(s) * total_rows) * 2]);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   float l = 0.0f, acc[E] = {};
 #pragma unroll 4
-  for (int s = wave % W; s < a.nsplit; s += W) {
+  for (int s = wave % W; s < shares; s += W) {
     const int64_t at = first + static_cast<int64_t>(s) * total_rows;
     const float ms = a.part_ml[at * 2];
     // a share without a maximum saw nothing (or only NaN): its sums count as they are, zeros (or NaN)
@@ -822,7 +843,6 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, int64_t all_
       for (int e = 0; e < E; ++e) acc[e] += lds[w][lane * E + e];
     }
   }
-  if (!in) return;
   const int t = rho / a.group, h = hk * a.group + rho % a.group;
   if (t >= sp.count) l = 0.0f;
   else if (sp.broken) l = __builtin_nanf("");
@@ -853,21 +873,27 @@ Shape shape_of(int32_t batch, int32_t kv_heads, int32_t group, int32_t rows, int
   if (total <= 32) {
     s.nt = total <= 16 ? 1 : 2;
     s.groups = heads;
-    // about four workgroups for every CU, none of less than four blocks a wave
-    const int64_t fill = spr::ceil_div(1024, s.groups);
+    // Three workgroups for every CU, in one round, where there is one sequence; shares of its keys that
+    // are not alike even out over more of them where there are several (their lengths are not known
+    // here).  None of less than four blocks a wave.
+    const int64_t fill = std::max<int64_t>(1, (batch == 1 ? 768 : 2048) / s.groups);
     const int64_t most = std::max<int64_t>(1, max_length / (4 * FEW_WAVES * FEW_KEYS));
     s.nsplit = static_cast<int32_t>(std::min({fill, most, int64_t{256}}));
     return s;
   }
   s.halves = total <= 128;
   s.groups = heads * spr::ceil_div(total, s.halves ? 128 : 256);
+  const int64_t chunks = std::max<int64_t>(1, spr::ceil_div(max_length, MANY_KEYS));
+  if (batch > 1) {
+    s.nsplit = static_cast<int32_t>(std::min({std::max<int64_t>(1, 1024 / s.groups), std::max<int64_t>(1, chunks / 8), int64_t{64}}));
+    return s;
+  }
   // one workgroup a CU, so a call takes whole rounds of 256: the shares that come out fastest, at about
   // 1 us a chunk (half that with two waves to a row) and 4 TB/s for the partial results
-  const double chunks = static_cast<double>(spr::ceil_div(std::max<int64_t>(max_length, 1), MANY_KEYS));
   double best = 0.0;
-  for (int32_t n = 1; n <= 64 && (n == 1 || chunks >= 8.0 * n); ++n) {
+  for (int32_t n = 1; n <= 64 && (n == 1 || chunks >= 8 * n); ++n) {
     const double rounds = static_cast<double>(spr::ceil_div(s.groups * n, 256));
-    const double each = (s.halves ? 0.6 : 1.0) * (chunks / n + 3.0);
+    const double each = (s.halves ? 0.6 : 1.0) * (static_cast<double>(chunks) / n + 3.0);
     const double merge = n == 1 ? 0.0 : 6.0 + 8e-6 / 4.0 * d * static_cast<double>(heads * total) * n;
     const double us = rounds * each + merge;
     if (n == 1 || us < best) best = us, s.nsplit = n;
@@ -882,7 +908,7 @@ void launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
     if (s.nt == 1) kv4_few_kernel<D, 1, F16><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
     else kv4_few_kernel<D, 2, F16><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
   } else {
-    const unsigned grid = static_cast<unsigned>(spr::ceil_div(s.groups * s.nsplit, 8) * 8);
+    const unsigned grid = static_cast<unsigned>(spr::ceil_div(s.groups * s.nsplit, 8 * RUN) * (8 * RUN));
     if (s.halves) kv4_many_kernel<D, F16, true><<<grid, 64 * MANY_WAVES, 0, stream>>>(a);
     else kv4_many_kernel<D, F16, false><<<grid, 64 * MANY_WAVES, 0, stream>>>(a);
   }
@@ -928,7 +954,8 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
               "%s: %d rows of %d heads in %d sequences are too many for one call", what, rows, heads, batch);
   if (batch == 0 || rows == 0) return SPR_OK;
   const int32_t group = heads / kv_heads;
-  const Shape s = shape_of(batch, kv_heads, group, rows, d, std::min<int64_t>(max_length, static_cast<int64_t>(wide) * page_size));
+  const int64_t longest = std::min<int64_t>(max_length, static_cast<int64_t>(wide) * page_size);
+  const Shape s = shape_of(batch, kv_heads, group, rows, d, longest);
   const size_t part = static_cast<size_t>(batch) * heads * rows * s.nsplit;
   if (s.nsplit > 1 && (workspace == nullptr || workspace_bytes < part * (d + 2) * sizeof(float))) {
     spr_set_error("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, part * (d + 2) * sizeof(float));
@@ -946,7 +973,11 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
   a.page_stride = kv_heads * spr::kv4_head_bytes(page_size, d);
   a.batch = batch, a.kv_heads = kv_heads, a.group = group, a.rows = rows, a.sequences = sequences, a.wide = wide;
   a.log_s = 31 - __builtin_clz(static_cast<unsigned>(page_size));
-  a.num_pages = num_pages, a.nsplit = s.nsplit, a.causal = causal;
+  a.num_pages = num_pages, a.causal = causal;
+  a.nsplit = s.nsplit;
+  a.block_keys = s.nt != 0 ? FEW_KEYS : MANY_KEYS;
+  a.tile_rows = s.nt != 0 ? 16 * s.nt : s.halves ? 128 : 256;
+  a.share = static_cast<int32_t>(spr::ceil_div(std::max<int64_t>(longest, 1), static_cast<int64_t>(a.block_keys) * s.nsplit));
   a.scale_log2 = scale * LOG2E;
   if (d == 128) {
     if (dtype == 1) launch<128, true>(a, s, stream);

@@ -47,53 +47,55 @@ def kv4_page_bytes(page_size: int, head_dim: int) -> int:
 
 
 def _page_size(pages: torch.Tensor, head_dim: int, what: str) -> int:
+    """Tokens of a page, from the pages of one layer and the head dim."""
+    shape = pages.shape
+    if pages.dtype is not torch.uint8 or len(shape) != 3 or not pages.is_contiguous() or pages.numel() == 0:
+        raise RuntimeError(f"{what}: pages must be a contiguous uint8 tensor [P, Hkv, bytes], got {pages.dtype} "
+                           f"{tuple(shape)}")
     if head_dim not in HEAD_DIMS:
         raise RuntimeError(f"{what}: head dim {head_dim} not supported {HEAD_DIMS}")
-    size = pages.shape[-1] // (head_dim + head_dim // 16)
-    if size not in PAGE_SIZES or pages.shape[-1] != kv4_page_bytes(size, head_dim):
-        raise RuntimeError(f"{what}: pages of {pages.shape[-1]} bytes a head are not whole pages of head dim {head_dim}")
+    size = shape[2] // (head_dim + head_dim // 16)
+    if size not in PAGE_SIZES or shape[2] != size * (head_dim + head_dim // 16):
+        raise RuntimeError(f"{what}: pages of {shape[2]} bytes a head are not whole pages of head dim {head_dim}")
     return size
 
 
-def _int32(t: torch.Tensor, shape: tuple, name: str, what: str) -> torch.Tensor:
-    """An int32 tensor of this shape, as the kernels read it."""
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
-        raise RuntimeError(f"{what}: {name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} "
+def _int32(t: torch.Tensor, n: int, name: str, what: str) -> None:
+    """An int32 vector of n, as the kernels read it."""
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise RuntimeError(f"{what}: {name} must be a contiguous int32 tensor of shape {(n,)}, got {t.dtype} "
                            f"{tuple(t.shape)}")
-    return t
-
-
-def _check_pool(pages: torch.Tensor, what: str) -> None:
-    if pages.dtype != torch.uint8 or pages.ndim != 3 or not pages.is_contiguous() or pages.numel() == 0:
-        raise RuntimeError(f"{what}: pages must be a contiguous uint8 tensor [P, Hkv, bytes], got {pages.dtype} "
-                           f"{tuple(pages.shape)}")
 
 
 def _check_table(block_table: torch.Tensor, what: str) -> tuple[int, int]:
-    if block_table.dtype != torch.int32 or block_table.ndim != 2 or not block_table.is_contiguous():
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or not block_table.is_contiguous():
         raise RuntimeError(f"{what}: block_table must be a contiguous int32 tensor [sequences, wide], got "
                            f"{block_table.dtype} {tuple(block_table.shape)}")
-    return block_table.shape[0], block_table.shape[1]
+    return block_table.shape
 
 
-def _batch_ids(seq_ids, batch: int, sequences: int, what: str):
-    if seq_ids is None:
-        if batch > sequences:
-            raise RuntimeError(f"{what}: a batch of {batch} without seq_ids on a table of {sequences} sequences")
-        return None
-    return _int32(seq_ids, (batch,), "seq_ids", what)
+def _check_entries(batch: int, sequences: int, seq_ids, counts, what: str) -> None:
+    if seq_ids is not None:
+        _int32(seq_ids, batch, "seq_ids", what)
+    elif batch > sequences:
+        raise RuntimeError(f"{what}: a batch of {batch} without seq_ids on a table of {sequences} sequences")
+    if counts is not None:
+        _int32(counts, batch, "counts", what)
 
 
-def _rows_in_place(x: torch.Tensor) -> torch.Tensor:
-    """x [B, H, T, D] by its strides where rows are packed and 16-byte aligned, else a copy."""
-    step = 16 // x.element_size()
-    ok = (x.stride(3) == 1 and x.data_ptr() % 16 == 0
-          and all(x.shape[i] <= 1 or (x.stride(i) % step == 0 and x.stride(i) >= 0) for i in range(3)))
-    return x if ok else x.contiguous()
-
-
-def _strides(x: torch.Tensor) -> list[int]:
-    return [x.stride(i) if x.shape[i] > 1 else 0 for i in range(3)]
+def _by_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """x [B, H, T, D] and the strides of its first three dims: itself where rows are packed and 16-byte
+    aligned, else a copy."""
+    (b, h, t, d), (sb, sh, st, sd) = x.shape, x.stride()
+    if b == 1:
+        sb = 0
+    if h == 1:
+        sh = 0
+    if t == 1:
+        st = 0
+    if sd == 1 and x.data_ptr() % 16 == 0 and (sb | sh | st) * x.element_size() % 16 == 0:
+        return x, sb, sh, st
+    return x.contiguous(), h * t * d, t * d, d
 
 
 def kv4_store(pages: torch.Tensor, block_table: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
@@ -106,8 +108,7 @@ def kv4_store(pages: torch.Tensor, block_table: torch.Tensor, k: torch.Tensor, v
     A group of 32 dims with an infinity or a NaN is stored as NaN."""
     what = "4-bit cache store"
     dev = _lib.require_gpu(pages, block_table, k, v, starts, counts, seq_ids, what=what)
-    _check_pool(pages, what)
-    if k.ndim != 4 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _lib.DTYPE_CODE:
+    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _lib.DTYPE_CODE:
         raise RuntimeError(f"{what}: K and V must be [B, Hkv, T, D] of one dtype (bfloat16, float16, float32), got "
                            f"{k.dtype} {tuple(k.shape)} / {v.dtype} {tuple(v.shape)}")
     b, h, t, d = k.shape
@@ -115,17 +116,15 @@ def kv4_store(pages: torch.Tensor, block_table: torch.Tensor, k: torch.Tensor, v
     if pages.shape[1] != h:
         raise RuntimeError(f"{what}: K has {h} heads, the pages {pages.shape[1]}")
     sequences, wide = _check_table(block_table, what)
-    ids = _batch_ids(seq_ids, b, sequences, what)
-    _int32(starts, (b,), "starts", what)
-    if counts is not None:
-        _int32(counts, (b,), "counts", what)
+    _check_entries(b, sequences, seq_ids, counts, what)
+    _int32(starts, b, "starts", what)
     if k.numel() == 0:
         return
-    kc, vc = _rows_in_place(k), _rows_in_place(v)
-    with torch.cuda.device(dev):
-        _lib.call("spr_kv4_store", _lib.ptr(pages), pages.shape[0], h, size, d, _lib.ptr(block_table), sequences, wide,
-                  _lib.ptr(ids), _lib.ptr(starts), _lib.ptr(counts), _lib.ptr(kc), _lib.ptr(vc),
-                  _lib.DTYPE_CODE[k.dtype], b, t, *_strides(kc), *_strides(vc), _lib.stream(dev))
+    k, *k_strides = _by_rows(k)
+    v, *v_strides = _by_rows(v)
+    _lib.launch("spr_kv4_store", dev, pages.data_ptr(), pages.shape[0], h, size, d, block_table.data_ptr(), sequences,
+                wide, _lib.ptr(seq_ids), starts.data_ptr(), _lib.ptr(counts), k.data_ptr(), v.data_ptr(),
+                _lib.DTYPE_CODE[k.dtype], b, t, *k_strides, *v_strides)
 
 
 def kv4_load(pages: torch.Tensor, block_table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, rows: int,
@@ -134,25 +133,21 @@ def kv4_load(pages: torch.Tensor, block_table: torch.Tensor, starts: torch.Tenso
     in `dtype` (exact in bf16 and fp32); rows past the count are 0, rows with no page NaN."""
     what = "4-bit cache load"
     dev = _lib.require_gpu(pages, block_table, starts, counts, seq_ids, what=what)
-    _check_pool(pages, what)
     size = _page_size(pages, head_dim, what)
     if dtype not in _lib.DTYPE_CODE:
         raise RuntimeError(f"{what}: dtype must be bfloat16, float16 or float32, got {dtype}")
-    if rows < 0 or starts.ndim != 1:
+    if rows < 0 or starts.dim() != 1:
         raise RuntimeError(f"{what}: rows {rows}, starts {tuple(starts.shape)}")
     b, h = starts.shape[0], pages.shape[1]
     sequences, wide = _check_table(block_table, what)
-    ids = _batch_ids(seq_ids, b, sequences, what)
-    _int32(starts, (b,), "starts", what)
-    _int32(counts, (b,), "counts", what)
+    _check_entries(b, sequences, seq_ids, counts, what)
+    _int32(starts, b, "starts", what)
     k = torch.empty((b, h, rows, head_dim), dtype=dtype, device=dev)
     v = torch.empty_like(k)
-    if k.numel() == 0:
-        return k, v
-    with torch.cuda.device(dev):
-        _lib.call("spr_kv4_load", _lib.ptr(pages), pages.shape[0], h, size, head_dim, _lib.ptr(block_table), sequences,
-                  wide, _lib.ptr(ids), _lib.ptr(starts), _lib.ptr(counts), _lib.ptr(k), _lib.ptr(v),
-                  _lib.DTYPE_CODE[dtype], b, rows, _lib.stream(dev))
+    if k.numel() > 0:
+        _lib.launch("spr_kv4_load", dev, pages.data_ptr(), pages.shape[0], h, size, head_dim, block_table.data_ptr(),
+                    sequences, wide, _lib.ptr(seq_ids), starts.data_ptr(), counts.data_ptr(), k.data_ptr(),
+                    v.data_ptr(), _lib.DTYPE_CODE[dtype], b, rows)
     return k, v
 
 
@@ -169,8 +164,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     longest length the caller knows of (default: what the table can hold), only sizes the launch."""
     what = "4-bit cache attention"
     dev = _lib.require_gpu(q, pages, block_table, lengths, counts, seq_ids, what=what)
-    _check_pool(pages, what)
-    if q.ndim != 4 or q.dtype not in (torch.bfloat16, torch.float16):
+    if q.dim() != 4 or q.dtype not in (torch.bfloat16, torch.float16):
         raise RuntimeError(f"{what}: q must be [B, Hq, T, D] in bfloat16 or float16, got {q.dtype} {tuple(q.shape)}")
     b, h, t, d = q.shape
     size = _page_size(pages, d, what)
@@ -178,61 +172,56 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     if h == 0 or h % hk != 0:
         raise RuntimeError(f"{what}: Q heads ({h}) must be a multiple of KV heads ({hk})")
     sequences, wide = _check_table(block_table, what)
-    ids = _batch_ids(seq_ids, b, sequences, what)
-    _int32(lengths, (sequences,), "lengths", what)
-    if counts is not None:
-        _int32(counts, (b,), "counts", what)
+    _check_entries(b, sequences, seq_ids, counts, what)
+    _int32(lengths, sequences, "lengths", what)
     longest = wide * size if max_length is None else min(int(max_length), wide * size)
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(d)
     out = torch.empty((b, h, t, d), dtype=q.dtype, device=dev)
     lse = torch.empty((b, h, t), dtype=torch.float32, device=dev) if return_lse else None
     if out.numel() > 0:
-        qc = _rows_in_place(q)
-        need = int(_lib.query("spr_kv4_attention_workspace", b, h, hk, t, d, longest))
+        q, *strides = _by_rows(q)
+        need = _lib.query("spr_kv4_attention_workspace", b, h, hk, t, d, longest)
         ws = _lib.workspace(need, dev) if need > 0 else None
-        with torch.cuda.device(dev):
-            _lib.call("spr_kv4_attention", _lib.ptr(qc), *_strides(qc), _lib.DTYPE_CODE[q.dtype], b, h, hk, t, d,
-                      _lib.ptr(pages), pages.shape[0], size, _lib.ptr(block_table), sequences, wide, _lib.ptr(lengths),
-                      _lib.ptr(counts), _lib.ptr(ids), int(causal), sc, longest, _lib.ptr(out), _lib.ptr(lse),
-                      _lib.ptr(ws), need, _lib.stream(dev))
+        _lib.launch("spr_kv4_attention", dev, q.data_ptr(), *strides, _lib.DTYPE_CODE[q.dtype], b, h, hk, t, d,
+                    pages.data_ptr(), pages.shape[0], size, block_table.data_ptr(), sequences, wide, lengths.data_ptr(),
+                    _lib.ptr(counts), _lib.ptr(seq_ids), int(causal), sc, longest, out.data_ptr(), _lib.ptr(lse),
+                    _lib.ptr(ws), need)
     return (out, lse) if return_lse else out
 
 
-def _check_metadata(block_table, lengths, ref_count, page_size, what):
+def _check_metadata(block_table, lengths, ref_count, page_size, status, what):
     sequences, wide = _check_table(block_table, what)
     if lengths is not None:
-        _int32(lengths, (sequences,), "lengths", what)
-    if ref_count.ndim != 1 or ref_count.shape[0] == 0:
+        _int32(lengths, sequences, "lengths", what)
+    if ref_count.dim() != 1 or ref_count.shape[0] == 0:
         raise RuntimeError(f"{what}: ref_count must be [P], got {tuple(ref_count.shape)}")
-    _int32(ref_count, (ref_count.shape[0],), "ref_count", what)
+    _int32(ref_count, ref_count.shape[0], "ref_count", what)
     if page_size not in PAGE_SIZES:
         raise RuntimeError(f"{what}: page size {page_size} not supported {PAGE_SIZES}")
+    if status is not None:
+        _int32(status, 1, "status", what)
     return sequences, wide
 
 
 def _named(ids: torch.Tensor, name: str, what: str) -> int:
-    if ids.ndim != 1 or ids.shape[0] > MAX_NAMED:
+    if ids.dim() != 1 or ids.shape[0] > MAX_NAMED:
         raise RuntimeError(f"{what}: {name} must be a vector of at most {MAX_NAMED}, got {tuple(ids.shape)}")
-    _int32(ids, (ids.shape[0],), name, what)
+    _int32(ids, ids.shape[0], name, what)
     return ids.shape[0]
-
-
-def _check_status(status, what):
-    return None if status is None else _int32(status, (1,), "status", what)
 
 
 def _layers(pages: torch.Tensor, num_pages: int, what: str) -> tuple[int, int, int]:
     """(bytes of a page, bytes from layer to layer, layers) of [P, H, bytes] or [layers, P, H, bytes]."""
-    p = pages if pages.ndim == 4 else pages.unsqueeze(0)
-    if pages.dtype != torch.uint8 or p.ndim != 4 or p.numel() == 0 or not p.is_contiguous():
+    shape = pages.shape if pages.dim() == 4 else (1, *pages.shape)
+    if pages.dtype is not torch.uint8 or len(shape) != 4 or pages.numel() == 0 or not pages.is_contiguous():
         raise RuntimeError(f"{what}: pages must be a contiguous uint8 tensor [P, Hkv, bytes] or [layers, P, Hkv, "
                            f"bytes], got {pages.dtype} {tuple(pages.shape)}")
-    if p.shape[1] != num_pages:
-        raise RuntimeError(f"{what}: {p.shape[1]} pages, ref_count of {num_pages}")
-    if (p.shape[2] * p.shape[3]) % 16 != 0:
-        raise RuntimeError(f"{what}: pages of {p.shape[2]} x {p.shape[3]} bytes are not whole 16-byte pieces")
-    page = p.shape[2] * p.shape[3]
-    return page, page * num_pages, p.shape[0]
+    if shape[1] != num_pages:
+        raise RuntimeError(f"{what}: {shape[1]} pages, ref_count of {num_pages}")
+    page = shape[2] * shape[3]
+    if page % 16 != 0:
+        raise RuntimeError(f"{what}: pages of {shape[2]} x {shape[3]} bytes are not whole 16-byte pieces")
+    return page, page * num_pages, shape[0]
 
 
 def kv4_reserve(block_table: torch.Tensor, lengths: torch.Tensor, ref_count: torch.Tensor, page_size: int,
@@ -243,16 +232,14 @@ def kv4_reserve(block_table: torch.Tensor, lengths: torch.Tensor, ref_count: tor
     first new token of each, or -1 for all when the call could not happen."""
     what = "4-bit cache reserve"
     dev = _lib.require_gpu(block_table, lengths, ref_count, counts, seq_ids, status, what=what)
-    sequences, wide = _check_metadata(block_table, lengths, ref_count, page_size, what)
+    sequences, wide = _check_metadata(block_table, lengths, ref_count, page_size, status, what)
     n = _named(counts, "counts", what)
-    ids = _batch_ids(seq_ids, n, sequences, what)
-    _check_status(status, what)
+    _check_entries(n, sequences, seq_ids, None, what)
     starts = torch.empty(n, dtype=torch.int32, device=dev)
     ws = _lib.workspace(_lib.query("spr_kv4_pages_workspace", ref_count.shape[0]), dev)
-    with torch.cuda.device(dev):
-        _lib.call("spr_kv4_reserve", _lib.ptr(block_table), _lib.ptr(lengths), _lib.ptr(ref_count), _lib.ptr(counts),
-                  _lib.ptr(ids), n, sequences, wide, page_size, ref_count.shape[0], _lib.ptr(starts), _lib.ptr(status),
-                  _lib.ptr(ws), ws.numel(), _lib.stream(dev))
+    _lib.launch("spr_kv4_reserve", dev, block_table.data_ptr(), lengths.data_ptr(), ref_count.data_ptr(),
+                counts.data_ptr(), _lib.ptr(seq_ids), n, sequences, wide, page_size, ref_count.shape[0],
+                starts.data_ptr(), _lib.ptr(status), ws.data_ptr(), ws.numel())
     return starts
 
 
@@ -264,17 +251,15 @@ def kv4_free(block_table: torch.Tensor, lengths: torch.Tensor, ref_count: torch.
     close up and the length loses the tokens that lay there.  A page is free when nobody holds it."""
     what = "4-bit cache free"
     dev = _lib.require_gpu(block_table, lengths, ref_count, seq_ids, first_pages, page_counts, status, what=what)
-    sequences, wide = _check_metadata(block_table, lengths, ref_count, page_size, what)
+    sequences, wide = _check_metadata(block_table, lengths, ref_count, page_size, status, what)
     n = _named(seq_ids, "seq_ids", what)
     for t, name in ((first_pages, "first_pages"), (page_counts, "page_counts")):
         if t is not None:
-            _int32(t, (n,), name, what)
-    _check_status(status, what)
+            _int32(t, n, name, what)
     ws = _lib.workspace(_lib.query("spr_kv4_pages_workspace", ref_count.shape[0]), dev)
-    with torch.cuda.device(dev):
-        _lib.call("spr_kv4_free", _lib.ptr(block_table), _lib.ptr(lengths), _lib.ptr(ref_count), _lib.ptr(seq_ids),
-                  _lib.ptr(first_pages), _lib.ptr(page_counts), n, sequences, wide, page_size, ref_count.shape[0],
-                  _lib.ptr(status), _lib.ptr(ws), ws.numel(), _lib.stream(dev))
+    _lib.launch("spr_kv4_free", dev, block_table.data_ptr(), lengths.data_ptr(), ref_count.data_ptr(),
+                seq_ids.data_ptr(), _lib.ptr(first_pages), _lib.ptr(page_counts), n, sequences, wide, page_size,
+                ref_count.shape[0], _lib.ptr(status), ws.data_ptr(), ws.numel())
 
 
 def kv4_fork(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, ref_count: torch.Tensor,
@@ -285,16 +270,14 @@ def kv4_fork(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tens
     A source may be named more than once, and in every layer of `pages` the same pages are copied."""
     what = "4-bit cache fork"
     dev = _lib.require_gpu(pages, block_table, lengths, ref_count, src, dst, status, what=what)
-    sequences, wide = _check_metadata(block_table, lengths, ref_count, page_size, what)
+    sequences, wide = _check_metadata(block_table, lengths, ref_count, page_size, status, what)
     n = _named(src, "src", what)
-    _int32(dst, (n,), "dst", what)
-    _check_status(status, what)
+    _int32(dst, n, "dst", what)
     page, layer, layers = _layers(pages, ref_count.shape[0], what)
     ws = _lib.workspace(_lib.query("spr_kv4_pages_workspace", ref_count.shape[0]), dev)
-    with torch.cuda.device(dev):
-        _lib.call("spr_kv4_fork", _lib.ptr(pages), page, layer, layers, _lib.ptr(block_table), _lib.ptr(lengths),
-                  _lib.ptr(ref_count), _lib.ptr(src), _lib.ptr(dst), n, sequences, wide, page_size, ref_count.shape[0],
-                  int(share), _lib.ptr(status), _lib.ptr(ws), ws.numel(), _lib.stream(dev))
+    _lib.launch("spr_kv4_fork", dev, pages.data_ptr(), page, layer, layers, block_table.data_ptr(), lengths.data_ptr(),
+                ref_count.data_ptr(), src.data_ptr(), dst.data_ptr(), n, sequences, wide, page_size,
+                ref_count.shape[0], int(share), _lib.ptr(status), ws.data_ptr(), ws.numel())
 
 
 def kv4_compact(pages: torch.Tensor, block_table: torch.Tensor, ref_count: torch.Tensor) -> torch.Tensor:
@@ -303,11 +286,10 @@ def kv4_compact(pages: torch.Tensor, block_table: torch.Tensor, ref_count: torch
     there on are free, and a pool cut to that many holds all sequences."""
     what = "4-bit cache compact"
     dev = _lib.require_gpu(pages, block_table, ref_count, what=what)
-    sequences, wide = _check_metadata(block_table, None, ref_count, PAGE_SIZES[0], what)
+    sequences, wide = _check_metadata(block_table, None, ref_count, PAGE_SIZES[0], None, what)
     page, layer, layers = _layers(pages, ref_count.shape[0], what)
     live = torch.empty((), dtype=torch.int32, device=dev)
     ws = _lib.workspace(_lib.query("spr_kv4_pages_workspace", ref_count.shape[0]), dev)
-    with torch.cuda.device(dev):
-        _lib.call("spr_kv4_compact", _lib.ptr(pages), page, layer, layers, _lib.ptr(block_table), _lib.ptr(ref_count),
-                  sequences, wide, ref_count.shape[0], _lib.ptr(live), _lib.ptr(ws), ws.numel(), _lib.stream(dev))
+    _lib.launch("spr_kv4_compact", dev, pages.data_ptr(), page, layer, layers, block_table.data_ptr(),
+                ref_count.data_ptr(), sequences, wide, ref_count.shape[0], live.data_ptr(), ws.data_ptr(), ws.numel())
     return live
