@@ -450,7 +450,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
 // ---------------------------------------------------------------------------- many rows
 
 constexpr int MANY_WAVES = 8;
-constexpr int MANY_KEYS = 64;  // keys of a chunk
+constexpr int MANY_KEYS = 128;  // keys of a chunk
 constexpr int RUN = 4;
 
 __device__ __forceinline__ float max_xor32(float x) {
@@ -462,13 +462,14 @@ __device__ __forceinline__ float sum_xor32(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// 256 query rows (HALVES false: a wave has 32 rows and all keys) or 128 (true: waves w and w + 4 have
-// the same 32 rows, w the first 32 keys of every chunk and w + 4 the second, merged at the end) of one
-// kv head against a share of its keys.  One workgroup per CU, two waves per SIMD.
+// 32 * RB query rows (RB 8, 4 or 2) of one kv head against a share of its keys.  One workgroup per CU,
+// two waves per SIMD.  Wave w has row block w % RB and part w / RB of every chunk of 128 keys, all of
+// it, 64 or 32 keys; the parts of a row block are merged at the end.
 //
-// A chunk of 64 keys is brought from its codes to bf16 once for all eight waves: a thread turns 32
-// values of one row (16 bytes of codes, one scale) into 64 bytes of a row-major LDS tile, 16 conversions
-// and 4 writes.  The codes of chunk x + 3 are loaded and those of x + 2 written at the end of chunk x.
+// A chunk is brought from its codes to bf16 once for all eight waves: a thread turns 32 values of one
+// row (16 bytes of codes, one scale) into 64 bytes of a row-major LDS tile, 16 conversions and 4 writes.
+// Two tiles each for K and V: the codes of chunk x + 2 are loaded and those of x + 1 written during
+// chunk x, with one barrier a chunk.
 // Scores and output are S^T = K Q^T and O^T += V^T P^T by 32x32x16 MFMA with a lane owning one query
 // row; V^T comes from the transposing read, P from the accumulator in the same order of keys.  S of the
 // next 32 keys is computed beside the exponentials of the current ones.
@@ -477,21 +478,21 @@ __device__ __forceinline__ float sum_xor32(float x) {
 // (D = 128; within the eight pieces of a row for D = 64, p ^ (r >> 1 & 7) and p ^ (4 (r >> 1 & 1) +
 // (r >> 2 & 3))): the conversion's writes of 16 rows, K's reads of 16 rows and V's transposing reads of
 // four rows by 64 bytes each meet every bank once.
-// K: two tiles (the chunk's second half is read before its barrier, the tile written behind it); V:
-// three (the second half is read behind the barrier).
-template <int D, bool F16, bool HALVES>
+template <int D, bool F16, int RB>
 __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a) {
   using Part = spr::Kv4Part<D>;
   constexpr int ROW = 2 * D;
   constexpr int TILE = MANY_KEYS * ROW;
   constexpr int KSTEPS = D / 16, DBLK = D / 32;
-  constexpr int TROWS = HALVES ? 128 : 256;
-  constexpr int GROUPS = D / spr::KV4_GROUP;        // scales of a row
-  constexpr int CONV = MANY_KEYS * GROUPS;          // threads that convert K (and as many V)
-  __shared__ __align__(1024) uint8_t k_tiles[2][TILE];
-  __shared__ __align__(1024) uint8_t v_tiles[3][TILE];
-  __shared__ uint32_t v_bytes[3][MANY_KEYS];  // the V scale bytes of every key
-  __shared__ float merge_ml[4][64][2];
+  constexpr int TROWS = 32 * RB;
+  constexpr int PARTS = MANY_WAVES / RB;
+  constexpr int HALVES = MANY_KEYS / 32 / PARTS;  // pieces of 32 keys a wave has of a chunk
+  constexpr int GROUPS = D / spr::KV4_GROUP;      // scales of a row
+  constexpr int ITEMS = D / 64;                   // D = 128: a thread converts K and V, D = 64: K or V
+  constexpr int CONV = MANY_KEYS * GROUPS;        // items of K
+  __shared__ __align__(1024) uint8_t tiles_lds[2][2][TILE];  // [buffer][K, V]
+  __shared__ uint32_t v_bytes[2][MANY_KEYS];                 // the V scale bytes of every key
+  __shared__ float merge_ml[MANY_WAVES][64][2];
 
   // runs of RUN consecutive tiles of one head and share on one XCD (workgroup b runs on XCD b mod 8):
   // they read the same codes, and shares of unlike length still spread over all XCDs
@@ -507,8 +508,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int blk = HALVES ? (wave & 3) : wave;
-  const int only = HALVES ? (wave >> 2) : 0;  // HALVES: which half of a chunk
+  const int blk = wave % RB, part = wave / RB;
   const Span sp = span_of(a, b);
   const int row0 = tile * TROWS;
   const int32_t most = most_of(a, sp, row0), least = least_of(a, sp, row0);
@@ -541,11 +541,11 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
 
   // ---- codes to tiles
   const int64_t head = static_cast<int64_t>(hk) * spr::kv4_head_bytes(1 << a.log_s, D);
-  const bool conv = threadIdx.x < 2 * CONV, conv_v = threadIdx.x >= CONV;
   const int ci = threadIdx.x & (CONV - 1);
   const int cr = (ci & 15) + 16 * (ci / (16 * GROUPS)), cg = (ci >> 4) & (GROUPS - 1);
-  u32x4 code = {0, 0, 0, 0};
-  uint32_t byte = 127;
+  const int first_v = ITEMS == 1 ? threadIdx.x / CONV : 0;  // what item 0 is: K or V
+  u32x4 code[ITEMS];
+  uint32_t byte[ITEMS];
   int32_t next_page = -1;
   auto look = [&](int c) {  // the page of this thread's row of chunk c
     const int32_t key = (c0 + c) * MANY_KEYS + cr;
@@ -554,29 +554,36 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
   auto fetch = [&](int c) {
     const int32_t key = (c0 + c) * MANY_KEYS + cr;
     const bool ok = next_page >= 0 && next_page < a.num_pages;
-    code = u32x4{0, 0, 0, 0};
-    byte = key < most ? 255 : 127;  // a page outside the pool is NaN; past the end nothing is read
-    if (ok && conv) {
-      const uint8_t* part = a.pages + next_page * a.page_stride + head;
-      const int32_t r = key & ((1 << a.log_s) - 1);
-      code = *reinterpret_cast<const u32x4*>(part + (conv_v ? Part::v_codes(a.log_s) : 0) + r * Part::CODE_ROW + cg * 16);
-      byte = part[(conv_v ? Part::v_scales(a.log_s) : Part::k_scales(a.log_s)) + r * Part::SCALE_ROW + cg];
+    const uint8_t* from = a.pages + (ok ? next_page : 0) * a.page_stride + head;
+    const int32_t r = key & ((1 << a.log_s) - 1);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const bool v = i + first_v != 0;
+      code[i] = u32x4{0, 0, 0, 0};
+      byte[i] = key < most ? 255 : 127;  // a page outside the pool is NaN; past the end nothing is read
+      if (ok) {
+        code[i] = *reinterpret_cast<const u32x4*>(from + (v ? Part::v_codes(a.log_s) : 0) + r * Part::CODE_ROW + cg * 16);
+        byte[i] = from[(v ? Part::v_scales(a.log_s) : Part::k_scales(a.log_s)) + r * Part::SCALE_ROW + cg];
+      }
     }
   };
   const int swz_k = D == 128 ? (cr & 15) : ((cr >> 1) & 7);
   const int swz_v = D == 128 ? 4 * (cr & 3) + ((cr >> 2) & 3) : 4 * ((cr >> 1) & 1) + ((cr >> 2) & 3);
   auto stash = [&](int c) {
-    if (!conv) return;
     const int32_t end = (c0 + c + 1) * MANY_KEYS;
-    uint8_t* to = (conv_v ? v_tiles[c % 3] : k_tiles[c & 1]) + cr * ROW;
-    const int x = conv_v ? swz_v : swz_k;
-    // a chunk that some row does not see whole keeps NaN V scales out of the products (0 * NaN); they
-    // are put in row by row
-    const float sc = spr::kv4_scale(conv_v && byte == 255 && end > least ? 127 : byte);
-    const uint32_t w[4] = {code.x, code.y, code.z, code.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(to + (((4 * cg + i) ^ x) << 4)) = spr::kv4_eight(w[i], sc);
-    if (conv_v) reinterpret_cast<uint8_t*>(&v_bytes[c % 3][cr])[cg] = static_cast<uint8_t>(byte);
+    for (int i = 0; i < ITEMS; ++i) {
+      const int v = i + first_v;
+      uint8_t* to = tiles_lds[c & 1][v] + cr * ROW;
+      const int x = v != 0 ? swz_v : swz_k;
+      // a chunk that some row does not see whole keeps NaN V scales out of the products (0 * NaN); they
+      // are put in row by row
+      const float sc = spr::kv4_scale(v != 0 && byte[i] == 255 && end > least ? 127 : byte[i]);
+      const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(to + (((4 * cg + j) ^ x) << 4)) = spr::kv4_eight(w[j], sc);
+      if (v != 0) reinterpret_cast<uint8_t*>(&v_bytes[c & 1][cr])[cg] = static_cast<uint8_t>(byte[i]);
+    }
   };
 
   // ---- products
@@ -594,15 +601,6 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
     const u32x2 r0 = lds_read_tr16(at + ((p ^ v_x) << 4));
     const u32x2 r1 = lds_read_tr16(at + 8 * ROW + ((p ^ v_x ^ 2) << 4));
     return u32x4{r0[0], r0[1], r1[0], r1[1]};
-  };
-  auto s_mma = [&](f32x16& acc, const uint8_t* kt, int hf) {
-    acc = f32x16{};
-#pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) {
-      const u32x4 k = kfrag(kt, hf, s);
-      acc = mfma32(k, qh[s], acc);
-      if constexpr (F16) acc = mfma32(k, ql[s], acc);
-    }
   };
   // mask, row maximum and lazy rescale of the 32 keys from `key` on
   auto row_max = [&](f32x16& acc, int32_t key) {
@@ -630,134 +628,152 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
       neg_m = m_new == NEG_INF ? 0.0f : -m_new;
     }
   };
-  // S of 32 keys (kt_n, hf_n) into acc_next beside the exponentials of acc, then O += P V (vt, hf)
-  auto step = [&](f32x16& acc_next, const uint8_t* kt_n, int hf_n, const f32x16& acc, const uint8_t* vt, int hf) {
+  // S of 32 keys (piece hf_n of kt) into acc_next beside the exponentials of acc, as far as asked for;
+  // then O += P V (piece hf of vt)
+  auto step = [&](auto with_s, auto with_p, f32x16& acc_next, const uint8_t* kt, int hf_n, const f32x16& acc, const uint8_t* vt, int hf) {
+    constexpr bool S = decltype(with_s)::value, P = decltype(with_p)::value;
     uint32_t ph[2][4], pl[2][4];
     float sum0 = 0.0f, sum1 = 0.0f;
-    acc_next = f32x16{};
+    if constexpr (S) acc_next = f32x16{};
     constexpr int EACH = 16 / KSTEPS;  // elements of P beside each step of S
     u32x4 ka[3];
-    ka[0] = kfrag(kt_n, hf_n, 0);
-    ka[1] = kfrag(kt_n, hf_n, 1);
+    if constexpr (S) {
+      ka[0] = kfrag(kt, hf_n, 0);
+      ka[1] = kfrag(kt, hf_n, 1);
+    }
 #pragma unroll
     for (int st = 0; st < KSTEPS; ++st) {
-      if (st + 2 < KSTEPS) ka[(st + 2) % 3] = kfrag(kt_n, hf_n, st + 2);
-      acc_next = mfma32(ka[st % 3], qh[st], acc_next);
-      if constexpr (F16) acc_next = mfma32(ka[st % 3], ql[st], acc_next);
+      if constexpr (S) {
+        if (st + 2 < KSTEPS) ka[(st + 2) % 3] = kfrag(kt, hf_n, st + 2);
+        acc_next = mfma32(ka[st % 3], qh[st], acc_next);
+        if constexpr (F16) acc_next = mfma32(ka[st % 3], ql[st], acc_next);
+      }
+      if constexpr (P) {
 #pragma unroll
-      for (int e = EACH * st; e < EACH * (st + 1); e += 2) {
-        const float p0 = exp2_hw(__builtin_fmaf(acc[e], a.scale_log2, neg_m));
-        const float p1 = exp2_hw(__builtin_fmaf(acc[e + 1], a.scale_log2, neg_m));
-        sum0 += p0;
-        sum1 += p1;
-        const uint32_t w = spr::pack_bf16x2(p0, p1);
-        ph[e / 8][(e % 8) / 2] = w;
-        if constexpr (F16) pl[e / 8][(e % 8) / 2] = spr::pack_bf16x2(p0 - spr::bf16_lo(w), p1 - spr::bf16_hi(w));
+        for (int e = EACH * st; e < EACH * (st + 1); e += 2) {
+          const float p0 = exp2_hw(__builtin_fmaf(acc[e], a.scale_log2, neg_m));
+          const float p1 = exp2_hw(__builtin_fmaf(acc[e + 1], a.scale_log2, neg_m));
+          const uint32_t w = spr::pack_bf16x2(p0, p1);
+          sum0 += p0;
+          sum1 += p1;
+          ph[e / 8][(e % 8) / 2] = w;
+          if constexpr (F16) pl[e / 8][(e % 8) / 2] = spr::pack_bf16x2(p0 - spr::bf16_lo(w), p1 - spr::bf16_hi(w));
+        }
       }
     }
-    l_run += sum0 + sum1;
-    u32x4 va[3];
-    va[0] = vfrag(vt, hf, 0);
-    va[1] = vfrag(vt, hf, 1);
+    if constexpr (P) {
+      l_run += sum0 + sum1;
+      u32x4 va[3];
+      va[0] = vfrag(vt, hf, 0);
+      va[1] = vfrag(vt, hf, 1);
 #pragma unroll
-    for (int f = 0; f < 2 * DBLK; ++f) {
-      if (f + 2 < 2 * DBLK) va[(f + 2) % 3] = vfrag(vt, hf, f + 2);
-      const int k = f / DBLK;
-      o_acc[f % DBLK] = mfma32(va[f % 3], u32x4{ph[k][0], ph[k][1], ph[k][2], ph[k][3]}, o_acc[f % DBLK]);
-      if constexpr (F16) o_acc[f % DBLK] = mfma32(va[f % 3], u32x4{pl[k][0], pl[k][1], pl[k][2], pl[k][3]}, o_acc[f % DBLK]);
+      for (int f = 0; f < 2 * DBLK; ++f) {
+        if (f + 2 < 2 * DBLK) va[(f + 2) % 3] = vfrag(vt, hf, f + 2);
+        const int k = f / DBLK;
+        o_acc[f % DBLK] = mfma32(va[f % 3], u32x4{ph[k][0], ph[k][1], ph[k][2], ph[k][3]}, o_acc[f % DBLK]);
+        if constexpr (F16) o_acc[f % DBLK] = mfma32(va[f % 3], u32x4{pl[k][0], pl[k][1], pl[k][2], pl[k][3]}, o_acc[f % DBLK]);
+      }
     }
   };
   // NaN V scales of a chunk that some row does not see whole: their dims of the rows that see the key
   auto put_nan = [&](int c) {
     const int32_t first = (c0 + c) * MANY_KEYS;
     if (first + MANY_KEYS <= least) return;
-    const uint32_t w = v_bytes[c % 3][lane];
-    uint32_t mine = 0;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) mine |= ((w >> (8 * g)) & 255) == 255 ? 1u << g : 0;
-    uint64_t keys = __ballot(mine != 0);
-    while (keys != 0) {
-      const int k = __builtin_ctzll(keys);
-      keys &= keys - 1;
-      const uint32_t groups = __builtin_amdgcn_readlane(mine, k);
-      if (HALVES && (k >> 5) != only) continue;
+    for (int k0 = 0; k0 < MANY_KEYS; k0 += 64) {
+      const uint32_t w = v_bytes[c & 1][k0 + lane];
+      uint32_t mine = 0;
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        if (((groups >> g) & 1) != 0 && first + k < seen) {
+      for (int g = 0; g < GROUPS; ++g) mine |= ((w >> (8 * g)) & 255) == 255 ? 1u << g : 0;
+      uint64_t keys = __ballot(mine != 0);
+      while (keys != 0) {
+        const int k = __builtin_ctzll(keys);
+        keys &= keys - 1;
+        const uint32_t groups = __builtin_amdgcn_readlane(mine, k);
+        if ((k0 + k) / (32 * HALVES) != part) continue;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o_acc[g][e] = __builtin_nanf("");
+        for (int g = 0; g < GROUPS; ++g) {
+          if (((groups >> g) & 1) != 0 && first + k0 + k < seen) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o_acc[g][e] = __builtin_nanf("");
+          }
         }
       }
     }
   };
 
   if (nch > 0) {
-    look(0), fetch(0), look(1), stash(0);
-    if (nch > 1) {
-      fetch(1), look(2), stash(1);
-    }
-    fetch(2), look(3);
-    __syncthreads();
-    f32x16 s_a, s_b;
-    if (wave_live) s_mma(s_a, k_tiles[0], only);
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    look(0), fetch(0), look(1);
+    stash(0);
+    fetch(1), look(2);
+    // the two waves of a SIMD (w and w + 4) convert at opposite ends of a chunk: one's conversions run
+    // beside the other's products (frame of 3600 rows 5.30 -> 5.24 ms)
+    auto refill = [&](int x) {
+      if (x + 1 < nch) {
+        stash(x + 1);
+        fetch(x + 2);
+        look(x + 3);
+      }
+    };
+    f32x16 s[2];
     for (int x = 0; x < nch; ++x) {
-      const int32_t key = (c0 + x) * MANY_KEYS;
-      const uint8_t *kt = k_tiles[x & 1], *kt1 = k_tiles[(x + 1) & 1], *vt = v_tiles[x % 3];
-      // the last chunk computes a next S from an old tile, unused: the same straight code
-      if constexpr (HALVES) {
-        if (wave_live) row_max(s_a, key + 32 * only);
-        __syncthreads();
-        if (wave_live) {
-          step(s_b, kt1, only, s_a, vt, only);
-          s_a = s_b;
-          put_nan(x);
+      spr::lds_barrier();  // chunk x is written; nobody reads chunk x - 1 any more
+      const uint8_t *kt = tiles_lds[x & 1][0], *vt = tiles_lds[x & 1][1];
+      const int32_t key = (c0 + x) * MANY_KEYS + part * (32 * HALVES);
+      const int h0 = part * HALVES;
+      if (wave >= 4) refill(x);
+      if (wave_live) {
+        step(yes, no, s[0], kt, h0, s[1], vt, h0);
+#pragma unroll
+        for (int i = 0; i < HALVES; ++i) {
+          row_max(s[i & 1], key + 32 * i);
+          if (i + 1 < HALVES) step(yes, yes, s[(i + 1) & 1], kt, h0 + i + 1, s[i & 1], vt, h0 + i);
+          else step(no, yes, s[(i + 1) & 1], kt, h0, s[i & 1], vt, h0 + i);
         }
-      } else {
-        if (wave_live) {
-          row_max(s_a, key);
-          step(s_b, kt, 1, s_a, vt, 0);
-          row_max(s_b, key + 32);
-        }
-        __syncthreads();
-        if (wave_live) {
-          step(s_a, kt1, 0, s_b, vt, 1);
-          put_nan(x);
-        }
+        put_nan(x);
       }
-      if (x + 2 < nch) {
-        stash(x + 2);
-        fetch(x + 3);
-        look(x + 4);
-      }
+      if (wave < 4) refill(x);
     }
   }
 
   float l_tot = sum_xor32(l_run);
-  if constexpr (HALVES) {
-    // waves 4 .. 7 hand (m, l, O) to waves 0 .. 3 through the tiles: 32 rows of D floats each
-    float* po = reinterpret_cast<float*>(blk < 2 ? k_tiles[blk] : v_tiles[blk - 2]);
+  if constexpr (PARTS > 1) {
+    // the other parts hand (m, l, O) to part 0 through the tiles: 32 rows of D floats each
     __syncthreads();
-    if (only == 1) {
+    float* po = reinterpret_cast<float*>(&tiles_lds[0][0][0]);
+    if (part > 0) {
+      float* mine = po + (wave - RB) * (32 * D);
 #pragma unroll
       for (int i = 0; i < DBLK; ++i) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) po[(i * 16 + e) * 64 + lane] = o_acc[i][e];
+        for (int e = 0; e < 16; ++e) mine[(i * 16 + e) * 64 + lane] = o_acc[i][e];
       }
-      merge_ml[blk][lane][0] = m_run;
-      merge_ml[blk][lane][1] = l_tot;
+      merge_ml[wave][lane][0] = m_run;
+      merge_ml[wave][lane][1] = l_tot;
     }
     __syncthreads();
-    if (only == 1) return;
-    const float m1 = merge_ml[blk][lane][0], l1 = merge_ml[blk][lane][1];
-    const float top = fmaxf(m_run, m1);
+    if (part > 0) return;
+    float top = m_run;
+#pragma unroll
+    for (int p = 1; p < PARTS; ++p) top = fmaxf(top, merge_ml[wave + p * RB][lane][0]);
     // one without a maximum has no sum (or NaN)
-    const float f0 = m_run == NEG_INF ? 1.0f : exp2_hw(m_run - top), f1 = m1 == NEG_INF ? 1.0f : exp2_hw(m1 - top);
+    const float f0 = m_run == NEG_INF ? 1.0f : exp2_hw(m_run - top);
+    l_tot *= f0;
 #pragma unroll
-    for (int i = 0; i < DBLK; ++i) {
+    for (int i = 0; i < DBLK; ++i) o_acc[i] *= f0;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o_acc[i][e] = o_acc[i][e] * f0 + po[(i * 16 + e) * 64 + lane] * f1;
+    for (int p = 1; p < PARTS; ++p) {
+      const float m1 = merge_ml[wave + p * RB][lane][0], f1 = m1 == NEG_INF ? 1.0f : exp2_hw(m1 - top);
+      const float* theirs = po + (wave + (p - 1) * RB) * (32 * D);
+      l_tot += merge_ml[wave + p * RB][lane][1] * f1;
+#pragma unroll
+      for (int i = 0; i < DBLK; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o_acc[i][e] += theirs[(i * 16 + e) * 64 + lane] * f1;
+      }
     }
-    l_tot = l_tot * f0 + l1 * f1;
     m_run = top;
   }
   if (!in) return;
@@ -858,11 +874,11 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, int64_t all_
 
 // ---------------------------------------------------------------------------- host
 
-// How a call is cut up: by the few-row kernel in 16 * nt rows, or by the many-row one in 128 (halves)
-// or 256 rows, and the keys in nsplit shares.
+// How a call is cut up: by the few-row kernel in 16 * nt rows, or by the many-row one in 64, 128 or 256
+// rows, and the keys in nsplit shares.
 struct Shape {
   int32_t nt;  // 0: the many-row kernel
-  bool halves;
+  int32_t rb;  // its row blocks of 32
   int32_t nsplit;
   int64_t groups;  // workgroups to a share
 };
@@ -881,19 +897,19 @@ Shape shape_of(int32_t batch, int32_t kv_heads, int32_t group, int32_t rows, int
     s.nsplit = static_cast<int32_t>(std::min({fill, most, int64_t{256}}));
     return s;
   }
-  s.halves = total <= 128;
-  s.groups = heads * spr::ceil_div(total, s.halves ? 128 : 256);
+  s.rb = total <= 64 ? 2 : total <= 128 ? 4 : 8;
+  s.groups = heads * spr::ceil_div(total, 32 * s.rb);
   const int64_t chunks = std::max<int64_t>(1, spr::ceil_div(max_length, MANY_KEYS));
   if (batch > 1) {
-    s.nsplit = static_cast<int32_t>(std::min({std::max<int64_t>(1, 1024 / s.groups), std::max<int64_t>(1, chunks / 8), int64_t{64}}));
+    s.nsplit = static_cast<int32_t>(std::min({std::max<int64_t>(1, 1024 / s.groups), std::max<int64_t>(1, chunks / 4), int64_t{64}}));
     return s;
   }
-  // one workgroup a CU, so a call takes whole rounds of 256: the shares that come out fastest, at about
-  // 1 us a chunk (half that with two waves to a row) and 4 TB/s for the partial results
+  // one workgroup a CU, so a call takes whole rounds of 256: the shares that come out fastest, at what a
+  // chunk takes and 4 TB/s for the partial results
   double best = 0.0;
-  for (int32_t n = 1; n <= 64 && (n == 1 || chunks >= 8 * n); ++n) {
+  for (int32_t n = 1; n <= 64 && (n == 1 || chunks >= 4 * n); ++n) {
     const double rounds = static_cast<double>(spr::ceil_div(s.groups * n, 256));
-    const double each = (s.halves ? 0.6 : 1.0) * (static_cast<double>(chunks) / n + 3.0);
+    const double each = (s.rb == 8 ? 3.8 : s.rb == 4 ? 2.1 : 1.2) * (static_cast<double>(chunks) / n + 2.0);
     const double merge = n == 1 ? 0.0 : 6.0 + 8e-6 / 4.0 * d * static_cast<double>(heads * total) * n;
     const double us = rounds * each + merge;
     if (n == 1 || us < best) best = us, s.nsplit = n;
@@ -909,8 +925,9 @@ void launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
     else kv4_few_kernel<D, 2, F16><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
   } else {
     const unsigned grid = static_cast<unsigned>(spr::ceil_div(s.groups * s.nsplit, 8 * RUN) * (8 * RUN));
-    if (s.halves) kv4_many_kernel<D, F16, true><<<grid, 64 * MANY_WAVES, 0, stream>>>(a);
-    else kv4_many_kernel<D, F16, false><<<grid, 64 * MANY_WAVES, 0, stream>>>(a);
+    if (s.rb == 8) kv4_many_kernel<D, F16, 8><<<grid, 64 * MANY_WAVES, 0, stream>>>(a);
+    else if (s.rb == 4) kv4_many_kernel<D, F16, 4><<<grid, 64 * MANY_WAVES, 0, stream>>>(a);
+    else kv4_many_kernel<D, F16, 2><<<grid, 64 * MANY_WAVES, 0, stream>>>(a);
   }
   if (s.nsplit > 1) {
     const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.group * a.rows;
@@ -976,7 +993,7 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
   a.num_pages = num_pages, a.causal = causal;
   a.nsplit = s.nsplit;
   a.block_keys = s.nt != 0 ? FEW_KEYS : MANY_KEYS;
-  a.tile_rows = s.nt != 0 ? 16 * s.nt : s.halves ? 128 : 256;
+  a.tile_rows = s.nt != 0 ? 16 * s.nt : 32 * s.rb;
   a.share = static_cast<int32_t>(spr::ceil_div(std::max<int64_t>(longest, 1), static_cast<int64_t>(a.block_keys) * s.nsplit));
   a.scale_log2 = scale * LOG2E;
   if (d == 128) {
