@@ -320,16 +320,15 @@ __device__ __forceinline__ int64_t pages_for(int64_t tokens, int log_s) { return
 
 // Room for counts[b] more tokens in every named sequence, and the sequences' lengths with them.  One
 // workgroup.  starts[b] is the first new token's place, or -1 for all when the call cannot happen.
-__global__ __launch_bounds__(PLAN_THREADS) void kv4_reserve_kernel(int32_t* __restrict__ table,
-                                                                   int32_t* __restrict__ lengths,
+__global__ __launch_bounds__(PLAN_THREADS) void kv4_reserve_kernel(int32_t* __restrict__ table, int32_t* lengths,
                                                                    int32_t* __restrict__ refs,
-                                                                   const int32_t* __restrict__ counts,
-                                                                   const int32_t* __restrict__ seq_ids, int32_t n,
-                                                                   int32_t sequences, int32_t wide, int32_t log_s,
-                                                                   int32_t num_pages, int32_t* __restrict__ starts,
+                                                                   const int32_t* counts, const int32_t* seq_ids,
+                                                                   int32_t n, int32_t sequences, int32_t wide,
+                                                                   int32_t log_s, int32_t num_pages,
+                                                                   int32_t* __restrict__ starts,
                                                                    int32_t* __restrict__ status,
                                                                    int32_t* __restrict__ list) {
-  __shared__ int32_t ids[MAX_NAMED], sums[MAX_NAMED + 1], olds[MAX_NAMED];
+  __shared__ int32_t ids[MAX_NAMED], sums[MAX_NAMED + 1], olds[MAX_NAMED], news[MAX_NAMED];
   __shared__ int scratch[PLAN_THREADS / 64];
   const int64_t room = static_cast<int64_t>(wide) << log_s;
   bool bad_id = false, bad_count = false, bad_length = false, full = false;
@@ -337,16 +336,19 @@ __global__ __launch_bounds__(PLAN_THREADS) void kv4_reserve_kernel(int32_t* __re
     const int32_t id = seq_ids != nullptr ? seq_ids[i] : i;
     ids[i] = id;
     olds[i] = 0;
+    news[i] = 0;
     sums[i] = 0;
     if (id < 0 || id >= sequences) {
       bad_id = true;
       continue;
     }
+    // all is read before anything is written: counts may be the lengths themselves
     const int32_t old = lengths[id], more = counts[i];
     bad_length |= old < 0 || old > room;
     bad_count |= more < 0;
     full |= static_cast<int64_t>(old) + more > room;
     olds[i] = old;
+    news[i] = static_cast<int32_t>(min(static_cast<int64_t>(old) + more, room));
     sums[i] = static_cast<int32_t>(pages_for(static_cast<int64_t>(old) + more, log_s) - pages_for(old, log_s));
   }
   __syncthreads();
@@ -372,7 +374,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void kv4_reserve_kernel(int32_t* __re
   }
   for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
     starts[i] = olds[i];
-    lengths[ids[i]] = olds[i] + counts[i];
+    lengths[ids[i]] = news[i];
   }
 }
 

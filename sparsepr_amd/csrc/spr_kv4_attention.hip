@@ -814,14 +814,13 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
 
 // ---------------------------------------------------------------------------- merge of key shares
 
-// W waves a row take its shares in turn, each lane D / 64 dims; 4 / W rows a workgroup.
-template <int D, bool F16, int W>
+// 16 lanes have all dims of a row, and P such teams share a row's shares; 16 / P rows a workgroup.
+template <int D, bool F16, int P>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, int64_t all_rows) {
-  constexpr int E = D / 64;
-  __shared__ float lds[4][D];
-  __shared__ float lds_l[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / W) + wave / W;
+  constexpr int E = D / 16;  // dims of a lane
+  __shared__ float lds[P > 1 ? 16 : 1][D + 1];
+  const int lane = threadIdx.x & 15, team = threadIdx.x >> 4;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (16 / P) + team / P;
   const int total_rows = a.rows * a.group;
   const bool in = row < all_rows;
   const int64_t bh = in ? row / total_rows : 0;
@@ -829,34 +828,41 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, int64_t all_
   const int b = static_cast<int>(bh / a.kv_heads), hk = static_cast<int>(bh % a.kv_heads);
   const Span sp = span_of(a, b);
   const int32_t shares = in ? deal_of(a, most_of(a, sp, rho / a.tile_rows * a.tile_rows)).shares : 1;
-  static_assert(W == 1 || W == 4, "waves of a workgroup leave together or wait for nobody");
-  if (shares == 1) return;  // written already, or no row
+  if (P == 1 && shares == 1) return;  // written already, or no row
   const int64_t first = bh * a.nsplit * total_rows + rho;
   float top = NEG_INF;
-  for (int s = lane; s < shares; s += 64) top = fmaxf(top, a.part_ml[(first + static_cast<int64_t>(s) * total_rows) * 2]);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   float l = 0.0f, acc[E] = {};
+  if (shares > 1) {
+    for (int s = lane; s < shares; s += 16) top = fmaxf(top, a.part_ml[(first + static_cast<int64_t>(s) * total_rows) * 2]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 16));
 #pragma unroll 4
-  for (int s = wave % W; s < shares; s += W) {
-    const int64_t at = first + static_cast<int64_t>(s) * total_rows;
-    const float ms = a.part_ml[at * 2];
-    // a share without a maximum saw nothing (or only NaN): its sums count as they are, zeros (or NaN)
-    const float f = ms == NEG_INF ? 1.0f : exp2_hw(ms - top);
-    l += f * a.part_ml[at * 2 + 1];
+    for (int s = team % P; s < shares; s += P) {
+      const int64_t at = first + static_cast<int64_t>(s) * total_rows;
+      const float ms = a.part_ml[at * 2];
+      // a share without a maximum saw nothing (or only NaN): its sums count as they are, zeros (or NaN)
+      const float f = ms == NEG_INF ? 1.0f : exp2_hw(ms - top);
+      l += f * a.part_ml[at * 2 + 1];
+      const f32x4* o = reinterpret_cast<const f32x4*>(a.part_o + at * D + lane * E);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += f * a.part_o[at * D + lane * E + e];
+      for (int e = 0; e < E; e += 4) {
+        const f32x4 x = o[e / 4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[e + i] += f * x[i];
+      }
+    }
   }
-  if constexpr (W > 1) {
+  if constexpr (P > 1) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) lds[wave][lane * E + e] = acc[e];
-    if (lane == 0) lds_l[wave] = l;
+    for (int e = 0; e < E; ++e) lds[team][lane * E + e] = acc[e];
+    if (lane == 0) lds[team][D] = l;
     __syncthreads();
-    if (wave % W != 0) return;
-    for (int w = wave + 1; w < wave + W; ++w) {
-      l += lds_l[w];
+    if (team % P != 0 || shares == 1) return;
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += lds[w][lane * E + e];
+    for (int w = 1; w < P; ++w) {
+      l += lds[team + w][D];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += lds[team + w][lane * E + e];
     }
   }
   const int t = rho / a.group, h = hk * a.group + rho % a.group;
@@ -865,9 +871,10 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, int64_t all_
   const int64_t at = (static_cast<int64_t>(b) * a.kv_heads * a.group + h) * a.rows + t;
   const float inv = 1.0f / l;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float o = l == 0.0f ? 0.0f : acc[e] * inv;
-    a.out[at * D + lane * E + e] = F16 ? spr::f32_to_f16(o) : spr::f32_to_bf16(o);
+  for (int e = 0; e < E; e += 4) {
+    u32x2 w = {0, 0};
+    if (l != 0.0f) w = u32x2{pack_out<F16>(acc[e] * inv, acc[e + 1] * inv), pack_out<F16>(acc[e + 2] * inv, acc[e + 3] * inv)};
+    *reinterpret_cast<u32x2*>(a.out + at * D + lane * E + e) = w;
   }
   if (lane == 0 && a.lse != nullptr) a.lse[at] = l == 0.0f ? NEG_INF : (top + __builtin_amdgcn_logf(l)) * LN2;
 }
@@ -931,9 +938,11 @@ void launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   }
   if (s.nsplit > 1) {
     const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.group * a.rows;
-    // four waves a row where there are many shares, one where there are many rows
-    if (s.nsplit >= 8) kv4_merge_kernel<D, F16, 4><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a, rows);
-    else kv4_merge_kernel<D, F16, 1><<<static_cast<unsigned>(spr::ceil_div(rows, 4)), 256, 0, stream>>>(a, rows);
+    // as many teams to a row as there are shares and room for on the card
+    const unsigned all = static_cast<unsigned>(rows);
+    if (s.nsplit >= 16 && rows <= 4096) kv4_merge_kernel<D, F16, 16><<<all, 256, 0, stream>>>(a, rows);
+    else if (s.nsplit >= 4 && rows <= 16384) kv4_merge_kernel<D, F16, 4><<<(all + 3) / 4, 256, 0, stream>>>(a, rows);
+    else kv4_merge_kernel<D, F16, 1><<<(all + 15) / 16, 256, 0, stream>>>(a, rows);
   }
 }
 
@@ -959,9 +968,9 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
   SPR_REQUIRE(spr::kv4_page_size_ok(page_size), "%s: page size %d (32, 64, 128 or 256)", what, page_size);
   SPR_REQUIRE(num_pages >= 1 && sequences >= 1 && wide >= 1 && static_cast<int64_t>(wide) * page_size <= INT32_MAX,
               "%s: %d pages, a block table of %d x %d", what, num_pages, sequences, wide);
-  SPR_REQUIRE(batch >= 0 && batch <= 65535 && rows >= 0 && kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0,
+  SPR_REQUIRE(batch >= 0 && batch <= 65535 && rows >= 0 && kv_heads >= 1 && kv_heads <= 65535 && heads >= 1 && heads % kv_heads == 0,
               "%s: batch %d, rows %d, %d query heads on %d kv heads", what, batch, rows, heads, kv_heads);
-  SPR_REQUIRE(scale > 0.0f && scale <= 3.402823466e38f, "%s: the scale must be positive and finite", what);
+  SPR_REQUIRE(scale > 0.0f && scale <= 1e38f, "%s: the scale must be positive and at most 1e38", what);
   SPR_REQUIRE(max_length >= 0, "%s: max_length %lld", what, static_cast<long long>(max_length));
   SPR_REQUIRE(q_b % 8 == 0 && q_h % 8 == 0 && q_t % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(pages) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,

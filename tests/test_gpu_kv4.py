@@ -558,3 +558,117 @@ def test_calls_on_two_streams_and_repeats_give_the_same_bits(dev):
                 got.append([c.attend(x, causal=True) for x in q])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+
+
+# ------------------------------------------------------------------ refusals, odd calls
+
+
+def test_calls_with_the_wrong_tensors_are_refused(dev):
+    from sparsepr_amd.kernels import kv4
+
+    n, h, d, size = 4, 2, 64, 32
+    pages = torch.zeros((n, h, kv4.kv4_page_bytes(size, d)), dtype=torch.uint8, device=dev)
+    table = torch.zeros((3, 2), dtype=torch.int32, device=dev)
+    lengths, refs, one = (torch.zeros(k, dtype=torch.int32, device=dev) for k in (3, n, 1))
+    x = torch.zeros((1, h, 5, d), dtype=torch.bfloat16, device=dev)
+
+    def store(p=pages, t=table, k=x, v=x, s=one, **kw):
+        kv4.kv4_store(p, t, k, v, s, **kw)
+
+    def load(p=pages, t=table, s=one, c=one, rows=5, dim=d, **kw):
+        kv4.kv4_load(p, t, s, c, rows, dim, **kw)
+
+    def attend(q=x, p=pages, t=table, n=lengths, **kw):
+        kv4.kv4_attention(q, p, t, n, **kw)
+
+    for call, text in [
+        (lambda: store(p=pages.int()), "contiguous uint8"), (lambda: store(p=pages[:, :1]), "contiguous uint8"),
+        (lambda: store(p=pages[..., :-16].contiguous()), "not whole pages"), (lambda: store(p=pages[:0]), "contiguous uint8"),
+        (lambda: store(k=x[..., :32], v=x[..., :32]), "head dim 32"), (lambda: store(v=x.float()), "of one dtype"),
+        (lambda: store(k=x.int(), v=x.int()), "of one dtype"), (lambda: store(v=x[:, :, :4]), "of one dtype"),
+        (lambda: store(k=x[:, :1], v=x[:, :1]), "K has 1 heads, the pages 2"),
+        (lambda: store(t=table.long()), "block_table must be"), (lambda: store(t=table[0]), "block_table must be"),
+        (lambda: store(t=table.t()), "block_table must be"), (lambda: store(s=lengths), "starts must be"),
+        (lambda: store(s=one.long()), "starts must be"), (lambda: store(counts=lengths), "counts must be"),
+        (lambda: store(seq_ids=lengths), "seq_ids must be"), (lambda: store(s=one.cpu()), "require GPU tensors"),
+        (lambda: store(k=x.expand(5, h, 5, d), v=x.expand(5, h, 5, d), s=torch.zeros(5, dtype=torch.int32, device=dev)),
+         "a batch of 5 without seq_ids"),
+        (lambda: load(dim=128), "not whole pages"), (lambda: load(rows=-1), "rows -1"),
+        (lambda: load(dtype=torch.float64), "dtype must be"), (lambda: load(c=lengths), "counts must be"),
+        (lambda: attend(q=x.float()), "bfloat16 or float16"), (lambda: attend(q=x[0]), "bfloat16 or float16"),
+        (lambda: attend(q=x[:, :1]), "multiple of KV heads"), (lambda: attend(n=one), "lengths must be"),
+        (lambda: attend(counts=lengths), "counts must be"), (lambda: attend(scale=0.0), "scale must be positive"),
+        (lambda: attend(scale=float("nan")), "scale must be positive"), (lambda: attend(max_length=-1), "max_length -1"),
+        (lambda: kv4.kv4_reserve(table, lengths, refs, 48, lengths), "page size 48"),
+        (lambda: kv4.kv4_reserve(table, one, refs, size, lengths), "lengths must be"),
+        (lambda: kv4.kv4_reserve(table, lengths, refs, size, refs), "a batch of 4 without seq_ids"),
+        (lambda: kv4.kv4_reserve(table, lengths, refs, size, lengths, status=lengths), "status must be"),
+        (lambda: kv4.kv4_free(table, lengths, refs, size, one, first_pages=lengths), "first_pages must be"),
+        (lambda: kv4.kv4_free(table, lengths, refs, size, one.float()), "seq_ids must be"),
+        (lambda: kv4.kv4_fork(pages, table, lengths, refs, size, one, lengths), "dst must be"),
+        (lambda: kv4.kv4_fork(pages, table, lengths, one, size, one, one), "4 pages, ref_count of 1"),
+        (lambda: kv4.kv4_compact(pages.float(), table, refs), "contiguous uint8"),
+        (lambda: kv4.kv4_compact(pages[None, None], table, refs), "contiguous uint8"),
+    ]:
+        with pytest.raises(RuntimeError, match=text):
+            call()
+    assert int(pages.sum()) == 0
+
+
+def test_empty_calls_and_no_sequences(dev):
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    cache = KV4Cache(4, 2, 64, 3, page_size=32, device=dev)
+    x = torch.zeros((0, 2, 5, 64), dtype=torch.bfloat16, device=dev)
+    assert cache.attend(x).shape == x.shape
+    out, lse = cache.attend(torch.ones((3, 4, 0, 64), dtype=torch.float16, device=dev), return_lse=True)
+    assert out.shape == (3, 4, 0, 64) and lse.shape == (3, 4, 0)
+    out, lse = cache.attend(torch.ones((3, 4, 2, 64), dtype=torch.float16, device=dev), return_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all()  # sequences without tokens
+    out, lse = cache.attend(torch.ones((3, 4, 40, 64), dtype=torch.float16, device=dev), causal=True, return_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    assert cache.reserve(none, none).shape == (0,)
+    cache.free(none), cache.fork(none, none), cache.store(x, x, none)
+    k, v = cache.load([0, 0, 0], [0, 0, 0], 0)
+    assert k.shape == (3, 2, 0, 64)
+    k, v = cache.load([0, 0, 0], [0, 1, 0], 2)
+    assert (k[[0, 2]] == 0).all() and torch.isnan(k[1, :, 0]).all() and (v[1, :, 1] == 0).all()
+    assert int(cache.compact()) == 0
+    cache.check()
+    # the lengths themselves as counts: sequences twice as long
+    cache.reserve([20, 0, 30])
+    starts = cache.reserve(cache.lengths)
+    assert starts.tolist() == [20, 0, 30] and cache.lengths.tolist() == [40, 0, 60]
+
+
+def test_a_window_that_slides_over_a_video(dev):
+    """Frame after frame: reserve, store, attend, and past four frames the oldest whole pages but the
+    first go; attention is over what is left, in order."""
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    rng = np.random.default_rng(14)
+    h, d, size, frame, layers = 3, 128, 32, 50, 2
+    cache = KV4Cache(9, h, d, 2, page_size=size, max_pages=9, layers=layers, device=dev)
+    kept = [np.zeros((2, h, 0, d)) for _ in range(layers)]
+    for i in range(12):
+        starts = cache.reserve([frame], [1])
+        for layer in range(layers):
+            k, v = torch.randn((2, 1, frame, h, d), device=dev).to(torch.bfloat16).transpose(2, 3)
+            cache.store(k, v, starts, seq_ids=[1], layer=layer)
+            new = np.stack([model.decode(*model.encode(y[0].double().cpu().numpy())) for y in (k, v)])
+            kept[layer] = np.concatenate([kept[layer], new], 2)
+            q = torch.randn((1, h, frame, d), device=dev).to(torch.bfloat16)
+            out, lse = cache.attend(q, seq_ids=[1], layer=layer, return_lse=True)
+            n = kept[layer].shape[2]
+            assert int(cache.lengths[1]) == n
+            # 2^-8 for each rounding (probabilities, output), and as much again for what is in fp32
+            ref, ref_lse, spread, _ = model.attend(q[0].double().cpu().numpy(), *kept[layer], frame, False, d**-0.5)
+            assert (np.abs(out[0].double().cpu().numpy() - ref) <= 2.0**-7 * (spread + np.abs(ref)) + 1e-6).all()
+            got = cache.load([0], [n], n, seq_ids=[1], layer=layer)
+            assert all(np.array_equal(g[0].double().cpu().numpy(), w) for g, w in zip(got, kept[layer]))
+        over = (n - 3 * frame) // size
+        if over > 0:
+            cache.free([1], first_pages=[1], page_counts=[over])
+            kept = [np.delete(x, np.s_[size:size * (1 + over)], 2) for x in kept]
+    cache.check()
