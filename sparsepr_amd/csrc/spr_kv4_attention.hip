@@ -8,7 +8,7 @@
 // list of rows * group query rows.
 //
 // K and V values (code times scale) are exact in bf16, so the conversion to the MFMA's operand loses
-// nothing; fp16 queries and probabilities go in as two bf16 terms (hi + lo) and lose at most 2^-16
+// nothing; fp16 queries and probabilities go in as two bf16 terms (hi + lo) and lose at most 2^-14
 // of themselves.  Scores, the running maximum and sum and the output are fp32; bf16 calls round each
 // probability to bf16 once, relative to a maximum at most 2^8 below the row's own.
 #include <algorithm>
@@ -189,7 +189,12 @@ struct Held {
 // own wave (no barrier) and comes back transposed (ds_read_b64_tr_b16).  A 32-byte unit u of row r sits
 // at u ^ (r & 7) (D = 128; u ^ ((r >> 1) & 3) for D = 64), its halves swapped in rows 8 .. 15: the
 // transposing read of eight rows meets every bank once, and so does the write of sixteen.
-template <int D, int NT, bool F16>
+//
+// TWICE: at most 8 rows, each in two of the 16 columns (m and m + 8), one for the upper eight
+// significant bits of its probabilities and one for the next eight, so P loses 2^-14 of itself instead of
+// the 2^-8 of a rounding to bf16, for two VALU operations an element and no product more.  (As a second
+// product of the remainders it cost 3 to 9 %.)
+template <int D, int NT, bool F16, bool TWICE>
 __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kernel(AttnArgs a) {
   using Part = spr::Kv4Part<D>;
   constexpr int KS = D / 32;   // MFMA steps over the dims
@@ -212,7 +217,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
   int32_t seen[NT];  // keys this lane's query row sees
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int rho = n * 16 + m;
+    const int rho = TWICE ? (m & 7) : n * 16 + m;
     const bool in = rho < total_rows;
     const int t = in ? rho / a.group : 0, h = hk * a.group + (in ? rho % a.group : 0);
     seen[n] = in ? visible_of(a, sp, t) : 0;
@@ -228,6 +233,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
   const int32_t least = least_of(a, sp, 0);
   const int32_t last = min(deal.blocks, (split + 1) * deal.per);
 
+  const uint32_t cut = TWICE && m >= 8 ? 0xffff0000u : 0u;
   f32x4 acc[NT][VT];
   float mx[NT], sum[NT];
 #pragma unroll
@@ -326,6 +332,17 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
         p[e] = exp2_hw(y[e] - off);
         sum[n] += p[e];
       }
+      if constexpr (TWICE) {
+        // columns 0 .. 7 cut p to its upper bits, columns 8 .. 15 take what that leaves
+        uint32_t x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = __float_as_uint(p[e] - __uint_as_float(__float_as_uint(p[e]) & cut));
+        }
+        ph[n] = u32x4{__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u),
+                      __builtin_amdgcn_perm(x[5], x[4], 0x07060302u), __builtin_amdgcn_perm(x[7], x[6], 0x07060302u)};
+        continue;
+      }
       ph[n] = u32x4{spr::pack_bf16x2(p[0], p[1]), spr::pack_bf16x2(p[2], p[3]), spr::pack_bf16x2(p[4], p[5]),
                     spr::pack_bf16x2(p[6], p[7])};
       if constexpr (F16) {
@@ -345,7 +362,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         acc[n][v] = mfma16(vf, ph[n], acc[n][v]);
-        if constexpr (F16) acc[n][v] = mfma16(vf, pl[n], acc[n][v]);
+        if constexpr (F16 && !TWICE) acc[n][v] = mfma16(vf, pl[n], acc[n][v]);
       }
     }
     if constexpr (MASKED) {
@@ -407,7 +424,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
     }
     __syncthreads();
     constexpr int PIECES = D / 4;  // 16-byte pieces of a row
-    for (int i = threadIdx.x; i < 16 * PIECES; i += 64 * FEW_WAVES) {
+    for (int i = threadIdx.x; i < (TWICE ? 8 : 16) * PIECES; i += 64 * FEW_WAVES) {
       const int r = i / PIECES, p = i % PIECES;
       const int rho = n * 16 + r;
       if (rho >= total_rows) continue;
@@ -421,7 +438,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
         const float mw = lds_ml[w][0][r];
         const float f = mw == NEG_INF ? 0.0f : exp2_hw(mw - top);
         const float lw = lds_ml[w][1][r];
-        const f32x4 ow = *reinterpret_cast<const f32x4*>(lds + w * (FEW_KEYS * ROW) + r * (4 * D) + ((p ^ r) & (D / 4 - 1)) * 16);
+        auto row_of = [&](int c) {
+          return *reinterpret_cast<const f32x4*>(lds + w * (FEW_KEYS * ROW) + c * (4 * D) + ((p ^ c) & (D / 4 - 1)) * 16);
+        };
+        f32x4 ow = row_of(r);
+        if constexpr (TWICE) ow += row_of(r + 8);
         // a wave whose scores were all NaN keeps maximum -inf and a NaN sum
         l += mw == NEG_INF ? (lw == lw ? 0.0f : lw) : f * lw;
         o += mw == NEG_INF && lw == lw ? f32x4{0, 0, 0, 0} : (mw == NEG_INF ? ow : f * ow);
@@ -928,8 +949,10 @@ template <int D, bool F16>
 void launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   if (s.nt != 0) {
     const dim3 grid(a.nsplit, a.kv_heads, a.batch);
-    if (s.nt == 1) kv4_few_kernel<D, 1, F16><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
-    else kv4_few_kernel<D, 2, F16><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
+    const int64_t total = static_cast<int64_t>(a.rows) * a.group;
+    if (total <= 8) kv4_few_kernel<D, 1, F16, true><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
+    else if (s.nt == 1) kv4_few_kernel<D, 1, F16, false><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
+    else kv4_few_kernel<D, 2, F16, false><<<grid, 64 * FEW_WAVES, 0, stream>>>(a);
   } else {
     const unsigned grid = static_cast<unsigned>(spr::ceil_div(s.groups * s.nsplit, 8 * RUN) * (8 * RUN));
     if (s.rb == 8) kv4_many_kernel<D, F16, 8><<<grid, 64 * MANY_WAVES, 0, stream>>>(a);

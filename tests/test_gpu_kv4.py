@@ -152,12 +152,13 @@ def _check_attention(got, lse, q, pages, table, lengths, counts, size, causal, s
     - a score is a sum of D exact products in fp32, D u sum|q k| at most, times the scale (2 u more);
       with the subtraction and the argument of exp2 in fp32 and exp2 good to 2^-22, a probability is off
       by e = (D + 6) u L + 2^-21 of itself, L the row's largest sum |q k| scale;
-    - bf16 calls round it once more, 2^-8; fp16 calls hold it in two terms, 2^-16;
+    - bf16 calls round it once more, 2^-8; fp16 calls hold it in two bf16 terms, cut off or rounded: what
+      the first leaves is below 2^-7 of it, what the second leaves below 2^-7 of that, 2^-14;
     - sums of n terms in fp32, n u of softmax |v| = A; numerator and denominator: twice e and n u;
     - the output is rounded once, half a step of its type."""
     b, hq, t, d = q.shape
     u = 2.0**-24
-    rounds, last = (2.0**-8, 2.0**-8) if dtype == "bf16" else (2.0**-16, 2.0**-11)
+    rounds, last = (2.0**-8, 2.0**-8) if dtype == "bf16" else (2.0**-14, 2.0**-11)
     for i in range(b):
         s = i if ids is None else ids[i]
         n = int(lengths[s])
