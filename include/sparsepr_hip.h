@@ -539,8 +539,8 @@ int spr_kv4_load(const uint8_t* pages, int32_t num_pages, int32_t kv_heads, int3
                  int32_t rows, hipStream_t stream);
 /* Page calls.  Each checks on the device all it is asked for and then happens whole or not at all;
  * new pages are the lowest free ones, ascending, in the order of the named sequences (at most 2048 a
- * call).  status int32 [1] (nullable) gets, unless it holds one already, 1 a sequence outside the
- * table, 2 a sequence named twice, 3 a negative count or a range outside the sequence's pages, 4 more
+ * call).  status int32 [1] (nullable) gets, unless it holds one already, the lowest that applies of 1 a
+ * sequence outside the table, 2 a sequence named twice, 3 a negative count or a range outside the sequence's pages, 4 more
  * tokens than the table's row holds, 5 not enough free pages, 6 a fork onto a sequence that holds
  * tokens, 7 a length outside the table or a table entry outside the pool. */
 size_t spr_kv4_pages_workspace(int32_t num_pages);
@@ -552,7 +552,7 @@ int spr_kv4_reserve(int32_t* block_table, int32_t* lengths, int32_t* ref_count, 
                     hipStream_t stream);
 /* Pages [first_pages[i], first_pages[i] + page_counts[i]) of sequence seq_ids[i] are given back
  * (nullable: 0, and all from there on, as any negative count says), the pages behind close up, the
- * length loses their tokens. */
+ * length loses their tokens.  Up to 64 sequences need no workspace. */
 int spr_kv4_free(int32_t* block_table, int32_t* lengths, int32_t* ref_count, const int32_t* seq_ids,
                  const int32_t* first_pages, const int32_t* page_counts, int32_t n, int32_t sequences, int32_t wide,
                  int32_t page_size, int32_t num_pages, int32_t* status, void* workspace, size_t workspace_bytes,

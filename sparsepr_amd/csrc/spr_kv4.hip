@@ -230,9 +230,6 @@ __device__ __forceinline__ int block_scan(int v, int* scratch, int& all) {
   return before + incl - v;
 }
 
-// Whether any thread of the workgroup says yes.
-__device__ __forceinline__ bool block_any(bool yes) { return __syncthreads_or(yes ? 1 : 0) != 0; }
-
 // The lowest `want` pages with FREE (ref_count <= 0) or held (> 0) among [first, last), ascending, to
 // `list`; returns how many there are (at most want).  Tiles of four pages a thread; stops at the tile
 // that has the last one.
@@ -273,17 +270,40 @@ __device__ __forceinline__ int entry_of(const int32_t* sums, int n, int i) {
   return lo;
 }
 
+// What the workgroup found wrong: every thread's findings (bit c for status c) together, and of them
+// the lowest status.  `found` is a word of LDS that holds 0 before and after.
+__device__ __forceinline__ int lowest_code(uint32_t mine, uint32_t* found) {
+  if (mine != 0) atomicOr(found, mine);
+  __syncthreads();
+  const uint32_t all = *found;
+  __syncthreads();
+  if (threadIdx.x == 0) *found = 0;
+  return all != 0 ? __builtin_ctz(all) : 0;
+}
+
 __device__ __forceinline__ void report(int32_t* status, int code) {
   if (status != nullptr && threadIdx.x == 0 && status[0] == 0) status[0] = code;
 }
 
-// Whether ids[0, n) (in LDS) repeats itself; every thread of the workgroup gets the answer.
-__device__ bool any_repeated(const int32_t* ids, int n) {
-  bool again = false;
-  for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
-    for (int j = 0; j < i; ++j) again |= ids[j] == ids[i];
+// Whether a[j] of [0, upto) is `id` (LDS).
+__device__ __forceinline__ bool any_is(const int32_t* a, int upto, int32_t id) {
+  bool is = false;
+  for (int j = 0; j < upto; ++j) is |= a[j] == id;
+  return is;
+}
+
+// Whether a page of one of the n sequences (ids in LDS) lies outside the pool: a wave a sequence.
+__device__ __forceinline__ bool outside_pool(const int32_t* table, const int32_t* lengths, const int32_t* ids, int n,
+                                             int32_t wide, int log_s, int32_t num_pages) {
+  bool outside = false;
+  for (int i = threadIdx.x >> 6; i < n; i += PLAN_THREADS / 64) {
+    const int64_t held = (static_cast<int64_t>(lengths[ids[i]]) + (1 << log_s) - 1) >> log_s;
+    for (int64_t j = threadIdx.x & 63; j < held; j += 64) {
+      const int32_t p = table[static_cast<int64_t>(ids[i]) * wide + j];
+      outside |= p < 0 || p >= num_pages;
+    }
   }
-  return block_any(again);
+  return outside;
 }
 
 // sums[i] = need[0] + .. + need[i - 1] over n entries in LDS, in place of need (n + 1 words); false if
@@ -330,8 +350,10 @@ __global__ __launch_bounds__(PLAN_THREADS) void kv4_reserve_kernel(int32_t* __re
                                                                    int32_t* __restrict__ list) {
   __shared__ int32_t ids[MAX_NAMED], sums[MAX_NAMED + 1], olds[MAX_NAMED], news[MAX_NAMED];
   __shared__ int scratch[PLAN_THREADS / 64];
+  __shared__ uint32_t found;
   const int64_t room = static_cast<int64_t>(wide) << log_s;
-  bool bad_id = false, bad_count = false, bad_length = false, full = false;
+  if (threadIdx.x == 0) found = 0;
+  uint32_t wrong = 0;
   for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
     const int32_t id = seq_ids != nullptr ? seq_ids[i] : i;
     ids[i] = id;
@@ -339,26 +361,27 @@ __global__ __launch_bounds__(PLAN_THREADS) void kv4_reserve_kernel(int32_t* __re
     news[i] = 0;
     sums[i] = 0;
     if (id < 0 || id >= sequences) {
-      bad_id = true;
+      wrong |= 1u << KV4_BAD_SEQUENCE;
       continue;
     }
     // all is read before anything is written: counts may be the lengths themselves
     const int32_t old = lengths[id], more = counts[i];
-    bad_length |= old < 0 || old > room;
-    bad_count |= more < 0;
-    full |= static_cast<int64_t>(old) + more > room;
+    if (more < 0) wrong |= 1u << KV4_BAD_COUNT;
+    if (old < 0 || old > room) wrong |= 1u << KV4_BAD_LENGTH;
+    else if (static_cast<int64_t>(old) + more > room) wrong |= 1u << KV4_TABLE_FULL;
     olds[i] = old;
     news[i] = static_cast<int32_t>(min(static_cast<int64_t>(old) + more, room));
     sums[i] = static_cast<int32_t>(pages_for(static_cast<int64_t>(old) + more, log_s) - pages_for(old, log_s));
   }
   __syncthreads();
-  int code = KV4_OK, total = 0;
-  if (block_any(bad_id)) code = KV4_BAD_SEQUENCE;
-  else if (any_repeated(ids, n)) code = KV4_REPEATED;
-  else if (block_any(bad_count)) code = KV4_BAD_COUNT;
-  else if (block_any(bad_length)) code = KV4_BAD_LENGTH;
-  else if (block_any(full)) code = KV4_TABLE_FULL;
-  else if (!sum_needs(sums, n, num_pages, scratch, total)) code = KV4_NO_PAGES;
+  if (seq_ids != nullptr) {
+    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
+      if (any_is(ids, i, ids[i])) wrong |= 1u << KV4_REPEATED;
+    }
+  }
+  int code = lowest_code(wrong, &found), total = 0;
+  if (code != KV4_OK) {
+  } else if (!sum_needs(sums, n, num_pages, scratch, total)) code = KV4_NO_PAGES;
   else if (find_pages<true>(refs, 0, num_pages, total, list, scratch) < total) code = KV4_NO_PAGES;
   if (code != KV4_OK) {
     report(status, code);
@@ -433,38 +456,32 @@ __global__ __launch_bounds__(PLAN_THREADS) void kv4_free_check_kernel(int32_t* t
                                                                       PlanHeader* __restrict__ plan,
                                                                       int32_t* __restrict__ status) {
   __shared__ int32_t ids[MAX_NAMED];
+  __shared__ uint32_t found;
   const int64_t room = static_cast<int64_t>(wide) << log_s;
-  bool bad_id = false, bad_count = false, bad_length = false;
+  if (threadIdx.x == 0) found = 0;
+  uint32_t wrong = 0;
   for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
     const int32_t id = seq_ids[i];
     ids[i] = id;
     if (id < 0 || id >= sequences) {
-      bad_id = true;
+      wrong |= 1u << KV4_BAD_SEQUENCE;
       continue;
     }
     const int32_t len = lengths[id];
-    bad_length |= len < 0 || len > room;
+    if (len < 0 || len > room) wrong |= 1u << KV4_BAD_LENGTH;
     const FreeRange f = free_range(len, firsts, page_counts, i, log_s);
-    bad_count |= f.first < 0 || f.first > f.held || f.count < 0 || f.first + f.count > f.held;
+    if (f.first < 0 || f.first > f.held || f.count < 0 || f.first + f.count > f.held) wrong |= 1u << KV4_BAD_COUNT;
   }
   __syncthreads();
-  int code = KV4_OK;
-  if (block_any(bad_id)) code = KV4_BAD_SEQUENCE;
-  else if (any_repeated(ids, n)) code = KV4_REPEATED;
-  else if (block_any(bad_length)) code = KV4_BAD_LENGTH;
-  else if (block_any(bad_count)) code = KV4_BAD_COUNT;
-  if (code == KV4_OK) {
-    bool outside = false;
-    for (int i = threadIdx.x >> 6; i < n; i += PLAN_THREADS / 64) {  // a wave a row
-      const int64_t held = pages_for(lengths[ids[i]], log_s);
-      for (int64_t j = threadIdx.x & 63; j < held; j += 64) {
-        const int32_t p = table[static_cast<int64_t>(ids[i]) * wide + j];
-        outside |= p < 0 || p >= num_pages;
-      }
-    }
-    if (block_any(outside)) code = KV4_BAD_LENGTH;
+  for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
+    if (any_is(ids, i, ids[i])) wrong |= 1u << KV4_REPEATED;
   }
-  if (threadIdx.x == 0) plan->ok = code == KV4_OK ? 1 : 0;
+  int code = lowest_code(wrong, &found);
+  if (code == KV4_OK) {
+    __syncthreads();  // `found` is 0 again
+    code = lowest_code(outside_pool(table, lengths, ids, n, wide, log_s, num_pages) ? 1u << KV4_BAD_LENGTH : 0, &found);
+  }
+  if (plan != nullptr && threadIdx.x == 0) plan->ok = code == KV4_OK ? 1 : 0;
   report(status, code);
   if (n <= FREE_HERE && code == KV4_OK) {
     for (int i = threadIdx.x >> 6; i < n; i += PLAN_THREADS / 64) {
@@ -499,47 +516,38 @@ __global__ __launch_bounds__(PLAN_THREADS) void kv4_fork_plan_kernel(const int32
                                                                      int32_t* __restrict__ status) {
   __shared__ int32_t to[MAX_NAMED], from[MAX_NAMED], sums[MAX_NAMED + 1];
   __shared__ int scratch[PLAN_THREADS / 64];
+  __shared__ uint32_t found;
   const int64_t room = static_cast<int64_t>(wide) << log_s;
-  bool bad_id = false, bad_length = false, holds = false;
+  if (threadIdx.x == 0) found = 0;
+  uint32_t wrong = 0;
   for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
     const int32_t s = src[i], d = dst[i];
     from[i] = s;
     to[i] = d;
     sums[i] = 0;
     if (s < 0 || s >= sequences || d < 0 || d >= sequences) {
-      bad_id = true;
+      wrong |= 1u << KV4_BAD_SEQUENCE;
       continue;
     }
     const int32_t len = lengths[s];
-    bad_length |= len < 0 || len > room;
-    holds |= lengths[d] != 0;
+    if (len < 0 || len > room) wrong |= 1u << KV4_BAD_LENGTH;
+    if (lengths[d] != 0) wrong |= 1u << KV4_NOT_EMPTY;
     const int64_t every = pages_for(len, log_s), full = share != 0 ? (len >> log_s) : 0;
     sums[i] = static_cast<int32_t>(every - full);
   }
   __syncthreads();
-  int code = KV4_OK, total = 0;
-  if (block_any(bad_id)) code = KV4_BAD_SEQUENCE;
-  else if (any_repeated(to, n)) code = KV4_REPEATED;
-  else if (block_any(bad_length)) code = KV4_BAD_LENGTH;
-  else if (block_any(holds)) code = KV4_NOT_EMPTY;
-  if (code == KV4_OK) {
-    bool both = false;  // a sequence that is written and read (an empty one: nothing else can be both)
-    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
-      for (int j = 0; j < n; ++j) both |= from[j] == to[i];
-    }
-    bool outside = false;
-    for (int i = threadIdx.x >> 6; i < n; i += PLAN_THREADS / 64) {
-      const int64_t held = pages_for(lengths[from[i]], log_s);
-      for (int64_t j = threadIdx.x & 63; j < held; j += 64) {
-        const int32_t p = table[static_cast<int64_t>(from[i]) * wide + j];
-        outside |= p < 0 || p >= num_pages;
-      }
-    }
-    if (block_any(both)) code = KV4_REPEATED;
-    else if (block_any(outside)) code = KV4_BAD_LENGTH;
-    else if (!sum_needs(sums, n, num_pages, scratch, total)) code = KV4_NO_PAGES;
-    else if (find_pages<true>(refs, 0, num_pages, total, list, scratch) < total) code = KV4_NO_PAGES;
+  // one destination twice, or (an empty one: nothing else can be both) one that is a source too
+  for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
+    if (any_is(to, i, to[i]) || any_is(from, n, to[i])) wrong |= 1u << KV4_REPEATED;
   }
+  int code = lowest_code(wrong, &found), total = 0;
+  if (code == KV4_OK) {
+    __syncthreads();  // `found` is 0 again
+    code = lowest_code(outside_pool(table, lengths, from, n, wide, log_s, num_pages) ? 1u << KV4_BAD_LENGTH : 0, &found);
+  }
+  if (code != KV4_OK) {
+  } else if (!sum_needs(sums, n, num_pages, scratch, total)) code = KV4_NO_PAGES;
+  else if (find_pages<true>(refs, 0, num_pages, total, list, scratch) < total) code = KV4_NO_PAGES;
   if (code == KV4_OK) {
     for (int i = threadIdx.x; i <= n; i += PLAN_THREADS) sums_out[i] = sums[i];
   }
@@ -818,8 +826,10 @@ extern "C" int spr_kv4_free(int32_t* block_table, int32_t* lengths, int32_t* ref
   if (int st = check_table(what, sequences, wide, page_size)) return st;
   if (int st = check_named(what, n)) return st;
   if (n == 0) return SPR_OK;
-  if (int st = check_space(what, workspace, workspace_bytes, num_pages)) return st;
-  PlanHeader* plan = static_cast<PlanHeader*>(workspace);
+  if (n > FREE_HERE) {
+    if (int st = check_space(what, workspace, workspace_bytes, num_pages)) return st;
+  }
+  PlanHeader* plan = n > FREE_HERE ? static_cast<PlanHeader*>(workspace) : nullptr;
   const int log_s = log2_of(page_size);
   kv4_free_check_kernel<<<1, PLAN_THREADS, 0, stream>>>(block_table, lengths, ref_count, seq_ids, first_pages,
                                                         page_counts, n, sequences, wide, log_s, num_pages, plan,

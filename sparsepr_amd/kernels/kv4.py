@@ -256,10 +256,11 @@ def kv4_free(block_table: torch.Tensor, lengths: torch.Tensor, ref_count: torch.
     for t, name in ((first_pages, "first_pages"), (page_counts, "page_counts")):
         if t is not None:
             _int32(t, n, name, what)
-    ws = _lib.workspace(_lib.query("spr_kv4_pages_workspace", ref_count.shape[0]), dev)
+    # up to 64 sequences are one launch, which hands nothing on
+    ws = _lib.workspace(_lib.query("spr_kv4_pages_workspace", ref_count.shape[0]), dev) if n > 64 else None
     _lib.launch("spr_kv4_free", dev, block_table.data_ptr(), lengths.data_ptr(), ref_count.data_ptr(),
                 seq_ids.data_ptr(), _lib.ptr(first_pages), _lib.ptr(page_counts), n, sequences, wide, page_size,
-                ref_count.shape[0], _lib.ptr(status), ws.data_ptr(), ws.numel())
+                ref_count.shape[0], _lib.ptr(status), _lib.ptr(ws), 0 if ws is None else ws.numel())
 
 
 def kv4_fork(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, ref_count: torch.Tensor,

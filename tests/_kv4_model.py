@@ -147,12 +147,10 @@ class Pages:
         """(status, [(from, to), ..] page copies)"""
         if any(i < 0 or i >= len(self.lengths) for i in src + dst):
             return 1, []
-        if len(set(dst)) < len(dst):
+        if len(set(dst)) < len(dst) or set(src) & set(dst):
             return 2, []
         if any(self.lengths[i] for i in dst):
             return 6, []
-        if set(src) & set(dst):
-            return 2, []
         own = [[j for j in range(self._pages(self.lengths[s])) if not share or (j + 1) * self.size > self.lengths[s]]
                for s in src]
         free = self._free()

@@ -82,7 +82,7 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
     assert lib.spr_kv4_reserve(16, 16, 16, 16, 16, 1, 2, 4, 64, 8, 16, None, None, 0, None) == 3
     assert lib.spr_kv4_free(16, 16, 16, 16, None, None, 5000, 2, 4, 64, 8, None, 16, 1 << 20, None) == 1
     assert "5000 sequences in one call" in lib.spr_last_error().decode()
-    assert lib.spr_kv4_free(16, 16, 16, 16, None, None, 1, 2, 4, 64, 8, None, 16, 16, None) == 3
+    assert lib.spr_kv4_free(16, 16, 16, 16, None, None, 65, 2, 4, 64, 8, None, 16, 16, None) == 3
     assert lib.spr_kv4_fork(16, 24, 0, 1, 16, 16, 16, 16, 16, 1, 2, 4, 64, 8, 1, None, 16, 1 << 20, None) == 1
     assert lib.spr_kv4_fork(16, 32, 64, 2, 16, 16, 16, 16, 16, 1, 2, 4, 64, 8, 1, None, 16, 1 << 20, None) == 1
     assert lib.spr_kv4_compact(16, 32, 0, 1, 16, 16, 2, 4, 0, 16, 16, 1 << 20, None) == 1
