@@ -142,7 +142,7 @@ def kv4_load(pages: torch.Tensor, block_table: torch.Tensor, starts: torch.Tenso
     sequences, wide = _check_table(block_table, what)
     _check_entries(b, sequences, seq_ids, counts, what)
     _int32(starts, b, "starts", what)
-    k = torch.empty((b, h, rows, head_dim), dtype=dtype, device=dev)
+    k = pages.new_empty((b, h, rows, head_dim), dtype=dtype)
     v = torch.empty_like(k)
     if k.numel() > 0:
         _lib.launch("spr_kv4_load", dev, pages.data_ptr(), pages.shape[0], h, size, head_dim, block_table.data_ptr(),
@@ -176,8 +176,8 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     _int32(lengths, sequences, "lengths", what)
     longest = wide * size if max_length is None else min(int(max_length), wide * size)
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(d)
-    out = torch.empty((b, h, t, d), dtype=q.dtype, device=dev)
-    lse = torch.empty((b, h, t), dtype=torch.float32, device=dev) if return_lse else None
+    out = q.new_empty((b, h, t, d))
+    lse = q.new_empty((b, h, t), dtype=torch.float32) if return_lse else None
     if out.numel() > 0:
         q, *strides = _by_rows(q)
         need = _lib.query("spr_kv4_attention_workspace", b, h, hk, t, d, longest)
@@ -235,7 +235,7 @@ def kv4_reserve(block_table: torch.Tensor, lengths: torch.Tensor, ref_count: tor
     sequences, wide = _check_metadata(block_table, lengths, ref_count, page_size, status, what)
     n = _named(counts, "counts", what)
     _check_entries(n, sequences, seq_ids, None, what)
-    starts = torch.empty(n, dtype=torch.int32, device=dev)
+    starts = counts.new_empty(n)
     ws = _lib.workspace(_lib.query("spr_kv4_pages_workspace", ref_count.shape[0]), dev)
     _lib.launch("spr_kv4_reserve", dev, block_table.data_ptr(), lengths.data_ptr(), ref_count.data_ptr(),
                 counts.data_ptr(), _lib.ptr(seq_ids), n, sequences, wide, page_size, ref_count.shape[0],
@@ -289,7 +289,7 @@ def kv4_compact(pages: torch.Tensor, block_table: torch.Tensor, ref_count: torch
     dev = _lib.require_gpu(pages, block_table, ref_count, what=what)
     sequences, wide = _check_metadata(block_table, None, ref_count, PAGE_SIZES[0], None, what)
     page, layer, layers = _layers(pages, ref_count.shape[0], what)
-    live = torch.empty((), dtype=torch.int32, device=dev)
+    live = ref_count.new_empty(())
     ws = _lib.workspace(_lib.query("spr_kv4_pages_workspace", ref_count.shape[0]), dev)
     _lib.launch("spr_kv4_compact", dev, pages.data_ptr(), page, layer, layers, block_table.data_ptr(),
                 ref_count.data_ptr(), sequences, wide, ref_count.shape[0], live.data_ptr(), ws.data_ptr(), ws.numel())
