@@ -516,7 +516,7 @@ int spr_project_rows_ex(const float* x, const float* factor, const float* div, i
  * (sign, then 0, 0.5, 1, 1.5, 2, 3, 4, 6), the even dim in the low half of a byte; scale byte s is
  * 2^(s - 127) for 32 dims of a token, 255 a NaN.  block_table int32 [sequences, wide] names a
  * sequence's pages (-1: none), lengths int32 [sequences] its tokens, ref_count int32 [num_pages] how
- * many sequences hold a page (0: free); wide * page_size <= 2^31 - 1.  seq_ids int32 [batch]
+ * many sequences hold a page (0: free); wide * page_size <= 2^30.  seq_ids int32 [batch]
  * (nullable: 0, 1, ..) names the sequences of a call. */
 int64_t spr_kv4_page_bytes(int32_t kv_heads, int32_t page_size, int32_t d);
 /* K and V rows into the cache: row t < counts[b] (nullable: rows) of entry b becomes token

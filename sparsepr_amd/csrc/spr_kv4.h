@@ -13,6 +13,8 @@
 namespace spr {
 
 constexpr int KV4_GROUP = 32;  // dims that share a scale
+// Tokens a row of the block table may stand for: a token's place plus a chunk stays in 32 bits.
+constexpr int64_t KV4_MOST_TOKENS = int64_t{1} << 30;
 
 // Bytes of one head's part of a page.
 __host__ __device__ __forceinline__ int64_t kv4_head_bytes(int32_t page_size, int32_t d) {

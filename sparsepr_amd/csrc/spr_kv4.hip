@@ -694,8 +694,8 @@ int check_pool(const char* what, int32_t page_size, int32_t num_pages) {
 
 int check_table(const char* what, int32_t sequences, int32_t wide, int32_t page_size) {
   SPR_REQUIRE(sequences >= 1 && wide >= 1, "%s: a block table of %d x %d", what, sequences, wide);
-  SPR_REQUIRE(static_cast<int64_t>(wide) * page_size <= INT32_MAX, "%s: %d pages of %d tokens a sequence pass 2^31 tokens",
-              what, wide, page_size);
+  SPR_REQUIRE(static_cast<int64_t>(wide) * page_size <= spr::KV4_MOST_TOKENS,
+              "%s: %d pages of %d tokens a sequence pass 2^30 tokens", what, wide, page_size);
   return SPR_OK;
 }
 

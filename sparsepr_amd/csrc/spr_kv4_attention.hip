@@ -1004,7 +1004,7 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
   SPR_REQUIRE(dtype == 0 || dtype == 1, "%s: dtype code %d (0 bf16, 1 fp16)", what, dtype);
   SPR_REQUIRE(d == 64 || d == 128, "%s: head dim %d not supported (64, 128)", what, d);
   SPR_REQUIRE(spr::kv4_page_size_ok(page_size), "%s: page size %d (32, 64, 128 or 256)", what, page_size);
-  SPR_REQUIRE(num_pages >= 1 && sequences >= 1 && wide >= 1 && static_cast<int64_t>(wide) * page_size <= INT32_MAX,
+  SPR_REQUIRE(num_pages >= 1 && sequences >= 1 && wide >= 1 && static_cast<int64_t>(wide) * page_size <= spr::KV4_MOST_TOKENS,
               "%s: %d pages, a block table of %d x %d", what, num_pages, sequences, wide);
   SPR_REQUIRE(batch >= 0 && batch <= 65535 && rows >= 0 && kv_heads >= 1 && kv_heads <= 65535 && heads >= 1 && heads % kv_heads == 0,
               "%s: batch %d, rows %d, %d query heads on %d kv heads", what, batch, rows, heads, kv_heads);

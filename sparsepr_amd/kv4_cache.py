@@ -13,7 +13,9 @@ and kv head (136 for D = 128, against 512 in bf16):
     cache.fork([0], [1])                                   # a second branch on the same pages
     cache.check()                                          # the one call that synchronises
 
-No call but `check` waits for the GPU; each runs on torch's current stream of the cache's device.
+No call but `check` waits for the GPU; each runs on torch's current stream of the cache's device (calls
+on one cache from several streams are the caller's to order).  Lists become device tensors, which a
+captured graph cannot hold: pass int32 tensors there.
 The calls that change pages happen whole or not at all (kernels/kv4.py)."""
 
 from __future__ import annotations
@@ -26,15 +28,15 @@ from .kernels import kv4
 class KV4Cache:
     def __init__(self, num_pages: int, num_kv_heads: int, head_dim: int, max_sequences: int, *, page_size: int = 64,
                  max_pages: int | None = None, layers: int = 1, device: torch.device | str | None = None):
-        """`max_pages` is what one sequence can hold (default: all pages)."""
+        """`max_pages` is what one sequence can hold (default: all pages, at most 2^30 tokens)."""
         width = kv4.kv4_page_bytes(page_size, head_dim)
-        wide = num_pages if max_pages is None else max_pages
+        wide = min(num_pages, 2**30 // page_size) if max_pages is None else max_pages
         for name, n in (("num_pages", num_pages), ("num_kv_heads", num_kv_heads), ("max_sequences", max_sequences),
                         ("max_pages", wide), ("layers", layers)):
             if n < 1:
                 raise RuntimeError(f"4-bit cache: {name} must be at least 1, got {n}")
-        if wide * page_size >= 2**31:
-            raise RuntimeError(f"4-bit cache: {wide} pages of {page_size} tokens pass 2^31 tokens a sequence")
+        if wide * page_size > 2**30:
+            raise RuntimeError(f"4-bit cache: {wide} pages of {page_size} tokens pass 2^30 tokens a sequence")
         dev = torch.device("cuda" if device is None else device)
         self.page_size, self.head_dim = page_size, head_dim
         self.pages = torch.zeros((layers, num_pages, num_kv_heads, width), dtype=torch.uint8, device=dev)

@@ -673,3 +673,39 @@ def test_a_window_that_slides_over_a_video(dev):
             cache.free([1], first_pages=[1], page_counts=[over])
             kept = [np.delete(x, np.s_[size:size * (1 + over)], 2) for x in kept]
     cache.check()
+
+
+def test_captured_attention_with_shares_of_the_keys(dev):
+    """Calls whose keys are dealt in shares (workspaces, merges), of each kernel: two graphs over one
+    cache, replayed in turns with eager calls between, as the sequences grow."""
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    g = torch.Generator(device=dev).manual_seed(7)
+    h, d = 2, 64
+    cache = KV4Cache(220, h, d, 2, page_size=64, max_pages=110, device=dev)
+    k, v = torch.randn((2, 2, h, 6000, d), generator=g, device=dev).to(torch.bfloat16)
+    cache.append(k, v, counts=[6000, 1500])
+    qs = [torch.randn((2, 4, t, d), generator=g, device=dev).to(torch.bfloat16) for t in (1, 14, 30, 60, 200)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for q in qs:
+            cache.attend(q, causal=True, return_lse=True)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for part in (qs[:3], qs[3:]):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [cache.attend(q, causal=True, return_lse=True) for q in part]
+        graphs.append((graph, part, outs))
+    for step in range(4):
+        cache.append(k[:, :, :200], v[:, :, :200])
+        for graph, part, outs in graphs:
+            for q in part:
+                q.copy_(torch.randn(q.shape, generator=g, device=dev))
+            want = [cache.attend(q, causal=True, return_lse=True) for q in part]
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(outs, want):
+                assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]), step
+    cache.check()

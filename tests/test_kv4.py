@@ -54,7 +54,7 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
 
     for kw, text in [
         (dict(dtype=2), "dtype code 2"), (dict(d=96), "head dim 96"), (dict(page_size=48), "page size 48"),
-        (dict(page_size=512), "page size 512"), (dict(num_pages=0), "0 pages"), (dict(wide=2**26), "block table"),
+        (dict(page_size=512), "page size 512"), (dict(num_pages=0), "0 pages"), (dict(wide=2**24 + 1), "block table"),
         (dict(heads=3), "3 query heads on 2"), (dict(scale=0.0), "scale must be positive"),
         (dict(scale=float("inf")), "scale must be positive"), (dict(scale=float("nan")), "scale must be positive"), (dict(scale=2e38), "at most 1e38"), (dict(heads=70000, kv_heads=70000), "on 70000 kv heads"),
         (dict(q=8), "16-byte aligned"), (dict(q_t=100), "multiples of 8"), (dict(batch=70000), "batch 70000"),
@@ -114,7 +114,7 @@ def test_python_refuses_cpu_tensors_and_bad_geometry():
         with pytest.raises(RuntimeError, match=text):
             kv4.kv4_page_bytes(*args)
     for kw, text in [(dict(num_pages=0), "num_pages"), (dict(layers=0), "layers"), (dict(page_size=100), "page size"),
-                     (dict(max_pages=2**26), "2\\^31 tokens")]:
+                     (dict(max_pages=2**26), "2\\^30 tokens")]:
         args = dict(num_pages=4, num_kv_heads=1, head_dim=64, max_sequences=1, device="cpu") | kw
         with pytest.raises(RuntimeError, match=text):
             KV4Cache(**args)
