@@ -495,8 +495,9 @@ __device__ __forceinline__ float sum_xor32(float x) {
 //
 // A chunk is brought from its codes to bf16 once for all eight waves: a thread turns 32 values of one
 // row (16 bytes of codes, one scale) into 64 bytes of a row-major LDS tile, 16 conversions and 4 writes.
-// Two tiles each for K and V: the codes of chunk x + 2 are loaded and those of x + 1 written during
-// chunk x, with one barrier a chunk.
+// Two tiles each for K and V: the codes of chunk x + 3 are loaded and those of x + 1 written during
+// chunk x, with one barrier a chunk.  Two chunks a turn of the loop, so that tiles and registers in
+// flight are the same ones each time, by constant addresses (frame 5.13 -> 4.96 ms).
 // Scores and output are S^T = K Q^T and O^T += V^T P^T by 32x32x16 MFMA with a lane owning one query
 // row; V^T comes from the transposing read, P from the accumulator in the same order of keys.  S of the
 // next 32 keys is computed beside the exponentials of the current ones.
@@ -507,7 +508,7 @@ __device__ __forceinline__ float sum_xor32(float x) {
 // every bank once (the conversion's writes take 1.5 times their least cycles).
 //
 // Bound by neither unit alone: 3600 rows of 24 heads against 118,800 tokens of 128 dims, 5.26 TFLOP,
-// take 5.0 to 5.2 ms, 1010 to 1050 TFLOP/s, where a library product of 8192^3 reaches 1129 on this card;
+// take 4.9 to 5.1 ms, 1030 to 1070 TFLOP/s, where a library product of 8192^3 reaches 1129 on this card;
 // the clock is down to 1.8 GHz, the MFMA pipe is busy half of the time, VALU issue 55 %.  128 rows take
 // 0.23 ms (815 TFLOP/s): half the products to each conversion.  Row blocks by rows of the call, at
 // 24 x 118,800 x 128: 33 to 64 rows 156 us with RB 2 and 200 with RB 4; 17 to 32 rows 150 us with RB 2 and
@@ -524,7 +525,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
   constexpr int GROUPS = D / spr::KV4_GROUP;      // scales of a row
   constexpr int ITEMS = D / 64;                   // D = 128: a thread converts K and V, D = 64: K or V
   constexpr int CONV = MANY_KEYS * GROUPS;        // items of K
-  __shared__ __align__(1024) uint8_t tiles_lds[2][2][TILE];  // [buffer][K, V]
+  __shared__ __align__(1024) uint8_t tiles_lds[2][2][TILE];  // [K, V][chunk mod 2]
   __shared__ uint32_t v_bytes[2][MANY_KEYS];                 // the V scale bytes of every key
   __shared__ float merge_ml[MANY_WAVES][64][2];
 
@@ -578,14 +579,16 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
   const int ci = threadIdx.x & (CONV - 1);
   const int cr = (ci & 15) + 16 * (ci / (16 * GROUPS)), cg = (ci >> 4) & (GROUPS - 1);
   const int first_v = ITEMS == 1 ? threadIdx.x / CONV : 0;  // what item 0 is: K or V
-  u32x4 code[ITEMS];
-  uint32_t byte[ITEMS];
+  u32x4 codes[2][ITEMS];  // of the chunks mod 2 in flight
+  uint32_t bytes[2][ITEMS];
   int32_t next_page = -1;
   auto look = [&](int c) {  // the page of this thread's row of chunk c
     const int32_t key = (c0 + c) * MANY_KEYS + cr;
     next_page = key < most ? row_table[key >> a.log_s] : -1;
   };
-  auto fetch = [&](int c) {
+  auto fetch = [&](int c, auto par) {  // par: c mod 2
+    auto& code = codes[decltype(par)::value];
+    auto& byte = bytes[decltype(par)::value];
     const int32_t key = (c0 + c) * MANY_KEYS + cr;
     const bool ok = next_page >= 0 && next_page < a.num_pages;
     const uint8_t* from = a.pages + (ok ? next_page : 0) * a.page_stride + head;
@@ -603,12 +606,14 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
   };
   const int swz_k = D == 128 ? (cr & 15) : ((cr >> 1) & 7);
   const int swz_v = D == 128 ? 4 * (cr & 3) + ((cr >> 2) & 3) : 4 * ((cr >> 1) & 1) + ((cr >> 2) & 3);
-  auto stash = [&](int c) {
+  auto stash = [&](int c, auto par) {
+    auto& code = codes[decltype(par)::value];
+    auto& byte = bytes[decltype(par)::value];
     const int32_t end = (c0 + c + 1) * MANY_KEYS;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int v = i + first_v;
-      uint8_t* to = tiles_lds[c & 1][v] + cr * ROW;
+      uint8_t* to = tiles_lds[v][decltype(par)::value] + cr * ROW;
       const int x = v != 0 ? swz_v : swz_k;
       // a chunk that some row does not see whole keeps NaN V scales out of the products (0 * NaN); they
       // are put in row by row
@@ -616,7 +621,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
       const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(to + (((4 * cg + j) ^ x) << 4)) = spr::kv4_eight(w[j], sc);
-      if (v != 0) reinterpret_cast<uint8_t*>(&v_bytes[c & 1][cr])[cg] = static_cast<uint8_t>(byte[i]);
+      if (v != 0) reinterpret_cast<uint8_t*>(&v_bytes[decltype(par)::value][cr])[cg] = static_cast<uint8_t>(byte[i]);
     }
   };
 
@@ -739,25 +744,29 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
   if (nch > 0) {
     constexpr std::true_type yes{};
     constexpr std::false_type no{};
-    look(0), fetch(0), look(1);
-    stash(0);
-    fetch(1), look(2);
+    constexpr std::integral_constant<int, 0> even{};
+    constexpr std::integral_constant<int, 1> odd{};
+    look(0), fetch(0, even), look(1);
+    fetch(1, odd), look(2);
+    stash(0, even);
+    fetch(2, even), look(3);
     // the two waves of a SIMD (w and w + 4) convert at opposite ends of a chunk: one's conversions run
-    // beside the other's products (frame of 3600 rows 5.30 -> 5.24 ms)
-    auto refill = [&](int x) {
+    // beside the other's products (frame 5.30 -> 5.24 ms)
+    auto refill = [&](int x, auto par) {  // par: (x + 1) mod 2
       if (x + 1 < nch) {
-        stash(x + 1);
-        fetch(x + 2);
-        look(x + 3);
+        stash(x + 1, par);
+        fetch(x + 3, par);
+        look(x + 4);
       }
     };
     f32x16 s[2];
-    for (int x = 0; x < nch; ++x) {
+    auto chunk = [&](int x, auto par) {  // par: (x + 1) mod 2
       spr::lds_barrier();  // chunk x is written; nobody reads chunk x - 1 any more
-      const uint8_t *kt = tiles_lds[x & 1][0], *vt = tiles_lds[x & 1][1];
+      constexpr int BUF = 1 - decltype(par)::value;
+      const uint8_t *kt = tiles_lds[0][BUF], *vt = tiles_lds[1][BUF];
       const int32_t key = (c0 + x) * MANY_KEYS + part * (32 * HALVES);
       const int h0 = part * HALVES;
-      if (wave >= 4) refill(x);
+      if (wave >= 4) refill(x, par);
       if (wave_live) {
         step(yes, no, s[0], kt, h0, s[1], vt, h0);
 #pragma unroll
@@ -768,7 +777,11 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
         }
         put_nan(x);
       }
-      if (wave < 4) refill(x);
+      if (wave < 4) refill(x, par);
+    };
+    for (int x = 0; x < nch; x += 2) {
+      chunk(x, odd);
+      if (x + 1 < nch) chunk(x + 1, even);
     }
   }
 
