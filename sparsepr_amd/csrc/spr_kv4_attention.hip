@@ -212,7 +212,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4;
-  const int hk = blockIdx.y, b = blockIdx.z, split = blockIdx.x;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  // the shares turn from head to head: workgroup i runs on XCD i mod 8, so with 2, 4 or 8 shares every
+  // short sequence's only one would be on the same XCDs (48 ragged sequences in 8 shares 67 us)
+  const int split = (blockIdx.x + blockIdx.y + blockIdx.z) % a.nsplit;
   const int total_rows = a.rows * a.group;
   const Span sp = span_of(a, b);
   const Deal deal = deal_of(a, most_of(a, sp, 0));
@@ -251,7 +254,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
   }
 
   const int64_t head = static_cast<int64_t>(hk) * spr::kv4_head_bytes(1 << a.log_s, D);
-  auto fetch = [&](int blk, Held<D>& x) {
+  auto fetch = [&](int blk, Held<D>& x) __attribute__((always_inline)) {
     const int32_t key = blk * FEW_KEYS;
     bool ok;
     const uint8_t* part = a.pages + page_offset(a, row_table, key, ok) + head;
@@ -287,7 +290,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
   // 16-dim tile v
   auto tr_at = [&](int v) { return piece_at(4 * g + (m >> 2), 2 * v + ((m & 3) >> 1)) + (m & 1) * 8; };
 
-  auto step = [&](const Held<D>& x, int32_t key, auto masked) {
+  auto step = [&](const Held<D>& x, int32_t key, auto masked) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(masked)::value;
     f32x4 s[NT][2];
 #pragma unroll
@@ -399,15 +402,20 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
   const int whole = min(last, least / FEW_KEYS);
   int blk = split * deal.per + wave;
   if (blk < last) {
-    Held<D> now, next;
-    fetch(blk, now);
-    auto walk = [&](int end, auto masked) {
+    Held<D> x0, x1;
+    fetch(blk, x0);
+    auto walk = [&](int end, auto masked) __attribute__((always_inline)) {
       while (blk < end) {
-        const int after = blk + FEW_WAVES;
-        if (after < last) fetch(after, next);
-        step(now, blk * FEW_KEYS, masked);
-        now = next;
-        blk = after;
+        if (blk + FEW_WAVES < last) fetch(blk + FEW_WAVES, x1);
+        step(x0, blk * FEW_KEYS, masked);
+        blk += FEW_WAVES;
+        if (blk >= end) {
+          x0 = x1;
+          break;
+        }
+        if (blk + FEW_WAVES < last) fetch(blk + FEW_WAVES, x0);
+        step(x1, blk * FEW_KEYS, masked);
+        blk += FEW_WAVES;
       }
     };
     walk(whole, std::false_type{});
@@ -489,6 +497,20 @@ __device__ __forceinline__ float sum_xor32(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The batch entry that comes `at`-th: the longest sequences first, so that the call does not end with one
+// of their shares alone on a CU (8 sequences to 9,000 tokens 215..240 -> 176 us, 5 fp16 prompts 76..87 ->
+// 72..81).  Every wave ranks them itself, a lane each (more than 64 stay in order).
+__device__ __forceinline__ int sequence_at(const AttnArgs& a, int at, int lane) {
+  if (a.batch == 1 || a.batch > 64) return at;
+  const int32_t mine = lane < a.batch ? span_of(a, lane).length : -1;
+  int rank = 0;
+  for (int k = 0; k < a.batch; ++k) {
+    const int32_t other = __builtin_amdgcn_readlane(mine, k);
+    rank += other > mine || (other == mine && k < lane) ? 1 : 0;
+  }
+  return __builtin_ctzll(__ballot(lane < a.batch && rank == at));
+}
+
 // 32 * RB query rows (RB 8, 4 or 2) of one kv head against a share of its keys.  One workgroup per CU,
 // two waves per SIMD.  Wave w has row block w % RB and part w / RB of every chunk of 128 keys, all of
 // it, 64 or 32 keys; the parts of a row block are merged at the end.
@@ -537,11 +559,13 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
   const int64_t id = static_cast<int64_t>(blockIdx.x / (8 * RUN)) * (8 * RUN) + (blockIdx.x & 7) * RUN + (blockIdx.x >> 3) % RUN;
   if (id >= total) return;
   const int tile = static_cast<int>(id % tiles);
-  const int split = static_cast<int>(id / tiles % a.nsplit);
   const int64_t bh = id / tiles / a.nsplit;
-  const int hk = static_cast<int>(bh % a.kv_heads), b = static_cast<int>(bh / a.kv_heads);
-
+  // with few tiles a head the shares turn from head to head, as in the few-row kernel (4 sequences of 64
+  // rows 59 -> 54 us); with many it would only bring some of the long ones late (13 tiles 81 -> 105 us)
+  const int split = static_cast<int>((id / tiles + (tiles <= RUN ? bh : 0)) % a.nsplit);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hk = static_cast<int>(bh % a.kv_heads), b = sequence_at(a, static_cast<int>(bh / a.kv_heads), lane);
+
   const int col = lane & 31, half = lane >> 5;
   const int blk = wave % RB, part = wave / RB;
   const Span sp = span_of(a, b);
@@ -825,7 +849,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
   }
   if (!in) return;
   if (deal.shares > 1) {
-    const int64_t at = (bh * a.nsplit + split) * total_rows + rho;
+    const int64_t at = ((static_cast<int64_t>(b) * a.kv_heads + hk) * a.nsplit + split) * total_rows + rho;
 #pragma unroll
     for (int i = 0; i < DBLK; ++i) {
 #pragma unroll
@@ -945,10 +969,10 @@ Shape shape_of(int32_t batch, int32_t kv_heads, int32_t group, int32_t rows, int
   if (total <= 32) {
     s.nt = total <= 16 ? 1 : 2;
     s.groups = heads;
-    // Three workgroups for every CU, in one round, where there is one sequence; shares of its keys that
-    // are not alike even out over more of them where there are several (their lengths are not known
-    // here).  None of less than four blocks a wave.
-    const int64_t fill = std::max<int64_t>(1, (batch == 1 ? 768 : 2048) / s.groups);
+    // Three workgroups for every CU, in one round, where there is one sequence; two rounds where there are
+    // several, whose lengths are not known here, so that long ones are dealt finer (48 ragged ones in one
+    // round 55 us, in two 36; 16 alike 31 and 34).  None of less than four blocks a wave.
+    const int64_t fill = std::max<int64_t>(1, (batch == 1 ? 768 : 1536) / s.groups);
     const int64_t most = std::max<int64_t>(1, max_length / (4 * FEW_WAVES * FEW_KEYS));
     s.nsplit = static_cast<int32_t>(std::min({fill, most, int64_t{256}}));
     return s;

@@ -291,6 +291,46 @@ def test_sharp_scores_and_long_sequences(dev):
             _check_attention(out, lse, q, pages, table, [n], [rows], size, False, d**-0.5, "bf16")
 
 
+@pytest.mark.parametrize("rows,group", [(1, 4), (9, 1), (5, 5), (20, 2), (65, 1), (130, 2)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_ragged_batches_in_shares(dev, rows, group, dtype):
+    """Sequences of unlike length, in no order, with keys in several shares (long ones), in one and in
+    none, for every kernel: each row comes out with its own sequence's."""
+    from sparsepr_amd.kernels.kv4 import kv4_attention
+
+    rng = np.random.default_rng(15)
+    hk, d, size = 2, 64, 64
+    lengths = [700, 5000, 0, 31, 9000, 2500, 5000]
+    ids = [3, 0, 5, 2, 4, 1, 6, 5]
+    counts = [rows, rows, max(1, rows // 2), rows, rows, 0, rows, rows]
+    num = sum(-(-n // size) for n in lengths)
+    pages, table = _pool(rng, num, hk, size, d), _table(rng, lengths, size, num, 141)
+    q = torch.randn((len(ids), hk * group, rows, d), device=dev).to(DT[dtype])
+    for causal in (False, True):
+        out, lse = kv4_attention(q, _gpu(pages, dev, torch.uint8), _gpu(table, dev), _gpu(lengths, dev),
+                                 counts=_gpu(counts, dev), seq_ids=_gpu(ids, dev), causal=causal, return_lse=True)
+        # two heads and some rows of each, so that the reference stays quick
+        heads = [0, hk * group - 1]
+        for i, s in enumerate(ids):
+            k, v = model.tokens(pages, table[s], lengths[s], size, d)
+            n = lengths[s]
+            for h in heads:
+                for t in {0, counts[i] // 3, counts[i] - 1, rows - 1} - {-1}:
+                    one = q[i:i + 1, h:h + 1, t:t + 1]
+                    seen = (min(max(n - counts[i] + t + 1, 0), n) if causal else n) if t < counts[i] else 0
+                    kv = k[None, h // group, :seen], v[None, h // group, :seen]
+                    ref, ref_lse, spread, logit = model.attend(one[0].double().cpu().numpy(), *kv, 1, False, d**-0.5)
+                    u = 2.0**-24  # the bounds of _check_attention
+                    rounds, last = (2.0**-8, 2.0**-8) if dtype == "bf16" else (2.0**-14, 2.0**-11)
+                    e = (d + 6) * u * logit[0, 0] + 2.0**-21
+                    tol = spread * (rounds + 2 * e + 2 * n * u) + last * np.abs(ref) + 2.0**-25
+                    assert (np.abs(out[i, h, t].double().cpu().numpy() - ref[0, 0]) <= tol[0, 0]).all(), (i, h, t)
+                    if seen == 0:
+                        assert torch.isneginf(lse[i, h, t])
+                    else:
+                        assert abs(float(lse[i, h, t]) - ref_lse[0, 0]) <= e + n * u + 2.0**-21 + 4 * u * abs(ref_lse[0, 0])
+
+
 def test_pages_past_two_gigabytes(dev):
     from sparsepr_amd.kernels.kv4 import kv4_attention, kv4_compact, kv4_fork, kv4_load, kv4_store
 
