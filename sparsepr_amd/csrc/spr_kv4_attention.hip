@@ -193,8 +193,8 @@ struct Held {
 //
 // Bound by memory: one row of 24 heads against 118,800 tokens of 128 dims, 388 MB, takes 71 us, 5.5 TB/s
 // (a large copy moves 4.9), and 5 us more for the merge of its 32 shares; 48 ragged sequences of up to
-// 8,191 tokens, 32 heads on 8, 118 MB in 34 us; a short call of 301 tokens 5.9 us.  The next block's
-// codes are in flight while one is computed, with three or four waves a SIMD (126 registers for D = 128).
+// 8,191 tokens, 32 heads on 8, 119 MB in 33 us; a short call of 301 tokens 5.9 us.  The next block's
+// codes are in flight while one is computed, with three waves a SIMD (149 registers for D = 128).
 //
 // TWICE: at most 8 rows, each in two of the 16 columns (m and m + 8), one for the upper eight
 // significant bits of its probabilities and one for the next eight, so P loses 2^-14 of itself instead of
@@ -398,7 +398,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
   };
 
   // blocks that every row sees whole, then the others: two loops, since one that takes either step holds
-  // half as many registers again (181 against 126)
+  // half as many registers again.  Two sets of registers in turn: copying the next block's to the current
+  // one's cost 10 % on 48 sequences.  (Inlined by force: called, the steps keep them in scratch.)
   const int whole = min(last, least / FEW_KEYS);
   int blk = split * deal.per + wave;
   if (blk < last) {
@@ -531,8 +532,8 @@ __device__ __forceinline__ int sequence_at(const AttnArgs& a, int at, int lane) 
 //
 // Bound by neither unit alone: 3600 rows of 24 heads against 118,800 tokens of 128 dims, 5.26 TFLOP,
 // take 4.9 to 5.1 ms, 1030 to 1070 TFLOP/s, where a library product of 8192^3 reaches 1129 on this card;
-// the clock is down to 1.8 GHz, the MFMA pipe is busy half of the time, VALU issue 55 %.  128 rows take
-// 0.23 ms (815 TFLOP/s): half the products to each conversion.  Row blocks by rows of the call, at
+// the clock is down to 1.75 GHz, the MFMA pipe is busy half of the time, VALU issue as much.  128 rows take
+// 0.23 ms (830 TFLOP/s): half the products to each conversion.  Row blocks by rows of the call, at
 // 24 x 118,800 x 128: 33 to 64 rows 156 us with RB 2 and 200 with RB 4; 17 to 32 rows 150 us with RB 2 and
 // 115 with the few-row kernel; 65 to 128 rows 209 with RB 4.
 template <int D, bool F16, int RB>
