@@ -513,8 +513,9 @@ int spr_project_rows_ex(const float* x, const float* factor, const float* div, i
  * pages uint8 [num_pages, kv_heads, spr_kv4_page_bytes(1, page_size, d)], 16-byte aligned; one head's
  * part of a page of page_size (32, 64, 128 or 256) tokens is the K codes [page_size, d / 2], the V
  * codes, the K scales [page_size, d / 32] and the V scales; d is 64 or 128.  A code is a 4-bit float
- * (sign, then 0, 0.5, 1, 1.5, 2, 3, 4, 6), the even dim in the low half of a byte; scale byte s is
- * 2^(s - 127) for 32 dims of a token, 255 a NaN.  block_table int32 [sequences, wide] names a
+ * (sign, then 0, 0.5, 1, 1.5, 2, 3, 4, 6), the even dim in the low half of a byte; scale byte s (2 to
+ * 252) is 2^(s - 127) for 32 dims of a token, a larger one a NaN.  Slots that hold no token may have any
+ * bytes.  block_table int32 [sequences, wide] names a
  * sequence's pages (-1: none), lengths int32 [sequences] its tokens, ref_count int32 [num_pages] how
  * many sequences hold a page (0: free); wide * page_size <= 2^30.  seq_ids int32 [batch]
  * (nullable: 0, 1, ..) names the sequences of a call. */

@@ -3,9 +3,10 @@
 // pages [num_pages, kv_heads, head_bytes] uint8.  One head's part of a page of S tokens:
 //   K codes [S][D / 2], V codes [S][D / 2], K scales [S][D / 32], V scales [S][D / 32]
 // A code is a 4-bit float e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), two to a byte, the even dim
-// in the low half.  A scale byte b is the power of two 2^(b - 127) of 32 dims of one token, 255 a
-// NaN.  code * scale has two significant bits, so bf16 holds it exactly for every b in [2, 252],
-// and one v_cvt_scalef32_pk_bf16_fp4 makes two of them.
+// in the low half.  A scale byte b is the power of two 2^(b - 127) of 32 dims of one token, b in
+// [2, 252]; a larger byte is a NaN (253 and 254 would pass bf16's range, with infinities that 0 * inf
+// brings to rows that do not see the token).  code * scale has two significant bits, so bf16 holds it
+// exactly, and one v_cvt_scalef32_pk_bf16_fp4 makes two of them.
 #pragma once
 
 #include "spr_common.h"
@@ -46,7 +47,10 @@ __device__ __forceinline__ u32x4 kv4_eight(uint32_t w, float scale) {
   return u32x4{kv4_pair<0>(w, scale), kv4_pair<1>(w, scale), kv4_pair<2>(w, scale), kv4_pair<3>(w, scale)};
 }
 
-// A scale byte as the float that the conversions take (255: not a number).
-__device__ __forceinline__ float kv4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+// Whether a scale byte stands for no number.
+__device__ __forceinline__ bool kv4_nan(uint32_t byte) { return byte > 252; }
+
+// A scale byte as the float that the conversions take (exponent 255: not a number).
+__device__ __forceinline__ float kv4_scale(uint32_t byte) { return __uint_as_float((kv4_nan(byte) ? 255 : byte) << 23); }
 
 }  // namespace spr

@@ -307,8 +307,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
           if constexpr (F16) s[n][kt] = mfma16(kf, ql[n][w], s[n][kt]);
         }
       }
-      // in a masked block a NaN V scale is kept out of the product (0 * NaN) and put in below
-      const float vs = spr::kv4_scale(MASKED && x.vs[kt] == 255 ? 127 : x.vs[kt]);
+      // in a masked block a NaN V scale is kept out of the product (0 * NaN) and put in below; slots past
+      // the sequence's end may hold any bytes
+      const float vs = spr::kv4_scale(MASKED && spr::kv4_nan(x.vs[kt]) ? 127 : x.vs[kt]);
 #pragma unroll
       for (int w = 0; w < WORDS; ++w) {
         *reinterpret_cast<u32x4*>(mine + piece_at(kt * 16 + m, g * WORDS + w)) = spr::kv4_eight(x.v[kt][w], vs);
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
       // V scales that are NaN: their dims of every row that sees their key
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        uint64_t nan = __ballot(x.vs[kt] == 255);
+        uint64_t nan = __ballot(spr::kv4_nan(x.vs[kt]));
         while (nan != 0) {
           const int l = __builtin_ctzll(nan);
           nan &= nan - 1;
@@ -642,7 +643,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
       const int x = v != 0 ? swz_v : swz_k;
       // a chunk that some row does not see whole keeps NaN V scales out of the products (0 * NaN); they
       // are put in row by row
-      const float sc = spr::kv4_scale(v != 0 && byte[i] == 255 && end > least ? 127 : byte[i]);
+      const float sc = spr::kv4_scale(v != 0 && spr::kv4_nan(byte[i]) && end > least ? 127 : byte[i]);
       const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(to + (((4 * cg + j) ^ x) << 4)) = spr::kv4_eight(w[j], sc);
@@ -748,7 +749,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
       const uint32_t w = v_bytes[c & 1][k0 + lane];
       uint32_t mine = 0;
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) mine |= ((w >> (8 * g)) & 255) == 255 ? 1u << g : 0;
+      for (int g = 0; g < GROUPS; ++g) mine |= spr::kv4_nan((w >> (8 * g)) & 255) ? 1u << g : 0;
       uint64_t keys = __ballot(mine != 0);
       while (keys != 0) {
         const int k = __builtin_ctzll(keys);

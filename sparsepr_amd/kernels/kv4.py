@@ -5,7 +5,8 @@ take.
 
 pages        uint8 [P, Hkv, page_bytes], or [layers, P, Hkv, page_bytes] for the page calls: pages of
              page_size tokens, K and V as 4-bit floats with one power-of-two scale per 32 dims
-             (kv4_page_bytes; D + D / 16 bytes a token and kv head, against 4 D in bf16).
+             (kv4_page_bytes; D + D / 16 bytes a token and kv head, against 4 D in bf16).  What slots
+             without a token hold does not matter, so a pool need not be cleared.
 block_table  int32 [sequences, wide], a sequence's pages in order, -1 past the last.
 lengths      int32 [sequences], tokens.
 ref_count    int32 [P], how many sequences hold a page; 0 is free.

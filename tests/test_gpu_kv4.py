@@ -749,3 +749,57 @@ def test_captured_attention_with_shares_of_the_keys(dev):
             for a, b in zip(outs, want):
                 assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]), step
     cache.check()
+
+
+ROWS = [(1, 2), (9, 1), (10, 2), (20, 2), (70, 1), (140, 2)]  # both kernels, 8, 16, 32 rows, 64, 128 and 256
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows,group", ROWS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_slots_that_hold_no_token_change_nothing(dev, d, rows, group, dtype):
+    from sparsepr_amd.kernels.kv4 import kv4_attention
+
+    rng = np.random.default_rng(21)
+    hk, size, lengths = 2, 64, [1, 33, 200, 0, 95]
+    num = sum(-(-n // size) for n in lengths) + 2
+    pages, table = _pool(rng, num, hk, size, d), _table(rng, lengths, size, num, 5)
+    unused = np.ones((num, size), bool)
+    for i, n in enumerate(lengths):
+        for j in range(n):
+            unused[table[i, j // size], j % size] = False
+    unused = np.broadcast_to(unused[:, None], (num, hk, size))
+    q = torch.randn((len(lengths), hk * group, rows, d), device=dev).to(DT[dtype])
+    outs = []
+    for scale in (100, 252, 253, 254, 255, None):  # None: any bytes at all
+        for part in model.parts(pages, size, d)[:2]:
+            part[unused] = rng.integers(0, 256, part[unused].shape, np.uint8)
+        for part in model.parts(pages, size, d)[2:]:
+            part[unused] = rng.integers(0, 256, part[unused].shape, np.uint8) if scale is None else scale
+        for causal in (False, True):
+            outs.append(kv4_attention(q, _gpu(pages, dev, torch.uint8), _gpu(table, dev), _gpu(lengths, dev),
+                                      causal=causal, return_lse=True))
+    for i, got in enumerate(outs):
+        assert all(torch.equal(a, b) for a, b in zip(got, outs[i % 2])), i // 2
+    assert torch.isfinite(outs[0][0]).all()
+
+
+@pytest.mark.parametrize("byte", [253, 254])
+@pytest.mark.parametrize("rows", [1, 40, 130])
+def test_scale_bytes_past_the_encoders_are_nan(dev, rows, byte):
+    from sparsepr_amd.kernels.kv4 import kv4_attention, kv4_load
+
+    rng = np.random.default_rng(22)
+    hk, d, size, n = 2, 128, 64, 200
+    for where in (0, n - rows // 2 - 1, n - 1):
+        for part, group in ((2, 1), (3, 2)):
+            pages, table = _pool(rng, 4, hk, size, d), _table(rng, [n], size, 4, 4)
+            said = model.parts(pages[table[0, where // size]], size, d)[part][1, where % size]
+            said[group] = byte
+            gp, gt = _gpu(pages, dev, torch.uint8), _gpu(table, dev)
+            said[group] = 255
+            q = torch.randn((1, 2, rows, d), device=dev).to(torch.bfloat16)
+            out, lse = kv4_attention(q, gp, gt, _gpu([n], dev), causal=True, return_lse=True)
+            _check_attention(out, lse, q, pages, table, [n], [rows], size, True, d**-0.5, "bf16")
+            for got, want in zip(kv4_load(gp, gt, _gpu([0], dev), _gpu([n], dev), n, d), model.tokens(pages, table[0], n, size, d)):
+                assert np.array_equal(got[0].double().cpu().numpy(), want, equal_nan=True)
