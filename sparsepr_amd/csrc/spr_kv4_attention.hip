@@ -4,8 +4,8 @@
 //
 // over the visible tokens j of sequence b's pages: all of them, or (causal) those up to the query's
 // own, the last of the call's rows being the sequence's last token.  A row that sees nothing is 0
-// with lse -inf.  The query heads of one kv head share its K and V: their rows, token-major, are one
-// list of rows * group query rows.
+// with lse -inf, one that sees scores of -inf alone NaN.  The query heads of one kv head share its K
+// and V: their rows, token-major, are one list of rows * group query rows.
 //
 // K and V values (code times scale) are exact in bf16, so the conversion to the MFMA's operand loses
 // nothing; fp16 queries and probabilities go in as two bf16 terms (hi + lo) and lose at most 2^-14
@@ -72,6 +72,14 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
 __device__ __forceinline__ int32_t visible_of(const AttnArgs& a, const Span& s, int t) {
   if (t >= s.count) return 0;
   return a.causal != 0 ? min(max(s.length - s.count + t + 1, 0), s.length) : s.length;
+}
+
+// What row t's sum of weights l stands for: rows out of use were computed beside the others, and nothing
+// of that is kept (0); a row whose every score is -inf has no softmax, which only a row without keys may
+// be 0 for.
+__device__ __forceinline__ float sum_of(const AttnArgs& a, const Span& s, int t, float l) {
+  if (t >= s.count) return 0.0f;
+  return s.broken || (l == 0.0f && visible_of(a, s, t) > 0) ? __builtin_nanf("") : l;
 }
 
 // Keys that the rows [row0, row0 + tile_rows) see at most.  Rows are token-major: the last one in use
@@ -469,10 +477,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
         reinterpret_cast<f32x4*>(a.part_o + at * D)[p] = o;
         if (p == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = float2{top, l};
       } else {
-        // rows out of use went through unmasked blocks like the others: nothing of that is kept
-        const bool used = t < sp.count;
-        if (!used) l = 0.0f;
-        if (sp.broken && used) l = __builtin_nanf("");
+        l = sum_of(a, sp, t, l);
         o = l == 0.0f ? f32x4{0, 0, 0, 0} : o * (1.0f / l);
         const int64_t at = (static_cast<int64_t>(b) * a.kv_heads * a.group + h) * a.rows + t;
         *reinterpret_cast<u32x2*>(a.out + at * D + 4 * p) = u32x2{pack_out<F16>(o[0], o[1]), pack_out<F16>(o[2], o[3])};
@@ -863,9 +868,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
     if (half == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = float2{m_run, l_tot};
     return;
   }
-  // rows out of use were computed beside the others: nothing of that is kept
-  if (!used) l_tot = 0.0f;
-  else if (sp.broken) l_tot = __builtin_nanf("");
+  l_tot = sum_of(a, sp, t, l_tot);
   const float inv = 1.0f / l_tot;
   const int64_t at = (static_cast<int64_t>(b) * a.kv_heads * a.group + h) * a.rows + t;
 #pragma unroll
@@ -941,8 +944,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, int64_t all_
     }
   }
   const int t = rho / a.group, h = hk * a.group + rho % a.group;
-  if (t >= sp.count) l = 0.0f;
-  else if (sp.broken) l = __builtin_nanf("");
+  l = sum_of(a, sp, t, l);
   const int64_t at = (static_cast<int64_t>(b) * a.kv_heads * a.group + h) * a.rows + t;
   const float inv = 1.0f / l;
 #pragma unroll

@@ -803,3 +803,24 @@ def test_scale_bytes_past_the_encoders_are_nan(dev, rows, byte):
             _check_attention(out, lse, q, pages, table, [n], [rows], size, True, d**-0.5, "bf16")
             for got, want in zip(kv4_load(gp, gt, _gpu([0], dev), _gpu([n], dev), n, d), model.tokens(pages, table[0], n, size, d)):
                 assert np.array_equal(got[0].double().cpu().numpy(), want, equal_nan=True)
+
+
+@pytest.mark.parametrize("rows,group", ROWS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n", [1, 6000])
+def test_rows_whose_scores_are_all_minus_infinity_are_nan(dev, rows, group, dtype, n):
+    from sparsepr_amd.kernels.kv4 import kv4_attention
+
+    rng = np.random.default_rng(23)
+    d, size = 64, 64
+    num = -(-n // size)
+    pages, table = _pool(rng, num, 1, size, d), _table(rng, [n], size, num, num)
+    codes = model.parts(pages, size, d)[0]
+    codes[..., 0] = codes[..., 0] & 0xF0 | 2  # K's first dim is positive
+    q = torch.randn((1, group, rows, d), device=dev).to(DT[dtype])
+    q[0, 0, 0, 0] = -math.inf
+    out, lse = kv4_attention(q, _gpu(pages, dev, torch.uint8), _gpu(table, dev), _gpu([n], dev), return_lse=True)
+    bad = torch.zeros((1, group, rows), dtype=torch.bool, device=dev)
+    bad[0, 0, 0] = True
+    assert torch.equal(torch.isnan(lse), bad) and torch.equal(torch.isnan(out).all(-1), bad)
+    assert torch.equal(torch.isnan(out).any(-1), bad)
