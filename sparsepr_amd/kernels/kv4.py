@@ -47,8 +47,8 @@ def kv4_page_bytes(page_size: int, head_dim: int) -> int:
     return page_size * (head_dim + head_dim // 16)
 
 
-def _page_size(pages: torch.Tensor, head_dim: int, what: str) -> int:
-    """Tokens of a page, from the pages of one layer and the head dim."""
+def _page_size(pages: torch.Tensor, head_dim: int, page_size: int | None, what: str) -> int:
+    """Tokens of a page, from the pages of one layer and the head dim; `page_size`, if the caller gives it."""
     shape = pages.shape
     if pages.dtype is not torch.uint8 or len(shape) != 3 or not pages.is_contiguous() or pages.numel() == 0:
         raise RuntimeError(f"{what}: pages must be a contiguous uint8 tensor [P, Hkv, bytes], got {pages.dtype} "
@@ -58,6 +58,8 @@ def _page_size(pages: torch.Tensor, head_dim: int, what: str) -> int:
     size = shape[2] // (head_dim + head_dim // 16)
     if size not in PAGE_SIZES or shape[2] != size * (head_dim + head_dim // 16):
         raise RuntimeError(f"{what}: pages of {shape[2]} bytes a head are not whole pages of head dim {head_dim}")
+    if page_size is not None and size != page_size:
+        raise RuntimeError(f"{what}: pages of {shape[2]} bytes a head are not {page_size} tokens of head dim {head_dim}")
     return size
 
 
@@ -100,20 +102,22 @@ def _by_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
 
 
 def kv4_store(pages: torch.Tensor, block_table: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
-              *, counts: torch.Tensor | None = None, seq_ids: torch.Tensor | None = None) -> None:
+              *, counts: torch.Tensor | None = None, seq_ids: torch.Tensor | None = None,
+              page_size: int | None = None) -> None:
     """Write K and V rows [B, Hkv, T, D] (bf16, fp16 or fp32, any strides with packed rows) to the
     cache: row t < counts[b] becomes token starts[b] + t of sequence seq_ids[b] (default b).
 
     The pages have to be there (kv4_reserve): rows without one are not written.  No two rows of a call
     may name one token, and no other sequence may share the page written to (kv4_fork sees to that).
-    A group of 32 dims with an infinity or a NaN is stored as NaN."""
+    A group of 32 dims with an infinity or a NaN is stored as NaN.  `page_size` is for the caller's
+    check of what it hands over: a page of 2 n tokens of head dim 64 has the bytes of n of 128."""
     what = "4-bit cache store"
     dev = _lib.require_gpu(pages, block_table, k, v, starts, counts, seq_ids, what=what)
     if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _lib.DTYPE_CODE:
         raise RuntimeError(f"{what}: K and V must be [B, Hkv, T, D] of one dtype (bfloat16, float16, float32), got "
                            f"{k.dtype} {tuple(k.shape)} / {v.dtype} {tuple(v.shape)}")
     b, h, t, d = k.shape
-    size = _page_size(pages, d, what)
+    size = _page_size(pages, d, page_size, what)
     if pages.shape[1] != h:
         raise RuntimeError(f"{what}: K has {h} heads, the pages {pages.shape[1]}")
     sequences, wide = _check_table(block_table, what)
@@ -129,12 +133,14 @@ def kv4_store(pages: torch.Tensor, block_table: torch.Tensor, k: torch.Tensor, v
 
 
 def kv4_load(pages: torch.Tensor, block_table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, rows: int,
-             head_dim: int, *, seq_ids: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16):
+             head_dim: int, *, seq_ids: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16,
+             page_size: int | None = None):
     """Tokens starts[b] .. starts[b] + counts[b] - 1 of every named sequence as (K, V) [B, Hkv, rows, D]
-    in `dtype` (exact in bf16 and fp32); rows past the count are 0, rows with no page NaN."""
+    in `dtype` (exact in bf16 and fp32); rows past the count are 0, rows with no page NaN.  `page_size` is
+    checked, as in kv4_store."""
     what = "4-bit cache load"
     dev = _lib.require_gpu(pages, block_table, starts, counts, seq_ids, what=what)
-    size = _page_size(pages, head_dim, what)
+    size = _page_size(pages, head_dim, page_size, what)
     if dtype not in _lib.DTYPE_CODE:
         raise RuntimeError(f"{what}: dtype must be bfloat16, float16 or float32, got {dtype}")
     if rows < 0 or starts.dim() != 1:
@@ -154,7 +160,8 @@ def kv4_load(pages: torch.Tensor, block_table: torch.Tensor, starts: torch.Tenso
 
 def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, *,
                   counts: torch.Tensor | None = None, seq_ids: torch.Tensor | None = None, causal: bool = False,
-                  scale: float | None = None, max_length: int | None = None, return_lse: bool = False):
+                  scale: float | None = None, max_length: int | None = None, return_lse: bool = False,
+                  page_size: int | None = None):
     """softmax(q K^T * scale) V over the cached tokens: q [B, Hq, T, D] bf16 or fp16 (any strides with
     packed rows) -> out [B, Hq, T, D] in q's dtype (and lse fp32 [B, Hq, T], natural log).
 
@@ -162,13 +169,14 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     sequence seq_ids[b] (default b) with its first counts[b] rows (default all).  With `causal` the last
     row in use is the sequence's last token and each row sees the tokens up to its own (store them
     first).  Rows that see nothing, and rows past the count, are 0 with lse -inf.  `max_length`, the
-    longest length the caller knows of (default: what the table can hold), only sizes the launch."""
+    longest length the caller knows of (default: what the table can hold), only sizes the launch;
+    `page_size` is checked, as in kv4_store."""
     what = "4-bit cache attention"
     dev = _lib.require_gpu(q, pages, block_table, lengths, counts, seq_ids, what=what)
     if q.dim() != 4 or q.dtype not in (torch.bfloat16, torch.float16):
         raise RuntimeError(f"{what}: q must be [B, Hq, T, D] in bfloat16 or float16, got {q.dtype} {tuple(q.shape)}")
     b, h, t, d = q.shape
-    size = _page_size(pages, d, what)
+    size = _page_size(pages, d, page_size, what)
     hk = pages.shape[1]
     if h == 0 or h % hk != 0:
         raise RuntimeError(f"{what}: Q heads ({h}) must be a multiple of KV heads ({hk})")

@@ -58,7 +58,7 @@ class KV4Cache:
     def store(self, k, v, starts, *, counts=None, seq_ids=None, layer: int = 0) -> None:
         """kv4_store into one layer, at the places `reserve` gave."""
         kv4.kv4_store(self.pages[layer], self.block_table, k, v, self._ints(starts), counts=self._ints(counts),
-                      seq_ids=self._ints(seq_ids))
+                      seq_ids=self._ints(seq_ids), page_size=self.page_size)
 
     def append(self, k, v, *, counts=None, seq_ids=None) -> torch.Tensor:
         """reserve and store K and V [B, Hkv, T, D] of a cache of one layer; returns the starts."""
@@ -74,14 +74,14 @@ class KV4Cache:
     def load(self, starts, counts, rows: int, *, seq_ids=None, layer: int = 0, dtype: torch.dtype = torch.bfloat16):
         """kv4_load from one layer."""
         return kv4.kv4_load(self.pages[layer], self.block_table, self._ints(starts), self._ints(counts), rows,
-                            self.head_dim, seq_ids=self._ints(seq_ids), dtype=dtype)
+                            self.head_dim, seq_ids=self._ints(seq_ids), dtype=dtype, page_size=self.page_size)
 
     def attend(self, q, *, counts=None, seq_ids=None, layer: int = 0, causal: bool = False, scale: float | None = None,
                max_length: int | None = None, return_lse: bool = False):
         """kv4_attention over one layer."""
         return kv4.kv4_attention(q, self.pages[layer], self.block_table, self.lengths, counts=self._ints(counts),
                                  seq_ids=self._ints(seq_ids), causal=causal, scale=scale, max_length=max_length,
-                                 return_lse=return_lse)
+                                 return_lse=return_lse, page_size=self.page_size)
 
     def free(self, seq_ids, *, first_pages=None, page_counts=None) -> None:
         """kv4_free: whole sequences, or a range of each one's pages."""

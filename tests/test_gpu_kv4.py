@@ -824,3 +824,28 @@ def test_rows_whose_scores_are_all_minus_infinity_are_nan(dev, rows, group, dtyp
     bad[0, 0, 0] = True
     assert torch.equal(torch.isnan(lse), bad) and torch.equal(torch.isnan(out).all(-1), bad)
     assert torch.equal(torch.isnan(out).any(-1), bad)
+
+
+def test_tensors_of_another_head_dim_are_refused(dev):
+    from sparsepr_amd.kernels import kv4
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    for d, size, other in ((64, 64, 128), (64, 256, 128), (128, 32, 64), (128, 128, 64), (64, 32, 128)):
+        cache = KV4Cache(8, 2, d, 2, page_size=size, device=dev)
+        starts = cache.reserve([5], [0])
+        x = torch.ones((1, 2, 5, other), dtype=torch.bfloat16, device=dev)
+        for call in (lambda: cache.store(x, x, starts, seq_ids=[0]), lambda: cache.attend(x, seq_ids=[0])):
+            with pytest.raises(RuntimeError, match=f"head dim {other}|pages of"):
+                call()
+        assert int(cache.pages.sum()) == 0 and cache.lengths.tolist() == [5, 0]
+    # the same of the functions, where the caller says what the pages hold
+    x = torch.ones((1, 2, 5, 128), dtype=torch.bfloat16, device=dev)
+    pages = torch.zeros((2, 2, kv4.kv4_page_bytes(64, 64)), dtype=torch.uint8, device=dev)
+    table = torch.zeros((1, 1), dtype=torch.int32, device=dev)
+    five = torch.full((1,), 5, dtype=torch.int32, device=dev)
+    for call in (lambda **kw: kv4.kv4_store(pages, table, x, x, five, **kw),
+                 lambda **kw: kv4.kv4_attention(x, pages, table, five, **kw),
+                 lambda **kw: kv4.kv4_load(pages, table, five, five, 5, 128, **kw)):
+        with pytest.raises(RuntimeError, match="are not 64 tokens of head dim 128"):
+            call(page_size=64)
+        call(page_size=32)
