@@ -98,7 +98,8 @@ def _by_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
         st = 0
     if sd == 1 and x.data_ptr() % 16 == 0 and (sb | sh | st) * x.element_size() % 16 == 0:
         return x, sb, sh, st
-    return x.contiguous(), h * t * d, t * d, d
+    # (contiguous() hands packed rows that start off 16 bytes back as they are)
+    return x.clone(memory_format=torch.contiguous_format), h * t * d, t * d, d
 
 
 def kv4_store(pages: torch.Tensor, block_table: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,

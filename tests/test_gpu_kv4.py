@@ -849,3 +849,21 @@ def test_tensors_of_another_head_dim_are_refused(dev):
         with pytest.raises(RuntimeError, match="are not 64 tokens of head dim 128"):
             call(page_size=64)
         call(page_size=32)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_packed_rows_off_sixteen_bytes_are_taken(dev, dtype):
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    b, h, t, d = 2, 2, 9, 64
+    k, v, q = (torch.randn(b * h * t * d + 1, device=dev).to(DT[dtype]) for _ in range(3))
+    odd = [x[1:].view(b, h, t, d) for x in (k, v, q)]
+    assert all(x.is_contiguous() and x.data_ptr() % 16 != 0 for x in odd)
+    got = []
+    for x in (odd, [y.clone() for y in odd]):
+        cache = KV4Cache(4, h, d, b, page_size=32, device=dev)
+        cache.append(x[0], x[1])
+        got.append([cache.pages, *cache.load([0, 0], [t, t], t)])
+        if dtype != "fp32":
+            got[-1] += [cache.attend(x[2]), cache.attend(x[2][:, :1, :1].expand(b, h, t, d))]
+    assert all(torch.equal(a, b) for a, b in zip(*got))
