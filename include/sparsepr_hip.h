@@ -541,17 +541,22 @@ int spr_kv4_load(const uint8_t* pages, int32_t num_pages, int32_t kv_heads, int3
 /* Page calls.  Each checks on the device all it is asked for and then happens whole or not at all;
  * new pages are the lowest free ones, ascending, in the order of the named sequences (at most 2048 a
  * call).  status int32 [1] (nullable) gets, unless it holds one already, what was wrong: 1 a sequence
- * outside the table, 2 a sequence named twice, 3 a negative count or a range outside the sequence's
- * pages, 4 more tokens than the table's row holds, 6 a fork onto a sequence that holds tokens, 7 a
+ * outside the table, 2 a sequence named twice, 3 a negative count (or one past `most`) or a range
+ * outside the sequence's pages, 4 more tokens than the table's row holds, 6 a fork onto a sequence that holds tokens, 7 a
  * length outside the table or a table entry outside the pool (the lowest of these), or else 5 not
  * enough free pages. */
 size_t spr_kv4_pages_workspace(int32_t num_pages);
 /* Room for counts[i] more tokens of sequence seq_ids[i]; starts[i] (out) is the first one's place, -1
- * for all if the call did not happen. */
+ * for all if the call did not happen.  _ex refuses counts past `most`, the rows that a store after it
+ * has. */
 int spr_kv4_reserve(int32_t* block_table, int32_t* lengths, int32_t* ref_count, const int32_t* counts,
                     const int32_t* seq_ids, int32_t n, int32_t sequences, int32_t wide, int32_t page_size,
                     int32_t num_pages, int32_t* starts, int32_t* status, void* workspace, size_t workspace_bytes,
                     hipStream_t stream);
+int spr_kv4_reserve_ex(int32_t* block_table, int32_t* lengths, int32_t* ref_count, const int32_t* counts,
+                       const int32_t* seq_ids, int32_t n, int32_t most, int32_t sequences, int32_t wide,
+                       int32_t page_size, int32_t num_pages, int32_t* starts, int32_t* status, void* workspace,
+                       size_t workspace_bytes, hipStream_t stream);
 /* Pages [first_pages[i], first_pages[i] + page_counts[i]) of sequence seq_ids[i] are given back
  * (nullable: 0, and all from there on, as any negative count says), the pages behind close up, the
  * length loses their tokens.  Up to 64 sequences need no workspace. */

@@ -21,7 +21,7 @@ enum {
   KV4_OK = 0,
   KV4_BAD_SEQUENCE = 1,   // a sequence number outside the table
   KV4_REPEATED = 2,       // a sequence named twice
-  KV4_BAD_COUNT = 3,      // a negative count, or a range outside the sequence's pages
+  KV4_BAD_COUNT = 3,      // a negative count or one past `most`, or a range outside the sequence's pages
   KV4_TABLE_FULL = 4,     // more tokens than a row of the table has pages for
   KV4_NO_PAGES = 5,       // not enough free pages
   KV4_NOT_EMPTY = 6,      // a fork onto a sequence that holds tokens
@@ -341,11 +341,12 @@ __device__ bool sum_needs(int32_t* need, int n, int64_t most, int* scratch, int&
 __device__ __forceinline__ int64_t pages_for(int64_t tokens, int log_s) { return (tokens + (1 << log_s) - 1) >> log_s; }
 
 // Room for counts[b] more tokens in every named sequence, and the sequences' lengths with them.  One
-// workgroup.  starts[b] is the first new token's place, or -1 for all when the call cannot happen.
+// workgroup.  starts[b] is the first new token's place, or -1 for all when the call cannot happen.  No
+// count may pass `most`.
 __global__ __launch_bounds__(PLAN_THREADS) void kv4_reserve_kernel(int32_t* __restrict__ table, int32_t* lengths,
                                                                    int32_t* __restrict__ refs,
                                                                    const int32_t* counts, const int32_t* seq_ids,
-                                                                   int32_t n, int32_t sequences, int32_t wide,
+                                                                   int32_t n, int32_t most, int32_t sequences, int32_t wide,
                                                                    int32_t log_s, int32_t num_pages,
                                                                    int32_t* __restrict__ starts,
                                                                    int32_t* __restrict__ status,
@@ -368,7 +369,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void kv4_reserve_kernel(int32_t* __re
     }
     // all is read before anything is written: counts may be the lengths themselves
     const int32_t old = lengths[id], more = counts[i];
-    if (more < 0) wrong |= 1u << KV4_BAD_COUNT;
+    if (more < 0 || more > most) wrong |= 1u << KV4_BAD_COUNT;
     if (old < 0 || old > room) wrong |= 1u << KV4_BAD_LENGTH;
     else if (static_cast<int64_t>(old) + more > room) wrong |= 1u << KV4_TABLE_FULL;
     olds[i] = old;
@@ -805,10 +806,10 @@ extern "C" int spr_kv4_load(const uint8_t* pages, int32_t num_pages, int32_t kv_
   });
 }
 
-extern "C" int spr_kv4_reserve(int32_t* block_table, int32_t* lengths, int32_t* ref_count, const int32_t* counts,
-                               const int32_t* seq_ids, int32_t n, int32_t sequences, int32_t wide, int32_t page_size,
-                               int32_t num_pages, int32_t* starts, int32_t* status, void* workspace,
-                               size_t workspace_bytes, hipStream_t stream) {
+extern "C" int spr_kv4_reserve_ex(int32_t* block_table, int32_t* lengths, int32_t* ref_count, const int32_t* counts,
+                                  const int32_t* seq_ids, int32_t n, int32_t most, int32_t sequences, int32_t wide,
+                                  int32_t page_size, int32_t num_pages, int32_t* starts, int32_t* status,
+                                  void* workspace, size_t workspace_bytes, hipStream_t stream) {
   const char* what = "spr_kv4_reserve";
   if (int st = check_pool(what, page_size, num_pages)) return st;
   if (int st = check_table(what, sequences, wide, page_size)) return st;
@@ -816,11 +817,19 @@ extern "C" int spr_kv4_reserve(int32_t* block_table, int32_t* lengths, int32_t* 
   SPR_REQUIRE(seq_ids != nullptr || n <= sequences, "%s: %d counts for %d sequences", what, n, sequences);
   if (n == 0) return SPR_OK;
   if (int st = check_space(what, workspace, workspace_bytes, num_pages)) return st;
-  kv4_reserve_kernel<<<1, PLAN_THREADS, 0, stream>>>(block_table, lengths, ref_count, counts, seq_ids, n, sequences,
-                                                     wide, log2_of(page_size), num_pages, starts, status,
+  kv4_reserve_kernel<<<1, PLAN_THREADS, 0, stream>>>(block_table, lengths, ref_count, counts, seq_ids, n, most,
+                                                     sequences, wide, log2_of(page_size), num_pages, starts, status,
                                                      static_cast<int32_t*>(workspace) + HEADER_WORDS);
   SPR_LAUNCHED(what);
   return SPR_OK;
+}
+
+extern "C" int spr_kv4_reserve(int32_t* block_table, int32_t* lengths, int32_t* ref_count, const int32_t* counts,
+                               const int32_t* seq_ids, int32_t n, int32_t sequences, int32_t wide, int32_t page_size,
+                               int32_t num_pages, int32_t* starts, int32_t* status, void* workspace,
+                               size_t workspace_bytes, hipStream_t stream) {
+  return spr_kv4_reserve_ex(block_table, lengths, ref_count, counts, seq_ids, n, INT32_MAX, sequences, wide, page_size,
+                            num_pages, starts, status, workspace, workspace_bytes, stream);
 }
 
 extern "C" int spr_kv4_free(int32_t* block_table, int32_t* lengths, int32_t* ref_count, const int32_t* seq_ids,

@@ -30,7 +30,7 @@ MAX_NAMED = 2048
 STATUS = {
     1: "a sequence outside the table",
     2: "a sequence named twice",
-    3: "a negative count, or a range outside the sequence's pages",
+    3: "a negative count or one past the rows given, or a range outside the sequence's pages",
     4: "more tokens than a row of the block table has pages for",
     5: "not enough free pages",
     6: "a fork onto a sequence that holds tokens",
@@ -102,6 +102,36 @@ def _by_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
     return x.clone(memory_format=torch.contiguous_format), h * t * d, t * d, d
 
 
+def store_call(pages: torch.Tensor, block_table: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+               counts: torch.Tensor | None = None, seq_ids: torch.Tensor | None = None, page_size: int | None = None):
+    """Everything of kv4_store but the starts checked, as a function of them: whoever reserves first has
+    no refusal to expect after it."""
+    what = "4-bit cache store"
+    dev = _lib.require_gpu(pages, block_table, k, v, counts, seq_ids, what=what)
+    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _lib.DTYPE_CODE:
+        raise RuntimeError(f"{what}: K and V must be [B, Hkv, T, D] of one dtype (bfloat16, float16, float32), got "
+                           f"{k.dtype} {tuple(k.shape)} / {v.dtype} {tuple(v.shape)}")
+    b, h, t, d = k.shape
+    size = _page_size(pages, d, page_size, what)
+    if pages.shape[1] != h:
+        raise RuntimeError(f"{what}: K has {h} heads, the pages {pages.shape[1]}")
+    sequences, wide = _check_table(block_table, what)
+    _check_entries(b, sequences, seq_ids, counts, what)
+    code, live = _lib.DTYPE_CODE[k.dtype], k.numel() > 0
+    k, *k_strides = _by_rows(k)
+    v, *v_strides = _by_rows(v)
+
+    def put(starts: torch.Tensor) -> None:
+        _lib.require_gpu(pages, starts, what=what)
+        _int32(starts, b, "starts", what)
+        if live:
+            _lib.launch("spr_kv4_store", dev, pages.data_ptr(), pages.shape[0], h, size, d, block_table.data_ptr(),
+                        sequences, wide, _lib.ptr(seq_ids), starts.data_ptr(), _lib.ptr(counts), k.data_ptr(),
+                        v.data_ptr(), code, b, t, *k_strides, *v_strides)
+
+    return put
+
+
 def kv4_store(pages: torch.Tensor, block_table: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
               *, counts: torch.Tensor | None = None, seq_ids: torch.Tensor | None = None,
               page_size: int | None = None) -> None:
@@ -112,25 +142,7 @@ def kv4_store(pages: torch.Tensor, block_table: torch.Tensor, k: torch.Tensor, v
     may name one token, and no other sequence may share the page written to (kv4_fork sees to that).
     A group of 32 dims with an infinity or a NaN is stored as NaN.  `page_size` is for the caller's
     check of what it hands over: a page of 2 n tokens of head dim 64 has the bytes of n of 128."""
-    what = "4-bit cache store"
-    dev = _lib.require_gpu(pages, block_table, k, v, starts, counts, seq_ids, what=what)
-    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _lib.DTYPE_CODE:
-        raise RuntimeError(f"{what}: K and V must be [B, Hkv, T, D] of one dtype (bfloat16, float16, float32), got "
-                           f"{k.dtype} {tuple(k.shape)} / {v.dtype} {tuple(v.shape)}")
-    b, h, t, d = k.shape
-    size = _page_size(pages, d, page_size, what)
-    if pages.shape[1] != h:
-        raise RuntimeError(f"{what}: K has {h} heads, the pages {pages.shape[1]}")
-    sequences, wide = _check_table(block_table, what)
-    _check_entries(b, sequences, seq_ids, counts, what)
-    _int32(starts, b, "starts", what)
-    if k.numel() == 0:
-        return
-    k, *k_strides = _by_rows(k)
-    v, *v_strides = _by_rows(v)
-    _lib.launch("spr_kv4_store", dev, pages.data_ptr(), pages.shape[0], h, size, d, block_table.data_ptr(), sequences,
-                wide, _lib.ptr(seq_ids), starts.data_ptr(), _lib.ptr(counts), k.data_ptr(), v.data_ptr(),
-                _lib.DTYPE_CODE[k.dtype], b, t, *k_strides, *v_strides)
+    store_call(pages, block_table, k, v, counts=counts, seq_ids=seq_ids, page_size=page_size)(starts)
 
 
 def kv4_load(pages: torch.Tensor, block_table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, rows: int,
@@ -236,10 +248,11 @@ def _layers(pages: torch.Tensor, num_pages: int, what: str) -> tuple[int, int, i
 
 def kv4_reserve(block_table: torch.Tensor, lengths: torch.Tensor, ref_count: torch.Tensor, page_size: int,
                 counts: torch.Tensor, *, seq_ids: torch.Tensor | None = None,
-                status: torch.Tensor | None = None) -> torch.Tensor:
+                status: torch.Tensor | None = None, most: int | None = None) -> torch.Tensor:
     """Room for counts[i] more tokens of sequence seq_ids[i] (default i): new pages (the lowest free
     ones) in its row of the table, the length with them.  Returns starts int32 [n], the place of the
-    first new token of each, or -1 for all when the call could not happen."""
+    first new token of each, or -1 for all when the call could not happen, as where a count passes
+    `most`."""
     what = "4-bit cache reserve"
     dev = _lib.require_gpu(block_table, lengths, ref_count, counts, seq_ids, status, what=what)
     sequences, wide = _check_metadata(block_table, lengths, ref_count, page_size, status, what)
@@ -247,8 +260,8 @@ def kv4_reserve(block_table: torch.Tensor, lengths: torch.Tensor, ref_count: tor
     _check_entries(n, sequences, seq_ids, None, what)
     starts = counts.new_empty(n)
     ws = _lib.workspace(_lib.query("spr_kv4_pages_workspace", ref_count.shape[0]), dev)
-    _lib.launch("spr_kv4_reserve", dev, block_table.data_ptr(), lengths.data_ptr(), ref_count.data_ptr(),
-                counts.data_ptr(), _lib.ptr(seq_ids), n, sequences, wide, page_size, ref_count.shape[0],
+    _lib.launch("spr_kv4_reserve_ex", dev, block_table.data_ptr(), lengths.data_ptr(), ref_count.data_ptr(),
+                counts.data_ptr(), _lib.ptr(seq_ids), n, 2**31 - 1 if most is None else most, sequences, wide, page_size, ref_count.shape[0],
                 starts.data_ptr(), _lib.ptr(status), ws.data_ptr(), ws.numel())
     return starts
 

@@ -61,14 +61,20 @@ class KV4Cache:
                       seq_ids=self._ints(seq_ids), page_size=self.page_size)
 
     def append(self, k, v, *, counts=None, seq_ids=None) -> torch.Tensor:
-        """reserve and store K and V [B, Hkv, T, D] of a cache of one layer; returns the starts."""
+        """reserve and store K and V [B, Hkv, T, D] of a cache of one layer; returns the starts.  What a store
+        would refuse is refused before anything is reserved, and so are counts above T (on the device,
+        as reserve refuses)."""
         if self.pages.shape[0] != 1:
             raise RuntimeError("4-bit cache append: a cache of several layers takes reserve, then store per layer")
+        rows = k.shape[2] if k.dim() == 4 else 0
         if counts is None:
-            counts = torch.full((k.shape[0],), k.shape[2], dtype=torch.int32, device=self.pages.device)
+            counts = torch.full((k.shape[0],), rows, dtype=torch.int32, device=self.pages.device)
         counts, ids = self._ints(counts), self._ints(seq_ids)
-        starts = self.reserve(counts, ids)
-        self.store(k, v, starts, counts=counts, seq_ids=ids)
+        put = kv4.store_call(self.pages[0], self.block_table, k, v, counts=counts, seq_ids=ids,
+                             page_size=self.page_size)
+        starts = kv4.kv4_reserve(self.block_table, self.lengths, self.ref_count, self.page_size, counts, seq_ids=ids,
+                                 status=self.status, most=rows)
+        put(starts)
         return starts
 
     def load(self, starts, counts, rows: int, *, seq_ids=None, layer: int = 0, dtype: torch.dtype = torch.bfloat16):

@@ -867,3 +867,34 @@ def test_packed_rows_off_sixteen_bytes_are_taken(dev, dtype):
         if dtype != "fp32":
             got[-1] += [cache.attend(x[2]), cache.attend(x[2][:, :1, :1].expand(b, h, t, d))]
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_a_refused_append_changes_nothing(dev):
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    cache = KV4Cache(8, 2, 64, 3, page_size=32, device=dev)
+    x = torch.ones((1, 2, 5, 64), dtype=torch.bfloat16, device=dev)
+    cache.append(x, x, seq_ids=[1])
+    before = [t.clone() for t in (cache.pages, cache.block_table, cache.lengths, cache.ref_count)]
+    ints = lambda *a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+    for call in (
+        lambda: cache.append(x, x.float(), seq_ids=[1]), lambda: cache.append(x, x[:, :, :4], seq_ids=[1]),
+        lambda: cache.append(x[:, :1], x[:, :1], seq_ids=[1]), lambda: cache.append(x.int(), x.int(), seq_ids=[1]),
+        lambda: cache.append(x[..., :32], x[..., :32], seq_ids=[1]), lambda: cache.append(x[0], x[0], seq_ids=[1]),
+        lambda: cache.append(x.repeat(1, 1, 1, 2), x.repeat(1, 1, 1, 2), seq_ids=[1]),
+        lambda: cache.append(x, x, counts=[3, 3], seq_ids=[0, 1]), lambda: cache.append(x, x.cpu(), seq_ids=[1]),
+    ):
+        with pytest.raises(RuntimeError):
+            call()
+        for a, b in zip(before, (cache.pages, cache.block_table, cache.lengths, cache.ref_count)):
+            assert torch.equal(a, b)
+    cache.check()
+    # counts are looked at on the device
+    for counts in ([6], ints(6), [-1]):
+        assert cache.append(x, x, counts=counts, seq_ids=[1]).tolist() == [-1]
+        with pytest.raises(RuntimeError, match="past the rows given"):
+            cache.check()
+        for a, b in zip(before, (cache.pages, cache.block_table, cache.lengths, cache.ref_count)):
+            assert torch.equal(a, b)
+    assert cache.append(x, x, counts=ints(5), seq_ids=[1]).tolist() == [5] and cache.lengths.tolist() == [0, 10, 0]
+    cache.check()
