@@ -101,6 +101,7 @@ __device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t& byte)
 }
 
 constexpr int ROW_THREADS = 256;
+constexpr int64_t MOST_BLOCKS = 0xffffffffll / ROW_THREADS;  // a launch has fewer than 2^32 threads in x
 
 // D / 8 lanes a row, K and V of it: 16 bytes in and one code word out per lane and tensor.  Rows go
 // by token inside a head, so a workgroup's codes fill neighbouring lines of one page.  Bound by memory:
@@ -772,7 +773,7 @@ extern "C" int spr_kv4_store(uint8_t* pages, int32_t num_pages, int32_t kv_heads
                 "%s: pages, K and V must be 16-byte aligned", what);
     if (batch == 0 || rows == 0) return SPR_OK;
     const int64_t blocks = spr::ceil_div(static_cast<int64_t>(kv_heads) * rows, ROW_THREADS / (D / 8));
-    SPR_REQUIRE(blocks <= INT32_MAX, "%s: too many rows", what);
+    SPR_REQUIRE(blocks <= MOST_BLOCKS, "%s: %d rows of %d heads are too many for one call", what, rows, kv_heads);
     kv4_store_kernel<T, D><<<dim3(static_cast<unsigned>(blocks), batch), ROW_THREADS, 0, stream>>>(
         a, pages, static_cast<const T*>(k), static_cast<const T*>(v), k_b, k_h, k_t, v_b, v_h, v_t);
     SPR_LAUNCHED(what);
@@ -798,7 +799,7 @@ extern "C" int spr_kv4_load(const uint8_t* pages, int32_t num_pages, int32_t kv_
                 "%s: pages, K and V must be 16-byte aligned", what);
     if (batch == 0 || rows == 0) return SPR_OK;
     const int64_t blocks = spr::ceil_div(static_cast<int64_t>(kv_heads) * rows, ROW_THREADS / (D / 8));
-    SPR_REQUIRE(blocks <= INT32_MAX, "%s: too many rows", what);
+    SPR_REQUIRE(blocks <= MOST_BLOCKS, "%s: %d rows of %d heads are too many for one call", what, rows, kv_heads);
     kv4_load_kernel<T, D><<<dim3(static_cast<unsigned>(blocks), batch), ROW_THREADS, 0, stream>>>(
         a, pages, static_cast<T*>(k), static_cast<T*>(v));
     SPR_LAUNCHED(what);

@@ -1061,6 +1061,9 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
   const int32_t group = heads / kv_heads;
   const int64_t longest = std::min<int64_t>(max_length, static_cast<int64_t>(wide) * page_size);
   const Shape s = shape_of(batch, kv_heads, group, rows, d, longest);
+  // a launch has fewer than 2^32 threads in x (8 * RUN workgroups of 512 spare: the grid is rounded up)
+  SPR_REQUIRE(s.nt != 0 || s.groups * s.nsplit <= 0xffffffffll / (64 * MANY_WAVES) - 8 * RUN,
+              "%s: %d rows of %d heads in %d sequences are too many for one call", what, rows, heads, batch);
   const size_t part = static_cast<size_t>(batch) * heads * rows * s.nsplit;
   if (s.nsplit > 1 && (workspace == nullptr || workspace_bytes < part * (d + 2) * sizeof(float))) {
     spr_set_error("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, part * (d + 2) * sizeof(float));

@@ -117,6 +117,8 @@ def store_call(pages: torch.Tensor, block_table: torch.Tensor, k: torch.Tensor, 
         raise RuntimeError(f"{what}: K has {h} heads, the pages {pages.shape[1]}")
     sequences, wide = _check_table(block_table, what)
     _check_entries(b, sequences, seq_ids, counts, what)
+    if h * t * (d // 8) > 2**32 - 256:  # threads of a launch
+        raise RuntimeError(f"{what}: {t} rows of {h} heads are too many for one call")
     code, live = _lib.DTYPE_CODE[k.dtype], k.numel() > 0
     k, *k_strides = _by_rows(k)
     v, *v_strides = _by_rows(v)

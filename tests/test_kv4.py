@@ -118,3 +118,15 @@ def test_python_refuses_cpu_tensors_and_bad_geometry():
         args = dict(num_pages=4, num_kv_heads=1, head_dim=64, max_sequences=1, device="cpu") | kw
         with pytest.raises(RuntimeError, match=text):
             KV4Cache(**args)
+
+
+def test_calls_of_more_rows_than_a_launch_has_threads_are_refused():
+    lib = _lib()
+    for d, rows in ((128, 2**28), (64, 2**29)):
+        assert lib.spr_kv4_store(16, 4, 1, 64, d, 16, 1, 4, None, 16, None, 16, 16, 0, 1, rows, 0, 0, 0, 0, 0, 0, None) == 1
+        assert f"{rows} rows of 1 heads are too many" in lib.spr_last_error().decode()
+        assert lib.spr_kv4_load(16, 4, 1, 64, d, 16, 1, 4, None, 16, 16, 16, 16, 0, 1, rows, None) == 1
+        assert f"{rows} rows of 1 heads are too many" in lib.spr_last_error().decode()
+    assert lib.spr_kv4_attention(16, 0, 0, 0, 0, 65535, 129, 129, 33, 64, 16, 4, 64, 16, 1, 4, 16, None, 16, 0, 0.1, 256,
+                                 16, None, None, 0, None) == 1
+    assert "33 rows of 129 heads in 65535 sequences are too many" in lib.spr_last_error().decode()
