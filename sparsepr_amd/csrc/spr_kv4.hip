@@ -701,6 +701,17 @@ int check_table(const char* what, int32_t sequences, int32_t wide, int32_t page_
   return SPR_OK;
 }
 
+// Pages of all layers are counted in 32 bits.
+int check_layers(const char* what, const void* pages, int64_t page_bytes, int64_t layer_bytes, int32_t layers,
+                 int32_t num_pages) {
+  SPR_REQUIRE(page_bytes > 0 && page_bytes % 16 == 0 && layers >= 1 && layer_bytes % 16 == 0 &&
+                  (layers == 1 || layer_bytes >= page_bytes * num_pages) && reinterpret_cast<uintptr_t>(pages) % 16 == 0 &&
+                  static_cast<int64_t>(layers) * num_pages <= INT32_MAX,
+              "%s: %d pages of %lld bytes, %d layers %lld bytes apart", what, num_pages,
+              static_cast<long long>(page_bytes), layers, static_cast<long long>(layer_bytes));
+  return SPR_OK;
+}
+
 int check_named(const char* what, int32_t n) {
   SPR_REQUIRE(n >= 0 && n <= MAX_NAMED, "%s: %d sequences in one call (at most %d)", what, n, MAX_NAMED);
   return SPR_OK;
@@ -867,10 +878,7 @@ extern "C" int spr_kv4_fork(uint8_t* pages, int64_t page_bytes, int64_t layer_by
   if (int st = check_pool(what, page_size, num_pages)) return st;
   if (int st = check_table(what, sequences, wide, page_size)) return st;
   if (int st = check_named(what, n)) return st;
-  SPR_REQUIRE(page_bytes > 0 && page_bytes % 16 == 0 && layers >= 1 && layer_bytes % 16 == 0 &&
-                  (layers == 1 || layer_bytes >= page_bytes * num_pages) && reinterpret_cast<uintptr_t>(pages) % 16 == 0,
-              "%s: pages of %lld bytes, %d layers %lld bytes apart", what, static_cast<long long>(page_bytes), layers,
-              static_cast<long long>(layer_bytes));
+  if (int st = check_layers(what, pages, page_bytes, layer_bytes, layers, num_pages)) return st;
   if (n == 0) return SPR_OK;
   if (int st = check_space(what, workspace, workspace_bytes, num_pages)) return st;
   PlanHeader* plan = static_cast<PlanHeader*>(workspace);
@@ -896,10 +904,7 @@ extern "C" int spr_kv4_compact(uint8_t* pages, int64_t page_bytes, int64_t layer
   const char* what = "spr_kv4_compact";
   if (int st = check_pool(what, 32, num_pages)) return st;
   if (int st = check_table(what, sequences, wide, 1)) return st;
-  SPR_REQUIRE(page_bytes > 0 && page_bytes % 16 == 0 && layers >= 1 && layer_bytes % 16 == 0 &&
-                  (layers == 1 || layer_bytes >= page_bytes * num_pages) && reinterpret_cast<uintptr_t>(pages) % 16 == 0,
-              "%s: pages of %lld bytes, %d layers %lld bytes apart", what, static_cast<long long>(page_bytes), layers,
-              static_cast<long long>(layer_bytes));
+  if (int st = check_layers(what, pages, page_bytes, layer_bytes, layers, num_pages)) return st;
   if (int st = check_space(what, workspace, workspace_bytes, num_pages)) return st;
   PlanHeader* plan = static_cast<PlanHeader*>(workspace);
   int32_t* a = static_cast<int32_t*>(workspace) + HEADER_WORDS;

@@ -130,3 +130,13 @@ def test_calls_of_more_rows_than_a_launch_has_threads_are_refused():
     assert lib.spr_kv4_attention(16, 0, 0, 0, 0, 65535, 129, 129, 33, 64, 16, 4, 64, 16, 1, 4, 16, None, 16, 0, 0.1, 256,
                                  16, None, None, 0, None) == 1
     assert "33 rows of 129 heads in 65535 sequences are too many" in lib.spr_last_error().decode()
+
+
+def test_more_pages_of_all_layers_than_an_index_counts_are_refused():
+    lib = _lib()
+    pages, layers = 2**28, 8
+    space = lib.spr_kv4_pages_workspace(pages)
+    assert lib.spr_kv4_fork(16, 16, 16 * pages, layers, 16, 16, 16, 16, 16, 1, 2, 4, 64, pages, 1, None, 16, space, None) == 1
+    assert "8 layers" in lib.spr_last_error().decode()
+    assert lib.spr_kv4_compact(16, 16, 16 * pages, layers, 16, 16, 2, 4, pages, 16, 16, space, None) == 1
+    assert "8 layers" in lib.spr_last_error().decode()
