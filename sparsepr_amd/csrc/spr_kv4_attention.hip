@@ -968,6 +968,7 @@ struct Shape {
 };
 
 Shape shape_of(int32_t batch, int32_t kv_heads, int32_t group, int32_t rows, int32_t d, int64_t max_length) {
+  max_length = std::min(max_length, spr::KV4_MOST_TOKENS);
   const int64_t total = static_cast<int64_t>(rows) * group, heads = static_cast<int64_t>(batch) * kv_heads;
   Shape s = {};
   if (total <= 32) {
@@ -1059,8 +1060,8 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
               "%s: %d rows of %d heads in %d sequences are too many for one call", what, rows, heads, batch);
   if (batch == 0 || rows == 0) return SPR_OK;
   const int32_t group = heads / kv_heads;
-  const int64_t longest = std::min<int64_t>(max_length, static_cast<int64_t>(wide) * page_size);
-  const Shape s = shape_of(batch, kv_heads, group, rows, d, longest);
+  // as the workspace query, which does not know the table
+  const Shape s = shape_of(batch, kv_heads, group, rows, d, max_length);
   // a launch has fewer than 2^32 threads in x (8 * RUN workgroups of 512 spare: the grid is rounded up)
   SPR_REQUIRE(s.nt != 0 || s.groups * s.nsplit <= 0xffffffffll / (64 * MANY_WAVES) - 8 * RUN,
               "%s: %d rows of %d heads in %d sequences are too many for one call", what, rows, heads, batch);
@@ -1085,6 +1086,7 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
   a.nsplit = s.nsplit;
   a.block_keys = s.nt != 0 ? FEW_KEYS : MANY_KEYS;
   a.tile_rows = s.nt != 0 ? 16 * s.nt : 32 * s.rb;
+  const int64_t longest = std::min<int64_t>(max_length, static_cast<int64_t>(wide) * page_size);
   a.share = static_cast<int32_t>(spr::ceil_div(std::max<int64_t>(longest, 1), static_cast<int64_t>(a.block_keys) * s.nsplit));
   a.scale_log2 = scale * LOG2E;
   if (d == 128) {

@@ -898,3 +898,24 @@ def test_a_refused_append_changes_nothing(dev):
             assert torch.equal(a, b)
     assert cache.append(x, x, counts=ints(5), seq_ids=[1]).tolist() == [5] and cache.lengths.tolist() == [0, 10, 0]
     cache.check()
+
+
+def test_the_workspace_query_is_what_a_call_needs_for_the_same_arguments(dev):
+    from sparsepr_amd import _lib
+
+    size, d = 64, 128
+    for wide in (1, 3, 17, 40, 90):
+        for rows, heads in ((1, 2), (20, 4), (64, 3), (128, 24), (200, 7)):
+            q = torch.ones((1, heads, rows, d), dtype=torch.bfloat16, device=dev)
+            out = torch.empty_like(q)
+            pages = torch.zeros((1, heads, size * (d + d // 16)), dtype=torch.uint8, device=dev)
+            table = torch.zeros((1, wide), dtype=torch.int32, device=dev)
+            n = torch.full((1,), wide * size, dtype=torch.int32, device=dev)
+            for bound in (0, 500, 2000, 9000, 1 << 20, (1 << 63) - 1):
+                need = _lib.query("spr_kv4_attention_workspace", 1, heads, heads, rows, d, bound)
+                ws = _lib.workspace(need, dev)
+                out.fill_(7)
+                _lib.launch("spr_kv4_attention", dev, q.data_ptr(), *q.stride()[:3], 0, 1, heads, heads, rows, d,
+                            pages.data_ptr(), 1, size, table.data_ptr(), 1, wide, n.data_ptr(), None, None, 0, 0.1,
+                            bound, out.data_ptr(), None, ws.data_ptr(), need)
+                assert (out == 0).all()
