@@ -14,8 +14,9 @@ and kv head (136 for D = 128, against 512 in bf16):
     cache.check()                                          # the one call that synchronises
 
 No call but `check` waits for the GPU; each runs on torch's current stream of the cache's device (calls
-on one cache from several streams are the caller's to order).  Lists become device tensors, which a
-captured graph cannot hold: pass int32 tensors there.
+on one cache from several streams are the caller's to order).  Lists become device tensors, by a copy
+from pinned memory that nothing waits for (11 us of host time each); a captured graph, which would replay what that memory holds
+later, refuses them: pass int32 tensors there.
 The calls that change pages happen whole or not at all (kernels/kv4.py)."""
 
 from __future__ import annotations
@@ -48,7 +49,14 @@ class KV4Cache:
     def _ints(self, x) -> torch.Tensor | None:
         if x is None or isinstance(x, torch.Tensor):
             return x
-        return torch.tensor(list(x), dtype=torch.int32, device=self.pages.device)
+        dev = self.pages.device
+        if dev.type != "cuda":
+            return torch.tensor(list(x), dtype=torch.int32)
+        with torch.cuda.device(dev):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("4-bit cache: a captured graph cannot hold a list; pass an int32 tensor")
+            # the pinned memory goes back to torch's host allocator, which keeps it until the copy has ended
+            return torch.tensor(list(x), dtype=torch.int32, pin_memory=True).to(dev, non_blocking=True)
 
     def reserve(self, counts, seq_ids=None) -> torch.Tensor:
         """kv4_reserve: room for counts[i] more tokens of seq_ids[i]; the place of the first of each."""

@@ -919,3 +919,75 @@ def test_the_workspace_query_is_what_a_call_needs_for_the_same_arguments(dev):
                             pages.data_ptr(), 1, size, table.data_ptr(), 1, wide, n.data_ptr(), None, None, 0, 0.1,
                             bound, out.data_ptr(), None, ws.data_ptr(), need)
                 assert (out == 0).all()
+
+
+def test_calls_with_lists_do_not_wait_for_the_gpu(dev):
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    h, d = 2, 64
+    cache = KV4Cache(200, h, d, 3, page_size=32, max_pages=40, layers=2, device=dev)
+    one = KV4Cache(20, h, d, 3, page_size=32, device=dev)
+    k, v = torch.randn((2, 1, h, 8, d), device=dev).to(torch.bfloat16)
+
+    def run():
+        starts = cache.reserve([8], [0])
+        for layer in range(2):
+            cache.store(k, v, starts, counts=[8], seq_ids=[0], layer=layer)
+            cache.attend(k, seq_ids=[0], counts=[8], layer=layer, causal=True)
+        cache.fork([0], [1])
+        cache.load([0, 0], [8, 4], 8, seq_ids=[1, 0])
+        cache.free([0], first_pages=[0], page_counts=[1])
+        cache.free([1])
+        one.append(k, v, seq_ids=[0])
+        one.append(k, v, counts=[3], seq_ids=[0])
+        cache.compact()
+
+    run()
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        run()
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    cache.check(), one.check()
+    assert one.lengths.tolist() == [22, 0, 0]
+
+
+def test_lists_hold_what_they_held_when_the_call_was_made(dev):
+    """Hundreds of calls behind a GPU that is busy, with lists that are changed right after."""
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    rng = np.random.default_rng(26)
+    cache, m = KV4Cache(3000, 1, 64, 40, page_size=32, max_pages=200, device=dev), model.Pages(3000, 40, 200, 32)
+    busy = torch.randn((8192, 8192), device=dev).to(torch.bfloat16)
+    for _ in range(30):
+        busy @ busy
+    starts = []
+    for _ in range(300):
+        ids = rng.permutation(40)[:3].tolist()
+        counts = rng.integers(0, 20, 3).tolist()
+        starts.append((cache.reserve(counts, ids), m.reserve(ids, counts)[1]))
+        ids[:], counts[:] = [39, 39, 39], [-1, -1, -1]
+    for got, want in starts:
+        assert got.tolist() == want
+    _assert_same(cache, m)
+    cache.check()
+
+
+def test_a_captured_graph_refuses_lists(dev):
+    cache = _filled(dev, 3, 2, 64, [5, 6, 7], 8)
+    ids, q = _gpu([2, 0], dev), torch.randn((2, 2, 1, 64), device=dev).to(torch.bfloat16)
+    want = cache.attend(q, seq_ids=ids)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="pass an int32 tensor"):
+            cache.attend(q, seq_ids=[2, 0])
+        with pytest.raises(RuntimeError, match="pass an int32 tensor"):
+            cache.reserve([1], [0])
+        out = cache.attend(q, seq_ids=ids)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert cache.lengths.tolist() == [5, 6, 7]
