@@ -582,7 +582,7 @@ int spr_kv4_compact(uint8_t* pages, int64_t page_bytes, int64_t layer_bytes, int
  * (nullable: rows) rows in use the last is the sequence's last token, and a row sees the tokens up to
  * its own.  Rows that see nothing, and rows past the count, are 0 with lse -inf; a page outside the
  * pool, scores that are all -inf, a sequence outside the table or a length it cannot hold gives NaN.
- * max_length (a bound on the lengths, which may be exceeded) only sizes the launch. */
+ * max_length (a bound on the lengths, which may be exceeded) only sizes the launch and the workspace. */
 size_t spr_kv4_attention_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t rows, int32_t d,
                                    int64_t max_length);
 int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_t q_t, int32_t dtype, int32_t batch,

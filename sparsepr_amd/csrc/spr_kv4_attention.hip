@@ -39,11 +39,14 @@ struct AttnArgs {
   float* lse;            // nullable
   float* part_o;         // [batch][kv_heads][nsplit][rows * group][D], unnormalised
   float* part_ml;        // the same rows' (maximum, sum)
+  int32_t* share_out;    // the share that this call's lengths gave, for the merge
   int64_t q_b, q_h, q_t;  // strides in elements
   int64_t page_stride;    // bytes
   int32_t batch, kv_heads, group, rows, sequences, wide, log_s, num_pages, causal;
-  int32_t nsplit, share;          // shares of the keys, blocks of one
+  int32_t nsplit, least_share;    // shares of the keys at most, blocks of one at least
   int32_t tile_rows, block_keys;  // query rows of a workgroup, keys of a block
+  int32_t groups, chunk_cost;     // of split_cost
+  int64_t merge_cost;
   float scale_log2;  // softmax scale * log2(e)
 };
 
@@ -92,17 +95,74 @@ __device__ __forceinline__ int32_t least_of(const AttnArgs& a, const Span& s, in
   return visible_of(a, s, min(row0 / a.group, max(s.count - 1, 0)));
 }
 
-// The keys of a tile are dealt in shares of `share` blocks, for every sequence alike: a short one takes
-// one share, and that writes its rows straight to the output; more than nsplit shares (a length past
-// the caller's bound) make them longer.
-struct Deal {
-  int32_t blocks, per, shares;
+// What a one-sequence call of the many-row kernel takes with its keys in n shares, in units of 50 ns.  One
+// workgroup a CU, so it takes whole rounds of 256, each of them a share's chunks and two more; then the
+// merge of the partial results.  Whole numbers: every workgroup has to come to the same n.
+__host__ __device__ __forceinline__ uint64_t split_cost(int32_t groups, int32_t chunk_cost, int64_t merge_cost,
+                                                        int32_t chunks, int32_t n) {
+  const uint64_t rounds = static_cast<uint64_t>(groups * static_cast<int64_t>(n) + 255) / 256;
+  const uint32_t each = static_cast<uint32_t>(chunk_cost) * static_cast<uint32_t>(chunks + 2 * n) / static_cast<uint32_t>(n);
+  return rounds * each + (n == 1 ? 0 : 120 + static_cast<uint64_t>(merge_cost) * n);
+}
+// A share has four chunks at least.
+__host__ __device__ __forceinline__ bool split_fits(int32_t chunks, int32_t n) { return n == 1 || chunks >= 4 * n; }
+
+// The largest of 64 lanes: within rows of 16 by rotations, then over the rows.
+__device__ __forceinline__ uint32_t max_wave(uint32_t x) {
+  auto turned = [](uint32_t v, auto ror) {
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ror)::value, 0xF, 0xF, false)));
+  };
+  x = turned(x, std::integral_constant<int, 0x128>{});
+  x = turned(x, std::integral_constant<int, 0x124>{});
+  x = turned(x, std::integral_constant<int, 0x122>{});
+  x = turned(x, std::integral_constant<int, 0x121>{});
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return max(b[0], b[1]);
+}
+
+constexpr int32_t ONE_SHARE = 1 << 26;  // more blocks than any sequence has
+
+// Blocks of a share of the keys, alike for all of a call's sequences, and how many the longest of them
+// takes.  From the lengths as they are, not from the caller's bound, which may be the whole table: 24 heads
+// on a table of 262,144, by the bound 3,600 tokens were one share of 24 workgroups, one row 31 us instead
+// of 13, 128 rows 71 instead of 29, and against 20,000 tokens 74 instead of 21 and 204 instead of 55.
+// COSTED: of one sequence the n <= nsplit that costs least, a lane each; else as many as there are.
+// Uniform.
+struct Share {
+  int32_t blocks, count;
 };
-__device__ __forceinline__ Deal deal_of(const AttnArgs& a, int32_t keys) {
+template <bool COSTED>
+__device__ __forceinline__ Share share_of(const AttnArgs& a, int32_t length, int lane) {
+  if (a.nsplit == 1) return {ONE_SHARE, 1};
+  if (a.batch > 1) {
+    for (int b = lane; b < a.batch; b += 64) length = max(length, span_of(a, b).length);
+    length = static_cast<int32_t>(max_wave(length));
+  }
+  const int32_t blocks = (length + a.block_keys - 1) / a.block_keys;
+  int32_t n = a.nsplit;
+  if (COSTED && a.batch == 1) {
+    uint32_t left = 0;  // to the most that 32 bits hold
+    if (lane < a.nsplit && split_fits(blocks, lane + 1)) {
+      const uint64_t cost = split_cost(a.groups, a.chunk_cost, a.merge_cost, blocks, lane + 1);
+      left = cost < 0xffffffffu ? ~static_cast<uint32_t>(cost) : 1;
+    }
+    n = __builtin_ctzll(__ballot(left == max_wave(left))) + 1;
+  }
+  const int32_t share = __builtin_amdgcn_readfirstlane(max(a.least_share, (blocks + n - 1) / n));
+  return {share, __builtin_amdgcn_readfirstlane(max(1, (blocks + share - 1) / share))};
+}
+
+// The keys of a tile in shares of `share` blocks: a short sequence takes one share, and that writes its
+// rows straight to the output.
+struct Deal {
+  int32_t blocks, shares;
+};
+__device__ __forceinline__ Deal deal_of(const AttnArgs& a, int32_t share, int32_t keys) {
   Deal d;
   d.blocks = (keys + a.block_keys - 1) / a.block_keys;
-  d.per = max(a.share, (d.blocks + a.nsplit - 1) / a.nsplit);
-  d.shares = max(1, (d.blocks + d.per - 1) / d.per);
+  d.shares = max(1, (d.blocks + share - 1) / share);
   return d;
 }
 
@@ -226,7 +286,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
   const int split = (blockIdx.x + blockIdx.y + blockIdx.z) % a.nsplit;
   const int total_rows = a.rows * a.group;
   const Span sp = span_of(a, b);
-  const Deal deal = deal_of(a, most_of(a, sp, 0));
+  const int32_t share = share_of<false>(a, sp.length, lane).blocks;
+  const Deal deal = deal_of(a, share, most_of(a, sp, 0));
   if (split >= deal.shares) return;
   const int32_t* row_table = a.table + static_cast<int64_t>(sp.seq) * a.wide;
 
@@ -248,7 +309,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
     }
   }
   const int32_t least = least_of(a, sp, 0);
-  const int32_t last = min(deal.blocks, (split + 1) * deal.per);
+  const int32_t last = min(deal.blocks, (split + 1) * share);
 
   const uint32_t cut = TWICE && m >= 8 ? 0xffff0000u : 0u;
   f32x4 acc[NT][VT];
@@ -410,7 +471,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
   // half as many registers again.  Two sets of registers in turn: copying the next block's to the current
   // one's cost 10 % on 48 sequences.  (Inlined by force: called, the steps keep them in scratch.)
   const int whole = min(last, least / FEW_KEYS);
-  int blk = split * deal.per + wave;
+  int blk = split * share + wave;
   if (blk < last) {
     Held<D> x0, x1;
     fetch(blk, x0);
@@ -432,6 +493,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, NT == 1 ? 3 : 2) void kv4_few_kerne
     walk(last, std::true_type{});
   }
 
+  // (behind the walk: a store before it would keep the table's pages out of scalar loads, 76 -> 85 us)
+  if (a.nsplit > 1 && blockIdx.x + blockIdx.y + blockIdx.z == 0 && threadIdx.x == 0) *a.share_out = share;
   // merge the waves, one 16-row tile at a time, through the V rows
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -561,16 +624,20 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
   // runs of RUN consecutive tiles of one head and share on one XCD (workgroup b runs on XCD b mod 8):
   // they read the same codes, and shares of unlike length still spread over all XCDs
   const int total_rows = a.rows * a.group;
-  const int tiles = (total_rows + TROWS - 1) / TROWS;
-  const int64_t total = static_cast<int64_t>(tiles) * a.nsplit * a.kv_heads * a.batch;
-  const int64_t id = static_cast<int64_t>(blockIdx.x / (8 * RUN)) * (8 * RUN) + (blockIdx.x & 7) * RUN + (blockIdx.x >> 3) % RUN;
-  if (id >= total) return;
-  const int tile = static_cast<int>(id % tiles);
-  const int64_t bh = id / tiles / a.nsplit;
+  const uint32_t tiles = (total_rows + TROWS - 1) / TROWS;
+  const uint32_t heads = static_cast<uint32_t>(a.kv_heads) * a.batch;
+  const uint32_t id = blockIdx.x / (8 * RUN) * (8 * RUN) + (blockIdx.x & 7) * RUN + (blockIdx.x >> 3) % RUN;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Share dealt = share_of<true>(a, a.batch == 1 ? span_of(a, 0).length : 0, lane);
+  const int32_t share = dealt.blocks;
+  // the shares that the lengths leave empty are the grid's last workgroups, not between the others (128
+  // rows, 20,000 tokens on a table of 262,144: 90 -> 55 us)
+  const uint32_t bhs = id / tiles, bh = bhs / dealt.count;
+  const int tile = static_cast<int>(id - bhs * tiles);
+  if (bh >= heads) return;
   // with few tiles a head the shares turn from head to head, as in the few-row kernel (4 sequences of 64
   // rows 59 -> 54 us); with many it would only bring some of the long ones late (13 tiles 81 -> 105 us)
-  const int split = static_cast<int>((id / tiles + (tiles <= RUN ? bh : 0)) % a.nsplit);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int split = static_cast<int>((bhs + (tiles <= RUN ? bh : 0)) % dealt.count);
   const int hk = static_cast<int>(bh % a.kv_heads), b = sequence_at(a, static_cast<int>(bh / a.kv_heads), lane);
 
   const int col = lane & 31, half = lane >> 5;
@@ -578,7 +645,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
   const Span sp = span_of(a, b);
   const int row0 = tile * TROWS;
   const int32_t most = most_of(a, sp, row0), least = least_of(a, sp, row0);
-  const Deal deal = deal_of(a, most);
+  const Deal deal = deal_of(a, share, most);
   if (split >= deal.shares) return;
   const int32_t* row_table = a.table + static_cast<int64_t>(sp.seq) * a.wide;
 
@@ -590,7 +657,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
   const int w0 = row0 + blk * 32;
   const bool wave_live = w0 < total_rows && w0 / a.group < sp.count;
   const int32_t wave_least = least_of(a, sp, w0);
-  const int c0 = split * deal.per, nch = min(deal.blocks, c0 + deal.per) - c0;
+  const int c0 = split * share, nch = min(deal.blocks, c0 + share) - c0;
 
   u32x4 qh[KSTEPS], ql[F16 ? KSTEPS : 1];
   const uint16_t* qp = a.q + b * a.q_b + h * a.q_h + t * a.q_t + half * 8;
@@ -816,6 +883,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
     }
   }
 
+  if (a.nsplit > 1 && blockIdx.x == 0 && threadIdx.x == 0) *a.share_out = share;
   float l_tot = sum_xor32(l_run);
   if constexpr (PARTS > 1) {
     // the other parts hand (m, l, O) to part 0 through the tiles: 32 rows of D floats each
@@ -905,7 +973,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, int64_t all_
   const int rho = static_cast<int>(in ? row % total_rows : 0);
   const int b = static_cast<int>(bh / a.kv_heads), hk = static_cast<int>(bh % a.kv_heads);
   const Span sp = span_of(a, b);
-  const int32_t shares = in ? deal_of(a, most_of(a, sp, rho / a.tile_rows * a.tile_rows)).shares : 1;
+  const int32_t shares = in ? deal_of(a, *a.share_out, most_of(a, sp, rho / a.tile_rows * a.tile_rows)).shares : 1;
   if (P == 1 && shares == 1) return;  // written already, or no row
   const int64_t first = bh * a.nsplit * total_rows + rho;
   float top = NEG_INF;
@@ -959,46 +1027,59 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, int64_t all_
 // ---------------------------------------------------------------------------- host
 
 // How a call is cut up: by the few-row kernel in 16 * nt rows, or by the many-row one in 64, 128 or 256
-// rows, and the keys in nsplit shares.
+// rows, and the keys in at most nsplit shares.
 struct Shape {
-  int32_t nt;  // 0: the many-row kernel
-  int32_t rb;  // its row blocks of 32
-  int32_t nsplit;
-  int64_t groups;  // workgroups to a share
+  int32_t nt;           // 0: the many-row kernel
+  int32_t rb;           // its row blocks of 32
+  int32_t fill;         // shares of a sequence of any length
+  int32_t nsplit;       // and of one within max_length
+  int32_t least_share;  // blocks of a share at least
+  int64_t groups;       // workgroups to a share
+  int32_t chunk_cost;   // of split_cost
+  int64_t merge_cost;
 };
 
 Shape shape_of(int32_t batch, int32_t kv_heads, int32_t group, int32_t rows, int32_t d, int64_t max_length) {
   max_length = std::min(max_length, spr::KV4_MOST_TOKENS);
   const int64_t total = static_cast<int64_t>(rows) * group, heads = static_cast<int64_t>(batch) * kv_heads;
   Shape s = {};
+  auto within = [&](int64_t block_keys) {  // shares that sequences of max_length can take
+    const int64_t shares = spr::ceil_div(std::max<int64_t>(max_length, 1), block_keys * s.least_share);
+    return static_cast<int32_t>(std::min<int64_t>(s.fill, shares));
+  };
   if (total <= 32) {
     s.nt = total <= 16 ? 1 : 2;
     s.groups = heads;
     // Three workgroups for every CU, in one round, where there is one sequence; two rounds where there are
     // several, whose lengths are not known here, so that long ones are dealt finer (48 ragged ones in one
     // round 55 us, in two 36; 16 alike 31 and 34).  None of less than four blocks a wave.
-    const int64_t fill = std::max<int64_t>(1, (batch == 1 ? 768 : 1536) / s.groups);
-    const int64_t most = std::max<int64_t>(1, max_length / (4 * FEW_WAVES * FEW_KEYS));
-    s.nsplit = static_cast<int32_t>(std::min({fill, most, int64_t{256}}));
+    s.fill = static_cast<int32_t>(std::min<int64_t>(std::max<int64_t>(1, (batch == 1 ? 768 : 1536) / s.groups), 256));
+    s.least_share = 4 * FEW_WAVES;
+    s.nsplit = within(FEW_KEYS);
     return s;
   }
   s.rb = total <= 64 ? 2 : total <= 128 ? 4 : 8;
   s.groups = heads * spr::ceil_div(total, 32 * s.rb);
-  const int64_t chunks = std::max<int64_t>(1, spr::ceil_div(max_length, MANY_KEYS));
+  s.least_share = 4;
   if (batch > 1) {
-    s.nsplit = static_cast<int32_t>(std::min({std::max<int64_t>(1, 1024 / s.groups), std::max<int64_t>(1, chunks / 4), int64_t{64}}));
+    s.fill = static_cast<int32_t>(std::min<int64_t>(std::max<int64_t>(1, 1024 / s.groups), 64));
+    s.nsplit = within(MANY_KEYS);
     return s;
   }
-  // one workgroup a CU, so a call takes whole rounds of 256: the shares that come out fastest, at what a
-  // chunk takes and 4 TB/s for the partial results
-  double best = 0.0;
-  for (int32_t n = 1; n <= 64 && (n == 1 || chunks >= 4 * n); ++n) {
-    const double rounds = static_cast<double>(spr::ceil_div(s.groups * n, 256));
-    const double each = (s.rb == 8 ? 3.8 : s.rb == 4 ? 2.1 : 1.2) * (static_cast<double>(chunks) / n + 2.0);
-    const double merge = n == 1 ? 0.0 : 6.0 + 8e-6 / 4.0 * d * static_cast<double>(heads * total) * n;
-    const double us = rounds * each + merge;
-    if (n == 1 || us < best) best = us, s.nsplit = n;
-  }
+  // the shares that come out fastest, at what a chunk takes and 4 TB/s for the partial results
+  s.chunk_cost = s.rb == 8 ? 76 : s.rb == 4 ? 42 : 24;
+  s.merge_cost = heads * total * d / 25000;
+  const int32_t groups = static_cast<int32_t>(std::min<int64_t>(s.groups, INT32_MAX));
+  auto best = [&](int64_t length) {
+    const int32_t chunks = static_cast<int32_t>(std::max<int64_t>(1, spr::ceil_div(length, MANY_KEYS)));
+    int32_t at = 1;
+    for (int32_t n = 2; n <= 64 && split_fits(chunks, n); ++n) {
+      if (split_cost(groups, s.chunk_cost, s.merge_cost, chunks, n) < split_cost(groups, s.chunk_cost, s.merge_cost, chunks, at)) at = n;
+    }
+    return at;
+  };
+  s.fill = best(spr::KV4_MOST_TOKENS);
+  s.nsplit = best(max_length);
   return s;
 }
 
@@ -1018,13 +1099,17 @@ void launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   }
   if (s.nsplit > 1) {
     const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.group * a.rows;
-    // as many teams to a row as there are shares and room for on the card
+    // as many teams to a row as a long sequence has shares and there is room for on the card (200 rows of
+    // 4 heads 37 us by teams of 16, 35 by 4; 72 rows of 30 shares 23 and 27)
     const unsigned all = static_cast<unsigned>(rows);
-    if (s.nsplit >= 16 && rows <= 4096) kv4_merge_kernel<D, F16, 16><<<all, 256, 0, stream>>>(a, rows);
-    else if (s.nsplit >= 4 && rows <= 16384) kv4_merge_kernel<D, F16, 4><<<(all + 3) / 4, 256, 0, stream>>>(a, rows);
+    if (s.fill >= 16 && rows <= 512) kv4_merge_kernel<D, F16, 16><<<all, 256, 0, stream>>>(a, rows);
+    else if (s.fill >= 4 && rows <= 16384) kv4_merge_kernel<D, F16, 4><<<(all + 3) / 4, 256, 0, stream>>>(a, rows);
     else kv4_merge_kernel<D, F16, 1><<<(all + 15) / 16, 256, 0, stream>>>(a, rows);
   }
 }
+
+// `part` partial rows, their (maximum, sum) and the share.
+size_t workspace_bytes_of(size_t part, int32_t d) { return part * (d + 2) * sizeof(float) + 16; }
 
 }  // namespace
 
@@ -1033,7 +1118,7 @@ extern "C" size_t spr_kv4_attention_workspace(int32_t batch, int32_t heads, int3
   if (batch <= 0 || kv_heads <= 0 || rows <= 0 || heads % kv_heads != 0) return 0;
   const Shape s = shape_of(batch, kv_heads, heads / kv_heads, rows, d, max_length);
   if (s.nsplit <= 1) return 0;
-  return static_cast<size_t>(batch) * heads * rows * s.nsplit * (d + 2) * sizeof(float);
+  return workspace_bytes_of(static_cast<size_t>(batch) * heads * rows * s.nsplit, d);
 }
 
 extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_t q_t, int32_t dtype, int32_t batch,
@@ -1066,8 +1151,8 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
   SPR_REQUIRE(s.nt != 0 || s.groups * s.nsplit <= 0xffffffffll / (64 * MANY_WAVES) - 8 * RUN,
               "%s: %d rows of %d heads in %d sequences are too many for one call", what, rows, heads, batch);
   const size_t part = static_cast<size_t>(batch) * heads * rows * s.nsplit;
-  if (s.nsplit > 1 && (workspace == nullptr || workspace_bytes < part * (d + 2) * sizeof(float))) {
-    spr_set_error("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, part * (d + 2) * sizeof(float));
+  if (s.nsplit > 1 && (workspace == nullptr || workspace_bytes < workspace_bytes_of(part, d))) {
+    spr_set_error("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, workspace_bytes_of(part, d));
     return SPR_EWORKSPACE;
   }
   AttnArgs a;
@@ -1078,16 +1163,17 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
   a.lse = lse;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + part * d;
+  a.share_out = reinterpret_cast<int32_t*>(a.part_ml + part * 2);
   a.q_b = q_b, a.q_h = q_h, a.q_t = q_t;
   a.page_stride = kv_heads * spr::kv4_head_bytes(page_size, d);
   a.batch = batch, a.kv_heads = kv_heads, a.group = group, a.rows = rows, a.sequences = sequences, a.wide = wide;
   a.log_s = 31 - __builtin_clz(static_cast<unsigned>(page_size));
   a.num_pages = num_pages, a.causal = causal;
-  a.nsplit = s.nsplit;
+  a.nsplit = s.nsplit, a.least_share = s.least_share;
+  a.groups = static_cast<int32_t>(std::min<int64_t>(s.groups, INT32_MAX));
+  a.chunk_cost = s.chunk_cost, a.merge_cost = s.merge_cost;
   a.block_keys = s.nt != 0 ? FEW_KEYS : MANY_KEYS;
   a.tile_rows = s.nt != 0 ? 16 * s.nt : 32 * s.rb;
-  const int64_t longest = std::min<int64_t>(max_length, static_cast<int64_t>(wide) * page_size);
-  a.share = static_cast<int32_t>(spr::ceil_div(std::max<int64_t>(longest, 1), static_cast<int64_t>(a.block_keys) * s.nsplit));
   a.scale_log2 = scale * LOG2E;
   if (d == 128) {
     if (dtype == 1) launch<128, true>(a, s, stream);

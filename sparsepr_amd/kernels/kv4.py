@@ -184,8 +184,9 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     sequence seq_ids[b] (default b) with its first counts[b] rows (default all).  With `causal` the last
     row in use is the sequence's last token and each row sees the tokens up to its own (store them
     first).  Rows that see nothing, and rows past the count, are 0 with lse -inf.  `max_length`, the
-    longest length the caller knows of (default: what the table can hold), only sizes the launch;
-    `page_size` is checked, as in kv4_store."""
+    longest length the caller knows of (default: what the table can hold), only sizes the launch and its
+    workspace, and may be passed: the keys are dealt by the lengths as they are.  `page_size` is checked,
+    as in kv4_store."""
     what = "4-bit cache attention"
     dev = _lib.require_gpu(q, pages, block_table, lengths, counts, seq_ids, what=what)
     if q.dim() != 4 or q.dtype not in (torch.bfloat16, torch.float16):

@@ -991,3 +991,21 @@ def test_a_captured_graph_refuses_lists(dev):
         torch.cuda.synchronize()
         assert torch.equal(out, want)
     assert cache.lengths.tolist() == [5, 6, 7]
+
+
+@pytest.mark.parametrize("rows,heads,lengths", [
+    (1, 24, [3600]), (1, 24, [20000]), (12, 24, [3600]), (30, 8, [20000]), (128, 24, [3600]), (128, 24, [20000]),
+    (1, 8, [3600, 0, 9000]), (64, 4, [3600, 9000, 33])])
+def test_a_loose_bound_deals_the_keys_as_the_exact_one(dev, rows, heads, lengths):
+    """The bits depend on how the keys are dealt out: they do not move with `max_length`."""
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    d, b = 128, len(lengths)
+    cache = KV4Cache(sum(-(-n // 64) for n in lengths), heads, d, b, max_pages=4096, device=dev)
+    k, v = torch.randn((2, b, heads, max(lengths), d), device=dev).to(torch.bfloat16)
+    cache.append(k, v, counts=lengths)
+    q = torch.randn((b, heads, rows, d), device=dev).to(torch.bfloat16)
+    want = cache.attend(q, max_length=max(lengths), return_lse=True)
+    for bound in (max(lengths) + 1000, 60000, None):
+        got = cache.attend(q, max_length=bound, return_lse=True)
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), bound
