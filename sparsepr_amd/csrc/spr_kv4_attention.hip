@@ -101,7 +101,8 @@ __device__ __forceinline__ int32_t least_of(const AttnArgs& a, const Span& s, in
 __host__ __device__ __forceinline__ uint64_t split_cost(int32_t groups, int32_t chunk_cost, int64_t merge_cost,
                                                         int32_t chunks, int32_t n) {
   const uint64_t rounds = static_cast<uint64_t>(groups * static_cast<int64_t>(n) + 255) / 256;
-  const uint32_t each = static_cast<uint32_t>(chunk_cost) * static_cast<uint32_t>(chunks + 2 * n) / static_cast<uint32_t>(n);
+  const uint32_t all = static_cast<uint32_t>(chunk_cost) * static_cast<uint32_t>(chunks + 2 * n);
+  const uint32_t each = all / static_cast<uint32_t>(n);
   return rounds * each + (n == 1 ? 0 : 120 + static_cast<uint64_t>(merge_cost) * n);
 }
 // A share has four chunks at least.
@@ -110,7 +111,8 @@ __host__ __device__ __forceinline__ bool split_fits(int32_t chunks, int32_t n) {
 // The largest of 64 lanes: within rows of 16 by rotations, then over the rows.
 __device__ __forceinline__ uint32_t max_wave(uint32_t x) {
   auto turned = [](uint32_t v, auto ror) {
-    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ror)::value, 0xF, 0xF, false)));
+    const int w = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ror)::value, 0xF, 0xF, false);
+    return max(v, static_cast<uint32_t>(w));
   };
   x = turned(x, std::integral_constant<int, 0x128>{});
   x = turned(x, std::integral_constant<int, 0x124>{});
@@ -1039,7 +1041,7 @@ struct Shape {
   int64_t merge_cost;
 };
 
-Shape shape_of(int32_t batch, int32_t kv_heads, int32_t group, int32_t rows, int32_t d, int64_t max_length) {
+Shape shape_of(int32_t batch, int32_t kv_heads, int32_t group, int32_t rows, int32_t d, bool f16, int64_t max_length) {
   max_length = std::min(max_length, spr::KV4_MOST_TOKENS);
   const int64_t total = static_cast<int64_t>(rows) * group, heads = static_cast<int64_t>(batch) * kv_heads;
   Shape s = {};
@@ -1066,15 +1068,20 @@ Shape shape_of(int32_t batch, int32_t kv_heads, int32_t group, int32_t rows, int
     s.nsplit = within(MANY_KEYS);
     return s;
   }
-  // the shares that come out fastest, at what a chunk takes and 4 TB/s for the partial results
-  s.chunk_cost = s.rb == 8 ? 76 : s.rb == 4 ? 42 : 24;
+  // the shares that come out fastest, at what a chunk takes (256 workgroups on K and V of their own, 8,192
+  // and 24,576 keys; units of 50 ns) and 4 TB/s for the partial results
+  constexpr int32_t chunk[2][2][3] = {{{20, 30, 50}, {24, 41, 77}},  // [D 64, 128][bf16, fp16][RB 2, 4, 8]
+                                      {{31, 47, 80}, {43, 74, 142}}};
+  s.chunk_cost = chunk[d == 128 ? 1 : 0][f16 ? 1 : 0][s.rb == 8 ? 2 : s.rb == 4 ? 1 : 0];
   s.merge_cost = heads * total * d / 25000;
   const int32_t groups = static_cast<int32_t>(std::min<int64_t>(s.groups, INT32_MAX));
   auto best = [&](int64_t length) {
     const int32_t chunks = static_cast<int32_t>(std::max<int64_t>(1, spr::ceil_div(length, MANY_KEYS)));
     int32_t at = 1;
+    uint64_t least = split_cost(groups, s.chunk_cost, s.merge_cost, chunks, 1);
     for (int32_t n = 2; n <= 64 && split_fits(chunks, n); ++n) {
-      if (split_cost(groups, s.chunk_cost, s.merge_cost, chunks, n) < split_cost(groups, s.chunk_cost, s.merge_cost, chunks, at)) at = n;
+      const uint64_t cost = split_cost(groups, s.chunk_cost, s.merge_cost, chunks, n);
+      if (cost < least) least = cost, at = n;
     }
     return at;
   };
@@ -1116,9 +1123,11 @@ size_t workspace_bytes_of(size_t part, int32_t d) { return part * (d + 2) * size
 extern "C" size_t spr_kv4_attention_workspace(int32_t batch, int32_t heads, int32_t kv_heads, int32_t rows, int32_t d,
                                               int64_t max_length) {
   if (batch <= 0 || kv_heads <= 0 || rows <= 0 || heads % kv_heads != 0) return 0;
-  const Shape s = shape_of(batch, kv_heads, heads / kv_heads, rows, d, max_length);
-  if (s.nsplit <= 1) return 0;
-  return workspace_bytes_of(static_cast<size_t>(batch) * heads * rows * s.nsplit, d);
+  int32_t nsplit = 1;  // of either type
+  for (bool f16 : {false, true}) {
+    nsplit = std::max(nsplit, shape_of(batch, kv_heads, heads / kv_heads, rows, d, f16, max_length).nsplit);
+  }
+  return nsplit == 1 ? 0 : workspace_bytes_of(static_cast<size_t>(batch) * heads * rows * nsplit, d);
 }
 
 extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_t q_t, int32_t dtype, int32_t batch,
@@ -1146,7 +1155,7 @@ extern "C" int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_
   if (batch == 0 || rows == 0) return SPR_OK;
   const int32_t group = heads / kv_heads;
   // as the workspace query, which does not know the table
-  const Shape s = shape_of(batch, kv_heads, group, rows, d, max_length);
+  const Shape s = shape_of(batch, kv_heads, group, rows, d, dtype == 1, max_length);
   // a launch has fewer than 2^32 threads in x (8 * RUN workgroups of 512 spare: the grid is rounded up)
   SPR_REQUIRE(s.nt != 0 || s.groups * s.nsplit <= 0xffffffffll / (64 * MANY_WAVES) - 8 * RUN,
               "%s: %d rows of %d heads in %d sequences are too many for one call", what, rows, heads, batch);

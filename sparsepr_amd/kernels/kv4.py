@@ -264,8 +264,8 @@ def kv4_reserve(block_table: torch.Tensor, lengths: torch.Tensor, ref_count: tor
     starts = counts.new_empty(n)
     ws = _lib.workspace(_lib.query("spr_kv4_pages_workspace", ref_count.shape[0]), dev)
     _lib.launch("spr_kv4_reserve_ex", dev, block_table.data_ptr(), lengths.data_ptr(), ref_count.data_ptr(),
-                counts.data_ptr(), _lib.ptr(seq_ids), n, 2**31 - 1 if most is None else most, sequences, wide, page_size, ref_count.shape[0],
-                starts.data_ptr(), _lib.ptr(status), ws.data_ptr(), ws.numel())
+                counts.data_ptr(), _lib.ptr(seq_ids), n, 2**31 - 1 if most is None else most, sequences, wide,
+                page_size, ref_count.shape[0], starts.data_ptr(), _lib.ptr(status), ws.data_ptr(), ws.numel())
     return starts
 
 

@@ -15,8 +15,8 @@ and kv head (136 for D = 128, against 512 in bf16):
 
 No call but `check` waits for the GPU; each runs on torch's current stream of the cache's device (calls
 on one cache from several streams are the caller's to order).  Lists become device tensors, by a copy
-from pinned memory that nothing waits for (11 us of host time each); a captured graph, which would replay what that memory holds
-later, refuses them: pass int32 tensors there.
+from pinned memory that nothing waits for (11 us of host time each); a captured graph, which would
+replay what that memory holds later, refuses them: pass int32 tensors there.
 The calls that change pages happen whole or not at all (kernels/kv4.py)."""
 
 from __future__ import annotations

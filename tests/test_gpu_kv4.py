@@ -801,7 +801,8 @@ def test_scale_bytes_past_the_encoders_are_nan(dev, rows, byte):
             q = torch.randn((1, 2, rows, d), device=dev).to(torch.bfloat16)
             out, lse = kv4_attention(q, gp, gt, _gpu([n], dev), causal=True, return_lse=True)
             _check_attention(out, lse, q, pages, table, [n], [rows], size, True, d**-0.5, "bf16")
-            for got, want in zip(kv4_load(gp, gt, _gpu([0], dev), _gpu([n], dev), n, d), model.tokens(pages, table[0], n, size, d)):
+            loaded = kv4_load(gp, gt, _gpu([0], dev), _gpu([n], dev), n, d)
+            for got, want in zip(loaded, model.tokens(pages, table[0], n, size, d)):
                 assert np.array_equal(got[0].double().cpu().numpy(), want, equal_nan=True)
 
 
@@ -900,13 +901,14 @@ def test_a_refused_append_changes_nothing(dev):
     cache.check()
 
 
-def test_the_workspace_query_is_what_a_call_needs_for_the_same_arguments(dev):
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_the_workspace_query_is_what_a_call_needs_for_the_same_arguments(dev, dtype):
     from sparsepr_amd import _lib
 
     size, d = 64, 128
     for wide in (1, 3, 17, 40, 90):
         for rows, heads in ((1, 2), (20, 4), (64, 3), (128, 24), (200, 7)):
-            q = torch.ones((1, heads, rows, d), dtype=torch.bfloat16, device=dev)
+            q = torch.ones((1, heads, rows, d), dtype=DT[dtype], device=dev)
             out = torch.empty_like(q)
             pages = torch.zeros((1, heads, size * (d + d // 16)), dtype=torch.uint8, device=dev)
             table = torch.zeros((1, wide), dtype=torch.int32, device=dev)
@@ -915,9 +917,9 @@ def test_the_workspace_query_is_what_a_call_needs_for_the_same_arguments(dev):
                 need = _lib.query("spr_kv4_attention_workspace", 1, heads, heads, rows, d, bound)
                 ws = _lib.workspace(need, dev)
                 out.fill_(7)
-                _lib.launch("spr_kv4_attention", dev, q.data_ptr(), *q.stride()[:3], 0, 1, heads, heads, rows, d,
-                            pages.data_ptr(), 1, size, table.data_ptr(), 1, wide, n.data_ptr(), None, None, 0, 0.1,
-                            bound, out.data_ptr(), None, ws.data_ptr(), need)
+                _lib.launch("spr_kv4_attention", dev, q.data_ptr(), *q.stride()[:3], _lib.DTYPE_CODE[q.dtype], 1, heads,
+                            heads, rows, d, pages.data_ptr(), 1, size, table.data_ptr(), 1, wide, n.data_ptr(), None,
+                            None, 0, 0.1, bound, out.data_ptr(), None, ws.data_ptr(), need)
                 assert (out == 0).all()
 
 
