@@ -1011,3 +1011,58 @@ def test_a_loose_bound_deals_the_keys_as_the_exact_one(dev, rows, heads, lengths
     for bound in (max(lengths) + 1000, 60000, None):
         got = cache.attend(q, max_length=bound, return_lse=True)
         assert all(torch.equal(x, y) for x, y in zip(got, want)), bound
+
+
+@pytest.mark.parametrize("count", [1, 63, 64, 65, 100, -1])
+def test_ranges_of_long_rows_close_up(dev, count):
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    tokens = [300 * 32, 130 * 32 - 5, 257 * 32 + 1]
+    for firsts in ([0, 199, 1], [63, 1, 30], [128, 64, 0]):
+        cache = KV4Cache(700, 1, 64, 3, page_size=32, max_pages=300, device=dev)
+        m = model.Pages(700, 3, 300, 32)
+        cache.reserve(tokens), m.reserve([0, 1, 2], tokens)
+        cache.free([2, 0, 1], first_pages=firsts, page_counts=[count] * 3)
+        assert m.free([2, 0, 1], firsts, [count] * 3) == 0
+        _assert_same(cache, m)
+        cache.check()
+
+
+def test_ranges_of_more_sequences_than_one_launch_frees(dev):
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    rng = np.random.default_rng(24)
+    n = 70
+    tokens = rng.integers(1, 130 * 32, n).tolist()
+    num = sum(-(-t // 32) for t in tokens) + n
+    cache, m = KV4Cache(num, 1, 64, 2 * n, page_size=32, max_pages=130, device=dev), model.Pages(num, 2 * n, 130, 32)
+    cache.reserve(tokens, list(range(n))), m.reserve(list(range(n)), tokens)
+    cache.fork(list(range(n)), list(range(n, 2 * n))), m.fork(list(range(n)), list(range(n, 2 * n)), True)
+    ids = rng.permutation(2 * n)[:100].tolist()
+    held = [-(-tokens[i % n] // 32) for i in ids]
+    firsts = [int(rng.integers(0, k + 1)) for k in held]
+    counts = [int(rng.integers(-1, k - f + 1)) for f, k in zip(firsts, held)]
+    cache.free(ids, first_pages=firsts, page_counts=counts)
+    assert m.free(ids, firsts, counts) == 0
+    _assert_same(cache, m)
+    before = m.table.copy()
+    cache.free(ids, first_pages=[0] * 99 + [131], page_counts=[0] * 99 + [1])  # refused whole
+    assert _status(cache) == 3 and np.array_equal(before, m.table)
+    _assert_same(cache, m)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_more_sequences_than_a_wave_ranks(dev, rows):
+    from sparsepr_amd.kernels.kv4 import kv4_attention
+
+    rng = np.random.default_rng(25)
+    hk, d, size, n = 1, 64, 64, 70
+    lengths = rng.integers(0, 900, n).tolist()
+    lengths[5] = 2900  # several shares, and the last one in the batch
+    num = sum(-(-t // size) for t in lengths)
+    pages, table = _pool(rng, num, hk, size, d), _table(rng, lengths, size, num, 46)
+    ids = [i for i in rng.permutation(n).tolist() if i != 5] + [5]
+    q = torch.randn((n, 1, rows, d), device=dev).to(torch.bfloat16)
+    out, lse = kv4_attention(q, _gpu(pages, dev, torch.uint8), _gpu(table, dev), _gpu(lengths, dev),
+                             seq_ids=_gpu(ids, dev), causal=True, return_lse=True)
+    _check_attention(out, lse, q, pages, table, lengths, [rows] * n, size, True, d**-0.5, "bf16", ids)
