@@ -105,7 +105,7 @@ constexpr int64_t MOST_BLOCKS = 0xffffffffll / ROW_THREADS;  // a launch has few
 
 // D / 8 lanes a row, K and V of it: 16 bytes in and one code word out per lane and tensor.  Rows go
 // by token inside a head, so a workgroup's codes fill neighbouring lines of one page.  Bound by memory:
-// a frame of 3600 tokens of 24 heads of 128 dims, 56 MB, takes 11.5 us, 4.9 TB/s (a large copy: 4.9);
+// a frame of 3600 tokens of 24 heads of 128 dims, 56 MB, takes 11.8 us, 4.8 TB/s (a large copy: 4.9);
 // 48 new tokens of 8 heads 3.2 us, a launch.
 template <typename T, int D>
 __global__ __launch_bounds__(ROW_THREADS) void kv4_store_kernel(RowArgs a, uint8_t* __restrict__ pages,
@@ -156,7 +156,7 @@ __device__ __forceinline__ void write8(T* p, u32x4 x) {
 }
 
 // The same walk the other way: out [b, kv_heads, rows, D].  Rows past the entry's count are zeros,
-// rows with no page NaN.  11.5 us for the same frame.
+// rows with no page NaN.  11.6 us for the same frame.
 template <typename T, int D>
 __global__ __launch_bounds__(ROW_THREADS) void kv4_load_kernel(RowArgs a, const uint8_t* __restrict__ pages,
                                                                T* __restrict__ k, T* __restrict__ v) {

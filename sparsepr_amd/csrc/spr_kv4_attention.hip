@@ -9,8 +9,10 @@
 //
 // K and V values (code times scale) are exact in bf16, so the conversion to the MFMA's operand loses
 // nothing; fp16 queries and probabilities go in as two bf16 terms (hi + lo) and lose at most 2^-14
-// of themselves.  Scores, the running maximum and sum and the output are fp32; bf16 calls round each
-// probability to bf16 once, relative to a maximum at most 2^8 below the row's own.
+// of themselves.  Scores, the running maximum and sum and the output are fp32.  bf16 calls of more than
+// 8 rows round each probability to bf16 once, relative to a maximum at most 2^8 below the row's own: the
+// output is off by 0.0023 of its norm where its own rounding leaves 0.0017, and a second term for the rest
+// costs 25 to 38 % from 33 rows on (a frame 5.00 -> 6.90 ms).
 #include <algorithm>
 #include <type_traits>
 
@@ -262,9 +264,10 @@ struct Held {
 // LDS is busy a third of the time).
 //
 // Bound by memory: one row of 24 heads against 118,800 tokens of 128 dims, 388 MB, takes 71 us, 5.5 TB/s
-// (a large copy moves 4.9), and 5 us more for the merge of its 32 shares; 48 ragged sequences of up to
-// 8,191 tokens, 32 heads on 8, 119 MB in 33 us; a short call of 301 tokens 5.9 us.  The next block's
-// codes are in flight while one is computed, with three waves a SIMD (149 registers for D = 128).
+// (a large copy moves 4.9), and 5 us more for the merge of its 32 shares; 16 rows 74 us, 32 rows 118 (210
+// registers, two waves a SIMD); 48 ragged sequences of up to 8,191 tokens, 32 heads on 8, 119 MB in 35 us; a
+// short call of 301 tokens 6.2 us.  The next block's codes are in flight while one is computed, with three
+// waves a SIMD (151 registers for D = 128).
 //
 // TWICE: at most 8 rows, each in two of the 16 columns (m and m + 8), one for the upper eight
 // significant bits of its probabilities and one for the next eight, so P loses 2^-14 of itself instead of
@@ -602,11 +605,11 @@ __device__ __forceinline__ int sequence_at(const AttnArgs& a, int at, int lane) 
 // every bank once (the conversion's writes take 1.5 times their least cycles).
 //
 // Bound by neither unit alone: 3600 rows of 24 heads against 118,800 tokens of 128 dims, 5.26 TFLOP,
-// take 4.9 to 5.1 ms, 1030 to 1070 TFLOP/s, where a library product of 8192^3 reaches 1129 on this card;
-// the clock is down to 1.75 GHz, the MFMA pipe is busy half of the time, VALU issue as much.  128 rows take
-// 0.23 ms (830 TFLOP/s): half the products to each conversion.  Row blocks by rows of the call, at
-// 24 x 118,800 x 128: 33 to 64 rows 156 us with RB 2 and 200 with RB 4; 17 to 32 rows 150 us with RB 2 and
-// 115 with the few-row kernel; 65 to 128 rows 209 with RB 4.
+// take 5.0 to 5.2 ms, 1010 to 1050 TFLOP/s, where a library product of 8192^3 reaches 1129 on this card;
+// the clock is down to 1.78 GHz, the MFMA pipe is busy half of the time, VALU issue as much.  128 rows take
+// 0.225 to 0.245 ms (760 to 830 TFLOP/s): half the products to each conversion.  Row blocks by rows of the
+// call, at 24 x 118,800 x 128: 33 to 64 rows 156 us with RB 2 and 200 with RB 4; 17 to 32 rows 150 us with RB 2
+// and 118 with the few-row kernel.
 template <int D, bool F16, int RB>
 __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a) {
   using Part = spr::Kv4Part<D>;
@@ -962,7 +965,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 1) void kv4_many_kernel(AttnArgs a
 
 // 16 lanes have all dims of a row, and P such teams share a row's shares; 16 / P rows a workgroup.
 // Bound by latency where rows are few (24 rows of 32 shares 5 us), by the partial results' bytes where
-// they are many (86,400 rows of 7 shares, 310 MB, 64 us).
+// they are many (86,400 rows of 7 shares, 310 MB, 64 us).  The share is the attention kernel's.
 template <int D, bool F16, int P>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, int64_t all_rows) {
   constexpr int E = D / 16;  // dims of a lane

@@ -186,7 +186,11 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     first).  Rows that see nothing, and rows past the count, are 0 with lse -inf.  `max_length`, the
     longest length the caller knows of (default: what the table can hold), only sizes the launch and its
     workspace, and may be passed: the keys are dealt by the lengths as they are.  `page_size` is checked,
-    as in kv4_store."""
+    as in kv4_store.
+
+    Sums, maxima and scores are fp32.  Probabilities keep 16 bits into the product with V in fp16 calls and
+    in bf16 calls of up to 8 rows (T * Hq // Hkv); in longer bf16 calls they are rounded to bf16 once.  A
+    row whose scores are all -inf is NaN."""
     what = "4-bit cache attention"
     dev = _lib.require_gpu(q, pages, block_table, lengths, counts, seq_ids, what=what)
     if q.dim() != 4 or q.dtype not in (torch.bfloat16, torch.float16):

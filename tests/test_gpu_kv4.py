@@ -923,6 +923,7 @@ def test_the_workspace_query_is_what_a_call_needs_for_the_same_arguments(dev, dt
                 assert (out == 0).all()
 
 
+@pytest.mark.filterwarnings("ignore:Synchronization debug mode")
 def test_calls_with_lists_do_not_wait_for_the_gpu(dev):
     from sparsepr_amd.kv4_cache import KV4Cache
 
