@@ -542,9 +542,9 @@ int spr_kv4_load(const uint8_t* pages, int32_t num_pages, int32_t kv_heads, int3
  * new pages are the lowest free ones, ascending, in the order of the named sequences (at most 2048 a
  * call).  status int32 [1] (nullable) gets, unless it holds one already, what was wrong: 1 a sequence
  * outside the table, 2 a sequence named twice, 3 a negative count (or one past `most`) or a range
- * outside the sequence's pages, 4 more tokens than the table's row holds, 6 a fork onto a sequence that holds tokens, 7 a
- * length outside the table or a table entry outside the pool (the lowest of these), or else 5 not
- * enough free pages. */
+ * outside the sequence's pages, 4 more tokens than the table's row holds, 6 a fork onto a sequence that
+ * holds tokens, 7 a length outside the table or a table entry outside the pool (the lowest of these),
+ * or else 5 not enough free pages. */
 size_t spr_kv4_pages_workspace(int32_t num_pages);
 /* Room for counts[i] more tokens of sequence seq_ids[i]; starts[i] (out) is the first one's place, -1
  * for all if the call did not happen.  _ex refuses counts past `most`, the rows that a store after it
