@@ -1067,3 +1067,33 @@ def test_more_sequences_than_a_wave_ranks(dev, rows):
     out, lse = kv4_attention(q, _gpu(pages, dev, torch.uint8), _gpu(table, dev), _gpu(lengths, dev),
                              seq_ids=_gpu(ids, dev), causal=True, return_lse=True)
     _check_attention(out, lse, q, pages, table, lengths, [rows] * n, size, True, d**-0.5, "bf16", ids)
+
+
+def test_a_captured_call_deals_a_growing_sequence_as_eager_calls_do(dev):
+    """One sequence, no bound: the shares follow its length from replay to replay."""
+    from sparsepr_amd.kv4_cache import KV4Cache
+
+    g = torch.Generator(device=dev).manual_seed(9)
+    h, d = 3, 128
+    cache = KV4Cache(400, h, d, 2, page_size=64, max_pages=300, device=dev)
+    ids = _gpu([1], dev)
+    k, v = torch.randn((2, 1, h, 1500, d), generator=g, device=dev).to(torch.bfloat16)
+    qs = [torch.randn((1, 6, t, d), generator=g, device=dev).to(dt)
+          for t, dt in ((1, DT["bf16"]), (12, DT["fp16"]), (20, DT["bf16"]), (60, DT["fp16"]), (300, DT["bf16"]))]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for q in qs:
+            cache.attend(q, seq_ids=ids, return_lse=True)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [cache.attend(q, seq_ids=ids, return_lse=True) for q in qs]
+    for count in (0, 1, 600, 1500, 1500, 1500, 1500, 1500, 1500):
+        cache.append(k[:, :, :count], v[:, :, :count], seq_ids=ids)
+        want = [cache.attend(q, seq_ids=ids, return_lse=True) for q in qs]
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]), int(cache.lengths[1])
+    cache.check()
