@@ -592,6 +592,55 @@ int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_t q_t, int3
                       int32_t causal, float scale, int64_t max_length, void* out, float* lse, void* workspace,
                       size_t workspace_bytes, hipStream_t stream);
 
+/* ---------------------------------------------------------------- norm of the hidden rows
+ * No counterpart in the reference: what its model blocks leave to torch in front of the QKV projection.
+ * x [n0, n1, width] of dtype with strides x_s0, x_s1 (elements) and packed rows; width 1 .. 16384.
+ *   s = x + residual, rounded to residual_dtype (dtype or 2); s = x where residual is null
+ *   y = s / sqrt(mean(s^2) + epsilon) * weight (null: ones; weight_dtype dtype or 2)
+ * out: y of dtype, contiguous; where `scales` is not null, e4m3 codes [rows, width rounded up to 16] (8-byte
+ * aligned) with a scale byte per 128 channels, scales [rows, width / 128 rounded up].  sum: s, contiguous
+ * (with a residual). */
+int spr_rms_norm(const void* x, int64_t x_s0, int64_t x_s1, const void* residual, int64_t res_s0, int64_t res_s1,
+                 int32_t n0, int32_t n1, int32_t width, int32_t dtype, int32_t residual_dtype, const void* weight,
+                 int32_t weight_dtype, float epsilon, void* out, uint8_t* scales, void* sum, hipStream_t stream);
+/* Its gradient: dx (sum_dtype, contiguous) = r (g - s r^2 mean(g s)) + dsum with g = dy weight and
+ * r = 1 / sqrt(mean(s^2) + epsilon); dweight fp32 [width] = sum over rows of dy s r.  s and dsum (null: zeros)
+ * are of sum_dtype (dtype or 2).  dweight null: not computed, and no workspace is needed. */
+size_t spr_rms_norm_backward_workspace(int64_t rows, int32_t width);
+int spr_rms_norm_backward(const void* dy, int64_t dy_s0, int64_t dy_s1, const void* s, int64_t s_s0, int64_t s_s1,
+                          const void* dsum, int64_t ds_s0, int64_t ds_s1, int32_t n0, int32_t n1, int32_t width,
+                          int32_t dtype, int32_t sum_dtype, const void* weight, int32_t weight_dtype, float epsilon,
+                          void* dx, float* dweight, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------- 8-bit matrices
+ * No counterpart in the reference.  e4m3 codes [rows, width rounded up to 16], zeros behind the width, with a
+ * scale byte b, 2^(b - 127) (255: NaN), per 128 values of a row, scales [rows, width / 128 rounded up], or
+ * (square) per 128 x 128 values, [rows / 128 rounded up, ...].
+ * Quantise x [rows, width] of dtype with row stride ld; transpose: the 8-bit matrix of x^T. */
+int spr_fp8_quantize(const void* x, int64_t ld, int64_t rows, int32_t width, int32_t dtype, int32_t square,
+                     int32_t transpose, uint8_t* codes, uint8_t* scales, hipStream_t stream);
+/* out [rows, width] of dtype, contiguous; width a multiple of 16, codes 16-byte aligned, ld a multiple of 16. */
+int spr_fp8_dequantize(const uint8_t* codes, int64_t ld, const uint8_t* scales, int64_t scales_ld, int32_t square,
+                       int64_t rows, int32_t width, int32_t dtype, void* out, hipStream_t stream);
+/* out [M, N] of out_dtype = a b^T + bias: a [M, K], b [N, K], K a multiple of 16 up to 2^22, codes 16-byte aligned,
+ * row strides multiples of 16 up to 2^22; bias [N] of bias_dtype or null.  Sums are fp32. */
+int spr_fp8_matmul(const uint8_t* a, int64_t a_ld, const uint8_t* a_scales, int64_t a_scales_ld, int32_t a_square,
+                   const uint8_t* b, int64_t b_ld, const uint8_t* b_scales, int64_t b_scales_ld, int32_t b_square,
+                   int64_t M, int64_t N, int32_t K, const void* bias, int32_t bias_dtype, int32_t out_dtype, void* out,
+                   hipStream_t stream);
+
+/* ---------------------------------------------------------------- rotary positions with several axes
+ * The QKV fusions above take tables; this one the tokens' places.  Q [batch, q_heads, tokens, dim] and K (k_heads
+ * may be 0) of dtype with strides in elements and packed rows -> q_out, k_out, contiguous.  Pair i < rotated / 2
+ * turns by positions[b, t, axis[i]] * freqs[i] radians (inverse: back); halves: dims (i, i + rotated / 2), else
+ * (2i, 2i + 1).  positions [tokens, axes] (position_b 0) or [batch, tokens, axes] (position_b = tokens * axes),
+ * position_code 0 int32, 1 int64, 2 fp32, 3 fp64.  dim and rotated are multiples of 8, dim at most 1024. */
+int spr_axial_rope(const void* q, int64_t q_b, int64_t q_h, int64_t q_t, int32_t q_heads, const void* k, int64_t k_b,
+                   int64_t k_h, int64_t k_t, int32_t k_heads, int32_t dtype, int64_t batch, int64_t tokens, int32_t dim,
+                   int32_t rotated, const void* positions, int32_t position_code, int64_t position_b, int32_t axes,
+                   const double* freqs, const int32_t* axis, int32_t halves, int32_t inverse, void* q_out, void* k_out,
+                   hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -146,6 +146,19 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "spr_kv4_attention_workspace": (_sz, [_i32, _i32, _i32, _i32, _i32, _i64]),
     "spr_kv4_attention": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _i32, _i32,
                                          _vp, _i32, _i32, _vp, _vp, _vp, _i32, _f32, _i64, _vp, _vp, _vp, _sz, _vp]),
+    # rms_norm.hip
+    "spr_rms_norm": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64] + [_i32] * 5 + [_vp, _i32, _f32] + [_vp] * 4),
+    "spr_rms_norm_backward_workspace": (_sz, [_i64, _i32]),
+    "spr_rms_norm_backward": (ctypes.c_int, [_vp, _i64, _i64] * 3 + [_i32] * 5 + [_vp, _i32, _f32, _vp, _vp, _vp, _sz,
+                                                                                  _vp]),
+    # fp8.hip
+    "spr_fp8_quantize": (ctypes.c_int, [_vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "spr_fp8_dequantize": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp]),
+    # fp8_matmul.hip
+    "spr_fp8_matmul": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32] * 2 + [_i64, _i64, _i32, _vp, _i32, _i32, _vp, _vp]),
+    # axial_rope.hip
+    "spr_axial_rope": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i32] * 2 + [_i32, _i64, _i64, _i32, _i32, _vp, _i32, _i64,
+                                                                          _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp]),
 }
 
 _LIB: ctypes.CDLL | None = None

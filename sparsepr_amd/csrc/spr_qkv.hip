@@ -26,82 +26,17 @@
 // token loaded before any arithmetic, its sines and cosines computed once into LDS).
 #pragma clang fp contract(off)
 
-#include "spr_common.h"
+#include "spr_elem.h"
 
 namespace {
 
 constexpr int QKV_THREADS = 256;
 
-template <int DT>
-struct Elem;
-template <>
-struct Elem<0> {  // bf16
-  using S = uint16_t;
-  __device__ static float to_f(S s) { return spr::bf16_to_f32(s); }
-  __device__ static S from_f(float f) { return spr::f32_to_bf16(f); }
-};
-template <>
-struct Elem<1> {  // fp16
-  using S = uint16_t;
-  __device__ static float to_f(S s) { return static_cast<float>(__builtin_bit_cast(_Float16, s)); }
-  __device__ static S from_f(float f) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f)); }
-};
-template <>
-struct Elem<2> {  // fp32
-  using S = float;
-  __device__ static float to_f(S s) { return s; }
-  __device__ static S from_f(float f) { return f; }
-};
-
-// 8 consecutive elements <-> float[8] (16 bytes for 16-bit types, 32 for fp32).
-template <int DT>
-__device__ __forceinline__ void load8(const typename Elem<DT>::S* p, float (&x)[8]) {
-  if constexpr (DT == 2) {
-    const spr::f32x4 a = reinterpret_cast<const spr::f32x4*>(p)[0];
-    const spr::f32x4 b = reinterpret_cast<const spr::f32x4*>(p)[1];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[e] = a[e];
-      x[e + 4] = b[e];
-    }
-  } else {
-    const spr::u32x4 r = *reinterpret_cast<const spr::u32x4*>(p);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[2 * e] = Elem<DT>::to_f(static_cast<uint16_t>(w[e] & 0xFFFFu));
-      x[2 * e + 1] = Elem<DT>::to_f(static_cast<uint16_t>(w[e] >> 16));
-    }
-  }
-}
-template <int DT>
-__device__ __forceinline__ void store8(typename Elem<DT>::S* p, const float (&x)[8]) {
-  if constexpr (DT == 2) {
-    reinterpret_cast<spr::f32x4*>(p)[0] = spr::f32x4{x[0], x[1], x[2], x[3]};
-    reinterpret_cast<spr::f32x4*>(p)[1] = spr::f32x4{x[4], x[5], x[6], x[7]};
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      w[e] = static_cast<uint32_t>(Elem<DT>::from_f(x[2 * e])) |
-             (static_cast<uint32_t>(Elem<DT>::from_f(x[2 * e + 1])) << 16);
-    }
-    *reinterpret_cast<spr::u32x4*>(p) = spr::u32x4{w[0], w[1], w[2], w[3]};
-  }
-}
-template <int DT>
-__device__ __forceinline__ void copy8(const typename Elem<DT>::S* src, typename Elem<DT>::S* dst) {
-  if constexpr (DT == 2) {
-    reinterpret_cast<spr::u32x4*>(dst)[0] = reinterpret_cast<const spr::u32x4*>(src)[0];
-    reinterpret_cast<spr::u32x4*>(dst)[1] = reinterpret_cast<const spr::u32x4*>(src)[1];
-  } else {
-    *reinterpret_cast<spr::u32x4*>(dst) = *reinterpret_cast<const spr::u32x4*>(src);
-  }
-}
-template <int DT>
-__device__ __forceinline__ float round_t(float x) {
-  return Elem<DT>::to_f(Elem<DT>::from_f(x));
-}
+using spr::copy8;
+using spr::Elem;
+using spr::load8;
+using spr::round_t;
+using spr::store8;
 
 __device__ __forceinline__ float inv_rms(float ss, float n, float eps) {
   return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, n), eps)));

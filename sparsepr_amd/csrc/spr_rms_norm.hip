@@ -1,0 +1,387 @@
+// Root-mean-square norm of rows, with the residual's addition in front, 8-bit codes behind, and its gradient.
+//
+//   s = x + residual (rounded once, to the residual's type; s = x without one)
+//   r = 1 / sqrt(mean(s^2) + eps),   y = s r w
+//   out: y rounded to x's type, or e4m3 codes with a scale byte per 128 channels (spr_fp8.h)
+// The norm reads the sum as it is stored, so that the gradient and a later call see the same one.
+//
+//   gradient, with g = dy w:   dx = r (g - s r^2 mean(g s)) + dsum,   dw = sum over rows of dy s r
+//
+// Sums are fp32, in an order that depends on the sizes only.  Bound by memory: every input is read
+// once and kept in registers over the reduction, vectors of 8 channels a lane.
+#include "spr_fp8.h"
+
+namespace {
+
+using spr::Elem;
+using spr::load8n;
+using spr::load8n_any;
+using spr::store8n;
+
+constexpr int MAX_WIDTH = 16384;
+
+// Rows of a [n0, n1, width] tensor with any strides of its first two dims.
+struct Rows {
+  const void* p;
+  int64_t s0, s1;
+  int32_t n1;
+};
+__device__ __forceinline__ int64_t row_at(const Rows& t, uint32_t row) {
+  const uint32_t a = row / static_cast<uint32_t>(t.n1);
+  return a * t.s0 + (row - a * static_cast<uint32_t>(t.n1)) * t.s1;
+}
+
+// The sum of a over the TPR threads of a row, in each of them; `red` has one float per wave.
+template <int TPR, int THREADS>
+__device__ __forceinline__ float row_total(float a, float* red) {
+  a = spr::row_sum(a);
+  if constexpr (TPR > 16) {
+    a += __shfl_xor(a, 16, 64);
+    a += __shfl_xor(a, 32, 64);
+  }
+  if constexpr (TPR > 64) {
+    static_assert(TPR == THREADS, "one row a workgroup");
+    constexpr int WAVES = THREADS / 64;
+    __syncthreads();  // an earlier total has been read
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) a += red[w];
+  }
+  return a;
+}
+
+__device__ __forceinline__ float inverse_rms(float ss, int32_t width, float eps) {
+  return __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, static_cast<float>(width)) + eps));
+}
+
+// TPR threads a row, NV vectors of 8 channels a thread.  RES: 0 no residual, 1 of x's type, 2 fp32.
+template <int DT, int RES, bool FP8, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(
+    Rows x, Rows residual, const void* __restrict__ weight, int32_t weight_dtype, uint32_t rows, int32_t width,
+    float eps, void* __restrict__ out, uint8_t* __restrict__ scales, void* __restrict__ sum) {
+  constexpr int THREADS = TPR < 256 ? 256 : TPR;
+  constexpr int SDT = RES == 2 ? 2 : DT;
+  using S = typename Elem<DT>::S;
+  using R = typename Elem<SDT>::S;
+  __shared__ float red[THREADS / 64];
+  const uint32_t row = blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
+  if (TPR <= 64 && row >= rows) return;
+  const int lane = threadIdx.x % TPR;
+  const S* xr = static_cast<const S*>(x.p) + row_at(x, row);
+  float s[NV][8];
+  float ss = 0.0f;
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int c = (lane + u * TPR) * 8;
+    load8n<DT>(xr + c, width - c, s[u]);
+  }
+  if constexpr (RES != 0) {
+    const R* rr = static_cast<const R*>(residual.p) + row_at(residual, row);
+    R* sr = static_cast<R*>(sum) + static_cast<int64_t>(row) * width;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int c = (lane + u * TPR) * 8;
+      float t[8];
+      load8n<SDT>(rr + c, width - c, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[u][e] = spr::round_t<SDT>(s[u][e] + t[e]);
+      if (c < width) store8n<SDT>(sr + c, width - c, s[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < NV; ++u)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(s[u][e], s[u][e], ss);
+  const float inv = inverse_rms(row_total<TPR, THREADS>(ss, red), width, eps);
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int c = (lane + u * TPR) * 8;
+    float w[8];
+    if (weight != nullptr) {
+      load8n_any(weight, weight_dtype, c, width - c, w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = 1.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[u][e] = s[u][e] * inv * w[e];
+    if constexpr (FP8) {
+      // 16 lanes are a group of 128 channels; all of them come here
+      if (c + 8 > width) {  // 0 * inf and 0 * NaN behind the row's end
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[u][e] = c + e < width ? s[u][e] : 0.0f;
+      }
+      const uint32_t b = spr::fp8_scale_byte(spr::row_max(spr::magnitude_bits8(s[u])));
+      const int64_t wide = spr::fp8_width(width);
+      if (c < wide) {
+        const uint64_t codes = spr::fp8_codes8(s[u], spr::fp8_inverse_scale(b));
+        *reinterpret_cast<uint64_t*>(static_cast<uint8_t*>(out) + row * wide + c) = codes;
+        if (lane % 16 == 0) scales[row * spr::fp8_groups(width) + c / spr::FP8_GROUP] = static_cast<uint8_t>(b);
+      }
+    } else {
+      if (c < width) store8n<DT>(static_cast<S*>(out) + static_cast<int64_t>(row) * width + c, width - c, s[u]);
+    }
+  }
+}
+
+// The gradient: workgroups take rows in turn, each thread keeps the weight's gradient of its channels
+// over all of them, and the workgroups' parts are added by a second kernel in a fixed order.
+template <int DT, int SDT, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_kernel(
+    Rows dy, Rows s_in, Rows dsum, const void* __restrict__ weight, int32_t weight_dtype, uint32_t rows, int32_t width,
+    float eps, void* __restrict__ dx, float* __restrict__ parts) {
+  constexpr int THREADS = TPR < 256 ? 256 : TPR;
+  constexpr int PER = THREADS / TPR;  // rows at a time
+  using S = typename Elem<DT>::S;
+  using R = typename Elem<SDT>::S;
+  __shared__ float red[THREADS / 64];
+  const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  float w[NV][8], dw[NV][8];
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int c = (lane + u * TPR) * 8;
+    if (weight != nullptr) {
+      load8n_any(weight, weight_dtype, c, width - c, w[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[u][e] = 1.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[u][e] = 0.0f;
+  }
+  for (uint32_t row = blockIdx.x * PER + sub; row < rows; row += gridDim.x * PER) {
+    const S* dyr = static_cast<const S*>(dy.p) + row_at(dy, row);
+    const R* sr = static_cast<const R*>(s_in.p) + row_at(s_in, row);
+    float g[NV][8], s[NV][8];
+    float ss = 0.0f, gs = 0.0f;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int c = (lane + u * TPR) * 8;
+      load8n<DT>(dyr + c, width - c, g[u]);
+      load8n<SDT>(sr + c, width - c, s[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        ss = __builtin_fmaf(s[u][e], s[u][e], ss);
+        gs = __builtin_fmaf(g[u][e] * w[u][e], s[u][e], gs);
+      }
+    ss = row_total<TPR, THREADS>(ss, red);
+    gs = row_total<TPR, THREADS>(gs, red);
+    const float inv = inverse_rms(ss, width, eps);
+    const float along = inv * inv * __fdiv_rn(gs, static_cast<float>(width));
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int c = (lane + u * TPR) * 8;
+      float d[8];
+      if (dsum.p != nullptr) {
+        load8n<SDT>(static_cast<const R*>(dsum.p) + row_at(dsum, row) + c, width - c, d);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float n = s[u][e] * inv;
+        dw[u][e] = __builtin_fmaf(g[u][e], n, dw[u][e]);
+        d[e] = __builtin_fmaf(inv, __builtin_fmaf(-s[u][e], along, g[u][e] * w[u][e]), d[e]);
+      }
+      if (c < width) store8n<SDT>(static_cast<R*>(dx) + static_cast<int64_t>(row) * width + c, width - c, d);
+    }
+  }
+  if (parts == nullptr) return;
+  // the rows that a workgroup takes at a time, added in LDS; then one row of `parts` each
+  if constexpr (PER > 1) {
+    __shared__ float add[PER * TPR * 8];
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) add[(sub * TPR + lane) * 8 + e] = dw[u][e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < TPR * 8; i += THREADS) {
+        float t = 0.0f;
+        for (int p = 0; p < PER; ++p) t += add[p * TPR * 8 + i];
+        const int c = u * TPR * 8 + i;
+        if (c < width) parts[static_cast<int64_t>(blockIdx.x) * width + c] = t;
+      }
+      __syncthreads();
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int c = (lane + u * TPR) * 8;
+      if (c < width) store8n<2>(parts + static_cast<int64_t>(blockIdx.x) * width + c, width - c, dw[u]);
+    }
+  }
+}
+
+// dw[c] = sum over the workgroups' parts: 64 channels a workgroup, 4 waves over the parts.
+__global__ __launch_bounds__(256) void norm_weight_gradient_kernel(const float* __restrict__ parts, int32_t n,
+                                                                  int32_t width, float* __restrict__ dw) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane;
+  float t = 0.0f;
+  if (c < width)
+    for (int p = wave; p < n; p += 4) t += parts[static_cast<int64_t>(p) * width + c];
+  red[wave][lane] = t;
+  __syncthreads();
+  if (wave == 0 && c < width) dw[c] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+}
+
+// Lanes of a row and vectors a lane: a quarter wave to 128 channels, a wave to 2048, a workgroup above.
+#define SPR_BY_WIDTH(CALL)           \
+  if (width <= 128) CALL(16, 1);     \
+  else if (width <= 512) CALL(64, 1); \
+  else if (width <= 2048) CALL(64, 4); \
+  else if (width <= 8192) CALL(256, 4); \
+  else CALL(1024, 2)
+
+template <int DT, int RES, bool FP8>
+void launch_norm(const Rows& x, const Rows& residual, const void* weight, int32_t weight_dtype, uint32_t rows,
+                 int32_t width, float eps, void* out, uint8_t* scales, void* sum, hipStream_t stream) {
+#define SPR_NORM(TPR, NV)                                                                                    \
+  norm_kernel<DT, RES, FP8, TPR, NV>                                                                         \
+      <<<static_cast<uint32_t>(spr::ceil_div(rows, TPR < 256 ? 256 / TPR : 1)), TPR < 256 ? 256 : TPR, 0, stream>>>( \
+          x, residual, weight, weight_dtype, rows, width, eps, out, scales, sum)
+  SPR_BY_WIDTH(SPR_NORM);
+#undef SPR_NORM
+}
+
+template <int DT, int RES>
+void launch_norm(bool fp8, const Rows& x, const Rows& residual, const void* weight, int32_t weight_dtype,
+                 uint32_t rows, int32_t width, float eps, void* out, uint8_t* scales, void* sum, hipStream_t stream) {
+  if (fp8) launch_norm<DT, RES, true>(x, residual, weight, weight_dtype, rows, width, eps, out, scales, sum, stream);
+  else launch_norm<DT, RES, false>(x, residual, weight, weight_dtype, rows, width, eps, out, scales, sum, stream);
+}
+
+int32_t rows_at_a_time(int32_t width) { return width <= 128 ? 16 : width <= 2048 ? 4 : 1; }
+
+// Workgroups of the gradient: enough to fill the chip a few times over, and few enough that their
+// parts of the weight's gradient are small beside the rows.
+int32_t backward_groups(int64_t rows, int32_t width) {
+  const int64_t most = width > 8192 ? 256 : 1024;
+  const int64_t all = spr::ceil_div(rows, rows_at_a_time(width));
+  return static_cast<int32_t>(all < most ? all : most);
+}
+
+template <int DT, int SDT>
+void launch_backward(const Rows& dy, const Rows& s, const Rows& dsum, const void* weight, int32_t weight_dtype,
+                     uint32_t rows, int32_t width, float eps, void* dx, float* parts, hipStream_t stream) {
+  const uint32_t groups = static_cast<uint32_t>(backward_groups(rows, width));
+#define SPR_NORM(TPR, NV)                                                                 \
+  norm_backward_kernel<DT, SDT, TPR, NV><<<groups, TPR < 256 ? 256 : TPR, 0, stream>>>( \
+      dy, s, dsum, weight, weight_dtype, rows, width, eps, dx, parts)
+  SPR_BY_WIDTH(SPR_NORM);
+#undef SPR_NORM
+}
+
+// (a launch has fewer than 2^32 threads)
+bool launch_fits(int64_t n0, int64_t n1, int32_t width) {
+  const int64_t per = width <= 128 ? 16 : width <= 2048 ? 64 : width <= 8192 ? 256 : 1024;
+  return n0 * n1 < (int64_t(1) << 32) / per - 1024 && n0 * n1 < (int64_t(1) << 31);
+}
+
+bool rows_fit(int64_t n0, int64_t n1, int64_t s0, int64_t s1) {
+  return n0 <= 1 || n1 <= 1 || (s0 >= 0 && s1 >= 0);
+}
+
+}  // namespace
+
+extern "C" int spr_rms_norm(const void* x, int64_t x_s0, int64_t x_s1, const void* residual, int64_t res_s0,
+                            int64_t res_s1, int32_t n0, int32_t n1, int32_t width, int32_t dtype,
+                            int32_t residual_dtype, const void* weight, int32_t weight_dtype, float epsilon, void* out,
+                            uint8_t* scales, void* sum, hipStream_t stream) {
+  SPR_REQUIRE(dtype >= 0 && dtype <= 2, "spr_rms_norm: dtype %d not in {0, 1, 2}", dtype);
+  SPR_REQUIRE(width >= 1 && width <= MAX_WIDTH, "spr_rms_norm: width %d not in 1 .. %d", width, MAX_WIDTH);
+  SPR_REQUIRE(n0 >= 0 && n1 >= 0 && launch_fits(n0, n1, width), "spr_rms_norm: too many rows");
+  SPR_REQUIRE(epsilon >= 0.0f && epsilon < __builtin_huge_valf(), "spr_rms_norm: epsilon must be finite and not negative");
+  SPR_REQUIRE(weight == nullptr || weight_dtype == dtype || weight_dtype == 2,
+              "spr_rms_norm: weights of dtype %d for rows of %d", weight_dtype, dtype);
+  SPR_REQUIRE(residual == nullptr || residual_dtype == dtype || residual_dtype == 2,
+              "spr_rms_norm: a residual of dtype %d for rows of %d", residual_dtype, dtype);
+  if (n0 == 0 || n1 == 0) return SPR_OK;
+  SPR_REQUIRE(x && out && (residual == nullptr || sum), "spr_rms_norm: null pointer");
+  SPR_REQUIRE(rows_fit(n0, n1, x_s0, x_s1) && rows_fit(n0, n1, res_s0, res_s1), "spr_rms_norm: negative stride");
+  SPR_REQUIRE(scales == nullptr || (reinterpret_cast<uintptr_t>(out) & 7) == 0, "spr_rms_norm: codes must be 8-byte aligned");
+  const Rows xr{x, x_s0, x_s1, n1}, rr{residual, res_s0, res_s1, n1};
+  const uint32_t rows = static_cast<uint32_t>(n0) * static_cast<uint32_t>(n1);
+  const bool fp8 = scales != nullptr;
+  const int res = residual == nullptr ? 0 : residual_dtype == dtype ? 1 : 2;
+#define SPR_NORM(DT, RES) \
+  launch_norm<DT, RES>(fp8, xr, rr, weight, weight_dtype, rows, width, epsilon, out, scales, sum, stream)
+#define SPR_NORM_RES(DT)          \
+  if (res == 0) SPR_NORM(DT, 0);  \
+  else if (res == 1) SPR_NORM(DT, 1); \
+  else SPR_NORM(DT, 2)
+  if (dtype == 0) { SPR_NORM_RES(0); }
+  else if (dtype == 1) { SPR_NORM_RES(1); }
+  else if (res == 0) { SPR_NORM(2, 0); }
+  else { SPR_NORM(2, 1); }
+#undef SPR_NORM_RES
+#undef SPR_NORM
+  SPR_LAUNCHED("norm_kernel");
+  return SPR_OK;
+}
+
+extern "C" size_t spr_rms_norm_backward_workspace(int64_t rows, int32_t width) {
+  if (rows <= 0 || width < 1 || width > MAX_WIDTH) return 0;
+  return sizeof(float) * static_cast<size_t>(width) * backward_groups(rows, width);
+}
+
+extern "C" int spr_rms_norm_backward(const void* dy, int64_t dy_s0, int64_t dy_s1, const void* s, int64_t s_s0,
+                                     int64_t s_s1, const void* dsum, int64_t ds_s0, int64_t ds_s1, int32_t n0,
+                                     int32_t n1, int32_t width, int32_t dtype, int32_t sum_dtype, const void* weight,
+                                     int32_t weight_dtype, float epsilon, void* dx, float* dweight, void* workspace,
+                                     size_t workspace_bytes, hipStream_t stream) {
+  SPR_REQUIRE(dtype >= 0 && dtype <= 2, "spr_rms_norm_backward: dtype %d not in {0, 1, 2}", dtype);
+  SPR_REQUIRE(sum_dtype == dtype || sum_dtype == 2, "spr_rms_norm_backward: a sum of dtype %d for gradients of %d",
+              sum_dtype, dtype);
+  SPR_REQUIRE(width >= 1 && width <= MAX_WIDTH, "spr_rms_norm_backward: width %d not in 1 .. %d", width, MAX_WIDTH);
+  SPR_REQUIRE(n0 >= 0 && n1 >= 0 && launch_fits(n0, n1, width), "spr_rms_norm_backward: too many rows");
+  SPR_REQUIRE(epsilon >= 0.0f && epsilon < __builtin_huge_valf(),
+              "spr_rms_norm_backward: epsilon must be finite and not negative");
+  SPR_REQUIRE(weight == nullptr || weight_dtype == dtype || weight_dtype == 2,
+              "spr_rms_norm_backward: weights of dtype %d for gradients of %d", weight_dtype, dtype);
+  const uint32_t rows = static_cast<uint32_t>(n0) * static_cast<uint32_t>(n1);
+  const int32_t groups = rows == 0 ? 0 : backward_groups(rows, width);
+  if (rows == 0) {
+    if (dweight != nullptr) {
+      norm_weight_gradient_kernel<<<static_cast<uint32_t>(spr::ceil_div(width, 64)), 256, 0, stream>>>(nullptr, 0, width,
+                                                                                                      dweight);
+      SPR_LAUNCHED("norm_weight_gradient_kernel");
+    }
+    return SPR_OK;
+  }
+  SPR_REQUIRE(dy && s && dx, "spr_rms_norm_backward: null pointer");
+  SPR_REQUIRE(rows_fit(n0, n1, dy_s0, dy_s1) && rows_fit(n0, n1, s_s0, s_s1) && rows_fit(n0, n1, ds_s0, ds_s1),
+              "spr_rms_norm_backward: negative stride");
+  if (dweight != nullptr) {
+    const size_t need = spr_rms_norm_backward_workspace(rows, width);
+    if (workspace == nullptr || workspace_bytes < need) {
+      spr_set_error("spr_rms_norm_backward: workspace %zu < %zu bytes", workspace_bytes, need);
+      return SPR_EWORKSPACE;
+    }
+    SPR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "spr_rms_norm_backward: workspace not 16-byte aligned");
+  }
+  const Rows dyr{dy, dy_s0, dy_s1, n1}, sr{s, s_s0, s_s1, n1}, dsr{dsum, ds_s0, ds_s1, n1};
+  float* parts = dweight != nullptr ? static_cast<float*>(workspace) : nullptr;
+#define SPR_BACK(DT, SDT) \
+  launch_backward<DT, SDT>(dyr, sr, dsr, weight, weight_dtype, rows, width, epsilon, dx, parts, stream)
+  if (dtype == 2) SPR_BACK(2, 2);
+  else if (dtype == 0 && sum_dtype == 0) SPR_BACK(0, 0);
+  else if (dtype == 0) SPR_BACK(0, 2);
+  else if (sum_dtype == 1) SPR_BACK(1, 1);
+  else SPR_BACK(1, 2);
+#undef SPR_BACK
+  SPR_LAUNCHED("norm_backward_kernel");
+  if (dweight != nullptr) {
+    norm_weight_gradient_kernel<<<static_cast<uint32_t>(spr::ceil_div(width, 64)), 256, 0, stream>>>(parts, groups, width,
+                                                                                                    dweight);
+    SPR_LAUNCHED("norm_weight_gradient_kernel");
+  }
+  return SPR_OK;
+}

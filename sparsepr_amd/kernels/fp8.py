@@ -1,0 +1,135 @@
+"""8-bit matrices and their product on the HIP kernels of csrc/spr_fp8.hip and csrc/spr_fp8_matmul.hip.
+
+A matrix in 8 bits is two tensors:
+  codes   float8_e4m3fn [rows, wide], wide = the row's width rounded up to 16, zeros behind the width
+  scales  uint8 [rows, blocks], blocks = the width / 128 rounded up: the byte b of 128 values of a row
+          stands for 2^(b - 127); or [rows / 128 rounded up, blocks] for 128 x 128 values ("square")
+The exponent is the smallest one with which the group's largest magnitude is at most 448, so scaling
+is exact and a value is off by half a step of its code alone.  A group with an infinity or a NaN has the
+byte 255 and is NaN.
+
+The products of a linear layer y = x W^T are all `fp8_matmul`, which sums along the rows of both sides:
+  y   fp8_matmul(*fp8_quantize(x), *fp8_quantize(w, square=True))
+  dx  fp8_matmul(*fp8_quantize(dy), *fp8_quantize(w, square=True, transpose=True))
+  dw  fp8_matmul(*fp8_quantize(dy, transpose=True), *fp8_quantize(x, transpose=True))
+Square blocks hold the same values either way round, so y and dx see one weight.  None of the functions
+is recorded by autograd: inputs that require a gradient are refused while it records."""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+
+BLOCK = 128
+CODES = torch.float8_e4m3fn
+
+
+def no_gradient(what: str, *tensors: torch.Tensor | None) -> None:
+    """Refuse what autograd would lose without a word."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what}: autograd does not record this call; call it under torch.no_grad() and use the "
+                           "gradient functions beside it")
+
+
+def _packed_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """x [R, C] and its row stride: itself where rows are packed, else a copy."""
+    if x.shape[1] == 1 or x.stride(1) == 1:
+        if x.shape[0] <= 1 or x.stride(0) >= 0:
+            return x, x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    x = x.contiguous()
+    return x, x.shape[1]
+
+
+def _check_matrix(codes: torch.Tensor, scales: torch.Tensor, what: str, name: str) -> tuple[int, int, int]:
+    """(rows, width, whether a scale is of 128 rows) of an 8-bit matrix."""
+    if codes.dtype is not CODES or codes.dim() != 2:
+        raise RuntimeError(f"{what}: {name} must be float8_e4m3fn [rows, width], got {codes.dtype} {tuple(codes.shape)}")
+    rows, width = codes.shape
+    if width % 16 != 0:
+        raise RuntimeError(f"{what}: the width of {name} ({width}) must be a multiple of 16 (zeros behind the row)")
+    blocks = -(-width // BLOCK)
+    if scales.dtype is not torch.uint8 or scales.dim() != 2 or scales.shape[1] != blocks \
+            or scales.shape[0] not in (rows, -(-rows // BLOCK)):
+        raise RuntimeError(f"{what}: the scales of {name} must be uint8 [{rows} or {-(-rows // BLOCK)}, {blocks}], got "
+                           f"{scales.dtype} {tuple(scales.shape)}")
+    return rows, width, int(scales.shape[0] != rows)
+
+
+def _as_read(codes: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, int, torch.Tensor, int]:
+    """Codes with packed rows that start on 16 bytes and scales with packed rows, and their row strides."""
+    codes, ld = _packed_rows(codes)
+    if codes.data_ptr() % 16 != 0 or ld % 16 != 0 or ld < codes.shape[1]:
+        codes = codes.clone(memory_format=torch.contiguous_format)
+        ld = codes.shape[1]
+    scales, scales_ld = _packed_rows(scales)
+    return codes, ld, scales, scales_ld
+
+
+def fp8_quantize(x: torch.Tensor, *, square: bool = False, transpose: bool = False):
+    """x [R, C] in bf16, fp16 or fp32 -> (codes, scales), see the module's text.
+
+    `square`: one scale for 128 x 128 values, else for 128 values of a row.  `transpose`: the 8-bit matrix
+    of x^T, codes [C, R rounded up to 16], its groups along x's columns."""
+    what = "8-bit quantisation"
+    dev = _lib.require_gpu(x, what=what)
+    no_gradient(what, x)
+    if x.dim() != 2 or x.dtype not in _lib.DTYPE_CODE:
+        raise RuntimeError(f"{what}: x must be [rows, width] in bfloat16, float16 or float32, got {x.dtype} "
+                           f"{tuple(x.shape)}")
+    rows, width = x.shape[::-1] if transpose else x.shape
+    codes = x.new_empty((rows, -(-width // 16) * 16), dtype=CODES)
+    scales = x.new_empty((-(-rows // BLOCK) if square else rows, -(-width // BLOCK)), dtype=torch.uint8)
+    if x.numel() > 0:
+        x, ld = _packed_rows(x)
+        _lib.launch("spr_fp8_quantize", dev, x.data_ptr(), ld, *x.shape, _lib.DTYPE_CODE[x.dtype], int(square),
+                    int(transpose), codes.data_ptr(), scales.data_ptr())
+    return codes, scales
+
+
+def fp8_dequantize(codes: torch.Tensor, scales: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of an 8-bit matrix, [rows, wide] in `dtype`: exact in fp32, and in bf16 but at the ends of its
+    range (fp16 rounds and overflows)."""
+    what = "8-bit values"
+    dev = _lib.require_gpu(codes, scales, what=what)
+    rows, width, square = _check_matrix(codes, scales, what, "codes")
+    if dtype not in _lib.DTYPE_CODE:
+        raise RuntimeError(f"{what}: dtype must be bfloat16, float16 or float32, got {dtype}")
+    out = codes.new_empty((rows, width), dtype=dtype)
+    if out.numel() > 0:
+        codes, ld, scales, scales_ld = _as_read(codes, scales)
+        _lib.launch("spr_fp8_dequantize", dev, codes.data_ptr(), ld, scales.data_ptr(), scales_ld, square, rows, width,
+                    _lib.DTYPE_CODE[dtype], out.data_ptr())
+    return out
+
+
+def fp8_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, *,
+               bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a b^T + bias for 8-bit matrices a [M, K] and b [N, K]: out [M, N] in `out_dtype` (bf16, fp16 or fp32),
+    summed in fp32 and rounded once.  bias [N] in any of the three types.
+
+    Rows that do not start on 16 bytes are copied first."""
+    what = "8-bit product"
+    dev = _lib.require_gpu(a, a_scales, b, b_scales, bias, what=what)
+    no_gradient(what, bias)
+    m, k, a_square = _check_matrix(a, a_scales, what, "a")
+    n, kb, b_square = _check_matrix(b, b_scales, what, "b")
+    if k != kb:
+        raise RuntimeError(f"{what}: a is [{m}, {k}], b [{n}, {kb}]")
+    if out_dtype not in _lib.DTYPE_CODE:
+        raise RuntimeError(f"{what}: out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype not in _lib.DTYPE_CODE:
+            raise RuntimeError(f"{what}: bias must be [{n}] in bfloat16, float16 or float32, got {bias.dtype} "
+                               f"{tuple(bias.shape)}")
+        bias = bias.contiguous()
+    if k == 0:
+        raise RuntimeError(f"{what}: nothing to sum over (a is [{m}, 0])")
+    out = a.new_empty((m, n), dtype=out_dtype)
+    if out.numel() > 0:
+        a, a_ld, a_scales, a_scales_ld = _as_read(a, a_scales)
+        b, b_ld, b_scales, b_scales_ld = _as_read(b, b_scales)
+        _lib.launch("spr_fp8_matmul", dev, a.data_ptr(), a_ld, a_scales.data_ptr(), a_scales_ld, a_square, b.data_ptr(),
+                    b_ld, b_scales.data_ptr(), b_scales_ld, b_square, m, n, k, _lib.ptr(bias),
+                    0 if bias is None else _lib.DTYPE_CODE[bias.dtype], _lib.DTYPE_CODE[out_dtype], out.data_ptr())
+    return out
