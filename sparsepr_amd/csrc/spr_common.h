@@ -131,17 +131,21 @@ __device__ __forceinline__ int32_t lds_base(const uint8_t* lds) {
   return __builtin_amdgcn_readfirstlane(
       static_cast<int32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)lds)));
 }
-__device__ __forceinline__ void lds_dma16x2(i32x4_s desc0, const uint8_t* lds0, int32_t voff0, i32x4_s desc1,
-                                            const uint8_t* lds1, int32_t voff1) {
+__device__ __forceinline__ void lds_dma16x2(i32x4_s desc0, int32_t lds0, int32_t voff0, i32x4_s desc1, int32_t lds1,
+                                            int32_t voff1) {
 #if defined(__HIP_DEVICE_COMPILE__)
   int32_t kept;
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 2\n\t"
                "buffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\t"
                "buffer_load_dwordx4 %5, %6, 0 offen lds\n\ts_mov_b32 m0, %0"
                : "=&s"(kept)
-               : "s"(lds_base(lds0)), "v"(voff0), "s"(desc0), "s"(lds_base(lds1)), "v"(voff1), "s"(desc1)
+               : "s"(lds0), "v"(voff0), "s"(desc0), "s"(lds1), "v"(voff1), "s"(desc1)
                : "memory");
 #endif
+}
+__device__ __forceinline__ void lds_dma16x2(i32x4_s desc0, const uint8_t* lds0, int32_t voff0, i32x4_s desc1,
+                                            const uint8_t* lds1, int32_t voff1) {
+  lds_dma16x2(desc0, lds_base(lds0), voff0, desc1, lds_base(lds1), voff1);
 }
 
 // Workgroup barrier behind this wave's LDS accesses, with no wait for the DMA in flight.

@@ -83,21 +83,86 @@ __device__ __forceinline__ f32x4 product(const Operand<true>& n, const Operand<t
   return c;
 }
 
+__device__ __forceinline__ float bias_at(const Output& o, int32_t n) {
+  return o.bias_dtype == 0   ? Elem<0>::to_f(static_cast<const uint16_t*>(o.bias)[n])
+         : o.bias_dtype == 1 ? Elem<1>::to_f(static_cast<const uint16_t*>(o.bias)[n])
+                             : static_cast<const float*>(o.bias)[n];
+}
+
+// The bias of the four columns from n on, zeros without one and behind the last.
+__device__ __forceinline__ f32x4 bias4(const Output& o, int32_t n, int32_t N) {
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (o.bias_dtype >= 0) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = n + e < N ? bias_at(o, n + e) : 0.0f;
+  }
+  return v;
+}
+
+// 64 columns of 16 rows: c[j] holds columns 16 j + 4 g .. + 3 of row r = lane % 16 in lane group g.  In 16 bits the
+// groups first exchange them, so that a lane has the 16 columns from 16 g on and a row's 128 bytes are one line.
+template <int DT>
+__device__ __forceinline__ void put64(const Output& o, const f32x4 (&c)[4], int64_t m, bool in, int32_t n0, int32_t N,
+                                      int lane) {
+  using S = typename Elem<DT>::S;
+  const int g = lane >> 4;
+  if constexpr (DT == 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int32_t n = n0 + 16 * j + 4 * g;
+      S* p = static_cast<S*>(o.out) + m * N + n;
+      if (in && n + 4 <= N) {
+        __builtin_memcpy(p, &c[j], 16);
+      } else if (in) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < N) p[e] = c[j][e];
+      }
+    }
+  } else {
+    uint32_t w[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[j][h] = static_cast<uint32_t>(Elem<DT>::from_f(c[j][2 * h])) |
+                  (static_cast<uint32_t>(Elem<DT>::from_f(c[j][2 * h + 1])) << 16);
+    // groups 2, 3 of w[j] against groups 0, 1 of w[j + 2], then groups 1, 3 of w[j] against 0, 2 of w[j + 1]
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const auto s = __builtin_amdgcn_permlane32_swap(w[j][h], w[j + 2][h], false, false);
+        w[j][h] = s[0], w[j + 2][h] = s[1];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        const auto s = __builtin_amdgcn_permlane16_swap(w[j][h], w[j + 1][h], false, false);
+        w[j][h] = s[0], w[j + 1][h] = s[1];
+      }
+    }
+    if (!in) return;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int32_t n = n0 + 16 * g + 8 * q;
+      S* p = static_cast<S*>(o.out) + m * N + n;
+      const uint32_t v[4] = {w[2 * q][0], w[2 * q][1], w[2 * q + 1][0], w[2 * q + 1][1]};
+      if (n + 8 <= N) {
+        __builtin_memcpy(p, v, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + e < N) p[e] = static_cast<S>(v[e / 2] >> (e % 2 * 16));
+      }
+    }
+  }
+}
+
 template <int DT>
 __device__ __forceinline__ void put4(const Output& o, f32x4 v, int64_t m, int32_t n, int32_t N) {
   using S = typename Elem<DT>::S;
   S* p = static_cast<S*>(o.out) + m * N + n;
-  float x[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = v[e];
-  if (o.bias_dtype >= 0) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < N)
-        x[e] += o.bias_dtype == 0   ? Elem<0>::to_f(static_cast<const uint16_t*>(o.bias)[n + e])
-                : o.bias_dtype == 1 ? Elem<1>::to_f(static_cast<const uint16_t*>(o.bias)[n + e])
-                                    : static_cast<const float*>(o.bias)[n + e];
-  }
+  const f32x4 x = v + bias4(o, n, N);
   if (n + 4 <= N) {
     S r[4];
 #pragma unroll
@@ -169,20 +234,30 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
       spr::lds_dma16x2(desc_b, l, v0, desc_b, l + 1024, v1);
     }
   };
-  // the scale bytes of blocks kb .. kb + WIN - 1, rows past the end as their last one
+  // the scale bytes of blocks kb .. kb + WIN - 1, a row a thread; rows past the end as their last one
+  static_assert(SROWS == THREADS && WIN % 16 == 0, "a row of scales a thread");
   auto fetch_scales = [&](int32_t kb) {
-    for (int i = threadIdx.x; i < SROWS * (WIN / 4); i += THREADS) {
-      const int r = i % SROWS, j = kb + i / SROWS * 4;
-      const bool is_a = r < TM;
-      const int32_t row = is_a ? (m0 + r < a.rows ? m0 + r : a.rows - 1) >> a.shift
-                               : (n0 + r - TM < b.rows ? n0 + r - TM : b.rows - 1) >> b.shift;
-      const uint8_t* s = is_a ? a.scales + row * a.scales_ld : b.scales + row * b.scales_ld;
-      uint32_t w = 0;
+    const int r = threadIdx.x;
+    const bool is_a = r < TM;
+    const int32_t row = is_a ? (m0 + r < a.rows ? m0 + r : a.rows - 1) >> a.shift
+                             : (n0 + r - TM < b.rows ? n0 + r - TM : b.rows - 1) >> b.shift;
+    const uint8_t* s = (is_a ? a.scales + row * a.scales_ld : b.scales + row * b.scales_ld) + kb;
+    const int32_t left = blocks - kb;
+    spr::Packed16 v[WIN / 16] = {};
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (j + e < blocks) w |= static_cast<uint32_t>(s[j + e]) << (8 * e);
-      win[i] = w;
+    for (int c = 0; c < WIN / 16; ++c) {
+      if (16 * c + 16 <= left) {
+        __builtin_memcpy(&v[c], s + 16 * c, 16);
+      } else if (16 * c < left) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (16 * c + e < left) v[c].w[e / 4] |= static_cast<uint32_t>(s[16 * c + e]) << (e % 4 * 8);
+      }
     }
+#pragma unroll
+    for (int c = 0; c < WIN / 16; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) win[(4 * c + e) * SROWS + r] = v[c].w[e];
   };
 
   f32x4 acc[MF][NF];
@@ -234,14 +309,17 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
       for (int j = 0; j < NF; ++j) acc[i][j] = product(n[j], m, acc[i][j]);
     }
   }
+  static_assert(NF == 4, "put64 takes 64 columns of a wave");
+  const int32_t nw = n0 + wn * 64;
+  f32x4 bias[NF];
+#pragma unroll
+  for (int j = 0; j < NF; ++j) bias[j] = bias4(o, nw + j * 16 + 4 * (lane >> 4), b.rows);
 #pragma unroll
   for (int i = 0; i < MF; ++i) {
     const int32_t m = m0 + wm * (TM / WM) + i * 16 + (lane & 15);
 #pragma unroll
-    for (int j = 0; j < NF; ++j) {
-      const int32_t n = n0 + wn * (TN / WN) + j * 16 + 4 * (lane >> 4);
-      if (m < a.rows && n < b.rows) put4<DT>(o, acc[i][j], m, n, b.rows);
-    }
+    for (int j = 0; j < NF; ++j) acc[i][j] += bias[j];
+    put64<DT>(o, acc[i], m, m < a.rows, nw, b.rows, lane);
   }
 }
 
