@@ -100,7 +100,7 @@ __device__ __forceinline__ f32x4 bias4(const Output& o, int32_t n, int32_t N) {
 }
 
 // 64 columns of 16 rows: c[j] holds columns 16 j + 4 g .. + 3 of row r = lane % 16 in lane group g.  In 16 bits the
-// groups first exchange them, so that a lane has the 16 columns from 16 g on and a row's 128 bytes are one line.
+// groups first exchange them, so that a lane has 8 columns side by side and each store writes 64 bytes of a row.
 template <int DT>
 __device__ __forceinline__ void put64(const Output& o, const f32x4 (&c)[4], int64_t m, bool in, int32_t n0, int32_t N,
                                       int lane) {
@@ -127,24 +127,18 @@ __device__ __forceinline__ void put64(const Output& o, const f32x4 (&c)[4], int6
       for (int h = 0; h < 2; ++h)
         w[j][h] = static_cast<uint32_t>(Elem<DT>::from_f(c[j][2 * h])) |
                   (static_cast<uint32_t>(Elem<DT>::from_f(c[j][2 * h + 1])) << 16);
-    // groups 2, 3 of w[j] against groups 0, 1 of w[j + 2], then groups 1, 3 of w[j] against 0, 2 of w[j + 1]
+    // groups 1, 3 of w[j] against 0, 2 of w[j + 1]: group g then has columns 8 (g / 2) + 16 (g % 2) .. + 7 of each 32
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const auto s = __builtin_amdgcn_permlane32_swap(w[j][h], w[j + 2][h], false, false);
-        w[j][h] = s[0], w[j + 2][h] = s[1];
-      }
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int j = 0; j < 4; j += 2) {
         const auto s = __builtin_amdgcn_permlane16_swap(w[j][h], w[j + 1][h], false, false);
         w[j][h] = s[0], w[j + 1][h] = s[1];
       }
-    }
     if (!in) return;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int32_t n = n0 + 16 * g + 8 * q;
+      const int32_t n = n0 + 32 * q + 8 * (g / 2) + 16 * (g % 2);
       S* p = static_cast<S*>(o.out) + m * N + n;
       const uint32_t v[4] = {w[2 * q][0], w[2 * q][1], w[2 * q + 1][0], w[2 * q + 1][1]};
       if (n + 8 <= N) {
@@ -175,6 +169,48 @@ __device__ __forceinline__ void put4(const Output& o, f32x4 v, int64_t m, int32_
   }
 }
 
+// Workgroups come to the 8 XCDs in turn: each XCD gets a run of tiles, in groups of 8 tile rows, so that the
+// tiles that are on it at once share their rows and columns in its L2.
+template <int TM, int TN>
+__device__ __forceinline__ void tile_of(int32_t tiles_m, int32_t tiles_n, int32_t& m0, int32_t& n0) {
+  const int32_t tiles = tiles_m * tiles_n;
+  const int32_t xcd = blockIdx.x % 8, each = tiles / 8, more = tiles % 8;
+  const int32_t tile = xcd * each + (xcd < more ? xcd : more) + static_cast<int32_t>(blockIdx.x / 8);
+  const int32_t group = tile / (8 * tiles_n), first = group * 8;
+  const int32_t high = tiles_m - first < 8 ? tiles_m - first : 8;
+  const int32_t in = tile - group * 8 * tiles_n;
+  m0 = (first + in % high) * TM, n0 = in / high * TN;
+}
+
+// The scale bytes of a tile's rows for blocks kb .. kb + WIN - 1 into `win`, a dword for four blocks of a row, a
+// row a thread; rows past the end as their last one.
+template <int TM, int TN, int WIN>
+__device__ __forceinline__ void fetch_scales(const Matrix& a, const Matrix& b, int32_t m0, int32_t n0, int32_t kb,
+                                             int32_t blocks, uint32_t* win) {
+  static_assert(WIN % 16 == 0, "16 bytes of a row at a time");
+  const int r = threadIdx.x;
+  const bool is_a = r < TM;
+  const int32_t row = is_a ? (m0 + r < a.rows ? m0 + r : a.rows - 1) >> a.shift
+                           : (n0 + r - TM < b.rows ? n0 + r - TM : b.rows - 1) >> b.shift;
+  const uint8_t* s = (is_a ? a.scales + row * a.scales_ld : b.scales + row * b.scales_ld) + kb;
+  const int32_t left = blocks - kb;
+  spr::Packed16 v[WIN / 16] = {};
+#pragma unroll
+  for (int c = 0; c < WIN / 16; ++c) {
+    if (16 * c + 16 <= left) {
+      __builtin_memcpy(&v[c], s + 16 * c, 16);
+    } else if (16 * c < left) {  // (no branch for each byte: all in flight at once)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        v[c].w[e / 4] |= static_cast<uint32_t>(s[16 * c + e < left ? 16 * c + e : left - 1]) << (e % 4 * 8);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < WIN / 16; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) win[(4 * c + e) * (TM + TN) + r] = v[c].w[e];
+}
+
 // ------------------------------------------------------------------ tiles
 //
 // TM x TN outputs a workgroup, WM x WN waves.  A block of both sides (128 bytes a row) goes by DMA into
@@ -191,20 +227,14 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
   static_assert(PA % 2 == 0 && PB % 2 == 0, "the DMA goes two by two");
   constexpr int BUF = (TM + TN) * KB;
   constexpr int SROWS = TM + TN;
+  static_assert(SROWS == THREADS, "fetch_scales takes a row a thread");
   __shared__ alignas(1024) uint8_t lds[2 * BUF + SROWS * WIN];
   uint32_t* win = reinterpret_cast<uint32_t*>(lds + 2 * BUF);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
-  // Workgroups come to the 8 XCDs in turn: each XCD gets a run of tiles, in groups of 8 tile rows, so
-  // that the tiles that are on it at once share their rows and columns in its L2.
-  const int32_t tiles = tiles_m * tiles_n;
-  const int32_t xcd = blockIdx.x % 8, each = tiles / 8, more = tiles % 8;
-  const int32_t tile = xcd * each + (xcd < more ? xcd : more) + static_cast<int32_t>(blockIdx.x / 8);
-  const int32_t group = tile / (8 * tiles_n), first = group * 8;
-  const int32_t high = tiles_m - first < 8 ? tiles_m - first : 8;
-  const int32_t in = tile - group * 8 * tiles_n;
-  const int32_t m0 = (first + in % high) * TM, n0 = in / high * TN;
+  int32_t m0, n0;
+  tile_of<TM, TN>(tiles_m, tiles_n, m0, n0);
 
   const int32_t rows_m = a.rows - m0 < TM ? a.rows - m0 : TM, rows_n = b.rows - n0 < TN ? b.rows - n0 : TN;
   const auto desc_a = spr::buffer_desc(a.codes + m0 * a.ld, static_cast<int32_t>((rows_m - 1) * a.ld + K));
@@ -234,32 +264,6 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
       spr::lds_dma16x2(desc_b, l, v0, desc_b, l + 1024, v1);
     }
   };
-  // the scale bytes of blocks kb .. kb + WIN - 1, a row a thread; rows past the end as their last one
-  static_assert(SROWS == THREADS && WIN % 16 == 0, "a row of scales a thread");
-  auto fetch_scales = [&](int32_t kb) {
-    const int r = threadIdx.x;
-    const bool is_a = r < TM;
-    const int32_t row = is_a ? (m0 + r < a.rows ? m0 + r : a.rows - 1) >> a.shift
-                             : (n0 + r - TM < b.rows ? n0 + r - TM : b.rows - 1) >> b.shift;
-    const uint8_t* s = (is_a ? a.scales + row * a.scales_ld : b.scales + row * b.scales_ld) + kb;
-    const int32_t left = blocks - kb;
-    spr::Packed16 v[WIN / 16] = {};
-#pragma unroll
-    for (int c = 0; c < WIN / 16; ++c) {
-      if (16 * c + 16 <= left) {
-        __builtin_memcpy(&v[c], s + 16 * c, 16);
-      } else if (16 * c < left) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (16 * c + e < left) v[c].w[e / 4] |= static_cast<uint32_t>(s[16 * c + e]) << (e % 4 * 8);
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < WIN / 16; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) win[(4 * c + e) * SROWS + r] = v[c].w[e];
-  };
-
   f32x4 acc[MF][NF];
 #pragma unroll
   for (int i = 0; i < MF; ++i)
@@ -276,7 +280,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
     spr::wait_vm<0>();
     spr::lds_barrier();
     if (kb % WIN == 0) {
-      fetch_scales(kb);
+      fetch_scales<TM, TN, WIN>(a, b, m0, n0, kb, blocks, win);
       spr::lds_barrier();
     }
     if (kb + 1 < blocks) fetch(kb + 1);
@@ -320,6 +324,151 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
 #pragma unroll
     for (int j = 0; j < NF; ++j) acc[i][j] += bias[j];
     put64<DT>(o, acc[i], m, m < a.rows, nw, b.rows, lane);
+  }
+}
+
+// ------------------------------------------------------------------ large tiles, outputs in 16 bits
+//
+// 256 x 256 outputs a workgroup of eight waves, 128 x 64 each, two waves a SIMD that take turns: while the
+// first four read operands from LDS into registers, the other four multiply theirs, and the other way round,
+// with a barrier at each change.  (With all waves in step the matrix units waited for LDS at the beginning of
+// each block.)  Both groups run the same four turns a block, the second one turn later:
+//   read b's rows and the first half of a's, multiply, read the second half of a's, multiply
+// A part of LDS is filled again as soon as both groups have read it: the rows of the first turn (kb + 2's) in the
+// third, those of the third (kb + 1's) in the first.  Each DMA has five turns to land, and 80 KB are on their
+// way at a time.  (Whole blocks at once had three turns: 834 us instead of what it is now on 32,760 x 5120 x 5120.)
+template <int DT>
+__global__ __launch_bounds__(512) void turns_product_kernel(Matrix a, Matrix b, int32_t K, int32_t tiles_m,
+                                                           int32_t tiles_n, Output o) {
+  constexpr int T = 256, BUF = 2 * T * KB, SROWS = 2 * T, WIN = 64, NF = 4;
+  __shared__ alignas(1024) uint8_t lds[2 * BUF + SROWS * WIN];
+  uint32_t* win = reinterpret_cast<uint32_t*>(lds + 2 * BUF);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  int32_t m0, n0;
+  tile_of<T, T>(tiles_m, tiles_n, m0, n0);
+
+  const int32_t rows_m = a.rows - m0 < T ? a.rows - m0 : T, rows_n = b.rows - n0 < T ? b.rows - n0 : T;
+  const auto desc_a = spr::buffer_desc(a.codes + m0 * a.ld, static_cast<int32_t>((rows_m - 1) * a.ld + K));
+  const auto desc_b = spr::buffer_desc(b.codes + n0 * b.ld, static_cast<int32_t>((rows_n - 1) * b.ld + K));
+  const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
+  const int32_t ld_a = static_cast<int32_t>(a.ld), ld_b = static_cast<int32_t>(b.ld);
+  // of a's 128 rows that a half of the waves reads, the first turn takes 64 and the third 64: this wave's DMA
+  // brings rows 16 (wave % 4) .. + 15 of them for wave / 4's half
+  const int arow = wm * 128 + wn * 16, brow = wave * 32;
+  const int32_t off_a = (arow + (lane >> 3)) * ld_a + piece, off_b = (brow + (lane >> 3)) * ld_b + piece;
+  const int32_t blocks = (K + KB - 1) / KB;
+  const int32_t base = spr::lds_base(lds);
+  auto fetch_a = [&](int32_t kb, int half) {
+    const int32_t k = kb * KB, to = base + (kb & 1) * BUF + (arow + 64 * half) * KB;
+    const int32_t v = k + piece < K ? off_a + k : 0x7f000000;  // K is a multiple of 16: a piece is in or out, and
+    const int32_t r = 64 * half * ld_a;                        // what is out reads as zeros
+    spr::lds_dma16x2(desc_a, to, v + r, desc_a, to + 1024, v + r + 8 * ld_a);
+  };
+  auto fetch_b = [&](int32_t kb) {
+    const int32_t k = kb * KB, to = base + (kb & 1) * BUF + (T + brow) * KB;
+    const int32_t v = k + piece < K ? off_b + k : 0x7f000000;
+#pragma unroll
+    for (int i = 0; i < 4; i += 2)
+      spr::lds_dma16x2(desc_b, to + i * 1024, v + i * 8 * ld_b, desc_b, to + (i + 1) * 1024, v + (i + 1) * 8 * ld_b);
+  };
+
+  f32x4 acc[8][NF];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  Operand<false> m[4], n[NF];
+  uint32_t sm[8], sn[NF];
+  const int p0 = (lane & 15) * KB + (((lane >> 4) ^ (lane & 7)) * 16);
+  const int p1 = (lane & 15) * KB + ((((lane >> 4) + 4) ^ (lane & 7)) * 16);
+  auto read_scales = [&](int32_t kb) {
+    if (kb % 4 == 0) {
+      const uint32_t* s = win + (kb % WIN) / 4 * SROWS + (lane & 15);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sm[i] = s[wm * 128 + i * 16];
+#pragma unroll
+      for (int j = 0; j < NF; ++j) sn[j] = s[T + wn * 64 + j * 16];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sm[i] >>= 8;
+#pragma unroll
+      for (int j = 0; j < NF; ++j) sn[j] >>= 8;
+    }
+  };
+  auto read_b = [&](int32_t kb) {
+    const uint8_t* t = lds + (kb & 1) * BUF + (T + wn * 64) * KB;
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+      n[j].set(*reinterpret_cast<const i32x4*>(t + j * 16 * KB + p0),
+               *reinterpret_cast<const i32x4*>(t + j * 16 * KB + p1), sn[j]);
+  };
+  auto read_a = [&](int32_t kb, int half) {
+    const uint8_t* t = lds + (kb & 1) * BUF + (wm * 128 + 64 * half) * KB;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      m[i].set(*reinterpret_cast<const i32x4*>(t + i * 16 * KB + p0),
+               *reinterpret_cast<const i32x4*>(t + i * 16 * KB + p1), sm[4 * half + i]);
+  };
+  auto multiply = [&](int half) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NF; ++j) acc[4 * half + i][j] = product(n[j], m[i], acc[4 * half + i][j]);
+  };
+  auto change = [&]() {  // nothing moves over a change of turns, the matrix instructions neither
+    __builtin_amdgcn_sched_barrier(0);
+    spr::lds_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  fetch_scales<T, T, WIN>(a, b, m0, n0, 0, blocks, win);
+  fetch_b(0);
+  fetch_a(0, 0);
+  fetch_a(0, 1);
+  fetch_b(1);
+  fetch_a(1, 0);
+  spr::wait_vm<8>();  // the first turn's rows
+  change();
+  if (wave >= 4) change();  // the second group is one turn behind
+  for (int32_t k0 = 0; k0 < blocks; k0 += WIN) {
+    const int32_t end = blocks - k0 < WIN ? blocks : k0 + WIN;
+    if (k0 > 0) {  // (the scales in use are in registers; both groups have written before the first reads)
+      fetch_scales<T, T, WIN>(a, b, m0, n0, k0, blocks, win);
+      change();
+      change();
+    }
+    for (int32_t kb = k0; kb < end; ++kb) {
+      fetch_a(kb + 1, 1);
+      read_scales(kb);
+      read_b(kb);
+      read_a(kb, 0);
+      spr::wait_vm<8>();  // the second half of kb's rows: the six DMA of kb + 1's first turn and two more are behind it
+      change();
+      multiply(0);
+      change();
+      fetch_b(kb + 2);
+      fetch_a(kb + 2, 0);
+      read_a(kb, 1);
+      spr::wait_vm<8>();  // kb + 1's first turn: two and six are behind it
+      change();
+      multiply(1);
+      change();
+    }
+  }
+  if (wave < 4) change();
+  spr::wait_vm<0>();  // of zeros behind the last block
+
+  const int32_t nw = n0 + wn * 64;
+  f32x4 bias[NF];
+#pragma unroll
+  for (int j = 0; j < NF; ++j) bias[j] = bias4(o, nw + j * 16 + 4 * (lane >> 4), b.rows);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int32_t mm = m0 + wm * 128 + i * 16 + (lane & 15);
+#pragma unroll
+    for (int j = 0; j < NF; ++j) acc[i][j] += bias[j];
+    put64<DT>(o, acc[i], mm, mm < a.rows, nw, b.rows, lane);
   }
 }
 
@@ -412,10 +561,15 @@ int launch_product(const Matrix& a, const Matrix& b, int32_t K, const Output& o,
   const int64_t tm = spr::ceil_div(M, t), tn = spr::ceil_div(N, t);
   SPR_REQUIRE(tm * tn < (int64_t(1) << 23), "spr_fp8_matmul: too many outputs");
   const uint32_t grid = static_cast<uint32_t>(tm * tn);
-  if (t == 256)
-    product_kernel<DT, 256, 256, 2, 4, 64><<<grid, 512, 0, stream>>>(a, b, K, static_cast<int32_t>(tm),
-                                                                    static_cast<int32_t>(tn), o);
-  else
+  if constexpr (DT == 2) {
+    if (t == 256)
+      product_kernel<DT, 256, 256, 2, 4, 64><<<grid, 512, 0, stream>>>(a, b, K, static_cast<int32_t>(tm),
+                                                                      static_cast<int32_t>(tn), o);
+  } else {
+    if (t == 256)
+      turns_product_kernel<DT><<<grid, 512, 0, stream>>>(a, b, K, static_cast<int32_t>(tm), static_cast<int32_t>(tn), o);
+  }
+  if (t == 128)
     product_kernel<DT, 128, 128, 2, 2, 32><<<grid, 256, 0, stream>>>(a, b, K, static_cast<int32_t>(tm),
                                                                     static_cast<int32_t>(tn), o);
   SPR_LAUNCHED("product_kernel");
