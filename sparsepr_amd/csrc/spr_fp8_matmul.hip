@@ -334,9 +334,10 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
 // with a barrier at each change.  (With all waves in step the matrix units waited for LDS at the beginning of
 // each block.)  Both groups run the same four turns a block, the second one turn later:
 //   read b's rows and the first half of a's, multiply, read the second half of a's, multiply
-// A part of LDS is filled again as soon as both groups have read it: the rows of the first turn (kb + 2's) in the
-// third, those of the third (kb + 1's) in the first.  Each DMA has five turns to land, and 80 KB are on their
-// way at a time.  (Whole blocks at once had three turns: 834 us instead of what it is now on 32,760 x 5120 x 5120.)
+// The first turn has twice the third one's reads, so it ends when b's are there; a's come in while the
+// products begin.  A part of LDS is filled again as soon as both groups have read it: b's rows (kb + 2's) in the
+// third turn, a's first half in the fourth, its second half (kb + 1's) in the first.  Each DMA has four or five
+// turns to land.  (Whole blocks at once had three: 834 us instead of 703 on 32,760 x 5120 x 5120.)
 template <int DT>
 __global__ __launch_bounds__(512) void turns_product_kernel(Matrix a, Matrix b, int32_t K, int32_t tiles_m,
                                                            int32_t tiles_n, Output o) {
@@ -422,6 +423,12 @@ __global__ __launch_bounds__(512) void turns_product_kernel(Matrix a, Matrix b, 
     __builtin_amdgcn_sched_barrier(0);
   };
 
+  auto change_after_b = [&]() {  // the eight reads of a's first half may be on their way
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(8)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
   fetch_scales<T, T, WIN>(a, b, m0, n0, 0, blocks, win);
   fetch_b(0);
   fetch_a(0, 0);
@@ -442,16 +449,17 @@ __global__ __launch_bounds__(512) void turns_product_kernel(Matrix a, Matrix b, 
       fetch_a(kb + 1, 1);
       read_scales(kb);
       read_b(kb);
+      __builtin_amdgcn_sched_barrier(0);
       read_a(kb, 0);
-      spr::wait_vm<8>();  // the second half of kb's rows: the six DMA of kb + 1's first turn and two more are behind it
-      change();
+      spr::wait_vm<8>();  // a's second half of kb: behind it are kb + 1's b (4) and a's halves (2 and 2)
+      change_after_b();
       multiply(0);
       change();
       fetch_b(kb + 2);
-      fetch_a(kb + 2, 0);
       read_a(kb, 1);
-      spr::wait_vm<8>();  // kb + 1's first turn: two and six are behind it
+      spr::wait_vm<6>();  // kb + 1's b and a's first half: behind them are a's second (2) and kb + 2's b (4)
       change();
+      fetch_a(kb + 2, 0);
       multiply(1);
       change();
     }
