@@ -184,40 +184,41 @@ __device__ __forceinline__ void tile_of(int32_t tiles_m, int32_t tiles_n, int32_
 
 // The scale bytes of a tile's rows for blocks kb .. kb + WIN - 1 into `win`, a dword for four blocks of a row, a
 // row a thread; rows past the end as their last one.
-template <int TM, int TN, int WIN>
+template <int TM, int TN, int WIN, int THREADS>
 __device__ __forceinline__ void fetch_scales(const Matrix& a, const Matrix& b, int32_t m0, int32_t n0, int32_t kb,
                                              int32_t blocks, uint32_t* win) {
   static_assert(WIN % 16 == 0, "16 bytes of a row at a time");
-  const int r = threadIdx.x;
-  const bool is_a = r < TM;
-  const int32_t row = is_a ? (m0 + r < a.rows ? m0 + r : a.rows - 1) >> a.shift
-                           : (n0 + r - TM < b.rows ? n0 + r - TM : b.rows - 1) >> b.shift;
-  const uint8_t* s = (is_a ? a.scales + row * a.scales_ld : b.scales + row * b.scales_ld) + kb;
-  const int32_t left = blocks - kb;
-  spr::Packed16 v[WIN / 16] = {};
+  for (int r = threadIdx.x; r < TM + TN; r += THREADS) {
+    const bool is_a = r < TM;
+    const int32_t row = is_a ? (m0 + r < a.rows ? m0 + r : a.rows - 1) >> a.shift
+                             : (n0 + r - TM < b.rows ? n0 + r - TM : b.rows - 1) >> b.shift;
+    const uint8_t* s = (is_a ? a.scales + row * a.scales_ld : b.scales + row * b.scales_ld) + kb;
+    const int32_t left = blocks - kb;
+    spr::Packed16 v[WIN / 16] = {};
 #pragma unroll
-  for (int c = 0; c < WIN / 16; ++c) {
-    if (16 * c + 16 <= left) {
-      __builtin_memcpy(&v[c], s + 16 * c, 16);
-    } else if (16 * c < left) {  // (no branch for each byte: all in flight at once)
+    for (int c = 0; c < WIN / 16; ++c) {
+      if (16 * c + 16 <= left) {
+        __builtin_memcpy(&v[c], s + 16 * c, 16);
+      } else if (16 * c < left) {  // (no branch for each byte: all in flight at once)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        v[c].w[e / 4] |= static_cast<uint32_t>(s[16 * c + e < left ? 16 * c + e : left - 1]) << (e % 4 * 8);
+        for (int e = 0; e < 16; ++e)
+          v[c].w[e / 4] |= static_cast<uint32_t>(s[16 * c + e < left ? 16 * c + e : left - 1]) << (e % 4 * 8);
+      }
     }
+#pragma unroll
+    for (int c = 0; c < WIN / 16; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) win[(4 * c + e) * (TM + TN) + r] = v[c].w[e];
   }
-#pragma unroll
-  for (int c = 0; c < WIN / 16; ++c)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) win[(4 * c + e) * (TM + TN) + r] = v[c].w[e];
 }
 
 // ------------------------------------------------------------------ tiles
 //
 // TM x TN outputs a workgroup, WM x WN waves.  A block of both sides (128 bytes a row) goes by DMA into
-// one of two buffers in LDS while the products of the other run; one barrier a block.  A row's 16-byte
+// one of NBUF buffers in LDS while the products of an earlier one run; one barrier a block.  A row's 16-byte
 // pieces lie at piece ^ (row % 8): eight rows' reads of one piece then meet every bank.  The scale bytes
 // of the tile's rows lie in LDS for WIN blocks at a time, a dword for four blocks of a row.
-template <int DT, int TM, int TN, int WM, int WN, int WIN>
+template <int DT, int TM, int TN, int WM, int WN, int WIN, int NBUF>
 __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix b, int32_t K, int32_t tiles_m,
                                                               int32_t tiles_n, Output o) {
   constexpr bool WIDE = DT == 2;
@@ -227,9 +228,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
   static_assert(PA % 2 == 0 && PB % 2 == 0, "the DMA goes two by two");
   constexpr int BUF = (TM + TN) * KB;
   constexpr int SROWS = TM + TN;
-  static_assert(SROWS == THREADS, "fetch_scales takes a row a thread");
-  __shared__ alignas(1024) uint8_t lds[2 * BUF + SROWS * WIN];
-  uint32_t* win = reinterpret_cast<uint32_t*>(lds + 2 * BUF);
+  __shared__ alignas(1024) uint8_t lds[NBUF * BUF + SROWS * WIN];
+  uint32_t* win = reinterpret_cast<uint32_t*>(lds + NBUF * BUF);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
@@ -246,9 +246,9 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
   const int32_t blocks = (K + KB - 1) / KB;
 
   auto fetch = [&](int32_t kb) {
-    uint8_t* to = lds + (kb & 1) * BUF;
+    uint8_t* to = lds + kb % NBUF * BUF;
     const int32_t k = kb * KB;
-    const bool in_row = k + piece < K;  // K is a multiple of 16: a piece is in or out
+    const bool in_row = k + piece < K;  // K is a multiple of 16: a piece is in or out, and what is out reads as zeros
 #pragma unroll
     for (int i = 0; i < PA; i += 2) {
       const int32_t v0 = in_row ? off_a + i * 8 * ld_a + k : 0x7ffffff0;
@@ -275,16 +275,17 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
   const int p0 = (lane & 15) * KB + (((lane >> 4) ^ (lane & 7)) * 16);
   const int p1 = (lane & 15) * KB + ((((lane >> 4) + 4) ^ (lane & 7)) * 16);
 
-  fetch(0);
+#pragma unroll
+  for (int i = 0; i < NBUF - 1; ++i) fetch(i);
   for (int32_t kb = 0; kb < blocks; ++kb) {
-    spr::wait_vm<0>();
+    spr::wait_vm<(NBUF - 2) * (PA + PB)>();  // the DMA of kb has landed, those of the next NBUF - 2 blocks may be on their way
     spr::lds_barrier();
     if (kb % WIN == 0) {
-      fetch_scales<TM, TN, WIN>(a, b, m0, n0, kb, blocks, win);
+      fetch_scales<TM, TN, WIN, THREADS>(a, b, m0, n0, kb, blocks, win);
       spr::lds_barrier();
     }
-    if (kb + 1 < blocks) fetch(kb + 1);
-    const uint8_t* at = lds + (kb & 1) * BUF;
+    fetch(kb + NBUF - 1);  // into the buffer that all have read
+    const uint8_t* at = lds + kb % NBUF * BUF;
     if (kb % 4 == 0) {
       const uint32_t* s = win + (kb % WIN) / 4 * SROWS + (lane & 15);
 #pragma unroll
@@ -313,6 +314,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
       for (int j = 0; j < NF; ++j) acc[i][j] = product(n[j], m, acc[i][j]);
     }
   }
+  spr::wait_vm<0>();  // of zeros behind the last block
   static_assert(NF == 4, "put64 takes 64 columns of a wave");
   const int32_t nw = n0 + wn * 64;
   f32x4 bias[NF];
@@ -429,7 +431,7 @@ __global__ __launch_bounds__(512) void turns_product_kernel(Matrix a, Matrix b, 
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  fetch_scales<T, T, WIN>(a, b, m0, n0, 0, blocks, win);
+  fetch_scales<T, T, WIN, 512>(a, b, m0, n0, 0, blocks, win);
   fetch_b(0);
   fetch_a(0, 0);
   fetch_a(0, 1);
@@ -441,7 +443,7 @@ __global__ __launch_bounds__(512) void turns_product_kernel(Matrix a, Matrix b, 
   for (int32_t k0 = 0; k0 < blocks; k0 += WIN) {
     const int32_t end = blocks - k0 < WIN ? blocks : k0 + WIN;
     if (k0 > 0) {  // (the scales in use are in registers; both groups have written before the first reads)
-      fetch_scales<T, T, WIN>(a, b, m0, n0, k0, blocks, win);
+      fetch_scales<T, T, WIN, 512>(a, b, m0, n0, k0, blocks, win);
       change();
       change();
     }
@@ -553,10 +555,44 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Matrix a, Matrix b
   }
 }
 
+// Which kernel: by what the whole call takes, in hundredths of a microsecond, from measured times of a block
+// of the summed dim while the chip is full of tiles (`full` of them), half full or less.  K = 5120, us, outputs in
+// 16 bits:            256 x 256   128 x 128   64 x 128   few rows
+//   1 x 15,360                       29.0        20.5       18.5
+//   32 x 5120                        27.0        20.8       20.0
+//   64 x 15,360                      31.4        21.4       54.4
+//   512 x 5120           51.9        32.8        27.9
+//   1024 x 5120          53.5        37.1        46.9
+//   2048 x 5120          56.9        69.8        76.8
+//   4096 x 5120         115         112         140
+//   32,760 x 5120       673         845        1143
+enum Kernel { LARGE, MIDDLE, SMALL, FEW };
+struct Cost {
+  int32_t tm, tn, full, start, all, most, some;
+};
+Kernel pick_kernel(int64_t M, int64_t N, int32_t K, bool wide) {
+  static const Cost costs[2][3] = {{{256, 256, 256, 600, 168, 165, 139}, {128, 128, 512, 300, 95, 80, 70}, {64, 128, 512, 200, 71, 57, 43}},
+                                   {{256, 256, 256, 600, 335, 320, 306}, {128, 128, 512, 300, 184, 170, 160}, {64, 128, 512, 200, 117, 110, 84}}};
+  const int64_t blocks = spr::ceil_div(K, KB);
+  Kernel best = LARGE;
+  int64_t least = INT64_MAX;
+  for (int i = 0; i < 3; ++i) {
+    const Cost& c = costs[wide ? 1 : 0][i];
+    const int64_t tiles = spr::ceil_div(M, c.tm) * spr::ceil_div(N, c.tn), rest = tiles % c.full;
+    const int64_t cost = spr::ceil_div(tiles, c.full) * c.start +
+                         blocks * (tiles / c.full * c.all + (rest == 0 ? 0 : 2 * rest > c.full ? c.most : c.some));
+    if (cost < least) least = cost, best = static_cast<Kernel>(i);
+  }
+  // few rows: b's bytes once and a's for every 16 of b's rows, 0.15 us a MB
+  if (M <= 64 && 400 + N * K / 1000 * (16 + M) / 16 * 15 / 1000 < least) best = FEW;
+  return best;
+}
+
 template <int DT>
 int launch_product(const Matrix& a, const Matrix& b, int32_t K, const Output& o, hipStream_t stream) {
   const int32_t M = a.rows, N = b.rows;
-  if (M <= 64) {
+  const Kernel kernel = pick_kernel(M, N, K, DT == 2);
+  if (kernel == FEW) {
     const uint32_t grid = static_cast<uint32_t>(spr::ceil_div(N, 16));
     if (M <= 16) few_rows_kernel<DT, 1, 8><<<grid, 512, 0, stream>>>(a, b, K, o);
     else if (M <= 32) few_rows_kernel<DT, 2, 8><<<grid, 512, 0, stream>>>(a, b, K, o);
@@ -564,22 +600,19 @@ int launch_product(const Matrix& a, const Matrix& b, int32_t K, const Output& o,
     SPR_LAUNCHED("few_rows_kernel");
     return SPR_OK;
   }
-  const int64_t large = spr::ceil_div(M, 256) * spr::ceil_div(N, 256);
-  const int32_t t = large >= 192 ? 256 : 128;
-  const int64_t tm = spr::ceil_div(M, t), tn = spr::ceil_div(N, t);
-  SPR_REQUIRE(tm * tn < (int64_t(1) << 23), "spr_fp8_matmul: too many outputs");
+  const int32_t side = kernel == LARGE ? 256 : 128, high = kernel == SMALL ? 64 : side;
+  const int64_t tm = spr::ceil_div(M, high), tn = spr::ceil_div(N, side);
+  SPR_REQUIRE(tm * tn < (int64_t(1) << 22), "spr_fp8_matmul: too many outputs");
   const uint32_t grid = static_cast<uint32_t>(tm * tn);
-  if constexpr (DT == 2) {
-    if (t == 256)
-      product_kernel<DT, 256, 256, 2, 4, 64><<<grid, 512, 0, stream>>>(a, b, K, static_cast<int32_t>(tm),
-                                                                      static_cast<int32_t>(tn), o);
+  const int32_t rows = static_cast<int32_t>(tm), columns = static_cast<int32_t>(tn);
+  if (kernel == MIDDLE) {
+    product_kernel<DT, 128, 128, 2, 2, 32, 2><<<grid, 256, 0, stream>>>(a, b, K, rows, columns, o);
+  } else if (kernel == SMALL) {
+    product_kernel<DT, 64, 128, 2, 2, 32, 3><<<grid, 256, 0, stream>>>(a, b, K, rows, columns, o);
   } else {
-    if (t == 256)
-      turns_product_kernel<DT><<<grid, 512, 0, stream>>>(a, b, K, static_cast<int32_t>(tm), static_cast<int32_t>(tn), o);
+    if constexpr (DT == 2) product_kernel<DT, 256, 256, 2, 4, 64, 2><<<grid, 512, 0, stream>>>(a, b, K, rows, columns, o);
+    else turns_product_kernel<DT><<<grid, 512, 0, stream>>>(a, b, K, rows, columns, o);
   }
-  if (t == 128)
-    product_kernel<DT, 128, 128, 2, 2, 32><<<grid, 256, 0, stream>>>(a, b, K, static_cast<int32_t>(tm),
-                                                                    static_cast<int32_t>(tn), o);
   SPR_LAUNCHED("product_kernel");
   return SPR_OK;
 }

@@ -128,9 +128,11 @@ def test_products_of_whole_numbers_are_exact(dev, m, n, k, squares):
             assert torch.equal(got.cpu(), torch.from_numpy(want + _f64(bias)).to(out))
 
 
-@pytest.mark.parametrize("m,n,k", [(4000, 3500, 256), (3328, 4097, 8320), (49152 + 7, 260, 144)])
-def test_products_on_the_large_tiles_are_exact(dev, m, n, k):
-    """Tiles of 256 x 256, one past the edge of each side, more blocks than a window of scales."""
+@pytest.mark.parametrize("m,n,k", [(4000, 3500, 256), (3328, 4097, 8320), (49152 + 7, 260, 144), (4000, 3585, 16),
+                                   (1030, 5000, 4240), (300, 700, 4240), (90, 5000, 8208), (30, 16, 20016)])
+def test_products_on_tiles_of_every_size_are_exact(dev, m, n, k):
+    """Past the edges of tiles of 256 x 256, 128 x 128 and 64 x 128, and with more blocks than their windows of
+    scales hold; a summed dim shorter than a block on each."""
     from sparsepr_amd.kernels.fp8 import fp8_matmul
 
     g = torch.Generator(device=dev).manual_seed(3)
@@ -140,7 +142,7 @@ def test_products_on_the_large_tiles_are_exact(dev, m, n, k):
     spread = lambda s, r: torch.exp2(s.float() - 127)[torch.arange(r, device=dev) // (1 if len(s) == r else 128)]  # noqa: E731
     af = a.float() * spread(sa, m).repeat_interleave(128, 1)[:, :k]
     bf = b.float() * spread(sb, n).repeat_interleave(128, 1)[:, :k]
-    want = af @ bf.t()  # exact: |a b| <= 16 in steps of 1/4, 8320 of them
+    want = af @ bf.t()  # exact: |a b| <= 16 in steps of 1/4, 20,016 of them at most
     for out in DT.values():
         assert torch.equal(fp8_matmul(a, sa, b, sb, out_dtype=out), want.to(out))
 
