@@ -31,50 +31,64 @@ __device__ __forceinline__ int64_t row_at(const Rows& t, uint32_t row) {
   return a * t.s0 + (row - a * static_cast<uint32_t>(t.n1)) * t.s1;
 }
 
-// The sum of a over the TPR threads of a row, in each of them; `red` has one float per wave.
-template <int TPR, int THREADS>
-__device__ __forceinline__ float row_total(float a, float* red) {
-  a = spr::row_sum(a);
-  if constexpr (TPR > 16) {
-    a += __shfl_xor(a, 16, 64);
-    a += __shfl_xor(a, 32, 64);
-  }
-  if constexpr (TPR > 64) {
-    static_assert(TPR == THREADS, "one row a workgroup");
-    constexpr int WAVES = THREADS / 64;
-    __syncthreads();  // an earlier total has been read
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
-    __syncthreads();
-    a = 0.0f;
+// The sums of N values over the threads of a row, in each of them: TPR threads, or (0) the whole workgroup, whose
+// waves meet in `red`, 16 N floats.
+template <int TPR, int N>
+__device__ __forceinline__ void row_total(float (&a)[N], float* red) {
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) a += red[w];
+  for (int i = 0; i < N; ++i) {
+    a[i] = spr::row_sum(a[i]);
+    if constexpr (TPR != 16) {
+      a[i] += __shfl_xor(a[i], 16, 64);
+      a[i] += __shfl_xor(a[i], 32, 64);
+    }
   }
-  return a;
+  if constexpr (TPR == 0) {
+    const int waves = blockDim.x >> 6;
+    __syncthreads();  // earlier sums have been read
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) red[(threadIdx.x >> 6) * N + i] = a[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = 0.0f;
+    for (int w = 0; w < waves; ++w)
+#pragma unroll
+      for (int i = 0; i < N; ++i) a[i] += red[w * N + i];
+  }
 }
 
-__device__ __forceinline__ float inverse_rms(float ss, int32_t width, float eps) {
-  return __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, static_cast<float>(width)) + eps));
+// Eight partial sums of a lane as a tree.
+__device__ __forceinline__ float tree_sum(const float (&p)[8]) {
+  return ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 }
 
-// TPR threads a row, NV vectors of 8 channels a thread.  RES: 0 no residual, 1 of x's type, 2 fp32.
+// 1 / sqrt(ss / width + eps), rounded once: a value next to a border of its output's type then goes where the
+// formula in more digits sends it, but for the error of ss.  One step of Newton from the instruction's estimate.
+__device__ __forceinline__ float inverse_rms(float ss, double inv_width, float eps) {
+  const double v = static_cast<double>(ss) * inv_width + static_cast<double>(eps);
+  const double r = __builtin_amdgcn_rsq(v), e = __builtin_fma(-v * r, r, 1.0);
+  return static_cast<float>(__builtin_isfinite(e) ? r + 0.5 * r * e : r);  // (of 0 and infinity as they are)
+}
+
+// TPR threads a row (0: the workgroup), NV vectors of 8 channels a thread.  RES: 0 no residual, 1 of x's type, 2 fp32.
 template <int DT, int RES, bool FP8, int TPR, int NV>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(
+__global__ __launch_bounds__(TPR == 0 ? 1024 : 256) void norm_kernel(
     Rows x, Rows residual, const void* __restrict__ weight, int32_t weight_dtype, uint32_t rows, int32_t width,
-    float eps, void* __restrict__ out, uint8_t* __restrict__ scales, void* __restrict__ sum) {
-  constexpr int THREADS = TPR < 256 ? 256 : TPR;
+    double inv_width, float eps, void* __restrict__ out, uint8_t* __restrict__ scales, void* __restrict__ sum) {
   constexpr int SDT = RES == 2 ? 2 : DT;
   using S = typename Elem<DT>::S;
   using R = typename Elem<SDT>::S;
-  __shared__ float red[THREADS / 64];
-  const uint32_t row = blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
-  if (TPR <= 64 && row >= rows) return;
-  const int lane = threadIdx.x % TPR;
+  __shared__ float red[16];
+  const int lane = TPR == 0 ? threadIdx.x : threadIdx.x % TPR, step = TPR == 0 ? blockDim.x : TPR;
+  const uint32_t row = TPR == 0 ? blockIdx.x : blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  if (TPR != 0 && row >= rows) return;
   const S* xr = static_cast<const S*>(x.p) + row_at(x, row);
   float s[NV][8];
-  float ss = 0.0f;
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
-    const int c = (lane + u * TPR) * 8;
+    const int c = (lane + u * step) * 8;
     load8n<DT>(xr + c, width - c, s[u]);
   }
   if constexpr (RES != 0) {
@@ -82,7 +96,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(
     R* sr = static_cast<R*>(sum) + static_cast<int64_t>(row) * width;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int c = (lane + u * TPR) * 8;
+      const int c = (lane + u * step) * 8;
       float t[8];
       load8n<SDT>(rr + c, width - c, t);
 #pragma unroll
@@ -90,14 +104,17 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(
       if (c < width) store8n<SDT>(sr + c, width - c, s[u]);
     }
   }
+  float p[8] = {};
 #pragma unroll
   for (int u = 0; u < NV; ++u)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(s[u][e], s[u][e], ss);
-  const float inv = inverse_rms(row_total<TPR, THREADS>(ss, red), width, eps);
+    for (int e = 0; e < 8; ++e) p[e] = __builtin_fmaf(s[u][e], s[u][e], p[e]);
+  float ss[1] = {tree_sum(p)};
+  row_total<TPR>(ss, red);
+  const float inv = inverse_rms(ss[0], inv_width, eps);
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
-    const int c = (lane + u * TPR) * 8;
+    const int c = (lane + u * step) * 8;
     float w[8];
     if (weight != nullptr) {
       load8n_any(weight, weight_dtype, c, width - c, w);
@@ -129,19 +146,19 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(
 // The gradient: workgroups take rows in turn, each thread keeps the weight's gradient of its channels
 // over all of them, and the workgroups' parts are added by a second kernel in a fixed order.
 template <int DT, int SDT, int TPR, int NV>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_kernel(
+__global__ __launch_bounds__(TPR == 0 ? 1024 : 256) void norm_backward_kernel(
     Rows dy, Rows s_in, Rows dsum, const void* __restrict__ weight, int32_t weight_dtype, uint32_t rows, int32_t width,
-    float eps, void* __restrict__ dx, float* __restrict__ parts) {
-  constexpr int THREADS = TPR < 256 ? 256 : TPR;
-  constexpr int PER = THREADS / TPR;  // rows at a time
+    double inv_width, float eps, void* __restrict__ dx, float* __restrict__ parts) {
+  constexpr int PER = TPR == 0 ? 1 : 256 / TPR;  // rows at a time
   using S = typename Elem<DT>::S;
   using R = typename Elem<SDT>::S;
-  __shared__ float red[THREADS / 64];
-  const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  __shared__ float red[32];
+  const int lane = TPR == 0 ? threadIdx.x : threadIdx.x % TPR, step = TPR == 0 ? blockDim.x : TPR;
+  const int sub = TPR == 0 ? 0 : threadIdx.x / TPR;
   float w[NV][8], dw[NV][8];
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
-    const int c = (lane + u * TPR) * 8;
+    const int c = (lane + u * step) * 8;
     if (weight != nullptr) {
       load8n_any(weight, weight_dtype, c, width - c, w[u]);
     } else {
@@ -154,99 +171,114 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_kernel(
   for (uint32_t row = blockIdx.x * PER + sub; row < rows; row += gridDim.x * PER) {
     const S* dyr = static_cast<const S*>(dy.p) + row_at(dy, row);
     const R* sr = static_cast<const R*>(s_in.p) + row_at(s_in, row);
-    float g[NV][8], s[NV][8];
-    float ss = 0.0f, gs = 0.0f;
+    float g[NV][8], s[NV][8], d[NV][8];
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int c = (lane + u * TPR) * 8;
+      const int c = (lane + u * step) * 8;
       load8n<DT>(dyr + c, width - c, g[u]);
       load8n<SDT>(sr + c, width - c, s[u]);
     }
+    if (dsum.p != nullptr) {
+      const R* dr = static_cast<const R*>(dsum.p) + row_at(dsum, row);
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        const int c = (lane + u * step) * 8;
+        load8n<SDT>(dr + c, width - c, d[u]);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[u][e] = 0.0f;
+    }
+    float p[8] = {}, q[8] = {};
 #pragma unroll
     for (int u = 0; u < NV; ++u)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        ss = __builtin_fmaf(s[u][e], s[u][e], ss);
-        gs = __builtin_fmaf(g[u][e] * w[u][e], s[u][e], gs);
+        p[e] = __builtin_fmaf(s[u][e], s[u][e], p[e]);
+        q[e] = __builtin_fmaf(g[u][e] * w[u][e], s[u][e], q[e]);
       }
-    ss = row_total<TPR, THREADS>(ss, red);
-    gs = row_total<TPR, THREADS>(gs, red);
-    const float inv = inverse_rms(ss, width, eps);
-    const float along = inv * inv * __fdiv_rn(gs, static_cast<float>(width));
+    float t[2] = {tree_sum(p), tree_sum(q)};  // of s^2 and of g s
+    row_total<TPR>(t, red);
+    const float inv = inverse_rms(t[0], inv_width, eps);
+    const float along = inv * inv * (t[1] * static_cast<float>(inv_width));
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int c = (lane + u * TPR) * 8;
-      float d[8];
-      if (dsum.p != nullptr) {
-        load8n<SDT>(static_cast<const R*>(dsum.p) + row_at(dsum, row) + c, width - c, d);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = 0.0f;
-      }
+      const int c = (lane + u * step) * 8;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float n = s[u][e] * inv;
-        dw[u][e] = __builtin_fmaf(g[u][e], n, dw[u][e]);
-        d[e] = __builtin_fmaf(inv, __builtin_fmaf(-s[u][e], along, g[u][e] * w[u][e]), d[e]);
+        dw[u][e] = __builtin_fmaf(g[u][e], s[u][e] * inv, dw[u][e]);
+        d[u][e] = __builtin_fmaf(inv, __builtin_fmaf(-s[u][e], along, g[u][e] * w[u][e]), d[u][e]);
       }
-      if (c < width) store8n<SDT>(static_cast<R*>(dx) + static_cast<int64_t>(row) * width + c, width - c, d);
+      if (c < width) store8n<SDT>(static_cast<R*>(dx) + static_cast<int64_t>(row) * width + c, width - c, d[u]);
     }
   }
   if (parts == nullptr) return;
   // the rows that a workgroup takes at a time, added in LDS; then one row of `parts` each
   if constexpr (PER > 1) {
+    static_assert(NV == 1, "one vector a thread");
     __shared__ float add[PER * TPR * 8];
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) add[(sub * TPR + lane) * 8 + e] = dw[u][e];
-      __syncthreads();
-      for (int i = threadIdx.x; i < TPR * 8; i += THREADS) {
-        float t = 0.0f;
-        for (int p = 0; p < PER; ++p) t += add[p * TPR * 8 + i];
-        const int c = u * TPR * 8 + i;
-        if (c < width) parts[static_cast<int64_t>(blockIdx.x) * width + c] = t;
-      }
-      __syncthreads();
+    for (int e = 0; e < 8; ++e) add[(sub * TPR + lane) * 8 + e] = dw[0][e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < TPR * 8 && c < width; c += 256) {
+      float t = 0.0f;
+      for (int r = 0; r < PER; ++r) t += add[r * TPR * 8 + c];
+      parts[static_cast<int64_t>(blockIdx.x) * width + c] = t;
     }
   } else {
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int c = (lane + u * TPR) * 8;
+      const int c = (lane + u * step) * 8;
       if (c < width) store8n<2>(parts + static_cast<int64_t>(blockIdx.x) * width + c, width - c, dw[u]);
     }
   }
 }
 
-// dw[c] = sum over the workgroups' parts: 64 channels a workgroup, 4 waves over the parts.
-__global__ __launch_bounds__(256) void norm_weight_gradient_kernel(const float* __restrict__ parts, int32_t n,
-                                                                  int32_t width, float* __restrict__ dw) {
-  __shared__ float red[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
-  float t = 0.0f;
-  if (c < width)
-    for (int p = wave; p < n; p += 4) t += parts[static_cast<int64_t>(p) * width + c];
-  red[wave][lane] = t;
+// dw[c] = sum over the workgroups' parts: 32 channels a workgroup, 32 half waves over the parts.
+__global__ __launch_bounds__(1024) void norm_weight_gradient_kernel(const float* __restrict__ parts, int32_t n,
+                                                                   int32_t width, float* __restrict__ dw) {
+  __shared__ float red[32][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  float t[4] = {};
+  if (c < width) {
+    int p = slice;
+    for (; p + 96 < n; p += 128)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] += parts[static_cast<int64_t>(p + 32 * i) * width + c];
+    for (; p < n; p += 32) t[0] += parts[static_cast<int64_t>(p) * width + c];
+  }
+  red[slice][lane] = (t[0] + t[1]) + (t[2] + t[3]);
   __syncthreads();
-  if (wave == 0 && c < width) dw[c] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+  float sum = red[lane][slice];  // slice's channel, one part a lane
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 32);
+  if (lane == 0 && blockIdx.x * 32 + slice < width) dw[blockIdx.x * 32 + slice] = sum;
 }
 
-// Lanes of a row and vectors a lane: a quarter wave to 128 channels, a wave to 2048, a workgroup above.
-#define SPR_BY_WIDTH(CALL)           \
-  if (width <= 128) CALL(16, 1);     \
+// Lanes of a row and vectors a lane: a quarter wave to 128 channels, a wave to 512, above a workgroup of as many
+// waves as the row has 512 channels (1024 from 8192 on).
+#define SPR_BY_WIDTH(CALL)            \
+  if (width <= 128) CALL(16, 1);      \
   else if (width <= 512) CALL(64, 1); \
-  else if (width <= 2048) CALL(64, 4); \
-  else if (width <= 8192) CALL(256, 4); \
-  else CALL(1024, 2)
+  else if (width <= 8192) CALL(0, 1); \
+  else CALL(0, 2)
+
+uint32_t threads_of(int32_t width) {
+  if (width <= 512) return 256;
+  return 64 * static_cast<uint32_t>(spr::ceil_div(width, width <= 8192 ? 512 : 1024));
+}
+int32_t rows_at_a_time(int32_t width) { return width <= 128 ? 16 : width <= 512 ? 4 : 1; }
 
 template <int DT, int RES, bool FP8>
 void launch_norm(const Rows& x, const Rows& residual, const void* weight, int32_t weight_dtype, uint32_t rows,
                  int32_t width, float eps, void* out, uint8_t* scales, void* sum, hipStream_t stream) {
 #define SPR_NORM(TPR, NV)                                                                                    \
   norm_kernel<DT, RES, FP8, TPR, NV>                                                                         \
-      <<<static_cast<uint32_t>(spr::ceil_div(rows, TPR < 256 ? 256 / TPR : 1)), TPR < 256 ? 256 : TPR, 0, stream>>>( \
-          x, residual, weight, weight_dtype, rows, width, eps, out, scales, sum)
+      <<<static_cast<uint32_t>(spr::ceil_div(rows, rows_at_a_time(width))), threads_of(width), 0, stream>>>( \
+          x, residual, weight, weight_dtype, rows, width, 1.0 / width, eps, out, scales, sum)
   SPR_BY_WIDTH(SPR_NORM);
 #undef SPR_NORM
 }
@@ -257,8 +289,6 @@ void launch_norm(bool fp8, const Rows& x, const Rows& residual, const void* weig
   if (fp8) launch_norm<DT, RES, true>(x, residual, weight, weight_dtype, rows, width, eps, out, scales, sum, stream);
   else launch_norm<DT, RES, false>(x, residual, weight, weight_dtype, rows, width, eps, out, scales, sum, stream);
 }
-
-int32_t rows_at_a_time(int32_t width) { return width <= 128 ? 16 : width <= 2048 ? 4 : 1; }
 
 // Workgroups of the gradient: enough to fill the chip a few times over, and few enough that their
 // parts of the weight's gradient are small beside the rows.
@@ -273,16 +303,16 @@ void launch_backward(const Rows& dy, const Rows& s, const Rows& dsum, const void
                      uint32_t rows, int32_t width, float eps, void* dx, float* parts, hipStream_t stream) {
   const uint32_t groups = static_cast<uint32_t>(backward_groups(rows, width));
 #define SPR_NORM(TPR, NV)                                                                 \
-  norm_backward_kernel<DT, SDT, TPR, NV><<<groups, TPR < 256 ? 256 : TPR, 0, stream>>>( \
-      dy, s, dsum, weight, weight_dtype, rows, width, eps, dx, parts)
+  norm_backward_kernel<DT, SDT, TPR, NV><<<groups, threads_of(width), 0, stream>>>(       \
+      dy, s, dsum, weight, weight_dtype, rows, width, 1.0 / width, eps, dx, parts)
   SPR_BY_WIDTH(SPR_NORM);
 #undef SPR_NORM
 }
 
 // (a launch has fewer than 2^32 threads)
 bool launch_fits(int64_t n0, int64_t n1, int32_t width) {
-  const int64_t per = width <= 128 ? 16 : width <= 2048 ? 64 : width <= 8192 ? 256 : 1024;
-  return n0 * n1 < (int64_t(1) << 32) / per - 1024 && n0 * n1 < (int64_t(1) << 31);
+  const int64_t blocks = spr::ceil_div(n0 * n1, rows_at_a_time(width));
+  return n0 * n1 < (int64_t(1) << 31) && blocks * threads_of(width) < (int64_t(1) << 32);
 }
 
 bool rows_fit(int64_t n0, int64_t n1, int64_t s0, int64_t s1) {
@@ -350,7 +380,7 @@ extern "C" int spr_rms_norm_backward(const void* dy, int64_t dy_s0, int64_t dy_s
   const int32_t groups = rows == 0 ? 0 : backward_groups(rows, width);
   if (rows == 0) {
     if (dweight != nullptr) {
-      norm_weight_gradient_kernel<<<static_cast<uint32_t>(spr::ceil_div(width, 64)), 256, 0, stream>>>(nullptr, 0, width,
+      norm_weight_gradient_kernel<<<static_cast<uint32_t>(spr::ceil_div(width, 32)), 1024, 0, stream>>>(nullptr, 0, width,
                                                                                                       dweight);
       SPR_LAUNCHED("norm_weight_gradient_kernel");
     }
@@ -379,7 +409,7 @@ extern "C" int spr_rms_norm_backward(const void* dy, int64_t dy_s0, int64_t dy_s
 #undef SPR_BACK
   SPR_LAUNCHED("norm_backward_kernel");
   if (dweight != nullptr) {
-    norm_weight_gradient_kernel<<<static_cast<uint32_t>(spr::ceil_div(width, 64)), 256, 0, stream>>>(parts, groups, width,
+    norm_weight_gradient_kernel<<<static_cast<uint32_t>(spr::ceil_div(width, 32)), 1024, 0, stream>>>(parts, groups, width,
                                                                                                     dweight);
     SPR_LAUNCHED("norm_weight_gradient_kernel");
   }
