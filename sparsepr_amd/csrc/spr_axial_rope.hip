@@ -7,8 +7,8 @@
 //
 // The turn is 64 bits up to the part below one: at place 118,800 an angle in fp32 is off by 0.004.  Its
 // sine and cosine are fp32 (sincospif), the rotation fp32 with one rounding at the end.
-// Bound by memory (Q and K read and written once).  A lane holds 4 pairs of one token: it finds their
-// angles once and turns the same pairs of every PER-th head.
+// Bound by memory (Q and K read and written once): Q and K of 32,760 x 40 x 128 in bf16 take 267 us, 5.0 TB/s, what a
+// copy takes.  A lane holds 4 pairs of one token: it finds their angles once and turns the same pairs of several heads.
 #include "spr_elem.h"
 
 namespace {
@@ -24,19 +24,19 @@ struct Side {  // Q or K, [batch, heads, tokens, D], and the output, contiguous
   int32_t heads;
 };
 
-// Four values, from any address that an element may have.
-template <int DT>
-__device__ __forceinline__ void load4(const typename Elem<DT>::S* p, float (&x)[4]) {
-  typename Elem<DT>::S r[4];
+// N values, from any address that an element may have.
+template <int DT, int N>
+__device__ __forceinline__ void load(const typename Elem<DT>::S* p, float* x) {
+  typename Elem<DT>::S r[N];
   __builtin_memcpy(r, p, sizeof(r));
 #pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = Elem<DT>::to_f(r[e]);
+  for (int e = 0; e < N; ++e) x[e] = Elem<DT>::to_f(r[e]);
 }
-template <int DT>
-__device__ __forceinline__ void store4(typename Elem<DT>::S* p, const float (&x)[4]) {
-  typename Elem<DT>::S r[4];
+template <int DT, int N>
+__device__ __forceinline__ void store(typename Elem<DT>::S* p, const float* x) {
+  typename Elem<DT>::S r[N];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) r[e] = Elem<DT>::from_f(x[e]);
+  for (int e = 0; e < N; ++e) r[e] = Elem<DT>::from_f(x[e]);
   __builtin_memcpy(p, r, sizeof(r));
 }
 
@@ -64,17 +64,17 @@ __device__ __forceinline__ void angle_of(const void* positions, int32_t code, in
   s = sign * sn;
 }
 
-// Units of a row: R / 8 of 4 pairs, then (D - R) / 8 of 8 dims to copy.  `units` of them a token, `per`
-// tokens-and-head-slots (units lanes each) a workgroup; slots of one token take its heads in turn.
-template <int DT, bool HALVES>
+// Units of a row: R / 2P of P pairs, then (D - R) / 2P of 2P dims to copy, a lane each.  A workgroup has as many (token,
+// slot) pairs as its lanes hold rows; the slots of a token take its heads in turn, AHEAD of them on their way at once.
+template <int DT, bool HALVES, int P>
 __global__ __launch_bounds__(THREADS) void rope_kernel(Side q, Side k, const void* __restrict__ positions,
                                                        int32_t position_code, int64_t position_b, int32_t axes,
                                                        const double* __restrict__ freqs,
                                                        const int32_t* __restrict__ axis, int64_t rows, int64_t tokens,
-                                                       int32_t dim, int32_t rotated, int32_t units, int32_t slots,
-                                                       float sign) {
+                                                       int32_t dim, int32_t rotated, int32_t slots, float sign) {
   using S = typename Elem<DT>::S;
-  const int per = THREADS / units;  // (token, slot) pairs of a workgroup
+  constexpr int AHEAD = 4;
+  const int units = dim / (2 * P), per = THREADS / units;
   const int mine = threadIdx.x / units, unit = threadIdx.x - mine * units;
   if (mine >= per) return;
   const int64_t job = static_cast<int64_t>(blockIdx.x) * per + mine;
@@ -82,63 +82,81 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(Side q, Side k, const voi
   if (row >= rows) return;
   const int slot = static_cast<int>(job - row * slots);
   const int64_t b = row / tokens, t = row - b * tokens;
-  const bool turned = unit * 8 < rotated;
-  float c[4], s[4];
+  const bool turned = unit * 2 * P < rotated;
+  float c[P], s[P];
   if (turned) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      angle_of(positions, position_code, b * position_b + t * axes, axes, freqs, axis, unit * 4 + e, sign, c[e], s[e]);
+    for (int e = 0; e < P; ++e)
+      angle_of(positions, position_code, b * position_b + t * axes, axes, freqs, axis, unit * P + e, sign, c[e], s[e]);
   }
-  // the two groups of 4 dims of a unit
-  const int d0 = HALVES && turned ? unit * 4 : unit * 8;
-  const int d1 = HALVES && turned ? d0 + rotated / 2 : d0 + 4;
-  for (int h = slot; h < q.heads + k.heads; h += slots) {
-    const bool is_k = h >= q.heads;
-    const Side& side = is_k ? k : q;
-    const int hh = is_k ? h - q.heads : h;
-    const S* x = static_cast<const S*>(side.x) + b * side.b + hh * side.h + t * side.t;
-    S* o = static_cast<S*>(side.out) + ((b * side.heads + hh) * tokens + t) * dim;
-    float u[4], v[4];
-    load4<DT>(x + d0, u);
-    load4<DT>(x + d1, v);
-    if (turned) {
-      float p[4], r[4];
+  // the two groups of P dims of a unit: a pair's first and second dims, or (interleaved) one behind the other
+  const int d0 = HALVES && turned ? unit * P : unit * 2 * P;
+  const int d1 = HALVES && turned ? d0 + rotated / 2 : d0 + P;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const Side& side = which == 0 ? q : k;
+    const S* x = static_cast<const S*>(side.x) + b * side.b + t * side.t;
+    S* o = static_cast<S*>(side.out) + (b * side.heads * tokens + t) * dim;
+    for (int h0 = slot; h0 < side.heads; h0 += AHEAD * slots) {
+      float u[AHEAD][2 * P];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // pairs (2i, 2i + 1): the first two of a unit lie in u, the others in v
-        const float a = HALVES ? u[e] : e < 2 ? u[2 * e] : v[2 * e - 4];
-        const float w = HALVES ? v[e] : e < 2 ? u[2 * e + 1] : v[2 * e - 3];
-        p[e] = __builtin_fmaf(a, c[e], -(w * s[e]));
-        r[e] = __builtin_fmaf(w, c[e], a * s[e]);
+      for (int i = 0; i < AHEAD; ++i) {
+        const int h = h0 + i * slots;
+        if (h < side.heads) {
+          const S* p = x + h * side.h;
+          if constexpr (HALVES) {
+            load<DT, P>(p + d0, u[i]);
+            load<DT, P>(p + d1, u[i] + P);
+          } else {
+            load<DT, 2 * P>(p + d0, u[i]);
+          }
+        }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        u[e] = HALVES ? p[e] : e % 2 == 0 ? p[e / 2] : r[e / 2];
-        v[e] = HALVES ? r[e] : e % 2 == 0 ? p[2 + e / 2] : r[2 + e / 2];
+      for (int i = 0; i < AHEAD; ++i) {
+        const int h = h0 + i * slots;
+        if (h < side.heads) {
+          if (turned) {
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+              float& first = u[i][HALVES ? e : 2 * e];
+              float& second = u[i][HALVES ? P + e : 2 * e + 1];
+              const float f = __builtin_fmaf(first, c[e], -(second * s[e]));
+              second = __builtin_fmaf(second, c[e], first * s[e]);
+              first = f;
+            }
+          }
+          S* p = o + static_cast<int64_t>(h) * tokens * dim;
+          if constexpr (HALVES) {
+            store<DT, P>(p + d0, u[i]);
+            store<DT, P>(p + d1, u[i] + P);
+          } else {
+            store<DT, 2 * P>(p + d0, u[i]);
+          }
+        }
       }
     }
-    store4<DT>(o + d0, u);
-    store4<DT>(o + d1, v);
   }
 }
 
-template <int DT>
-int launch_rope(bool halves, const Side& q, const Side& k, const void* positions, int32_t code, int64_t position_b,
-                 int32_t axes, const double* freqs, const int32_t* axis, int64_t rows, int64_t tokens, int32_t dim,
-                 int32_t rotated, float sign, hipStream_t stream) {
-  const int32_t units = dim / 8, per = THREADS / units, heads = q.heads + k.heads;
-  // every head a slot of its own while that leaves CUs without work, else slots of 4 heads or more
-  int32_t slots = heads;
-  while (slots > 1 && rows * slots > 8192 * static_cast<int64_t>(per) && heads / slots < 8) slots = (slots + 1) / 2;
-  const int64_t wanted = spr::ceil_div(rows * slots, per);
-  SPR_REQUIRE(wanted < (int64_t(1) << 24), "spr_axial_rope: too many rows");  // 2^32 threads of a launch
-  const uint32_t blocks = static_cast<uint32_t>(wanted);
-#define SPR_ROPE(HALVES)                                                                                          \
-  rope_kernel<DT, HALVES><<<blocks, THREADS, 0, stream>>>(q, k, positions, code, position_b, axes, freqs, axis, rows, \
-                                                          tokens, dim, rotated, units, slots, sign)
-  if (halves) SPR_ROPE(true);
-  else SPR_ROPE(false);
-#undef SPR_ROPE
+// Slots of a token: a million lanes, two rounds of the chip's waves, and no more slots than heads; an angle serves the
+// heads that share its slot.  (32,760 tokens of 80 heads: 267 us, 276 with half as many; 8000 of 40: 31 us, 38 with
+// twice as many.)
+int32_t rope_slots(int64_t rows, int32_t units, int32_t heads) {
+  const int64_t wanted = spr::ceil_div(int64_t(1) << 20, rows * units);
+  return static_cast<int32_t>(wanted < heads ? wanted : heads);
+}
+
+template <int DT, bool HALVES, int P>
+int launch_rope(const Side& q, const Side& k, const void* positions, int32_t code, int64_t position_b, int32_t axes,
+                const double* freqs, const int32_t* axis, int64_t rows, int64_t tokens, int32_t dim, int32_t rotated,
+                float sign, hipStream_t stream) {
+  const int32_t units = dim / (2 * P), per = THREADS / units;
+  const int32_t slots = rope_slots(rows, units, q.heads > k.heads ? q.heads : k.heads);
+  const int64_t blocks = spr::ceil_div(rows * slots, per);
+  SPR_REQUIRE(blocks < (int64_t(1) << 24), "spr_axial_rope: too many rows");  // 2^32 threads of a launch
+  rope_kernel<DT, HALVES, P><<<static_cast<uint32_t>(blocks), THREADS, 0, stream>>>(
+      q, k, positions, code, position_b, axes, freqs, axis, rows, tokens, dim, rotated, slots, sign);
   SPR_LAUNCHED("rope_kernel");
   return SPR_OK;
 }
@@ -167,11 +185,11 @@ extern "C" int spr_axial_rope(const void* q, int64_t q_b, int64_t q_h, int64_t q
   SPR_REQUIRE(batch < (int64_t(1) << 40) / tokens / (q_heads + k_heads), "spr_axial_rope: too many rows");
   const Side qs{q, q_out, q_b, q_h, q_t, q_heads}, ks{k, k_out, k_b, k_h, k_t, k_heads};
   const float sign = inverse != 0 ? -1.0f : 1.0f;
-#define SPR_ROPE(DT)                                                                                            \
-  launch_rope<DT>(halves != 0, qs, ks, positions, position_code, position_b, axes, freqs, axis, batch * tokens, \
-                  tokens, dim, rotated, sign, stream)
-  if (dtype == 0) return SPR_ROPE(0);
-  if (dtype == 1) return SPR_ROPE(1);
-  return SPR_ROPE(2);
+  // 16 bytes of a row a lane, or (halves) 8 and 8 in 16 bits: 16 and 16 took 2 % longer on 118,800 tokens
+#define SPR_ROPE(DT, HALVES, P)                                                                                 \
+  launch_rope<DT, HALVES, P>(qs, ks, positions, position_code, position_b, axes, freqs, axis, batch * tokens, tokens, \
+                             dim, rotated, sign, stream)
+  if (halves != 0) return dtype == 0 ? SPR_ROPE(0, true, 4) : dtype == 1 ? SPR_ROPE(1, true, 4) : SPR_ROPE(2, true, 4);
+  return dtype == 0 ? SPR_ROPE(0, false, 4) : dtype == 1 ? SPR_ROPE(1, false, 4) : SPR_ROPE(2, false, 2);
 #undef SPR_ROPE
 }

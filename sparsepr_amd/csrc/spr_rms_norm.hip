@@ -31,19 +31,19 @@ __device__ __forceinline__ int64_t row_at(const Rows& t, uint32_t row) {
   return a * t.s0 + (row - a * static_cast<uint32_t>(t.n1)) * t.s1;
 }
 
-// The sums of N values over the threads of a row, in each of them: TPR threads, or (0) the whole workgroup, whose
-// waves meet in `red`, 16 N floats.
+// The sums of N values over the threads of a row, in each of them: 16, or (0) the whole workgroup, whose waves meet
+// in `red`, 16 N floats.
 template <int TPR, int N>
 __device__ __forceinline__ void row_total(float (&a)[N], float* red) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     a[i] = spr::row_sum(a[i]);
-    if constexpr (TPR != 16) {
+    if constexpr (TPR == 0) {
       a[i] += __shfl_xor(a[i], 16, 64);
       a[i] += __shfl_xor(a[i], 32, 64);
     }
   }
-  if constexpr (TPR == 0) {
+  if (TPR == 0 && blockDim.x > 64) {
     const int waves = blockDim.x >> 6;
     __syncthreads();  // earlier sums have been read
     if ((threadIdx.x & 63) == 0) {
@@ -258,28 +258,28 @@ __global__ __launch_bounds__(1024) void norm_weight_gradient_kernel(const float*
   if (lane == 0 && blockIdx.x * 32 + slice < width) dw[blockIdx.x * 32 + slice] = sum;
 }
 
-// Lanes of a row and vectors a lane: a quarter wave to 128 channels, a wave to 512, above a workgroup of as many
-// waves as the row has 512 channels (1024 from 8192 on).
-#define SPR_BY_WIDTH(CALL)            \
-  if (width <= 128) CALL(16, 1);      \
-  else if (width <= 512) CALL(64, 1); \
-  else if (width <= 8192) CALL(0, 1); \
-  else CALL(0, 2)
-
-uint32_t threads_of(int32_t width) {
-  if (width <= 512) return 256;
-  return 64 * static_cast<uint32_t>(spr::ceil_div(width, width <= 8192 ? 512 : 1024));
+// A row is a quarter wave's to 128 channels, a wave's to 512 and a workgroup's above.  The norm has one vector of 8
+// channels a lane to 512 and two above: 160 M values of 5120 channels to 8 bits take 197 us with two (five waves),
+// 250 with one (ten), 201 with four; 1024 and 8192 channels 183 and 192 with two, 187 and 204 with one.  The gradient
+// has one to 8192: 21 M values of 2560 and 5120 channels take 41 and 40 us with one, 46 and 47 with two.
+uint32_t norm_threads(int32_t width) {
+  return width <= 128 ? 256 : width <= 512 ? 64 : 64 * static_cast<uint32_t>(spr::ceil_div(width, 1024));
 }
-int32_t rows_at_a_time(int32_t width) { return width <= 128 ? 16 : width <= 512 ? 4 : 1; }
+uint32_t gradient_threads(int32_t width) {
+  return width <= 128 ? 256 : 64 * static_cast<uint32_t>(spr::ceil_div(width, width <= 8192 ? 512 : 1024));
+}
+int32_t rows_at_a_time(int32_t width) { return width <= 128 ? 16 : 1; }
 
 template <int DT, int RES, bool FP8>
 void launch_norm(const Rows& x, const Rows& residual, const void* weight, int32_t weight_dtype, uint32_t rows,
                  int32_t width, float eps, void* out, uint8_t* scales, void* sum, hipStream_t stream) {
 #define SPR_NORM(TPR, NV)                                                                                    \
   norm_kernel<DT, RES, FP8, TPR, NV>                                                                         \
-      <<<static_cast<uint32_t>(spr::ceil_div(rows, rows_at_a_time(width))), threads_of(width), 0, stream>>>( \
+      <<<static_cast<uint32_t>(spr::ceil_div(rows, rows_at_a_time(width))), norm_threads(width), 0, stream>>>( \
           x, residual, weight, weight_dtype, rows, width, 1.0 / width, eps, out, scales, sum)
-  SPR_BY_WIDTH(SPR_NORM);
+  if (width <= 128) SPR_NORM(16, 1);
+  else if (width <= 512) SPR_NORM(0, 1);
+  else SPR_NORM(0, 2);
 #undef SPR_NORM
 }
 
@@ -290,10 +290,11 @@ void launch_norm(bool fp8, const Rows& x, const Rows& residual, const void* weig
   else launch_norm<DT, RES, false>(x, residual, weight, weight_dtype, rows, width, eps, out, scales, sum, stream);
 }
 
-// Workgroups of the gradient: enough to fill the chip a few times over, and few enough that their
-// parts of the weight's gradient are small beside the rows.
+// Workgroups of the gradient: about 5120 waves, so that every SIMD has a few rows on their way and the parts of the
+// weight's gradient stay small beside the rows (2560 channels: 43, 41 and 47 us with 512, 1024 and 2048 of them;
+// 1024: 61, 44 and 42; 8192: 46 and 54 with 512 and 1024).
 int32_t backward_groups(int64_t rows, int32_t width) {
-  const int64_t most = width > 8192 ? 256 : 1024;
+  const int64_t waves = gradient_threads(width) / 64, most = 5120 / waves > 512 ? 5120 / waves : 512;
   const int64_t all = spr::ceil_div(rows, rows_at_a_time(width));
   return static_cast<int32_t>(all < most ? all : most);
 }
@@ -303,16 +304,18 @@ void launch_backward(const Rows& dy, const Rows& s, const Rows& dsum, const void
                      uint32_t rows, int32_t width, float eps, void* dx, float* parts, hipStream_t stream) {
   const uint32_t groups = static_cast<uint32_t>(backward_groups(rows, width));
 #define SPR_NORM(TPR, NV)                                                                 \
-  norm_backward_kernel<DT, SDT, TPR, NV><<<groups, threads_of(width), 0, stream>>>(       \
+  norm_backward_kernel<DT, SDT, TPR, NV><<<groups, gradient_threads(width), 0, stream>>>( \
       dy, s, dsum, weight, weight_dtype, rows, width, 1.0 / width, eps, dx, parts)
-  SPR_BY_WIDTH(SPR_NORM);
+  if (width <= 128) SPR_NORM(16, 1);
+  else if (width <= 8192) SPR_NORM(0, 1);
+  else SPR_NORM(0, 2);
 #undef SPR_NORM
 }
 
 // (a launch has fewer than 2^32 threads)
 bool launch_fits(int64_t n0, int64_t n1, int32_t width) {
   const int64_t blocks = spr::ceil_div(n0 * n1, rows_at_a_time(width));
-  return n0 * n1 < (int64_t(1) << 31) && blocks * threads_of(width) < (int64_t(1) << 32);
+  return n0 * n1 < (int64_t(1) << 31) && blocks * norm_threads(width) < (int64_t(1) << 32);
 }
 
 bool rows_fit(int64_t n0, int64_t n1, int64_t s0, int64_t s1) {
