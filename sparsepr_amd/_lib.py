@@ -226,19 +226,19 @@ def stream(device: torch.device) -> int:
 
 
 def require_gpu(*tensors: torch.Tensor | None, what: str = "tensor") -> torch.device:
-    dev = None
+    first, index = None, -1
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
             raise RuntimeError(f"{what}: SparsePR HIP kernels require GPU tensors (got {t.device})")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"{what}: tensors are on different devices ({dev} vs {t.device})")
-    if dev is None:
+        if first is None:
+            first, index = t, t.get_device()
+        elif t.get_device() != index:
+            raise RuntimeError(f"{what}: tensors are on different devices ({first.device} vs {t.device})")
+    if first is None:
         raise RuntimeError(f"{what}: no tensor given")
-    return dev
+    return first.device
 
 
 DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}

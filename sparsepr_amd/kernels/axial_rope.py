@@ -40,9 +40,11 @@ def grid_positions(frames: int, height: int, width: int, *, first=(0, 0, 0), dev
 
 def _strided(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
     """x [B, H, T, D] and its strides over the first three dims; a copy where rows are not packed."""
-    if x.shape[3] > 1 and x.stride(3) != 1:
+    b, h, t, d = x.stride()
+    if d != 1 and x.shape[3] > 1:
         x = x.contiguous()
-    return x, x.stride(0), x.stride(1), x.stride(2)
+        b, h, t, d = x.stride()
+    return x, b, h, t
 
 
 def axial_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, freqs: torch.Tensor,
@@ -61,34 +63,38 @@ def axial_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
         raise RuntimeError(f"{what}: q must be [B, H, T, D] in bfloat16, float16 or float32, got {q.dtype} "
                            f"{tuple(q.shape)}")
     b, h, t, d = q.shape
-    if k is not None and (k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], *k.shape[2:]) != (b, t, d)):
-        raise RuntimeError(f"{what}: k must be [{b}, heads, {t}, {d}] in {q.dtype}, got {k.dtype} {tuple(k.shape)}")
+    hk = 0
+    if k is not None:
+        shape = k.shape
+        hk = shape[1] if len(shape) == 4 else -1
+        if shape != (b, hk, t, d) or k.dtype is not q.dtype:
+            raise RuntimeError(f"{what}: k must be [{b}, heads, {t}, {d}] in {q.dtype}, got {k.dtype} {tuple(shape)}")
     if pairs not in ("interleaved", "halves"):
         raise RuntimeError(f"{what}: pairs must be 'interleaved' or 'halves', got {pairs!r}")
-    if positions.dtype not in POSITION_CODE or positions.dim() not in (2, 3) or positions.shape[-2] != t \
-            or (positions.dim() == 3 and positions.shape[0] != b):
+    place, axes = positions.shape, positions.shape[-1] if positions.dim() > 1 else 0
+    code = POSITION_CODE.get(positions.dtype)
+    if code is None or (place != (t, axes) and place != (b, t, axes)):
         raise RuntimeError(f"{what}: positions must be [{t}, axes] or [{b}, {t}, axes] in int32, int64, float32 or "
                            f"float64, got {positions.dtype} {tuple(positions.shape)}")
     if freqs.dtype is not torch.float64 or axis.dtype is not torch.int32 or freqs.dim() != 1 \
             or axis.shape != freqs.shape or not freqs.is_contiguous() or not axis.is_contiguous():
         raise RuntimeError(f"{what}: freqs must be contiguous float64 and axis contiguous int32 of one length, got "
                            f"{freqs.dtype} {tuple(freqs.shape)} / {axis.dtype} {tuple(axis.shape)}")
-    rotated, axes = 2 * freqs.shape[0], positions.shape[-1]
+    rotated = 2 * freqs.shape[0]
     if d % 8 != 0 or not 8 <= d <= 1024 or rotated % 8 != 0 or rotated > d:
         raise RuntimeError(f"{what}: {rotated} rotated dims of {d} (both multiples of 8, D at most 1024)")
     if not 1 <= axes <= 16:
         raise RuntimeError(f"{what}: {axes} axes, 1 to 16 are taken")
     q_out = q.new_empty((b, h, t, d))
-    k_out = None if k is None else k.new_empty(k.shape)
-    if q_out.numel() + (0 if k is None else k_out.numel()) > 0:
+    k_out = None if k is None else q.new_empty((b, hk, t, d))
+    if b * t * (h + hk) > 0:
         positions = positions.contiguous()
-        hk, k_strides = 0, (0, 0, 0)
+        k_strides = (0, 0, 0)
         q, *q_strides = _strided(q)
         if k is not None:
-            hk = k.shape[1]
             k, *k_strides = _strided(k)
         _lib.launch("spr_axial_rope", dev, q.data_ptr(), *q_strides, h, _lib.ptr(k), *k_strides, hk,
-                    _lib.DTYPE_CODE[q.dtype], b, t, d, rotated, positions.data_ptr(), POSITION_CODE[positions.dtype],
-                    t * axes if positions.dim() == 3 else 0, axes, freqs.data_ptr(), axis.data_ptr(),
+                    _lib.DTYPE_CODE[q.dtype], b, t, d, rotated, positions.data_ptr(), code,
+                    t * axes if len(place) == 3 else 0, axes, freqs.data_ptr(), axis.data_ptr(),
                     int(pairs == "halves"), int(inverse), q_out.data_ptr(), _lib.ptr(k_out))
     return q_out, k_out

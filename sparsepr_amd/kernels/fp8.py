@@ -27,18 +27,19 @@ CODES = torch.float8_e4m3fn
 
 def no_gradient(what: str, *tensors: torch.Tensor | None) -> None:
     """Refuse what autograd would lose without a word."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what}: autograd does not record this call; call it under torch.no_grad() and use the "
-                           "gradient functions beside it")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what}: autograd does not record this call; call it under torch.no_grad() and use the "
+                               "gradient functions beside it")
 
 
 def _packed_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     """x [R, C] and its row stride: itself where rows are packed, else a copy."""
-    if x.shape[1] == 1 or x.stride(1) == 1:
-        if x.shape[0] <= 1 or x.stride(0) >= 0:
-            return x, x.stride(0) if x.shape[0] > 1 else x.shape[1]
-    x = x.contiguous()
-    return x, x.shape[1]
+    rows, width = x.shape
+    step, packed = x.stride()
+    if packed == 1 or width == 1:
+        return x, step if rows > 1 else width
+    return x.contiguous(), width
 
 
 def _check_matrix(codes: torch.Tensor, scales: torch.Tensor, what: str, name: str) -> tuple[int, int, int]:
@@ -46,22 +47,23 @@ def _check_matrix(codes: torch.Tensor, scales: torch.Tensor, what: str, name: st
     if codes.dtype is not CODES or codes.dim() != 2:
         raise RuntimeError(f"{what}: {name} must be float8_e4m3fn [rows, width], got {codes.dtype} {tuple(codes.shape)}")
     rows, width = codes.shape
+    blocks = -(-width // BLOCK)
     if width % 16 != 0:
         raise RuntimeError(f"{what}: the width of {name} ({width}) must be a multiple of 16 (zeros behind the row)")
-    blocks = -(-width // BLOCK)
-    if scales.dtype is not torch.uint8 or scales.dim() != 2 or scales.shape[1] != blocks \
-            or scales.shape[0] not in (rows, -(-rows // BLOCK)):
+    shape = scales.shape
+    if scales.dtype is not torch.uint8 or len(shape) != 2 or shape[1] != blocks \
+            or (shape[0] != rows and shape[0] != -(-rows // BLOCK)):
         raise RuntimeError(f"{what}: the scales of {name} must be uint8 [{rows} or {-(-rows // BLOCK)}, {blocks}], got "
                            f"{scales.dtype} {tuple(scales.shape)}")
-    return rows, width, int(scales.shape[0] != rows)
+    return rows, width, int(shape[0] != rows)
 
 
 def _as_read(codes: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, int, torch.Tensor, int]:
     """Codes with packed rows that start on 16 bytes and scales with packed rows, and their row strides."""
+    width = codes.shape[1]
     codes, ld = _packed_rows(codes)
-    if codes.data_ptr() % 16 != 0 or ld % 16 != 0 or ld < codes.shape[1]:
-        codes = codes.clone(memory_format=torch.contiguous_format)
-        ld = codes.shape[1]
+    if codes.data_ptr() % 16 != 0 or ld % 16 != 0 or ld < width:
+        codes, ld = codes.clone(memory_format=torch.contiguous_format), width
     scales, scales_ld = _packed_rows(scales)
     return codes, ld, scales, scales_ld
 
