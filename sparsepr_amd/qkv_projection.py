@@ -1,0 +1,66 @@
+"""QKVProjection: what a model's block does in front of the attention, with the weights in 8 bits.
+
+    front = QKVProjection(weight, heads=40, norm_weight=g, axis_dims=(44, 42, 42))   # once: weight [3 * 40 * 128, C]
+    positions = grid_positions(21, 30, 52)                                           # or any [T, 3] / [B, T, 3]
+    q, k, v, x = front(y, positions, residual=x)       # x + y normed to 8 bits, projected, Q and K turned by place
+    out = SparsePRAttention(config)(q, k, v)
+
+The hidden rows are read once between the residual's addition and the 8-bit product; nothing is rounded to 16
+bits in between.  All calls are kernels/rms_norm.py's, kernels/fp8.py's and kernels/axial_rope.py's, on torch's
+current stream; none waits for the GPU, and a captured graph replays what an eager call does."""
+
+from __future__ import annotations
+
+import torch
+
+from .kernels.axial_rope import axial_frequencies, axial_rope
+from .kernels.fp8 import fp8_matmul, fp8_quantize
+from .kernels.rms_norm import rms_norm, rms_norm_fp8
+
+
+class QKVProjection:
+    def __init__(self, weight: torch.Tensor, *, heads: int, kv_heads: int | None = None, axis_dims, theta: float = 10000.0,
+                 pairs: str = "interleaved", norm_weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                 q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, epsilon: float = 1e-6):
+        """weight [(heads + 2 kv_heads) D, C]: the rows of Q, then K, then V, quantised here once (128 x 128 blocks).
+        norm_weight [C] and bias as in rms_norm and fp8_matmul.  q_norm and k_norm norm Q and K before they are
+        turned: [D] every head by itself, [heads * D] all channels together.  axis_dims: the rotated dims of each
+        axis of the positions (axial_frequencies)."""
+        kv_heads = heads if kv_heads is None else kv_heads
+        what = "QKV projection"
+        if heads < 1 or kv_heads < 1 or heads % kv_heads != 0:
+            raise RuntimeError(f"{what}: {heads} query heads on {kv_heads} kv heads")
+        if weight.dim() != 2 or weight.shape[0] % (heads + 2 * kv_heads) != 0 or weight.numel() == 0:
+            raise RuntimeError(f"{what}: weight {tuple(weight.shape)} is not [({heads} + 2 * {kv_heads}) D, C]")
+        self.heads, self.kv_heads = heads, kv_heads
+        self.head_dim = weight.shape[0] // (heads + 2 * kv_heads)
+        for t, h, name in ((q_norm, heads, "q_norm"), (k_norm, kv_heads, "k_norm")):
+            if t is not None and t.shape not in ((self.head_dim,), (h * self.head_dim,)):
+                raise RuntimeError(f"{what}: {name} must be [{self.head_dim}] or [{h * self.head_dim}], got {tuple(t.shape)}")
+        self.width = weight.shape[1]
+        self.weight = fp8_quantize(weight, square=True)
+        self.norm_weight, self.bias, self.q_norm, self.k_norm = norm_weight, bias, q_norm, k_norm
+        self.freqs, self.axis = axial_frequencies(axis_dims, theta=theta, device=weight.device)
+        self.pairs, self.epsilon = pairs, epsilon
+
+    def _heads(self, x: torch.Tensor, heads: int, weight: torch.Tensor | None) -> torch.Tensor:
+        """x [B, T, heads * D] -> [B, heads, T, D], normed where there is a weight."""
+        if weight is not None and weight.shape[0] != self.head_dim:
+            x = rms_norm(x, weight, epsilon=self.epsilon)
+        x = x.unflatten(-1, (heads, self.head_dim))
+        if weight is not None and weight.shape[0] == self.head_dim:
+            x = rms_norm(x, weight, epsilon=self.epsilon)
+        return x.transpose(1, 2)
+
+    def __call__(self, x: torch.Tensor, positions: torch.Tensor, *, residual: torch.Tensor | None = None):
+        """x [B, T, C] -> Q [B, heads, T, D], K and V [B, kv_heads, T, D] in x's type (V a view of the projection),
+        and with a residual the sum x + residual as well."""
+        if x.dim() != 3 or x.shape[2] != self.width:
+            raise RuntimeError(f"QKV projection: x must be [B, T, {self.width}], got {tuple(x.shape)}")
+        codes, scales, *total = rms_norm_fp8(x, self.norm_weight, residual=residual, epsilon=self.epsilon)
+        y = fp8_matmul(codes.flatten(0, 1), scales.flatten(0, 1), *self.weight, bias=self.bias, out_dtype=x.dtype)
+        kv = self.kv_heads * self.head_dim
+        q, k, v = y.view(*x.shape[:2], -1).split((self.heads * self.head_dim, kv, kv), -1)
+        q, k = axial_rope(self._heads(q, self.heads, self.q_norm), self._heads(k, self.kv_heads, self.k_norm), positions,
+                          self.freqs, self.axis, pairs=self.pairs)
+        return q, k, self._heads(v, self.kv_heads, None), *total
