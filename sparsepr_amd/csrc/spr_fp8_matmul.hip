@@ -39,6 +39,9 @@ struct Output {
   void* out;
   const void* bias;
   int32_t bias_dtype;  // -1: none
+  // Outputs that the 256 MB cache cannot hold are written past it: 335 MB 674 instead of 684 us, but 50 MB (5000 x 5000,
+  // K = 320) 42 instead of 26.
+  bool past_caches;
 };
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -101,6 +104,7 @@ __device__ __forceinline__ f32x4 bias4(const Output& o, int32_t n, int32_t N) {
 
 // 64 columns of 16 rows: c[j] holds columns 16 j + 4 g .. + 3 of row r = lane % 16 in lane group g.  In 16 bits the
 // groups first exchange them, so that a lane has 8 columns side by side and each store writes 64 bytes of a row.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 template <int DT>
 __device__ __forceinline__ void put64(const Output& o, const f32x4 (&c)[4], int64_t m, bool in, int32_t n0, int32_t N,
                                       int lane) {
@@ -142,7 +146,9 @@ __device__ __forceinline__ void put64(const Output& o, const f32x4 (&c)[4], int6
       S* p = static_cast<S*>(o.out) + m * N + n;
       const uint32_t v[4] = {w[2 * q][0], w[2 * q][1], w[2 * q + 1][0], w[2 * q + 1][1]};
       if (n + 8 <= N) {
-        __builtin_memcpy(p, v, 16);
+        const u32x4_any all = {v[0], v[1], v[2], v[3]};
+        if (o.past_caches) __builtin_nontemporal_store(all, reinterpret_cast<u32x4_any*>(p));
+        else *reinterpret_cast<u32x4_any*>(p) = all;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -245,25 +251,23 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
   const int32_t off_b = (wave * PB * 8 + (lane >> 3)) * ld_b + piece;
   const int32_t blocks = (K + KB - 1) / KB;
 
-  auto fetch = [&](int32_t kb) {
-    uint8_t* to = lds + kb % NBUF * BUF;
+  const int32_t base = spr::lds_base(lds);
+  auto fetch = [&](int32_t kb, int32_t buf) {  // into buffer `buf` (an offset)
     const int32_t k = kb * KB;
     const bool in_row = k + piece < K;  // K is a multiple of 16: a piece is in or out, and what is out reads as zeros
+    const int32_t va = in_row ? off_a + k : 0x7f000000, vb = in_row ? off_b + k : 0x7f000000;
 #pragma unroll
     for (int i = 0; i < PA; i += 2) {
-      const int32_t v0 = in_row ? off_a + i * 8 * ld_a + k : 0x7ffffff0;
-      const int32_t v1 = in_row ? off_a + (i + 1) * 8 * ld_a + k : 0x7ffffff0;
-      uint8_t* l = to + (wave * PA + i) * 1024;
-      spr::lds_dma16x2(desc_a, l, v0, desc_a, l + 1024, v1);
+      const int32_t l = base + buf + (wave * PA + i) * 1024;
+      spr::lds_dma16x2(desc_a, l, va + i * 8 * ld_a, desc_a, l + 1024, va + (i + 1) * 8 * ld_a);
     }
 #pragma unroll
     for (int i = 0; i < PB; i += 2) {
-      const int32_t v0 = in_row ? off_b + i * 8 * ld_b + k : 0x7ffffff0;
-      const int32_t v1 = in_row ? off_b + (i + 1) * 8 * ld_b + k : 0x7ffffff0;
-      uint8_t* l = to + TM * KB + (wave * PB + i) * 1024;
-      spr::lds_dma16x2(desc_b, l, v0, desc_b, l + 1024, v1);
+      const int32_t l = base + buf + TM * KB + (wave * PB + i) * 1024;
+      spr::lds_dma16x2(desc_b, l, vb + i * 8 * ld_b, desc_b, l + 1024, vb + (i + 1) * 8 * ld_b);
     }
   };
+
   f32x4 acc[MF][NF];
 #pragma unroll
   for (int i = 0; i < MF; ++i)
@@ -275,17 +279,9 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
   const int p0 = (lane & 15) * KB + (((lane >> 4) ^ (lane & 7)) * 16);
   const int p1 = (lane & 15) * KB + ((((lane >> 4) + 4) ^ (lane & 7)) * 16);
 
-#pragma unroll
-  for (int i = 0; i < NBUF - 1; ++i) fetch(i);
-  for (int32_t kb = 0; kb < blocks; ++kb) {
-    spr::wait_vm<(NBUF - 2) * (PA + PB)>();  // the DMA of kb has landed, those of the next NBUF - 2 blocks may be on their way
-    spr::lds_barrier();
-    if (kb % WIN == 0) {
-      fetch_scales<TM, TN, WIN, THREADS>(a, b, m0, n0, kb, blocks, win);
-      spr::lds_barrier();
-    }
-    fetch(kb + NBUF - 1);  // into the buffer that all have read
-    const uint8_t* at = lds + kb % NBUF * BUF;
+  Operand<WIDE> m[MF], n[NF];
+  auto read = [&](int32_t kb, int32_t buf) {
+    const uint8_t* at = lds + buf;
     if (kb % 4 == 0) {
       const uint32_t* s = win + (kb % WIN) / 4 * SROWS + (lane & 15);
 #pragma unroll
@@ -298,7 +294,6 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
 #pragma unroll
       for (int j = 0; j < NF; ++j) sn[j] >>= 8;
     }
-    Operand<WIDE> n[NF];
     const uint8_t* nt = at + TM * KB + wn * (TN / WN) * KB;
 #pragma unroll
     for (int j = 0; j < NF; ++j)
@@ -306,13 +301,35 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
                *reinterpret_cast<const i32x4*>(nt + j * 16 * KB + p1), sn[j]);
     const uint8_t* mt = at + wm * (TM / WM) * KB;
 #pragma unroll
-    for (int i = 0; i < MF; ++i) {
-      Operand<WIDE> m;
-      m.set(*reinterpret_cast<const i32x4*>(mt + i * 16 * KB + p0),
-            *reinterpret_cast<const i32x4*>(mt + i * 16 * KB + p1), sm[i]);
+    for (int i = 0; i < MF; ++i)
+      m[i].set(*reinterpret_cast<const i32x4*>(mt + i * 16 * KB + p0),
+               *reinterpret_cast<const i32x4*>(mt + i * 16 * KB + p1), sm[i]);
+  };
+  auto multiply = [&]() {
 #pragma unroll
-      for (int j = 0; j < NF; ++j) acc[i][j] = product(n[j], m, acc[i][j]);
+    for (int i = 0; i < MF; ++i)
+#pragma unroll
+      for (int j = 0; j < NF; ++j) acc[i][j] = product(n[j], m[i], acc[i][j]);
+  };
+
+#pragma unroll
+  for (int i = 0; i < NBUF - 1; ++i) fetch(i, i * BUF);
+  int32_t now = 0, next = (NBUF - 1) * BUF;  // the buffers of kb and of kb + NBUF - 1
+  for (int32_t kb = 0; kb < blocks; ++kb) {
+    spr::wait_vm<(NBUF - 2) * (PA + PB)>();  // the DMA of kb has landed, those of the next NBUF - 2 blocks may be on their way
+    spr::lds_barrier();
+    if (kb % WIN == 0) {
+      fetch_scales<TM, TN, WIN, THREADS>(a, b, m0, n0, kb, blocks, win);
+      spr::lds_barrier();
     }
+    // the next DMA, into the buffer that all have read: with two buffers it cannot start too early (41 instead of 37 us
+    // on 1024 x 5120 x 5120 behind the reads), with three the reads go first (19.0 instead of 20.6 us on 333 x 5000 x 4112)
+    if (NBUF == 2) fetch(kb + NBUF - 1, next);
+    read(kb, now);
+    if (NBUF > 2) fetch(kb + NBUF - 1, next);
+    multiply();
+    now = now == (NBUF - 1) * BUF ? 0 : now + BUF;
+    next = next == (NBUF - 1) * BUF ? 0 : next + BUF;
   }
   spr::wait_vm<0>();  // of zeros behind the last block
   static_assert(NF == 4, "put64 takes 64 columns of a wave");
@@ -556,35 +573,51 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Matrix a, Matrix b
 }
 
 // Which kernel: by what the whole call takes, in hundredths of a microsecond, from measured times of a block
-// of the summed dim while the chip is full of tiles (`full` of them), half full or less.  K = 5120, us, outputs in
-// 16 bits:            256 x 256   128 x 128   64 x 128   few rows
-//   1 x 15,360                       29.0        20.5       18.5
-//   32 x 5120                        27.0        20.8       20.0
-//   64 x 15,360                      31.4        21.4       54.4
-//   512 x 5120           51.9        32.8        27.9
-//   1024 x 5120          53.5        37.1        46.9
-//   2048 x 5120          56.9        69.8        76.8
-//   4096 x 5120         115         112         140
-//   32,760 x 5120       673         845        1143
-enum Kernel { LARGE, MIDDLE, SMALL, FEW };
+// of the summed dim while the chip is full of tiles (`full` of them), more than half full or less.  In us, outputs in
+// 16 bits, K = 5120 but for the last four:
+//                  256 x 256   128 x 128   64 x 128   64 x 64   few rows
+//   1 x 5120                                  17.5      12.3      10.1
+//   1 x 15,360                                18.4      14.1      18.6
+//   16 x 5120                                 17.5      12.4      14.1
+//   64 x 15,360                     30.7      20.2      15.7      54.4
+//   512 x 5120          51.4        32.2      27.8      30.8
+//   1024 x 5120         52.1        38.2      43.2      48.1
+//   2048 x 5120         53.5        67.7      68.9      92.0
+//   4096 x 5120          116         108       139       180
+//   32,760 x 5120        643         816      1072      1413
+//   333 x 5000 x 4112   45.6        27.4      18.1      22.4
+//   100 x 2560 x 2560   27.4        15.4      10.8       8.0
+//   64 x 500 x 14,000    130        65.5      41.9      28.6      31.4
+//   1000 x 1000 x 1008  16.2         8.9       6.9       5.6
+enum Kernel { LARGE, MIDDLE, SMALL, TINY, FEW };
 struct Cost {
   int32_t tm, tn, full, start, all, most, some;
 };
 Kernel pick_kernel(int64_t M, int64_t N, int32_t K, bool wide) {
-  static const Cost costs[2][3] = {{{256, 256, 256, 600, 168, 165, 139}, {128, 128, 512, 300, 95, 80, 70}, {64, 128, 512, 200, 71, 57, 43}},
-                                   {{256, 256, 256, 600, 335, 320, 306}, {128, 128, 512, 300, 184, 170, 160}, {64, 128, 512, 200, 117, 110, 84}}};
+  static const Cost costs[2][4] = {{{256, 256, 256, 600, 168, 165, 139},
+                                    {128, 128, 512, 300, 95, 80, 70},
+                                    {64, 128, 512, 200, 71, 57, 43},
+                                    {64, 64, 512, 200, 55, 50, 30}},
+                                   {{256, 256, 256, 600, 335, 320, 306},
+                                    {128, 128, 512, 300, 184, 170, 160},
+                                    {64, 128, 512, 200, 117, 110, 84},
+                                    {64, 64, 512, 200, 95, 80, 45}}};
   const int64_t blocks = spr::ceil_div(K, KB);
   Kernel best = LARGE;
   int64_t least = INT64_MAX;
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const Cost& c = costs[wide ? 1 : 0][i];
     const int64_t tiles = spr::ceil_div(M, c.tm) * spr::ceil_div(N, c.tn), rest = tiles % c.full;
     const int64_t cost = spr::ceil_div(tiles, c.full) * c.start +
                          blocks * (tiles / c.full * c.all + (rest == 0 ? 0 : 2 * rest > c.full ? c.most : c.some));
     if (cost < least) least = cost, best = static_cast<Kernel>(i);
   }
-  // few rows: b's bytes once and a's for every 16 of b's rows, 0.15 us a MB
-  if (M <= 64 && 400 + N * K / 1000 * (16 + M) / 16 * 15 / 1000 < least) best = FEW;
+  // few rows: b's bytes once and a's for every 16 of b's rows, 0.15 us a MB, or the blocks that a wave takes in turn
+  if (M <= 64) {
+    const int64_t bytes = N * K / 1000 * (16 + M) / 16 * 15 / 1000;
+    const int64_t turns = spr::ceil_div(blocks, 8) * (M <= 16 ? 80 : M <= 32 ? 120 : 200);
+    if (400 + (bytes > turns ? bytes : turns) < least) best = FEW;
+  }
   return best;
 }
 
@@ -600,8 +633,8 @@ int launch_product(const Matrix& a, const Matrix& b, int32_t K, const Output& o,
     SPR_LAUNCHED("few_rows_kernel");
     return SPR_OK;
   }
-  const int32_t side = kernel == LARGE ? 256 : 128, high = kernel == SMALL ? 64 : side;
-  const int64_t tm = spr::ceil_div(M, high), tn = spr::ceil_div(N, side);
+  const int64_t tm = spr::ceil_div(M, kernel == LARGE ? 256 : kernel == MIDDLE ? 128 : 64);
+  const int64_t tn = spr::ceil_div(N, kernel == LARGE ? 256 : kernel == TINY ? 64 : 128);
   SPR_REQUIRE(tm * tn < (int64_t(1) << 22), "spr_fp8_matmul: too many outputs");
   const uint32_t grid = static_cast<uint32_t>(tm * tn);
   const int32_t rows = static_cast<int32_t>(tm), columns = static_cast<int32_t>(tn);
@@ -609,6 +642,8 @@ int launch_product(const Matrix& a, const Matrix& b, int32_t K, const Output& o,
     product_kernel<DT, 128, 128, 2, 2, 32, 2><<<grid, 256, 0, stream>>>(a, b, K, rows, columns, o);
   } else if (kernel == SMALL) {
     product_kernel<DT, 64, 128, 2, 2, 32, 3><<<grid, 256, 0, stream>>>(a, b, K, rows, columns, o);
+  } else if (kernel == TINY) {
+    product_kernel<DT, 64, 64, 4, 1, 32, 4><<<grid, 256, 0, stream>>>(a, b, K, rows, columns, o);
   } else {
     if constexpr (DT == 2) product_kernel<DT, 256, 256, 2, 4, 64, 2><<<grid, 512, 0, stream>>>(a, b, K, rows, columns, o);
     else turns_product_kernel<DT><<<grid, 512, 0, stream>>>(a, b, K, rows, columns, o);
@@ -639,7 +674,7 @@ extern "C" int spr_fp8_matmul(const uint8_t* a, int64_t a_ld, const uint8_t* a_s
   SPR_REQUIRE(aligned16(a) && aligned16(b), "spr_fp8_matmul: codes must be 16-byte aligned");
   const Matrix am{a, a_ld, a_scales, a_scales_ld, a_square != 0 ? 7 : 0, static_cast<int32_t>(M)};
   const Matrix bm{b, b_ld, b_scales, b_scales_ld, b_square != 0 ? 7 : 0, static_cast<int32_t>(N)};
-  const Output o{out, bias, bias == nullptr ? -1 : bias_dtype};
+  const Output o{out, bias, bias == nullptr ? -1 : bias_dtype, M * N * (out_dtype == 2 ? 4 : 2) > (int64_t(256) << 20)};
   switch (out_dtype) {
     case 0: return launch_product<0>(am, bm, K, o, stream);
     case 1: return launch_product<1>(am, bm, K, o, stream);

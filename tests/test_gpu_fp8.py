@@ -101,7 +101,8 @@ def test_quantisation_reads_strided_rows_and_copies_others(dev):
 # ------------------------------------------------------------------ the product
 
 SIZES = [(1, 1, 16), (1, 16, 128), (1, 500, 1040), (3, 70, 144), (16, 48, 4112), (17, 33, 272), (33, 129, 640), (64, 64, 256),
-         (65, 130, 400), (128, 128, 128), (200, 300, 1168), (257, 129, 96), (333, 1000, 528)]
+         (65, 130, 400), (128, 128, 128), (200, 300, 1168), (257, 129, 96), (333, 1000, 528), (1, 500, 4112), (17, 33, 5136),
+         (60, 32, 20016)]  # the last three: the kernel of few rows, with 16, 32 and 64 of them
 
 
 def _whole(rng, m, k, square):
@@ -115,7 +116,7 @@ def _whole(rng, m, k, square):
 def test_products_of_whole_numbers_are_exact(dev, m, n, k, squares):
     from sparsepr_amd.kernels.fp8 import fp8_matmul
 
-    # |a b| <= 16 at scales up to 4, in steps of 1/4: sums of 4112 of them stay below 2^24 steps
+    # |a b| <= 16 at scales up to 4, in steps of 1/4: sums of 20,016 of them stay below 2^24 steps
     rng = np.random.default_rng(m * 1000 + n)
     a, b = _whole(rng, m, k, squares[0]), _whole(rng, n, k, squares[1])
     want = model.values(*a) @ model.values(*b).T
@@ -129,9 +130,9 @@ def test_products_of_whole_numbers_are_exact(dev, m, n, k, squares):
 
 
 @pytest.mark.parametrize("m,n,k", [(4000, 3500, 256), (3328, 4097, 8320), (49152 + 7, 260, 144), (4000, 3585, 16),
-                                   (1030, 5000, 4240), (300, 700, 4240), (90, 5000, 8208), (30, 16, 20016)])
+                                   (1030, 5000, 4240), (500, 5000, 4240), (300, 700, 4240), (90, 5000, 8208), (30, 16, 20016)])
 def test_products_on_tiles_of_every_size_are_exact(dev, m, n, k):
-    """Past the edges of tiles of 256 x 256, 128 x 128 and 64 x 128, and with more blocks than their windows of
+    """Past the edges of tiles of 256 x 256, 128 x 128, 64 x 128 and 64 x 64, and with more blocks than their windows of
     scales hold; a summed dim shorter than a block on each."""
     from sparsepr_amd.kernels.fp8 import fp8_matmul
 
@@ -148,7 +149,7 @@ def test_products_on_tiles_of_every_size_are_exact(dev, m, n, k):
 
 
 @pytest.mark.parametrize("out", DT)
-@pytest.mark.parametrize("m,n,k", [(1, 200, 2048), (40, 77, 592), (150, 190, 2064), (513, 260, 400)])
+@pytest.mark.parametrize("m,n,k", [(1, 200, 4096), (60, 24, 20000), (40, 77, 592), (150, 190, 2064), (513, 260, 400)])
 def test_products_of_rows_as_they_come(dev, out, m, n, k):
     from sparsepr_amd.kernels.fp8 import fp8_matmul, fp8_quantize
 
