@@ -64,8 +64,9 @@ __device__ __forceinline__ void angle_of(const void* positions, int32_t code, in
   s = sign * sn;
 }
 
-// Units of a row: R / 2P of P pairs, then (D - R) / 2P of 2P dims to copy, a lane each.  A workgroup has as many (token,
-// slot) pairs as its lanes hold rows; the slots of a token take its heads in turn, AHEAD of them on their way at once.
+// Units of a row: R / 2P of P pairs, then (D - R) / 2P of 2P dims to copy, a lane each.  A workgroup has as many
+// tokens as its lanes hold rows, one behind the other, so that it writes one run of each head; its slot takes every
+// `slots`-th head, AHEAD of them on their way at once.
 template <int DT, bool HALVES, int P>
 __global__ __launch_bounds__(THREADS) void rope_kernel(Side q, Side k, const void* __restrict__ positions,
                                                        int32_t position_code, int64_t position_b, int32_t axes,
@@ -77,10 +78,10 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(Side q, Side k, const voi
   const int units = dim / (2 * P), per = THREADS / units;
   const int mine = threadIdx.x / units, unit = threadIdx.x - mine * units;
   if (mine >= per) return;
-  const int64_t job = static_cast<int64_t>(blockIdx.x) * per + mine;
-  const int64_t row = job / slots;
+  const uint32_t group = blockIdx.x / static_cast<uint32_t>(slots);
+  const int64_t row = static_cast<int64_t>(group) * per + mine;
   if (row >= rows) return;
-  const int slot = static_cast<int>(job - row * slots);
+  const int slot = static_cast<int>(blockIdx.x - group * static_cast<uint32_t>(slots));
   const int64_t b = row / tokens, t = row - b * tokens;
   const bool turned = unit * 2 * P < rotated;
   float c[P], s[P];
@@ -139,12 +140,13 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(Side q, Side k, const voi
   }
 }
 
-// Slots of a token: a million lanes, two rounds of the chip's waves, and no more slots than heads; an angle serves the
-// heads that share its slot.  (32,760 tokens of 80 heads: 267 us, 276 with half as many; 8000 of 40: 31 us, 38 with
-// twice as many.)
+// Slots of a token: about 12 waves a SIMD of lanes, and as even a share of the heads as that allows; an angle serves the
+// heads that share its slot.  (Two slots of 40 heads on 32,760 tokens: 266 us, 274 with one; eight of 16 on 3 x 2311
+// tokens of 80 fp32 dims: 32 us, 35 with sixteen and 40 with one.)
 int32_t rope_slots(int64_t rows, int32_t units, int32_t heads) {
-  const int64_t wanted = spr::ceil_div(int64_t(1) << 20, rows * units);
-  return static_cast<int32_t>(wanted < heads ? wanted : heads);
+  const int64_t wanted = spr::ceil_div(int64_t(3) << 18, rows * units);
+  if (wanted >= heads) return heads;
+  return static_cast<int32_t>(spr::ceil_div(heads, spr::ceil_div(heads, wanted)));
 }
 
 template <int DT, bool HALVES, int P>
@@ -153,7 +155,7 @@ int launch_rope(const Side& q, const Side& k, const void* positions, int32_t cod
                 float sign, hipStream_t stream) {
   const int32_t units = dim / (2 * P), per = THREADS / units;
   const int32_t slots = rope_slots(rows, units, q.heads > k.heads ? q.heads : k.heads);
-  const int64_t blocks = spr::ceil_div(rows * slots, per);
+  const int64_t blocks = spr::ceil_div(rows, per) * slots;
   SPR_REQUIRE(blocks < (int64_t(1) << 24), "spr_axial_rope: too many rows");  // 2^32 threads of a launch
   rope_kernel<DT, HALVES, P><<<static_cast<uint32_t>(blocks), THREADS, 0, stream>>>(
       q, k, positions, code, position_b, axes, freqs, axis, rows, tokens, dim, rotated, slots, sign);
