@@ -140,12 +140,14 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(Side q, Side k, const voi
   }
 }
 
-// Slots of a token: about 12 waves a SIMD of lanes, and as even a share of the heads as that allows; an angle serves the
-// heads that share its slot.  (Two slots of 40 heads on 32,760 tokens: 266 us, 274 with one; eight of 16 on 3 x 2311
-// tokens of 80 fp32 dims: 32 us, 35 with sixteen and 40 with one.)
+// Slots of a token: a million lanes, as even a share of the heads as that allows, and two heads a slot at least where
+// that still leaves half a million lanes, since an angle serves the heads that share its slot.  (32,760 tokens of 40
+// heads: 264 us with three slots, 274 with two and one; 3 x 2311 tokens of 16 heads of 80 fp32 dims: 32 us with eight
+// slots, 35 with sixteen, 40 with one.)
 int32_t rope_slots(int64_t rows, int32_t units, int32_t heads) {
-  const int64_t wanted = spr::ceil_div(int64_t(3) << 18, rows * units);
-  if (wanted >= heads) return heads;
+  const int64_t lanes = rows * units, wanted = spr::ceil_div(int64_t(1) << 20, lanes);
+  const int64_t most = lanes * heads >= int64_t(1) << 20 ? spr::ceil_div(heads, 2) : heads;
+  if (wanted >= most) return static_cast<int32_t>(most);
   return static_cast<int32_t>(spr::ceil_div(heads, spr::ceil_div(heads, wanted)));
 }
 
