@@ -25,6 +25,8 @@ typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
 
 
 constexpr int KB = 128;  // of the summed dim, one block
+// An offset that no tile of a matrix reaches (256 rows of 2^22 bytes), nor with a tile's rows on it overflows.
+constexpr int32_t OUTSIDE = 1 << 30;
 
 struct Matrix {
   const uint8_t* codes;
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
   auto fetch = [&](int32_t kb, int32_t buf) {  // into buffer `buf` (an offset)
     const int32_t k = kb * KB;
     const bool in_row = k + piece < K;  // K is a multiple of 16: a piece is in or out, and what is out reads as zeros
-    const int32_t va = in_row ? off_a + k : 0x7f000000, vb = in_row ? off_b + k : 0x7f000000;
+    const int32_t va = in_row ? off_a + k : OUTSIDE, vb = in_row ? off_b + k : OUTSIDE;
 #pragma unroll
     for (int i = 0; i < PA; i += 2) {
       const int32_t l = base + buf + (wave * PA + i) * 1024;
@@ -381,13 +383,13 @@ __global__ __launch_bounds__(512) void turns_product_kernel(Matrix a, Matrix b, 
   const int32_t base = spr::lds_base(lds);
   auto fetch_a = [&](int32_t kb, int half) {
     const int32_t k = kb * KB, to = base + (kb & 1) * BUF + (arow + 64 * half) * KB;
-    const int32_t v = k + piece < K ? off_a + k : 0x7f000000;  // K is a multiple of 16: a piece is in or out, and
+    const int32_t v = k + piece < K ? off_a + k : OUTSIDE;  // K is a multiple of 16: a piece is in or out, and
     const int32_t r = 64 * half * ld_a;                        // what is out reads as zeros
     spr::lds_dma16x2(desc_a, to, v + r, desc_a, to + 1024, v + r + 8 * ld_a);
   };
   auto fetch_b = [&](int32_t kb) {
     const int32_t k = kb * KB, to = base + (kb & 1) * BUF + (T + brow) * KB;
-    const int32_t v = k + piece < K ? off_b + k : 0x7f000000;
+    const int32_t v = k + piece < K ? off_b + k : OUTSIDE;
 #pragma unroll
     for (int i = 0; i < 4; i += 2)
       spr::lds_dma16x2(desc_b, to + i * 1024, v + i * 8 * ld_b, desc_b, to + (i + 1) * 1024, v + (i + 1) * 8 * ld_b);
@@ -531,7 +533,7 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Matrix a, Matrix b
   for (int i = 0; i < MF; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   // rows past the end and pieces past the summed dim read as zeros (K is a multiple of 16)
   auto load = [&](auto desc, int32_t off, int32_t k) {
-    return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(desc, k < K - g * 16 ? off + k : 0x7ffffff0, 0, 0));
+    return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(desc, k < K - g * 16 ? off + k : OUTSIDE, 0, 0));
   };
   for (int32_t k0 = wave; k0 < blocks; k0 += WAVES * AHEAD) {
     i32x4 nv[AHEAD][2], mv[AHEAD][MF][2];
@@ -626,6 +628,7 @@ int launch_product(const Matrix& a, const Matrix& b, int32_t K, const Output& o,
   const int32_t M = a.rows, N = b.rows;
   const Kernel kernel = pick_kernel(M, N, K, DT == 2);
   if (kernel == FEW) {
+    SPR_REQUIRE(N < (1 << 27), "spr_fp8_matmul: too many outputs");  // 2^32 threads of a launch
     const uint32_t grid = static_cast<uint32_t>(spr::ceil_div(N, 16));
     if (M <= 16) few_rows_kernel<DT, 1, 8><<<grid, 512, 0, stream>>>(a, b, K, o);
     else if (M <= 32) few_rows_kernel<DT, 2, 8><<<grid, 512, 0, stream>>>(a, b, K, o);

@@ -125,9 +125,9 @@ def fp8_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
             raise RuntimeError(f"{what}: bias must be [{n}] in bfloat16, float16 or float32, got {bias.dtype} "
                                f"{tuple(bias.shape)}")
         bias = bias.contiguous()
-    if k == 0:
-        raise RuntimeError(f"{what}: nothing to sum over (a is [{m}, 0])")
     out = a.new_empty((m, n), dtype=out_dtype)
+    if k == 0:  # (no rows that a weight's gradient would be summed over)
+        return out.zero_() if bias is None else out.copy_(bias)
     if out.numel() > 0:
         a, a_ld, a_scales, a_scales_ld = _as_read(a, a_scales)
         b, b_ld, b_scales, b_scales_ld = _as_read(b, b_scales)

@@ -132,7 +132,8 @@ def test_values_refuse_bad_arguments_before_any_launch(kw, text):
     (dict(od=3), "output dtype 3"), (dict(bd=4), "bias dtype 4"), (dict(K=40), "sizes"), (dict(K=1 << 23), "sizes"),
     (dict(M=-1), "sizes"), (dict(M=1 << 31), "sizes"), (dict(K=0), "nothing to sum"), (dict(a=None), "null pointer"),
     (dict(a_ld=48), "row strides 48"), (dict(b_ld=72), "row strides 64, 72"), (dict(a=24), "16-byte aligned"),
-    (dict(s_ld=-1), "negative scale stride"), (dict(M=1 << 30, N=1 << 16), "too many outputs")])
+    (dict(s_ld=-1), "negative scale stride"), (dict(M=1 << 30, N=1 << 16), "too many outputs"),
+    (dict(M=1, N=1 << 29, K=16, a_ld=16, b_ld=16), "too many outputs"), (dict(M=1 << 22, N=1 << 22), "too many outputs")])
 def test_product_refuses_bad_arguments_before_any_launch(kw, text):
     lib = _lib()
     a = dict(a=16, a_ld=64, b_ld=64, s_ld=1, M=4, N=4, K=64, bd=0, od=0)
