@@ -23,7 +23,6 @@ using spr::f32x4;
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
 
-
 constexpr int KB = 128;  // of the summed dim, one block
 // An offset that no tile of a matrix reaches (256 rows of 2^22 bytes), nor with a tile's rows on it overflows.
 constexpr int32_t OUTSIDE = 1 << 30;
@@ -359,6 +358,9 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
 // products begin.  A part of LDS is filled again as soon as both groups have read it: b's rows (kb + 2's) in the
 // third turn, a's first half in the fourth, its second half (kb + 1's) in the first.  Each DMA has four or five
 // turns to land.  (Whole blocks at once had three: 834 us instead of 703 on 32,760 x 5120 x 5120.)
+// That size takes 643 to 688 us, 2.5 to 2.7 PFLOP/s: what bounds it is the matrix units, busy for 63 % of the cycles at
+// the 1.9 GHz that real codes leave them (2.34 with constant ones).  Alone, the products take 400 us, with the
+// LDS reads 511, with the DMA 641.  One wave a SIMD with 128 x 128 outputs, half the LDS reads, takes 761.
 template <int DT>
 __global__ __launch_bounds__(512) void turns_product_kernel(Matrix a, Matrix b, int32_t K, int32_t tiles_m,
                                                            int32_t tiles_n, Output o) {
@@ -615,7 +617,8 @@ Kernel pick_kernel(int64_t M, int64_t N, int32_t K, bool wide) {
     if (cost < least) least = cost, best = static_cast<Kernel>(i);
   }
   // few rows: b's bytes once and a's for every 16 of b's rows, 0.15 us a MB, or the blocks that a wave takes in turn
-  if (M <= 64) {
+  // (and 512 threads for 16 of b's rows, fewer than 2^32 in a launch)
+  if (M <= 64 && N <= (int64_t(1) << 26)) {
     const int64_t bytes = N * K / 1000 * (16 + M) / 16 * 15 / 1000;
     const int64_t turns = spr::ceil_div(blocks, 8) * (M <= 16 ? 80 : M <= 32 ? 120 : 200);
     if (400 + (bytes > turns ? bytes : turns) < least) best = FEW;

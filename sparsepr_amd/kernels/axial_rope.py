@@ -83,6 +83,8 @@ def axial_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     rotated = 2 * freqs.shape[0]
     if d % 8 != 0 or not 8 <= d <= 1024 or rotated % 8 != 0 or rotated > d:
         raise RuntimeError(f"{what}: {rotated} rotated dims of {d} (both multiples of 8, D at most 1024)")
+    if max(h, hk) >= 1 << 20:
+        raise RuntimeError(f"{what}: {h} and {hk} heads")
     if not 1 <= axes <= 16:
         raise RuntimeError(f"{what}: {axes} axes, 1 to 16 are taken")
     q_out = q.new_empty((b, h, t, d))

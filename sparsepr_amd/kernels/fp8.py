@@ -22,6 +22,8 @@ import torch
 from .. import _lib
 
 BLOCK = 128
+MAX_SIZE = 1 << 30  # of a dim: the entry points count columns in 32 bits
+MAX_SUM = 1 << 22  # terms of a product
 CODES = torch.float8_e4m3fn
 
 
@@ -48,6 +50,8 @@ def _check_matrix(codes: torch.Tensor, scales: torch.Tensor, what: str, name: st
         raise RuntimeError(f"{what}: {name} must be float8_e4m3fn [rows, width], got {codes.dtype} {tuple(codes.shape)}")
     rows, width = codes.shape
     blocks = -(-width // BLOCK)
+    if max(rows, width) > MAX_SIZE:
+        raise RuntimeError(f"{what}: {name} is {tuple(codes.shape)}, {MAX_SIZE} rows or columns at most")
     if width % 16 != 0:
         raise RuntimeError(f"{what}: the width of {name} ({width}) must be a multiple of 16 (zeros behind the row)")
     shape = scales.shape
@@ -79,6 +83,8 @@ def fp8_quantize(x: torch.Tensor, *, square: bool = False, transpose: bool = Fal
     if x.dim() != 2 or x.dtype not in _lib.DTYPE_CODE:
         raise RuntimeError(f"{what}: x must be [rows, width] in bfloat16, float16 or float32, got {x.dtype} "
                            f"{tuple(x.shape)}")
+    if max(x.shape) > MAX_SIZE:
+        raise RuntimeError(f"{what}: x is {tuple(x.shape)}, {MAX_SIZE} rows or columns at most")
     rows, width = x.shape[::-1] if transpose else x.shape
     codes = x.new_empty((rows, -(-width // 16) * 16), dtype=CODES)
     scales = x.new_empty((-(-rows // BLOCK) if square else rows, -(-width // BLOCK)), dtype=torch.uint8)
@@ -118,6 +124,8 @@ def fp8_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     n, kb, b_square = _check_matrix(b, b_scales, what, "b")
     if k != kb:
         raise RuntimeError(f"{what}: a is [{m}, {k}], b [{n}, {kb}]")
+    if k > MAX_SUM:
+        raise RuntimeError(f"{what}: sums of {k} terms, {MAX_SUM} are taken")
     if out_dtype not in _lib.DTYPE_CODE:
         raise RuntimeError(f"{what}: out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
     if bias is not None:

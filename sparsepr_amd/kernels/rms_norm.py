@@ -3,7 +3,8 @@ HIP kernels of csrc/spr_rms_norm.hip.
 
     s = x + residual (rounded once, to the residual's type);  y = s / sqrt(mean(s^2) + epsilon) * weight
 
-over the last dim of x [..., C], C up to 16384, sums in fp32.  The norm reads s as it is stored.  x and the
+over the last dim of x [..., C], C up to 16384, sums in fp32: a row whose sum of squares leaves its range gives
+what fp32 gives (zeros above 1.8e19, and with epsilon 0 infinities below 1e-23).  The norm reads s as it is stored.  x and the
 residual are bf16, fp16 or fp32, the residual of x's type or fp32; the weight is [C] of x's type or fp32,
 or None.  Rows may have any strides as long as they are packed and their dims merge into two (a Q or K
 slice of a projection, seen by heads); others are copied.  None of the functions is recorded by autograd:
@@ -57,6 +58,8 @@ def _check(x: torch.Tensor, weight: torch.Tensor | None, epsilon: float, what: s
     width = x.shape[-1]
     if not 1 <= width <= MAX_WIDTH:
         raise RuntimeError(f"{what}: width {width} not in 1 .. {MAX_WIDTH}")
+    if x.numel() // width >= 1 << 31:  # the entry points count rows in 32 bits
+        raise RuntimeError(f"{what}: too many rows in {tuple(x.shape)}")
     if weight is not None and (weight.shape != (width,) or weight.dtype not in (x.dtype, torch.float32)):
         raise RuntimeError(f"{what}: weight must be [{width}] in {x.dtype} or float32, got {weight.dtype} "
                            f"{tuple(weight.shape)}")

@@ -182,3 +182,14 @@ def test_replays_and_another_stream(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_more_heads_than_an_entry_point_counts(dev):
+    from sparsepr_amd.kernels.axial_rope import axial_frequencies, axial_rope
+
+    freqs, axis = axial_frequencies((8,))
+    one, place = torch.zeros(1, 1, 1, 8, device=dev), torch.zeros(1, 1, device=dev)
+    many = one.expand(1, 2**32 + 1, 1, 8)
+    for q, k in ((many, None), (one, many)):
+        with pytest.raises(RuntimeError, match="heads"):
+            axial_rope(q, k, place, freqs, axis)

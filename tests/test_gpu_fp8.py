@@ -312,3 +312,52 @@ def test_another_stream_and_replays(dev):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(y, want)
+
+
+def test_sizes_past_what_an_entry_point_counts(dev):
+    """Views of one value: a column count that 32 bits would cut down to a small one is refused before anything is
+    allocated."""
+    from sparsepr_amd.kernels.fp8 import fp8_dequantize, fp8_matmul, fp8_quantize
+
+    n = 2**32 + 16
+    x = torch.zeros(1, 1, device=dev)
+    for shape in ((1, n), (n, 1)):
+        for how in (dict(), dict(square=True), dict(transpose=True)):
+            with pytest.raises(RuntimeError, match="rows or columns"):
+                fp8_quantize(x.expand(shape), **how)
+    codes = torch.zeros(1, 1, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+    scale = torch.zeros(1, 1, dtype=torch.uint8, device=dev)
+    wide, scales = codes.expand(1, n), scale.expand(1, -(-n // 128))
+    with pytest.raises(RuntimeError, match="rows or columns"):
+        fp8_dequantize(wide, scales)
+    with pytest.raises(RuntimeError, match="rows or columns"):
+        fp8_matmul(wide, scales, wide, scales)
+    k = 2**22 + 16
+    wide, scales = codes.expand(1, k), scale.expand(1, -(-k // 128))
+    with pytest.raises(RuntimeError, match=f"sums of {k} terms"):
+        fp8_matmul(wide, scales, wide, scales)
+
+
+def test_more_rows_than_a_launch_of_tiles_has(dev):
+    from sparsepr_amd.kernels.fp8 import fp8_quantize
+
+    rows = 65535 * 128 + 100
+    x = (torch.arange(rows, device=dev)[:, None] % 1021 - 500 + torch.arange(8, device=dev)).to(torch.bfloat16)
+    codes, scales = (t.view(torch.uint8) for t in fp8_quantize(x))
+    for part in (slice(0, 1000), slice(rows - 1000, rows)):
+        c, s = (t.view(torch.uint8) for t in fp8_quantize(x[part].clone()))
+        assert torch.equal(codes[part], c) and torch.equal(scales[part], s)
+    with pytest.raises(RuntimeError, match="rows of 8"):
+        fp8_quantize(x, square=True)
+
+
+def test_one_row_on_more_columns_than_a_launch_of_few_rows_has(dev):
+    from sparsepr_amd.kernels.fp8 import fp8_matmul
+
+    n = 2**27 + 5
+    one = torch.full((1, 16), 0x38, dtype=torch.uint8, device=dev)  # 1.0
+    scale = torch.full((1, 1), 127, dtype=torch.uint8, device=dev)
+    b = torch.zeros(n, 16, dtype=torch.uint8, device=dev)
+    b[-3:] = 0x38
+    y = fp8_matmul(one.view(torch.float8_e4m3fn), scale, b.view(torch.float8_e4m3fn), scale.expand(n, 1))
+    assert (y[0, -3:] == 16).all() and not y[0, :-3].any()

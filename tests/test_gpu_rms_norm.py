@@ -230,3 +230,13 @@ def test_replays_and_another_stream(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_more_rows_than_an_entry_point_counts(dev):
+    """Views of one row: 2^32 + 8 rows, which 32 bits would cut down to 8, are refused before anything is allocated."""
+    from sparsepr_amd.kernels.rms_norm import rms_norm, rms_norm_backward, rms_norm_fp8
+
+    x = torch.zeros(1, 16, device=dev).expand(2**32 + 8, 16)
+    for call in (rms_norm, rms_norm_fp8, lambda t: rms_norm_backward(t, t)):
+        with pytest.raises(RuntimeError, match="too many rows"):
+            call(x)
