@@ -7,7 +7,7 @@
 //
 // The turn is 64 bits up to the part below one: at place 118,800 an angle in fp32 is off by 0.004.  Its
 // sine and cosine are fp32 (sincospif), the rotation fp32 with one rounding at the end.
-// Bound by memory (Q and K read and written once): Q and K of 32,760 x 40 x 128 in bf16 take 267 us, 5.0 TB/s, what a
+// Bound by memory (Q and K read and written once): Q and K of 32,760 x 40 x 128 in bf16 take 264 us, 5.1 TB/s, what a
 // copy takes.  A lane holds 4 pairs of one token: it finds their angles once and turns the same pairs of several heads.
 #include "spr_elem.h"
 
