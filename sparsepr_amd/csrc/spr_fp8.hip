@@ -185,7 +185,7 @@ extern "C" int spr_fp8_quantize(const void* x, int64_t ld, int64_t rows, int32_t
                                 int32_t transpose, uint8_t* codes, uint8_t* scales, hipStream_t stream) {
   SPR_REQUIRE(dtype >= 0 && dtype <= 2, "spr_fp8_quantize: dtype %d not in {0, 1, 2}", dtype);
   // (a launch of tiles has at most 65,535 of them one below the other)
-  SPR_REQUIRE(rows >= 0 && rows <= (square != 0 || transpose != 0 ? 65535 * int64_t(FP8_GROUP) : int64_t(1) << 30) &&
+  SPR_REQUIRE(rows >= 0 && rows < (int64_t(1) << 24) && (rows <= 65535 * int64_t(FP8_GROUP) || !(square || transpose)) &&
                   width >= 0 && width <= (1 << 30),
               "spr_fp8_quantize: %lld rows of %d", static_cast<long long>(rows), width);
   SPR_REQUIRE(rows * spr::fp8_groups(width) < (int64_t(1) << 28) - 64, "spr_fp8_quantize: too many groups");

@@ -76,7 +76,8 @@ def fp8_quantize(x: torch.Tensor, *, square: bool = False, transpose: bool = Fal
     """x [R, C] in bf16, fp16 or fp32 -> (codes, scales), see the module's text.
 
     `square`: one scale for 128 x 128 values, else for 128 values of a row.  `transpose`: the 8-bit matrix
-    of x^T, codes [C, R rounded up to 16], its groups along x's columns."""
+    of x^T, codes [C, R rounded up to 16], its groups along x's columns.  R is below 2^24, with either at most
+    65535 * 128."""
     what = "8-bit quantisation"
     dev = _lib.require_gpu(x, what=what)
     no_gradient(what, x)
