@@ -225,19 +225,27 @@ __device__ __forceinline__ void fetch_scales(const Matrix& a, const Matrix& b, i
 // one of NBUF buffers in LDS while the products of an earlier one run; one barrier a block.  A row's 16-byte
 // pieces lie at piece ^ (row % 8): eight rows' reads of one piece then meet every bank.  The scale bytes
 // of the tile's rows lie in LDS for WIN blocks at a time, a dword for four blocks of a row.
-template <int DT, int TM, int TN, int WM, int WN, int WIN, int NBUF>
-__global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix b, int32_t K, int32_t tiles_m,
+//
+// KG groups of such waves share one tile's blocks: a turn takes KG of them, each group one from buffers of its own,
+// and the first adds the other's sums at the end.  For few tiles, where a block is a chain of its DMA, reads
+// and products that one group alone leaves gaps in: 64 x 500 x 14,000 takes 25.7 us with two groups and 31.3 with one, in
+// fp32 42.9 and 54.9.  Where tiles are many it loses (512 x 5120 x 5120: 38 and 34), since the groups wait for one another;
+// four groups take 23.0 us on the first, but 21.4 instead of two's 19.0 on 300 x 1536 x 8960.
+template <int DT, int TM, int TN, int WM, int WN, int WIN, int NBUF, int KG>
+__global__ __launch_bounds__(64 * WM * WN * KG) void product_kernel(Matrix a, Matrix b, int32_t K, int32_t tiles_m,
                                                               int32_t tiles_n, Output o) {
   constexpr bool WIDE = DT == 2;
-  constexpr int NW = WM * WN, THREADS = 64 * NW;
+  constexpr int NW = WM * WN, THREADS = 64 * NW * KG;
   constexpr int MF = TM / WM / 16, NF = TN / WN / 16;
   constexpr int PA = TM / 8 / NW, PB = TN / 8 / NW;  // DMA instructions of a wave, 8 rows each
   static_assert(PA % 2 == 0 && PB % 2 == 0, "the DMA goes two by two");
   constexpr int BUF = (TM + TN) * KB;
   constexpr int SROWS = TM + TN;
-  __shared__ alignas(1024) uint8_t lds[NBUF * BUF + SROWS * WIN];
-  uint32_t* win = reinterpret_cast<uint32_t*>(lds + NBUF * BUF);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  static_assert(KG == 1 || KG == 2, "a dword of scales is for four or two turns");
+  __shared__ alignas(1024) uint8_t lds[KG * NBUF * BUF + SROWS * WIN];
+  uint32_t* win = reinterpret_cast<uint32_t*>(lds + KG * NBUF * BUF);
+  const int lane = threadIdx.x & 63, every = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = every / NW, wave = every % NW;
   const int wm = wave / WN, wn = wave % WN;
 
   int32_t m0, n0;
@@ -253,8 +261,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
   const int32_t blocks = (K + KB - 1) / KB;
 
   const int32_t base = spr::lds_base(lds);
-  auto fetch = [&](int32_t kb, int32_t buf) {  // into buffer `buf` (an offset)
-    const int32_t k = kb * KB;
+  auto fetch = [&](int32_t turn, int32_t buf) {  // into buffer `buf` (an offset)
+    const int32_t k = (turn * KG + kg) * KB;
     const bool in_row = k + piece < K;  // K is a multiple of 16: a piece is in or out, and what is out reads as zeros
     const int32_t va = in_row ? off_a + k : OUTSIDE, vb = in_row ? off_b + k : OUTSIDE;
 #pragma unroll
@@ -281,19 +289,19 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
   const int p1 = (lane & 15) * KB + ((((lane >> 4) + 4) ^ (lane & 7)) * 16);
 
   Operand<WIDE> m[MF], n[NF];
-  auto read = [&](int32_t kb, int32_t buf) {
+  auto read = [&](int32_t turn, int32_t buf) {
     const uint8_t* at = lds + buf;
-    if (kb % 4 == 0) {
-      const uint32_t* s = win + (kb % WIN) / 4 * SROWS + (lane & 15);
+    if (turn * KG % 4 == 0) {
+      const uint32_t* s = win + turn * KG % WIN / 4 * SROWS + (lane & 15);
 #pragma unroll
-      for (int i = 0; i < MF; ++i) sm[i] = s[wm * (TM / WM) + i * 16];
+      for (int i = 0; i < MF; ++i) sm[i] = s[wm * (TM / WM) + i * 16] >> (8 * kg);
 #pragma unroll
-      for (int j = 0; j < NF; ++j) sn[j] = s[TM + wn * (TN / WN) + j * 16];
+      for (int j = 0; j < NF; ++j) sn[j] = s[TM + wn * (TN / WN) + j * 16] >> (8 * kg);
     } else {
 #pragma unroll
-      for (int i = 0; i < MF; ++i) sm[i] >>= 8;
+      for (int i = 0; i < MF; ++i) sm[i] >>= 8 * KG;
 #pragma unroll
-      for (int j = 0; j < NF; ++j) sn[j] >>= 8;
+      for (int j = 0; j < NF; ++j) sn[j] >>= 8 * KG;
     }
     const uint8_t* nt = at + TM * KB + wn * (TN / WN) * KB;
 #pragma unroll
@@ -313,26 +321,46 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Matrix a, Matrix 
       for (int j = 0; j < NF; ++j) acc[i][j] = product(n[j], m[i], acc[i][j]);
   };
 
+  const int32_t mine = kg * NBUF * BUF, turns = (blocks + KG - 1) / KG;
 #pragma unroll
-  for (int i = 0; i < NBUF - 1; ++i) fetch(i, i * BUF);
-  int32_t now = 0, next = (NBUF - 1) * BUF;  // the buffers of kb and of kb + NBUF - 1
-  for (int32_t kb = 0; kb < blocks; ++kb) {
-    spr::wait_vm<(NBUF - 2) * (PA + PB)>();  // the DMA of kb has landed, those of the next NBUF - 2 blocks may be on their way
+  for (int i = 0; i < NBUF - 1; ++i) fetch(i, mine + i * BUF);
+  int32_t now = 0, next = (NBUF - 1) * BUF;  // the buffers of this turn and of the one NBUF - 1 later
+  for (int32_t turn = 0; turn < turns; ++turn) {
+    spr::wait_vm<(NBUF - 2) * (PA + PB)>();  // this turn's DMA has landed, those of the next NBUF - 2 may be on their way
     spr::lds_barrier();
-    if (kb % WIN == 0) {
-      fetch_scales<TM, TN, WIN, THREADS>(a, b, m0, n0, kb, blocks, win);
+    if (turn * KG % WIN == 0) {
+      fetch_scales<TM, TN, WIN, THREADS>(a, b, m0, n0, turn * KG, blocks, win);
       spr::lds_barrier();
     }
     // the next DMA, into the buffer that all have read: with two buffers it cannot start too early (41 instead of 37 us
     // on 1024 x 5120 x 5120 behind the reads), with three the reads go first (19.0 instead of 20.6 us on 333 x 5000 x 4112)
-    if (NBUF == 2) fetch(kb + NBUF - 1, next);
-    read(kb, now);
-    if (NBUF > 2) fetch(kb + NBUF - 1, next);
+    if (NBUF == 2) fetch(turn + NBUF - 1, mine + next);
+    read(turn, mine + now);
+    if (NBUF > 2) fetch(turn + NBUF - 1, mine + next);
     multiply();
     now = now == (NBUF - 1) * BUF ? 0 : now + BUF;
     next = next == (NBUF - 1) * BUF ? 0 : next + BUF;
   }
   spr::wait_vm<0>();  // of zeros behind the last block
+  if constexpr (KG > 1) {  // the groups' sums, in their order
+    static_assert((KG - 1) * MF * NF * NW * 1024 <= KG * NBUF * BUF, "the sums fit where the blocks were");
+    spr::lds_barrier();
+    f32x4* sums = reinterpret_cast<f32x4*>(lds) + wave * 64 + lane;
+    if (kg > 0) {
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) sums[(((kg - 1) * MF + i) * NF + j) * NW * 64] = acc[i][j];
+    }
+    spr::lds_barrier();
+    if (kg > 0) return;
+#pragma unroll
+    for (int q = 0; q < KG - 1; ++q)
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[i][j] += sums[((q * MF + i) * NF + j) * NW * 64];
+  }
   static_assert(NF == 4, "put64 takes 64 columns of a wave");
   const int32_t nw = n0 + wn * 64;
   f32x4 bias[NF];
@@ -578,38 +606,42 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Matrix a, Matrix b
 
 // Which kernel: by what the whole call takes, in hundredths of a microsecond, from measured times of a block
 // of the summed dim while the chip is full of tiles (`full` of them), more than half full or less.  In us, outputs in
-// 16 bits, K = 5120 but for the last four:
-//                  256 x 256   128 x 128   64 x 128   64 x 64   few rows
-//   1 x 5120                                  17.5      12.3      10.1
-//   1 x 15,360                                18.4      14.1      18.6
-//   16 x 5120                                 17.5      12.4      14.1
-//   64 x 15,360                     30.7      20.2      15.7      54.4
-//   512 x 5120          51.4        32.2      27.8      30.8
-//   1024 x 5120         52.1        38.2      43.2      48.1
-//   2048 x 5120         53.5        67.7      68.9      92.0
-//   4096 x 5120          116         108       139       180
-//   32,760 x 5120        643         816      1072      1413
-//   333 x 5000 x 4112   45.6        27.4      18.1      22.4
-//   100 x 2560 x 2560   27.4        15.4      10.8       8.0
-//   64 x 500 x 14,000    130        65.5      41.9      28.6      31.4
-//   1000 x 1000 x 1008  16.2         8.9       6.9       5.6
-enum Kernel { LARGE, MIDDLE, SMALL, TINY, FEW };
+// 16 bits, K = 5120 where none is given:
+//                     256 x 256  128 x 128  64 x 128  64 x 64  two groups  few rows
+//   1 x 5120                          26.7      17.9     13.2        11.5      10.1
+//   1 x 15,360                        28.4      19.0     15.1        14.8      18.2
+//   16 x 5120                         26.7      18.1     13.3        11.7      14.2
+//   64 x 15,360                       30.8      20.4     16.0        15.8      55.0
+//   512 x 5120             51.4       33.0      29.1     33.9        38.0
+//   1024 x 5120            52.1       41.9      47.3     54.6        63.8
+//   2048 x 5120            53.5       67.7      68.9     92.0
+//   4096 x 5120             116        108       139      180
+//   32,760 x 5120           643        816      1072     1413
+//   333 x 5000 x 4112      45.6       28.4      18.9     24.1        24.4
+//   100 x 2560 x 2560      27.4       15.8      11.1      8.5         7.8
+//   77 x 4096 x 4096                  21.7      15.1     11.2         9.6
+//   300 x 1536 x 8960                 45.6      29.6     22.7        19.0
+//   64 x 500 x 14,000       130       67.5      42.8     31.3        25.7      31.4
+//   1000 x 1000 x 1008     16.2        9.3       7.3      6.1         6.2
+enum Kernel { LARGE, MIDDLE, SMALL, TINY, TINY2, FEW };
 struct Cost {
   int32_t tm, tn, full, start, all, most, some;
 };
 Kernel pick_kernel(int64_t M, int64_t N, int32_t K, bool wide) {
-  static const Cost costs[2][4] = {{{256, 256, 256, 600, 168, 165, 139},
+  static const Cost costs[2][5] = {{{256, 256, 256, 600, 168, 165, 139},
                                     {128, 128, 512, 300, 95, 80, 70},
                                     {64, 128, 512, 200, 71, 57, 43},
-                                    {64, 64, 512, 200, 55, 50, 30}},
+                                    {64, 64, 512, 200, 55, 50, 30},
+                                    {64, 64, 256, 300, 30, 29, 21}},
                                    {{256, 256, 256, 600, 335, 320, 306},
                                     {128, 128, 512, 300, 184, 170, 160},
                                     {64, 128, 512, 200, 117, 110, 84},
-                                    {64, 64, 512, 200, 95, 80, 45}}};
+                                    {64, 64, 512, 200, 95, 80, 45},
+                                    {64, 64, 256, 300, 55, 50, 36}}};
   const int64_t blocks = spr::ceil_div(K, KB);
   Kernel best = LARGE;
   int64_t least = INT64_MAX;
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 5; ++i) {
     const Cost& c = costs[wide ? 1 : 0][i];
     const int64_t tiles = spr::ceil_div(M, c.tm) * spr::ceil_div(N, c.tn), rest = tiles % c.full;
     const int64_t cost = spr::ceil_div(tiles, c.full) * c.start +
@@ -617,8 +649,9 @@ Kernel pick_kernel(int64_t M, int64_t N, int32_t K, bool wide) {
     if (cost < least) least = cost, best = static_cast<Kernel>(i);
   }
   // few rows: b's bytes once and a's for every 16 of b's rows, 0.15 us a MB, or the blocks that a wave takes in turn
-  // (and 512 threads for 16 of b's rows, fewer than 2^32 in a launch)
-  if (M <= 64 && N <= (int64_t(1) << 26)) {
+  // (and 512 threads for 16 of b's rows, fewer than 2^32 in a launch; more than 32 rows pay beside two groups of waves only
+  // where those convert to bf16: 64 x 500 x 14,000 in fp32 takes 32.0 us, with two groups 42.9)
+  if (M <= (wide ? 64 : 32) && N <= (int64_t(1) << 26)) {
     const int64_t bytes = N * K / 1000 * (16 + M) / 16 * 15 / 1000;
     const int64_t turns = spr::ceil_div(blocks, 8) * (M <= 16 ? 80 : M <= 32 ? 120 : 200);
     if (400 + (bytes > turns ? bytes : turns) < least) best = FEW;
@@ -635,23 +668,25 @@ int launch_product(const Matrix& a, const Matrix& b, int32_t K, const Output& o,
     const uint32_t grid = static_cast<uint32_t>(spr::ceil_div(N, 16));
     if (M <= 16) few_rows_kernel<DT, 1, 8><<<grid, 512, 0, stream>>>(a, b, K, o);
     else if (M <= 32) few_rows_kernel<DT, 2, 8><<<grid, 512, 0, stream>>>(a, b, K, o);
-    else few_rows_kernel<DT, 4, 8><<<grid, 512, 0, stream>>>(a, b, K, o);
+    else if constexpr (DT == 2) few_rows_kernel<DT, 4, 8><<<grid, 512, 0, stream>>>(a, b, K, o);
     SPR_LAUNCHED("few_rows_kernel");
     return SPR_OK;
   }
   const int64_t tm = spr::ceil_div(M, kernel == LARGE ? 256 : kernel == MIDDLE ? 128 : 64);
-  const int64_t tn = spr::ceil_div(N, kernel == LARGE ? 256 : kernel == TINY ? 64 : 128);
+  const int64_t tn = spr::ceil_div(N, kernel == LARGE ? 256 : kernel >= TINY ? 64 : 128);
   SPR_REQUIRE(tm * tn < (int64_t(1) << 22), "spr_fp8_matmul: too many outputs");
   const uint32_t grid = static_cast<uint32_t>(tm * tn);
   const int32_t rows = static_cast<int32_t>(tm), columns = static_cast<int32_t>(tn);
   if (kernel == MIDDLE) {
-    product_kernel<DT, 128, 128, 2, 2, 32, 2><<<grid, 256, 0, stream>>>(a, b, K, rows, columns, o);
+    product_kernel<DT, 128, 128, 2, 2, 32, 2, 1><<<grid, 256, 0, stream>>>(a, b, K, rows, columns, o);
   } else if (kernel == SMALL) {
-    product_kernel<DT, 64, 128, 2, 2, 32, 3><<<grid, 256, 0, stream>>>(a, b, K, rows, columns, o);
+    product_kernel<DT, 64, 128, 2, 2, 32, 3, 1><<<grid, 256, 0, stream>>>(a, b, K, rows, columns, o);
   } else if (kernel == TINY) {
-    product_kernel<DT, 64, 64, 4, 1, 32, 4><<<grid, 256, 0, stream>>>(a, b, K, rows, columns, o);
+    product_kernel<DT, 64, 64, 4, 1, 32, 4, 1><<<grid, 256, 0, stream>>>(a, b, K, rows, columns, o);
+  } else if (kernel == TINY2) {
+    product_kernel<DT, 64, 64, 4, 1, 32, 3, 2><<<grid, 512, 0, stream>>>(a, b, K, rows, columns, o);
   } else {
-    if constexpr (DT == 2) product_kernel<DT, 256, 256, 2, 4, 64, 2><<<grid, 512, 0, stream>>>(a, b, K, rows, columns, o);
+    if constexpr (DT == 2) product_kernel<DT, 256, 256, 2, 4, 64, 2, 1><<<grid, 512, 0, stream>>>(a, b, K, rows, columns, o);
     else turns_product_kernel<DT><<<grid, 512, 0, stream>>>(a, b, K, rows, columns, o);
   }
   SPR_LAUNCHED("product_kernel");

@@ -361,3 +361,9 @@ def test_one_row_on_more_columns_than_a_launch_of_few_rows_has(dev):
     b[-3:] = 0x38
     y = fp8_matmul(one.view(torch.float8_e4m3fn), scale, b.view(torch.float8_e4m3fn), scale.expand(n, 1))
     assert (y[0, -3:] == 16).all() and not y[0, :-3].any()
+
+
+@pytest.mark.parametrize("m,n,k", [(64, 64, 640), (70, 100, 4496), (130, 700, 1296), (300, 1500, 8208), (77, 4096, 3984)])
+def test_products_of_few_tiles_whose_waves_share_the_sum_are_exact(dev, m, n, k):
+    """Odd and even counts of blocks between two groups of waves, more of them than a window of scales holds."""
+    test_products_on_tiles_of_every_size_are_exact(dev, m, n, k)
