@@ -7,9 +7,9 @@
 //
 //   gradient, with g = dy w:   dx = r (g - s r^2 mean(g s)) + dsum,   dw = sum over rows of dy s r
 //
-// Sums are fp32, in an order that depends on the sizes only.  Bound by memory: every input is read
+// Sums are fp32, the norm's over more than 16 lanes 64 bits, in an order that depends on the sizes only.  Bound by memory: every input is read
 // once and kept in registers over the reduction, vectors of 8 channels a lane.  32,760 rows of 5120 in bf16
-// with residual and codes (1.18 GB) take 214 to 238 us, 5.0 to 5.5 TB/s where a copy has 5.1; the gradient of
+// with residual and codes (1.18 GB) take 214 to 242 us, 4.9 to 5.5 TB/s where a copy has 5.1; the gradient of
 // 8191 rows of 2560 (294 MB) 55 us, and 6 us for the weight's partial sums.  One row of 5120 takes 3.7 us.
 #include "spr_fp8.h"
 
@@ -34,15 +34,15 @@ __device__ __forceinline__ int64_t row_at(const Rows& t, uint32_t row) {
 }
 
 // The sums of N values over the threads of a row, in each of them: 16, or (0) the whole workgroup, whose waves meet
-// in `red`, 16 N floats.
-template <int TPR, int N>
-__device__ __forceinline__ void row_total(float (&a)[N], float* red) {
+// in `red`, 16 N of T.  T double is for sums past 16 lanes in 64 bits: the roundings of those below average out.
+template <int TPR, typename T, int N>
+__device__ __forceinline__ void row_total(const float (&a)[N], T (&total)[N], T* red) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    a[i] = spr::row_sum(a[i]);
+    total[i] = spr::row_sum(a[i]);
     if constexpr (TPR == 0) {
-      a[i] += __shfl_xor(a[i], 16, 64);
-      a[i] += __shfl_xor(a[i], 32, 64);
+      total[i] += __shfl_xor(total[i], 16, 64);
+      total[i] += __shfl_xor(total[i], 32, 64);
     }
   }
   if (TPR == 0 && blockDim.x > 64) {
@@ -50,14 +50,14 @@ __device__ __forceinline__ void row_total(float (&a)[N], float* red) {
     __syncthreads();  // earlier sums have been read
     if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) red[(threadIdx.x >> 6) * N + i] = a[i];
+      for (int i = 0; i < N; ++i) red[(threadIdx.x >> 6) * N + i] = total[i];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i) a[i] = 0.0f;
+    for (int i = 0; i < N; ++i) total[i] = T(0);
     for (int w = 0; w < waves; ++w)
 #pragma unroll
-      for (int i = 0; i < N; ++i) a[i] += red[w * N + i];
+      for (int i = 0; i < N; ++i) total[i] += red[w * N + i];
   }
 }
 
@@ -66,12 +66,21 @@ __device__ __forceinline__ float tree_sum(const float (&p)[8]) {
   return ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 }
 
-// 1 / sqrt(ss / width + eps), rounded once: a value next to a border of its output's type then goes where the
-// formula in more digits sends it, but for the error of ss.  One step of Newton from the instruction's estimate.
-__device__ __forceinline__ float inverse_rms(float ss, double inv_width, float eps) {
-  const double v = static_cast<double>(ss) * inv_width + static_cast<double>(eps);
+// 1 / sqrt(ss / width + eps).  One step of Newton from the instruction's estimate.
+__device__ __forceinline__ double inverse_rms(double ss, double inv_width, float eps) {
+  const double v = ss * inv_width + static_cast<double>(eps);
   const double r = __builtin_amdgcn_rsq(v), e = __builtin_fma(-v * r, r, 1.0);
-  return static_cast<float>(__builtin_isfinite(e) ? r + 0.5 * r * e : r);  // (of 0 and infinity as they are)
+  return __builtin_isfinite(e) ? r + 0.5 * r * e : r;  // (of 0 and infinity as they are)
+}
+
+// s inv w with the roundings of the two products carried along, so rounded once to fp32: a value next to a border of its
+// output's type then goes where the formula in more digits sends it (of 10 M bf16 outputs 3 to 5 go elsewhere, 30 with two
+// roundings; 305 instead of 301 us on 32,760 rows of 5120).  Where a product is 0, infinite or NaN it is as it is.
+__device__ __forceinline__ float normed(float s, float inv, float inv_low, float w) {
+  const float a = s * inv, y = a * w;
+  const float low = __builtin_fmaf(s, inv_low, __builtin_fmaf(s, inv, -a));
+  const float exact = __builtin_fmaf(a, w, low * w);
+  return y != 0.0f && __builtin_isfinite(y) ? exact : y;
 }
 
 // TPR threads a row (0: the workgroup), NV vectors of 8 channels a thread.  RES: 0 no residual, 1 of x's type, 2 fp32.
@@ -82,7 +91,7 @@ __global__ __launch_bounds__(TPR == 0 ? 1024 : 256) void norm_kernel(
   constexpr int SDT = RES == 2 ? 2 : DT;
   using S = typename Elem<DT>::S;
   using R = typename Elem<SDT>::S;
-  __shared__ float red[16];
+  __shared__ double red[16];
   const int lane = TPR == 0 ? threadIdx.x : threadIdx.x % TPR, step = TPR == 0 ? blockDim.x : TPR;
   const uint32_t row = TPR == 0 ? blockIdx.x : blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
   if (TPR != 0 && row >= rows) return;
@@ -112,8 +121,11 @@ __global__ __launch_bounds__(TPR == 0 ? 1024 : 256) void norm_kernel(
 #pragma unroll
     for (int e = 0; e < 8; ++e) p[e] = __builtin_fmaf(s[u][e], s[u][e], p[e]);
   float ss[1] = {tree_sum(p)};
-  row_total<TPR>(ss, red);
-  const float inv = inverse_rms(ss[0], inv_width, eps);
+  double total[1];
+  row_total<TPR>(ss, total, red);
+  const double root = inverse_rms(total[0], inv_width, eps);
+  const float inv = static_cast<float>(root);
+  const float inv_low = __builtin_isfinite(inv) ? static_cast<float>(root - static_cast<double>(inv)) : 0.0f;
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
     const int c = (lane + u * step) * 8;
@@ -125,7 +137,7 @@ __global__ __launch_bounds__(TPR == 0 ? 1024 : 256) void norm_kernel(
       for (int e = 0; e < 8; ++e) w[e] = 1.0f;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s[u][e] = s[u][e] * inv * w[e];
+    for (int e = 0; e < 8; ++e) s[u][e] = normed(s[u][e], inv, inv_low, w[e]);
     if constexpr (FP8) {
       // 16 lanes are a group of 128 channels; all of them come here
       if (c + 8 > width) {  // 0 * inf and 0 * NaN behind the row's end
@@ -202,9 +214,10 @@ __global__ __launch_bounds__(TPR == 0 ? 1024 : 256) void norm_backward_kernel(
         q[e] = __builtin_fmaf(g[u][e] * w[u][e], s[u][e], q[e]);
       }
     float t[2] = {tree_sum(p), tree_sum(q)};  // of s^2 and of g s
-    row_total<TPR>(t, red);
-    const float inv = inverse_rms(t[0], inv_width, eps);
-    const float along = inv * inv * (t[1] * static_cast<float>(inv_width));
+    float total[2];  // (in 64 bits, as the norm's: 74 instead of 65 us on 8191 rows of 2560)
+    row_total<TPR>(t, total, red);
+    const float inv = static_cast<float>(inverse_rms(total[0], inv_width, eps));
+    const float along = inv * inv * (total[1] * static_cast<float>(inv_width));
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int c = (lane + u * step) * 8;
