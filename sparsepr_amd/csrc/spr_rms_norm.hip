@@ -74,7 +74,7 @@ __device__ __forceinline__ double inverse_rms(double ss, double inv_width, float
 }
 
 // s inv w with the roundings of the two products carried along, so rounded once to fp32: a value next to a border of its
-// output's type then goes where the formula in more digits sends it (of 10 M bf16 outputs 3 to 5 go elsewhere, 30 with two
+// output's type then goes where the formula in more digits sends it (of 5 M bf16 outputs 2 to 5 go elsewhere, 30 with two
 // roundings; 305 instead of 301 us on 32,760 rows of 5120).  Where a product is 0, infinite or NaN it is as it is.
 __device__ __forceinline__ float normed(float s, float inv, float inv_low, float w) {
   const float a = s * inv, y = a * w;
