@@ -194,12 +194,15 @@ def available() -> bool:
 
 def call(name: str, *args) -> int:
     """Call an entry point; raise RuntimeError on a nonzero status."""
-    lib = load()
-    status = getattr(lib, name)(*args)
+    status = getattr(_LIB or load(), name)(*args)
     if status != 0:
-        msg = lib.spr_last_error().decode(errors="replace")
-        raise RuntimeError(f"{name} failed (status {status}): {msg}")
+        _refused(name, status)
     return status
+
+
+def _refused(name: str, status: int):
+    msg = load().spr_last_error().decode(errors="replace")
+    raise RuntimeError(f"{name} failed (status {status}): {msg}")
 
 
 def launch(name: str, device: torch.device, *args) -> int:
@@ -207,10 +210,13 @@ def launch(name: str, device: torch.device, *args) -> int:
     What a call of a few microseconds spends on the host counts: the raw stream takes 0.1 us where
     torch.cuda.current_stream takes 2, and the device is entered only where it is not the current one."""
     index = device.index
-    if torch.cuda.current_device() != index:
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
             return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-    return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    status = getattr(_LIB or load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != 0:
+        _refused(name, status)
+    return status
 
 
 def query(name: str, *args):

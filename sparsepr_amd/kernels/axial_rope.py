@@ -59,31 +59,34 @@ def axial_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     what = "axial RoPE"
     dev = _lib.require_gpu(q, k, positions, freqs, axis, what=what)
     no_gradient(what, q, k, positions, freqs)
-    if q.dim() != 4 or q.dtype not in _lib.DTYPE_CODE:
+    shape, dtype = q.shape, _lib.DTYPE_CODE.get(q.dtype)
+    if len(shape) != 4 or dtype is None:
         raise RuntimeError(f"{what}: q must be [B, H, T, D] in bfloat16, float16 or float32, got {q.dtype} "
                            f"{tuple(q.shape)}")
-    b, h, t, d = q.shape
+    b, h, t, d = shape
     hk = 0
     if k is not None:
         shape = k.shape
         hk = shape[1] if len(shape) == 4 else -1
         if shape != (b, hk, t, d) or k.dtype is not q.dtype:
             raise RuntimeError(f"{what}: k must be [{b}, heads, {t}, {d}] in {q.dtype}, got {k.dtype} {tuple(shape)}")
-    if pairs not in ("interleaved", "halves"):
+    if pairs != "interleaved" and pairs != "halves":
         raise RuntimeError(f"{what}: pairs must be 'interleaved' or 'halves', got {pairs!r}")
-    place, axes = positions.shape, positions.shape[-1] if positions.dim() > 1 else 0
+    place = positions.shape
+    axes = place[-1] if len(place) > 1 else 0
     code = POSITION_CODE.get(positions.dtype)
     if code is None or (place != (t, axes) and place != (b, t, axes)):
         raise RuntimeError(f"{what}: positions must be [{t}, axes] or [{b}, {t}, axes] in int32, int64, float32 or "
                            f"float64, got {positions.dtype} {tuple(positions.shape)}")
-    if freqs.dtype is not torch.float64 or axis.dtype is not torch.int32 or freqs.dim() != 1 \
-            or axis.shape != freqs.shape or not freqs.is_contiguous() or not axis.is_contiguous():
+    turns = freqs.shape
+    if freqs.dtype is not torch.float64 or axis.dtype is not torch.int32 or len(turns) != 1 \
+            or axis.shape != turns or not freqs.is_contiguous() or not axis.is_contiguous():
         raise RuntimeError(f"{what}: freqs must be contiguous float64 and axis contiguous int32 of one length, got "
                            f"{freqs.dtype} {tuple(freqs.shape)} / {axis.dtype} {tuple(axis.shape)}")
-    rotated = 2 * freqs.shape[0]
+    rotated = 2 * turns[0]
     if d % 8 != 0 or not 8 <= d <= 1024 or rotated % 8 != 0 or rotated > d:
         raise RuntimeError(f"{what}: {rotated} rotated dims of {d} (both multiples of 8, D at most 1024)")
-    if max(h, hk) >= 1 << 20:
+    if h >= 1 << 20 or hk >= 1 << 20:
         raise RuntimeError(f"{what}: {h} and {hk} heads")
     if not 1 <= axes <= 16:
         raise RuntimeError(f"{what}: {axes} axes, 1 to 16 are taken")
@@ -91,12 +94,12 @@ def axial_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     k_out = None if k is None else q.new_empty((b, hk, t, d))
     if b * t * (h + hk) > 0:
         positions = positions.contiguous()
-        k_strides = (0, 0, 0)
-        q, *q_strides = _strided(q)
+        kb = kh = kt = k_at = k_to = 0
+        q, qb, qh, qt = _strided(q)
         if k is not None:
-            k, *k_strides = _strided(k)
-        _lib.launch("spr_axial_rope", dev, q.data_ptr(), *q_strides, h, _lib.ptr(k), *k_strides, hk,
-                    _lib.DTYPE_CODE[q.dtype], b, t, d, rotated, positions.data_ptr(), code,
-                    t * axes if len(place) == 3 else 0, axes, freqs.data_ptr(), axis.data_ptr(),
-                    int(pairs == "halves"), int(inverse), q_out.data_ptr(), _lib.ptr(k_out))
+            k, kb, kh, kt = _strided(k)
+            k_at, k_to = k.data_ptr(), k_out.data_ptr()
+        _lib.launch("spr_axial_rope", dev, q.data_ptr(), qb, qh, qt, h, k_at, kb, kh, kt, hk, dtype, b, t, d, rotated,
+                    positions.data_ptr(), code, t * axes if len(place) == 3 else 0, axes, freqs.data_ptr(),
+                    axis.data_ptr(), int(pairs == "halves"), int(inverse), q_out.data_ptr(), k_to)
     return q_out, k_out

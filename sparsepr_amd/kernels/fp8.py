@@ -35,9 +35,8 @@ def no_gradient(what: str, *tensors: torch.Tensor | None) -> None:
                                "gradient functions beside it")
 
 
-def _packed_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+def _packed_rows(x: torch.Tensor, rows: int, width: int) -> tuple[torch.Tensor, int]:
     """x [R, C] and its row stride: itself where rows are packed, else a copy."""
-    rows, width = x.shape
     step, packed = x.stride()
     if packed == 1 or width == 1:
         return x, step if rows > 1 else width
@@ -46,11 +45,12 @@ def _packed_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
 
 def _check_matrix(codes: torch.Tensor, scales: torch.Tensor, what: str, name: str) -> tuple[int, int, int]:
     """(rows, width, whether a scale is of 128 rows) of an 8-bit matrix."""
-    if codes.dtype is not CODES or codes.dim() != 2:
+    shape = codes.shape
+    if codes.dtype is not CODES or len(shape) != 2:
         raise RuntimeError(f"{what}: {name} must be float8_e4m3fn [rows, width], got {codes.dtype} {tuple(codes.shape)}")
-    rows, width = codes.shape
+    rows, width = shape
     blocks = -(-width // BLOCK)
-    if max(rows, width) > MAX_SIZE:
+    if rows > MAX_SIZE or width > MAX_SIZE:
         raise RuntimeError(f"{what}: {name} is {tuple(codes.shape)}, {MAX_SIZE} rows or columns at most")
     if width % 16 != 0:
         raise RuntimeError(f"{what}: the width of {name} ({width}) must be a multiple of 16 (zeros behind the row)")
@@ -62,13 +62,17 @@ def _check_matrix(codes: torch.Tensor, scales: torch.Tensor, what: str, name: st
     return rows, width, int(shape[0] != rows)
 
 
-def _as_read(codes: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, int, torch.Tensor, int]:
+def _as_read(codes: torch.Tensor, scales: torch.Tensor, rows: int, width: int) -> tuple[torch.Tensor, int, torch.Tensor, int]:
     """Codes with packed rows that start on 16 bytes and scales with packed rows, and their row strides."""
-    width = codes.shape[1]
-    codes, ld = _packed_rows(codes)
-    if codes.data_ptr() % 16 != 0 or ld % 16 != 0 or ld < width:
+    ld, packed = codes.stride()
+    if rows == 1:
+        ld = width
+    if packed != 1 or ld % 16 != 0 or ld < width or codes.data_ptr() % 16 != 0:  # (the width is 16 or more)
         codes, ld = codes.clone(memory_format=torch.contiguous_format), width
-    scales, scales_ld = _packed_rows(scales)
+    scales_ld, packed = scales.stride()
+    if packed != 1 and width > BLOCK:
+        scales = scales.contiguous()
+        scales_ld = scales.stride(0)
     return codes, ld, scales, scales_ld
 
 
@@ -81,18 +85,20 @@ def fp8_quantize(x: torch.Tensor, *, square: bool = False, transpose: bool = Fal
     what = "8-bit quantisation"
     dev = _lib.require_gpu(x, what=what)
     no_gradient(what, x)
-    if x.dim() != 2 or x.dtype not in _lib.DTYPE_CODE:
+    shape, code = x.shape, _lib.DTYPE_CODE.get(x.dtype)
+    if len(shape) != 2 or code is None:
         raise RuntimeError(f"{what}: x must be [rows, width] in bfloat16, float16 or float32, got {x.dtype} "
                            f"{tuple(x.shape)}")
-    if max(x.shape) > MAX_SIZE:
+    height, across = shape
+    if height > MAX_SIZE or across > MAX_SIZE:
         raise RuntimeError(f"{what}: x is {tuple(x.shape)}, {MAX_SIZE} rows or columns at most")
-    rows, width = x.shape[::-1] if transpose else x.shape
+    rows, width = (across, height) if transpose else (height, across)
     codes = x.new_empty((rows, -(-width // 16) * 16), dtype=CODES)
     scales = x.new_empty((-(-rows // BLOCK) if square else rows, -(-width // BLOCK)), dtype=torch.uint8)
-    if x.numel() > 0:
-        x, ld = _packed_rows(x)
-        _lib.launch("spr_fp8_quantize", dev, x.data_ptr(), ld, *x.shape, _lib.DTYPE_CODE[x.dtype], int(square),
-                    int(transpose), codes.data_ptr(), scales.data_ptr())
+    if height > 0 and across > 0:
+        x, ld = _packed_rows(x, height, across)
+        _lib.launch("spr_fp8_quantize", dev, x.data_ptr(), ld, height, across, code, int(square), int(transpose),
+                    codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
@@ -102,13 +108,14 @@ def fp8_dequantize(codes: torch.Tensor, scales: torch.Tensor, *, dtype: torch.dt
     what = "8-bit values"
     dev = _lib.require_gpu(codes, scales, what=what)
     rows, width, square = _check_matrix(codes, scales, what, "codes")
-    if dtype not in _lib.DTYPE_CODE:
+    code = _lib.DTYPE_CODE.get(dtype)
+    if code is None:
         raise RuntimeError(f"{what}: dtype must be bfloat16, float16 or float32, got {dtype}")
     out = codes.new_empty((rows, width), dtype=dtype)
-    if out.numel() > 0:
-        codes, ld, scales, scales_ld = _as_read(codes, scales)
+    if rows > 0 and width > 0:
+        codes, ld, scales, scales_ld = _as_read(codes, scales, rows, width)
         _lib.launch("spr_fp8_dequantize", dev, codes.data_ptr(), ld, scales.data_ptr(), scales_ld, square, rows, width,
-                    _lib.DTYPE_CODE[dtype], out.data_ptr())
+                    code, out.data_ptr())
     return out
 
 
@@ -127,20 +134,22 @@ def fp8_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
         raise RuntimeError(f"{what}: a is [{m}, {k}], b [{n}, {kb}]")
     if k > MAX_SUM:
         raise RuntimeError(f"{what}: sums of {k} terms, {MAX_SUM} are taken")
-    if out_dtype not in _lib.DTYPE_CODE:
+    code, bias_at, bias_code = _lib.DTYPE_CODE.get(out_dtype), 0, 0
+    if code is None:
         raise RuntimeError(f"{what}: out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
     if bias is not None:
-        if bias.shape != (n,) or bias.dtype not in _lib.DTYPE_CODE:
+        bias_code = _lib.DTYPE_CODE.get(bias.dtype)
+        if bias.shape != (n,) or bias_code is None:
             raise RuntimeError(f"{what}: bias must be [{n}] in bfloat16, float16 or float32, got {bias.dtype} "
                                f"{tuple(bias.shape)}")
         bias = bias.contiguous()
+        bias_at = bias.data_ptr()
     out = a.new_empty((m, n), dtype=out_dtype)
     if k == 0:  # (no rows that a weight's gradient would be summed over)
         return out.zero_() if bias is None else out.copy_(bias)
-    if out.numel() > 0:
-        a, a_ld, a_scales, a_scales_ld = _as_read(a, a_scales)
-        b, b_ld, b_scales, b_scales_ld = _as_read(b, b_scales)
+    if m > 0 and n > 0:
+        a, a_ld, a_scales, a_scales_ld = _as_read(a, a_scales, m, k)
+        b, b_ld, b_scales, b_scales_ld = _as_read(b, b_scales, n, k)
         _lib.launch("spr_fp8_matmul", dev, a.data_ptr(), a_ld, a_scales.data_ptr(), a_scales_ld, a_square, b.data_ptr(),
-                    b_ld, b_scales.data_ptr(), b_scales_ld, b_square, m, n, k, _lib.ptr(bias),
-                    0 if bias is None else _lib.DTYPE_CODE[bias.dtype], _lib.DTYPE_CODE[out_dtype], out.data_ptr())
+                    b_ld, b_scales.data_ptr(), b_scales_ld, b_square, m, n, k, bias_at, bias_code, code, out.data_ptr())
     return out

@@ -52,46 +52,53 @@ def _split(x: torch.Tensor, n0: int, n1: int) -> tuple[torch.Tensor, int, int]:
     return x, x.shape[-1] * n1, x.shape[-1]
 
 
-def _check(x: torch.Tensor, weight: torch.Tensor | None, epsilon: float, what: str) -> int:
-    if x.dim() < 1 or x.dtype not in _lib.DTYPE_CODE:
+def _check(x: torch.Tensor, weight: torch.Tensor | None, epsilon: float, what: str) -> tuple[torch.Size, int, int, int]:
+    """(x's shape, its last dim, codes of x's and of the weight's type)."""
+    shape, code = x.shape, _lib.DTYPE_CODE.get(x.dtype)
+    if len(shape) < 1 or code is None:
         raise RuntimeError(f"{what}: x must be [..., C] in bfloat16, float16 or float32, got {x.dtype} {tuple(x.shape)}")
-    width = x.shape[-1]
+    width, weight_code = shape[-1], 0
     if not 1 <= width <= MAX_WIDTH:
         raise RuntimeError(f"{what}: width {width} not in 1 .. {MAX_WIDTH}")
     if x.numel() // width >= 1 << 31:  # the entry points count rows in 32 bits
         raise RuntimeError(f"{what}: too many rows in {tuple(x.shape)}")
-    if weight is not None and (weight.shape != (width,) or weight.dtype not in (x.dtype, torch.float32)):
-        raise RuntimeError(f"{what}: weight must be [{width}] in {x.dtype} or float32, got {weight.dtype} "
-                           f"{tuple(weight.shape)}")
+    if weight is not None:
+        weight_code = _lib.DTYPE_CODE.get(weight.dtype)
+        if weight.shape != (width,) or weight_code not in (code, 2):
+            raise RuntimeError(f"{what}: weight must be [{width}] in {x.dtype} or float32, got {weight.dtype} "
+                               f"{tuple(weight.shape)}")
     if not 0.0 <= epsilon < float("inf"):
         raise RuntimeError(f"{what}: epsilon must be finite and not negative, got {epsilon}")
-    return width
+    return shape, width, code, weight_code
 
 
 def _norm(x, weight, residual, epsilon, fp8: bool, what: str):
     dev = _lib.require_gpu(x, weight, residual, what=what)
     no_gradient(what, x, weight, residual)
-    width = _check(x, weight, epsilon, what)
-    if residual is not None and (residual.shape != x.shape or residual.dtype not in (x.dtype, torch.float32)):
-        raise RuntimeError(f"{what}: residual must be {tuple(x.shape)} in {x.dtype} or float32, got {residual.dtype} "
-                           f"{tuple(residual.shape)}")
+    shape, width, code, weight_code = _check(x, weight, epsilon, what)
+    total, r_code = None, 0
+    if residual is not None:
+        r_code = _lib.DTYPE_CODE.get(residual.dtype)
+        if residual.shape != shape or r_code not in (code, 2):
+            raise RuntimeError(f"{what}: residual must be {tuple(x.shape)} in {x.dtype} or float32, got {residual.dtype} "
+                               f"{tuple(residual.shape)}")
+        total = residual.new_empty(shape)
+    scales = None
     if fp8:
-        out = x.new_empty((*x.shape[:-1], -(-width // 16) * 16), dtype=CODES)
-        scales = x.new_empty((*x.shape[:-1], -(-width // BLOCK)), dtype=torch.uint8)
+        rows = shape[:-1]
+        out = x.new_empty((*rows, -(-width // 16) * 16), dtype=CODES)
+        scales = x.new_empty((*rows, -(-width // BLOCK)), dtype=torch.uint8)
     else:
-        out, scales = x.new_empty(x.shape), None
-    total = None if residual is None else residual.new_empty(x.shape)
+        out = x.new_empty(shape)
     if x.numel() > 0:
-        code = _lib.DTYPE_CODE[x.dtype]
         x, n0, n1, s0, s1 = _by_rows(x)
-        r0 = r1 = r_code = 0
+        r_at = r0 = r1 = 0
         if residual is not None:
             residual, r0, r1 = _split(residual, n0, n1)
-            r_code = _lib.DTYPE_CODE[residual.dtype]
+            r_at = residual.data_ptr()
         weight = None if weight is None else weight.contiguous()
-        _lib.launch("spr_rms_norm", dev, x.data_ptr(), s0, s1, _lib.ptr(residual), r0, r1, n0, n1, width, code, r_code,
-                    _lib.ptr(weight), 0 if weight is None else _lib.DTYPE_CODE[weight.dtype], float(epsilon),
-                    out.data_ptr(), _lib.ptr(scales), _lib.ptr(total))
+        _lib.launch("spr_rms_norm", dev, x.data_ptr(), s0, s1, r_at, r0, r1, n0, n1, width, code, r_code,
+                    _lib.ptr(weight), weight_code, float(epsilon), out.data_ptr(), _lib.ptr(scales), _lib.ptr(total))
     return out, scales, total
 
 
@@ -119,7 +126,7 @@ def rms_norm_backward(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor | 
     what = "RMS norm's gradient"
     dev = _lib.require_gpu(dy, s, weight, dsum, what=what)
     no_gradient(what, dy, s, weight, dsum)
-    width = _check(dy, weight, epsilon, what)
+    _, width, code, weight_code = _check(dy, weight, epsilon, what)
     for t, name in ((s, "s"), (dsum, "dsum")):
         if t is not None and (t.shape != dy.shape or t.dtype not in (dy.dtype, torch.float32) or t.dtype != s.dtype):
             raise RuntimeError(f"{what}: {name} must be {tuple(dy.shape)} in {dy.dtype} or float32 (one type for both), "
@@ -137,7 +144,6 @@ def rms_norm_backward(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor | 
     need = 0 if dweight is None else _lib.query("spr_rms_norm_backward_workspace", n0 * n1, width)
     ws = _lib.workspace(need, dev) if need > 0 else None
     _lib.launch("spr_rms_norm_backward", dev, dy.data_ptr(), y0, y1, s.data_ptr(), s0, s1, _lib.ptr(dsum), d0, d1, n0, n1,
-                width, _lib.DTYPE_CODE[dy.dtype], _lib.DTYPE_CODE[s.dtype], _lib.ptr(weight),
-                0 if weight is None else _lib.DTYPE_CODE[weight.dtype], float(epsilon), dx.data_ptr(),
+                width, code, _lib.DTYPE_CODE[s.dtype], _lib.ptr(weight), weight_code, float(epsilon), dx.data_ptr(),
                 _lib.ptr(dweight), _lib.ptr(ws), need)
     return dx, dweight
