@@ -9,8 +9,9 @@
 //
 // Sums are fp32, the norm's over more than 16 lanes 64 bits, in an order that depends on the sizes only.  Bound by memory: every input is read
 // once and kept in registers over the reduction, vectors of 8 channels a lane.  32,760 rows of 5120 in bf16
-// with residual and codes (1.18 GB) take 214 to 242 us, 4.9 to 5.5 TB/s where a copy has 5.1; the gradient of
-// 8191 rows of 2560 (294 MB) 55 us, and 6 us for the weight's partial sums.  One row of 5120 takes 3.7 us.
+// with residual and codes (1.18 GB) take 215 us one behind the other, 5.5 TB/s where a copy has
+// 5.1, and 241 to 265 between other kernels; the gradient of
+// 8191 rows of 2560 (294 MB) 55 us, and 6 us for the weight's partial sums.  One row of 5120 takes 4.0 us.
 #include "spr_fp8.h"
 
 namespace {
