@@ -7,11 +7,11 @@
 //
 //   gradient, with g = dy w:   dx = r (g - s r^2 mean(g s)) + dsum,   dw = sum over rows of dy s r
 //
-// Sums are fp32, the norm's over more than 16 lanes 64 bits, in an order that depends on the sizes only.  Bound by memory: every input is read
-// once and kept in registers over the reduction, vectors of 8 channels a lane.  32,760 rows of 5120 in bf16
-// with residual and codes (1.18 GB) take 215 us one behind the other, 5.5 TB/s where a copy has
-// 5.1, and 241 to 265 between other kernels; the gradient of
-// 8191 rows of 2560 (294 MB) 55 us, and 6 us for the weight's partial sums.  One row of 5120 takes 4.0 us.
+// Sums are fp32, the norm's over more than 16 lanes 64 bits, in an order that depends on the sizes only.
+// Bound by memory: every input is read once and kept in registers over the reduction, vectors of 8 channels a
+// lane.  32,760 rows of 5120 in bf16 with residual and codes (1.18 GB) take 215 us one call behind the other, 5.5 TB/s
+// where a copy has 5.1, and 241 to 265 between other kernels; the gradient of 8191 rows of 2560 (294 MB) 55 us, and
+// 6 us for the weight's partial sums.  One row of 5120 takes 4.0 us.
 #include "spr_fp8.h"
 
 namespace {
