@@ -616,7 +616,8 @@ int spr_rms_norm_backward(const void* dy, int64_t dy_s0, int64_t dy_s1, const vo
  * No counterpart in the reference.  e4m3 codes [rows, width rounded up to 16], zeros behind the width, with a
  * scale byte b, 2^(b - 127) (255: NaN), per 128 values of a row, scales [rows, width / 128 rounded up], or
  * (square) per 128 x 128 values, [rows / 128 rounded up, ...].
- * Quantise x [rows, width] of dtype with row stride ld; transpose: the 8-bit matrix of x^T. */
+ * Quantise x [rows, width] of dtype with row stride ld, rows below 2^24 (square or transposed at most 65,535 * 128);
+ * transpose: the 8-bit matrix of x^T. */
 int spr_fp8_quantize(const void* x, int64_t ld, int64_t rows, int32_t width, int32_t dtype, int32_t square,
                      int32_t transpose, uint8_t* codes, uint8_t* scales, hipStream_t stream);
 /* out [rows, width] of dtype, contiguous; width a multiple of 16, codes 16-byte aligned, ld a multiple of 16. */
