@@ -156,6 +156,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "spr_fp8_dequantize": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp]),
     # fp8_matmul.hip
     "spr_fp8_matmul": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32] * 2 + [_i64, _i64, _i32, _vp, _i32, _i32, _vp, _vp]),
+    "spr_fp8_matmul_ex": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32] * 2 + [_i64, _i64, _i32, _vp, _i32, _i32, _i32, _vp,
+                                                                            _vp]),
     # axial_rope.hip
     "spr_axial_rope": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i32] * 2 + [_i32, _i64, _i64, _i32, _i32, _vp, _i32, _i64,
                                                                           _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp]),

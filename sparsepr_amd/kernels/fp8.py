@@ -120,9 +120,16 @@ def fp8_dequantize(codes: torch.Tensor, scales: torch.Tensor, *, dtype: torch.dt
 
 
 def fp8_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, *,
-               bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+               bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+               fast_sums: bool = False) -> torch.Tensor:
     """a b^T + bias for 8-bit matrices a [M, K] and b [N, K]: out [M, N] in `out_dtype` (bf16, fp16 or fp32),
-    summed in fp32 and rounded once.  bias [N] in any of the three types.
+    summed in fp32 and rounded once.  bias [N] in any of the three types.  The values are multiplied as
+    fp8_dequantize gives them in bf16, exact for scale bytes 3 to 246.
+
+    `fast_sums`, for outputs in 16 bits: up to twice the rate, on the 8-bit matrix instruction.  It adds eight
+    neighbouring products at a time and keeps digits down to 2^-13 of the largest of them (the sums of the eights
+    are fp32).  What it cuts is 5e-5 of the norm on normal rows, a thirtieth of bf16's own rounding and a quarter
+    of fp16's; where large products cancel it may be all of an output.
 
     Rows that do not start on 16 bytes are copied first."""
     what = "8-bit product"
@@ -137,6 +144,8 @@ def fp8_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     code, bias_at, bias_code = _lib.DTYPE_CODE.get(out_dtype), 0, 0
     if code is None:
         raise RuntimeError(f"{what}: out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
+    if fast_sums and code == 2:
+        raise RuntimeError(f"{what}: fast sums are for outputs in 16 bits, got {out_dtype}")
     if bias is not None:
         bias_code = _lib.DTYPE_CODE.get(bias.dtype)
         if bias.shape != (n,) or bias_code is None:
@@ -150,6 +159,7 @@ def fp8_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     if m > 0 and n > 0:
         a, a_ld, a_scales, a_scales_ld = _as_read(a, a_scales, m, k)
         b, b_ld, b_scales, b_scales_ld = _as_read(b, b_scales, n, k)
-        _lib.launch("spr_fp8_matmul", dev, a.data_ptr(), a_ld, a_scales.data_ptr(), a_scales_ld, a_square, b.data_ptr(),
-                    b_ld, b_scales.data_ptr(), b_scales_ld, b_square, m, n, k, bias_at, bias_code, code, out.data_ptr())
+        _lib.launch("spr_fp8_matmul_ex", dev, a.data_ptr(), a_ld, a_scales.data_ptr(), a_scales_ld, a_square, b.data_ptr(),
+                    b_ld, b_scales.data_ptr(), b_scales_ld, b_square, m, n, k, bias_at, bias_code, code, int(fast_sums),
+                    out.data_ptr())
     return out

@@ -21,11 +21,12 @@ from .kernels.rms_norm import rms_norm, rms_norm_fp8
 class QKVProjection:
     def __init__(self, weight: torch.Tensor, *, heads: int, kv_heads: int | None = None, axis_dims, theta: float = 10000.0,
                  pairs: str = "interleaved", norm_weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
-                 q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, epsilon: float = 1e-6):
+                 q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, epsilon: float = 1e-6,
+                 fast_sums: bool = False):
         """weight [(heads + 2 kv_heads) D, C]: the rows of Q, then K, then V, quantised here once (128 x 128 blocks).
         norm_weight [C] and bias as in rms_norm and fp8_matmul.  q_norm and k_norm norm Q and K before they are
         turned: [D] every head by itself, [heads * D] all channels together.  axis_dims: the rotated dims of each
-        axis of the positions (axial_frequencies)."""
+        axis of the positions (axial_frequencies).  fast_sums: the product's (fp8_matmul)."""
         kv_heads = heads if kv_heads is None else kv_heads
         what = "QKV projection"
         if heads < 1 or kv_heads < 1 or heads % kv_heads != 0:
@@ -41,7 +42,7 @@ class QKVProjection:
         self.weight = fp8_quantize(weight, square=True)
         self.norm_weight, self.bias, self.q_norm, self.k_norm = norm_weight, bias, q_norm, k_norm
         self.freqs, self.axis = axial_frequencies(axis_dims, theta=theta, device=weight.device)
-        self.pairs, self.epsilon = pairs, epsilon
+        self.pairs, self.epsilon, self.fast_sums = pairs, epsilon, fast_sums
 
     def _heads(self, x: torch.Tensor, heads: int, weight: torch.Tensor | None) -> torch.Tensor:
         """x [B, T, heads * D] -> [B, heads, T, D], normed where there is a weight."""
@@ -58,7 +59,8 @@ class QKVProjection:
         if x.dim() != 3 or x.shape[2] != self.width:
             raise RuntimeError(f"QKV projection: x must be [B, T, {self.width}], got {tuple(x.shape)}")
         codes, scales, *total = rms_norm_fp8(x, self.norm_weight, residual=residual, epsilon=self.epsilon)
-        y = fp8_matmul(codes.flatten(0, 1), scales.flatten(0, 1), *self.weight, bias=self.bias, out_dtype=x.dtype)
+        y = fp8_matmul(codes.flatten(0, 1), scales.flatten(0, 1), *self.weight, bias=self.bias, out_dtype=x.dtype,
+                       fast_sums=self.fast_sums)
         kv = self.kv_heads * self.head_dim
         q, k, v = y.view(*x.shape[:2], -1).split((self.heads * self.head_dim, kv, kv), -1)
         q, k = axial_rope(self._heads(q, self.heads, self.q_norm), self._heads(k, self.kv_heads, self.k_norm), positions,

@@ -64,6 +64,22 @@ def values(codes, scales):
     return grid()[codes] * s.repeat(GROUP, 1)[:, :c]
 
 
+def cancelling(rng, m, n, k):
+    """Codes [m, k] and [n, k]: of eight neighbouring products one is +-2^12, alternating, the others are +-2^-2."""
+    at = np.arange(k)
+    big, flip = at % 8 == 0, np.where(at // 8 % 2 == 0, 1.0, -1.0)
+    a, b = (np.where(rng.random((r, k)) < 0.5, 0.5, -0.5) for r in (m, n))
+    a[:, big], b[:, big] = 64.0 * flip[big], 64.0
+    return encode(a), encode(b)
+
+
+def cut_product(a, b, digits):
+    """a b^T where of eight neighbouring products the digits below 2^-digits of the largest one's power of two are cut."""
+    p = (a[:, None, :] * b[None, :, :]).reshape(len(a), len(b), -1, 8)
+    unit = np.ldexp(1.0, np.frexp(np.abs(p).max(-1, keepdims=True))[1] - 1 - digits)
+    return (np.trunc(p / unit) * unit).sum((-1, -2))
+
+
 def norm(s, w, eps):
     """s / sqrt(mean(s^2) + eps) * w."""
     return s / np.sqrt((s * s).mean(-1, keepdims=True) + eps) * w

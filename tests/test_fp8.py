@@ -62,6 +62,26 @@ def test_gradient_formulas_against_differences():
             assert abs(diff.sum() / (2 * h) - back[i]) < 1e-7
 
 
+def test_rows_that_cancel_tell_full_sums_from_cut_ones():
+    """What the GPU tests of the sums are built on: cut at 2^-13, nothing is left of products that are 2^-14 of the
+    largest; fp32's 24 digits keep them all, and normal rows tell the cut from fp32 only by little."""
+    rng = np.random.default_rng(4)
+    a, b = (model.grid()[c] for c in model.cancelling(rng, 5, 7, 256))
+    want = a @ b.T
+    assert (want != 0).sum() > 25 and np.abs(want).max() <= 2.0**-2 * 224
+    assert (cut := model.cut_product(a, b, 13)).shape == want.shape and not cut.any()
+    assert np.array_equal(model.cut_product(a, b, 14), want)
+    a, b = (model.values(*model.quantise(rng.standard_normal((r, 512)))) for r in (6, 9))
+    off = np.abs(model.cut_product(a, b, 13) - a @ b.T)
+    assert off.max() > 0 and (off <= 7 * 2.0**-13 * (np.abs(a[:, None]) * np.abs(b)).reshape(6, 9, -1, 8).max(-1).sum(-1)).all()
+
+
+def test_products_entry_point_refuses_fast_sums_of_fp32_outputs():
+    lib = _lib()
+    st = lib.spr_fp8_matmul_ex(16, 64, 16, 1, 0, 16, 64, 16, 1, 0, 4, 4, 64, None, 0, 2, 1, 16, None)
+    assert "fast sums are for outputs in 16 bits" in _refused(lib, st)
+
+
 def _refused(lib, st):
     assert st in (1, 3)
     return lib.spr_last_error().decode()
