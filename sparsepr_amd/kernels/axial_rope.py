@@ -55,7 +55,7 @@ def axial_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     axis int32 [R / 2] (axial_frequencies), R a multiple of 8.  An axis that the positions do not have gives NaN.
 
     `inverse` turns back: with the gradients of q' and k' it gives those of q and k.  Autograd does not record the
-    call: inputs that require a gradient are refused while it records."""
+    call: inputs that require a gradient are refused while it records, and those with a tangent."""
     what = "axial RoPE"
     dev = _lib.require_gpu(q, k, positions, freqs, axis, what=what)
     no_gradient(what, q, k, positions, freqs)

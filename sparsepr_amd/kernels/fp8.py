@@ -13,11 +13,12 @@ The products of a linear layer y = x W^T are all `fp8_matmul`, which sums along 
   dx  fp8_matmul(*fp8_quantize(dy), *fp8_quantize(w, square=True, transpose=True))
   dw  fp8_matmul(*fp8_quantize(dy, transpose=True), *fp8_quantize(x, transpose=True))
 Square blocks hold the same values either way round, so y and dx see one weight.  None of the functions
-is recorded by autograd: inputs that require a gradient are refused while it records."""
+is recorded by autograd: inputs that require a gradient are refused while it records, and those with a tangent."""
 
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -28,11 +29,16 @@ CODES = torch.float8_e4m3fn
 
 
 def no_gradient(what: str, *tensors: torch.Tensor | None) -> None:
-    """Refuse what autograd would lose without a word."""
+    """Refuse what autograd would lose without a word: gradients that it records, and tangents (forward mode; no_grad
+    does not stop those, so they are looked for wherever a level is open)."""
     for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
+        if t is None:
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{what}: autograd does not record this call; call it under torch.no_grad() and use the "
                                "gradient functions beside it")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what}: autograd's forward mode would lose a tangent in this call; give it the primal")
 
 
 def _packed_rows(x: torch.Tensor, rows: int, width: int) -> tuple[torch.Tensor, int]:
@@ -107,6 +113,7 @@ def fp8_dequantize(codes: torch.Tensor, scales: torch.Tensor, *, dtype: torch.dt
     range (fp16 rounds and overflows)."""
     what = "8-bit values"
     dev = _lib.require_gpu(codes, scales, what=what)
+    no_gradient(what, codes)
     rows, width, square = _check_matrix(codes, scales, what, "codes")
     code = _lib.DTYPE_CODE.get(dtype)
     if code is None:
@@ -134,7 +141,7 @@ def fp8_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     Rows that do not start on 16 bytes are copied first."""
     what = "8-bit product"
     dev = _lib.require_gpu(a, a_scales, b, b_scales, bias, what=what)
-    no_gradient(what, bias)
+    no_gradient(what, a, b, bias)
     m, k, a_square = _check_matrix(a, a_scales, what, "a")
     n, kb, b_square = _check_matrix(b, b_scales, what, "b")
     if k != kb:

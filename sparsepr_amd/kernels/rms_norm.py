@@ -8,7 +8,8 @@ what fp32 gives (zeros above 1.8e19, and with epsilon 0 infinities below 1e-23).
 residual are bf16, fp16 or fp32, the residual of x's type or fp32; the weight is [C] of x's type or fp32,
 or None.  Rows may have any strides as long as they are packed and their dims merge into two (a Q or K
 slice of a projection, seen by heads); others are copied.  None of the functions is recorded by autograd:
-inputs that require a gradient are refused while it records, and `rms_norm_backward` is the gradient."""
+inputs that require a gradient are refused while it records, and those with a tangent; `rms_norm_backward` is the
+gradient."""
 
 from __future__ import annotations
 

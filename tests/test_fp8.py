@@ -199,3 +199,27 @@ def test_functions_refuse_host_tensors_and_host_tables_are_right():
     for bad in (dict(axis_dims=(3, 4)), dict(axis_dims=(4,), theta=0.0), dict(axis_dims=(-2,))):
         with pytest.raises(RuntimeError, match="axial RoPE"):
             axial_frequencies(bad.pop("axis_dims"), device="cpu", **bad)
+
+
+def test_lost_gradients_are_found():
+    from torch.autograd import forward_ad
+
+    from sparsepr_amd.kernels.fp8 import no_gradient
+
+    x = torch.ones(2, 3)
+    leaf = x.clone().requires_grad_()
+    no_gradient("call", x, None, torch.zeros(2, dtype=torch.uint8))
+    for lost in (leaf, leaf[1:], leaf.to(torch.float8_e4m3fn)):
+        with pytest.raises(RuntimeError, match="call: autograd does not record"):
+            no_gradient("call", x, lost)
+    with torch.no_grad():
+        no_gradient("call", leaf)
+    with forward_ad.dual_level():
+        no_gradient("call", x, torch.zeros(2, dtype=torch.uint8))
+        dual = forward_ad.make_dual(x, x)
+        for lost in (dual, dual[1:], dual.to(torch.float8_e4m3fn)):
+            with pytest.raises(RuntimeError, match="call: autograd's forward mode"):
+                no_gradient("call", lost)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward mode"):
+                no_gradient("call", x, lost)
+        no_gradient("call", forward_ad.unpack_dual(dual).primal)

@@ -163,3 +163,36 @@ def test_refusals(dev):
         front(w[None, :, :32], torch.zeros(192, 1, device=dev))
     with pytest.raises(RuntimeError, match="positions must be"):
         front(w[None], torch.zeros(191, 1, device=dev))
+
+
+def test_inputs_whose_gradient_or_tangent_would_be_lost_are_refused(dev):
+    """Every tensor input of every function in front of the attention."""
+    from torch.autograd import forward_ad
+
+    from sparsepr_amd.kernels.axial_rope import axial_frequencies, axial_rope
+    from sparsepr_amd.kernels.fp8 import fp8_dequantize, fp8_matmul, fp8_quantize
+    from sparsepr_amd.kernels.rms_norm import rms_norm, rms_norm_backward, rms_norm_fp8
+    from sparsepr_amd.qkv_projection import QKVProjection
+
+    x, w, place = torch.randn(4, 64, device=dev), torch.ones(64, device=dev), torch.ones(4, 1, device=dev)
+    codes, scales = fp8_quantize(x)
+    freqs, axis = axial_frequencies((64,))
+    front = QKVProjection(torch.randn(192, 64, device=dev), heads=1, axis_dims=(64,))
+    calls = [(rms_norm, x, w), (lambda a, b, c: rms_norm(a, b, residual=c), x, w, x), (rms_norm_fp8, x, w),
+             (lambda a, b, c: rms_norm_fp8(a, b, residual=c), x, w, x),
+             (lambda a, b, c, d: rms_norm_backward(a, b, c, dsum=d), x, x, w, x), (fp8_quantize, x),
+             (lambda a: fp8_dequantize(a, scales), codes),
+             (lambda a, b, c: fp8_matmul(a, scales, b, scales, bias=c), codes, codes, w[:4]),
+             (lambda a, b, c, d: axial_rope(a, b, c, d, axis), x[None, None], x[None, None], place, freqs),
+             (lambda a, b: front(a, place, residual=b), x[None], x[None])]
+    for call, *given in calls:
+        call(*given)
+        for i, t in enumerate(given):
+            leaf = t.float().clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="autograd does not record"):
+                call(*given[:i], leaf.to(t.dtype), *given[i + 1:])
+            with forward_ad.dual_level():
+                call(*given)
+                dual = forward_ad.make_dual(t.float(), torch.ones_like(t, dtype=torch.float32)).to(t.dtype)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward mode"):
+                    call(*given[:i], dual, *given[i + 1:])
