@@ -61,8 +61,8 @@ class QKVProjection:
         codes, scales, *total = rms_norm_fp8(x, self.norm_weight, residual=residual, epsilon=self.epsilon)
         y = fp8_matmul(codes.flatten(0, 1), scales.flatten(0, 1), *self.weight, bias=self.bias, out_dtype=x.dtype,
                        fast_sums=self.fast_sums)
-        kv = self.kv_heads * self.head_dim
-        q, k, v = y.view(*x.shape[:2], -1).split((self.heads * self.head_dim, kv, kv), -1)
+        q_dims, kv_dims = self.heads * self.head_dim, self.kv_heads * self.head_dim
+        q, k, v = y.view(*x.shape[:2], q_dims + 2 * kv_dims).split((q_dims, kv_dims, kv_dims), -1)
         q, k = axial_rope(self._heads(q, self.heads, self.q_norm), self._heads(k, self.kv_heads, self.k_norm), positions,
                           self.freqs, self.axis, pairs=self.pairs)
         return q, k, self._heads(v, self.kv_heads, None), *total

@@ -196,3 +196,17 @@ def test_inputs_whose_gradient_or_tangent_would_be_lost_are_refused(dev):
                 dual = forward_ad.make_dual(t.float(), torch.ones_like(t, dtype=torch.float32)).to(t.dtype)
                 with torch.no_grad(), pytest.raises(RuntimeError, match="forward mode"):
                     call(*given[:i], dual, *given[i + 1:])
+
+
+@pytest.mark.parametrize("norms", [None, "head", "all"])
+@pytest.mark.parametrize("b,t", [(0, 150), (2, 0), (0, 0)])
+def test_no_batch_and_no_tokens(dev, b, t, norms):
+    h, hk, d = 4, 2, 64
+    qn, kn = (None if norms is None else torch.ones(d if norms == "head" else n * d, device=dev) for n in (h, hk))
+    front, *_ = _front(dev, 2, h, hk, d, 384, torch.bfloat16, axis_dims=(24, 20, 20), q_norm=qn, k_norm=kn)
+    x = torch.zeros(b, t, 384, device=dev, dtype=torch.bfloat16)
+    for places in (torch.zeros(t, 3, device=dev), torch.zeros(b, t, 3, device=dev)):
+        for residual in (None, x, x.float()):
+            q, k, v, *total = front(x, places, residual=residual)
+            assert q.shape == (b, h, t, d) and k.shape == v.shape == (b, hk, t, d) and v.dtype == x.dtype
+            assert [s.shape for s in total] == ([] if residual is None else [(b, t, 384)])
