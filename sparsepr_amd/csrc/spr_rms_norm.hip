@@ -218,7 +218,8 @@ __global__ __launch_bounds__(TPR == 0 ? 1024 : 256) void norm_backward_kernel(
     float total[2];  // (in 64 bits, as the norm's: 74 instead of 65 us on 8191 rows of 2560)
     row_total<TPR>(t, total, red);
     const float inv = static_cast<float>(inverse_rms(total[0], inv_width, eps));
-    const float along = inv * inv * (total[1] * static_cast<float>(inv_width));
+    // (inv^2 by itself leaves fp32's range where rows below 2^-64 are normed with no epsilon)
+    const float along = inv * (inv * (total[1] * static_cast<float>(inv_width)));
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int c = (lane + u * step) * 8;

@@ -240,3 +240,25 @@ def test_more_rows_than_an_entry_point_counts(dev):
     for call in (rms_norm, rms_norm_fp8, lambda t: rms_norm_backward(t, t)):
         with pytest.raises(RuntimeError, match="too many rows"):
             call(x)
+
+
+@pytest.mark.parametrize("scale", [2.0**-66, 2.0**-60, 2.0**56])
+@pytest.mark.parametrize("width", [64, 300, 2000])
+def test_gradient_of_very_small_and_large_rows(dev, width, scale):
+    """With no epsilon, where 1 / mean(s^2) is outside of fp32's range: at 2^-66 a square is about 2^-132, a subnormal
+    that is off by 2^-150, so the sum by 2^-18 of itself, the root by half and its cube by three halves of that."""
+    from sparsepr_amd.kernels.rms_norm import rms_norm_backward
+
+    dy = _x(width, (20, width), torch.float32, dev, 0.3)
+    g = torch.Generator(device=dev).manual_seed(3)
+    s = (1 + torch.rand(20, width, generator=g, device=dev)) * scale * torch.where(torch.rand(20, width, generator=g, device=dev) < 0.5, 1, -1)
+    w = torch.linspace(0.5, 1.5, width, device=dev)
+    dx, dw = rms_norm_backward(dy, s, w, epsilon=0.0)
+    y64, s64, w64 = _f64(dy), _f64(s), _f64(w)
+    want_x, want_w = model.norm_backward(y64, s64, w64, 0.0, 0.0)
+    r = 1.0 / np.sqrt((s64 * s64).mean(-1, keepdims=True))
+    g = np.abs(y64 * w64)
+    size = r * (g + np.abs(s64) * r * r * (g * np.abs(s64)).mean(-1, keepdims=True))
+    low = 2.0**-17 if scale < 2.0**-63 else 0.0
+    assert (np.abs(_f64(dx) - want_x) <= (97 * F32 + low) * size).all()
+    assert (np.abs(_f64(dw) - want_w) <= (84 * F32 + low) * np.abs(y64 * s64 * r).sum(0)).all()
