@@ -24,7 +24,7 @@ from .. import _lib
 
 BLOCK = 128
 MAX_SIZE = 1 << 30  # of a dim: the entry points count columns in 32 bits
-MAX_SUM = 1 << 22  # terms of a product
+MAX_SUM = 1 << 22  # terms of a product, and bytes from row to row
 CODES = torch.float8_e4m3fn
 
 
@@ -68,12 +68,14 @@ def _check_matrix(codes: torch.Tensor, scales: torch.Tensor, what: str, name: st
     return rows, width, int(shape[0] != rows)
 
 
-def _as_read(codes: torch.Tensor, scales: torch.Tensor, rows: int, width: int) -> tuple[torch.Tensor, int, torch.Tensor, int]:
-    """Codes with packed rows that start on 16 bytes and scales with packed rows, and their row strides."""
+def _as_read(codes: torch.Tensor, scales: torch.Tensor, rows: int, width: int,
+             most: int = 1 << 62) -> tuple[torch.Tensor, int, torch.Tensor, int]:
+    """Codes with packed rows that start on 16 bytes, at most `most` bytes apart, and scales with packed rows, and their
+    row strides."""
     ld, packed = codes.stride()
     if rows == 1:
         ld = width
-    if packed != 1 or ld % 16 != 0 or ld < width or codes.data_ptr() % 16 != 0:  # (the width is 16 or more)
+    if packed != 1 or ld % 16 != 0 or not width <= ld <= most or codes.data_ptr() % 16 != 0:  # (the width is 16 or more)
         codes, ld = codes.clone(memory_format=torch.contiguous_format), width
     scales_ld, packed = scales.stride()
     if packed != 1 and width > BLOCK:
@@ -138,7 +140,7 @@ def fp8_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     are fp32).  What it cuts is 5e-5 of the norm on normal rows, a thirtieth of bf16's own rounding and a quarter
     of fp16's; where large products cancel it may be all of an output.
 
-    Rows that do not start on 16 bytes are copied first."""
+    Codes whose rows are not packed, do not start on 16 bytes or are more than 2^22 bytes apart are copied first."""
     what = "8-bit product"
     dev = _lib.require_gpu(a, a_scales, b, b_scales, bias, what=what)
     no_gradient(what, a, b, bias)
@@ -164,8 +166,8 @@ def fp8_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     if k == 0:  # (no rows that a weight's gradient would be summed over)
         return out.zero_() if bias is None else out.copy_(bias)
     if m > 0 and n > 0:
-        a, a_ld, a_scales, a_scales_ld = _as_read(a, a_scales, m, k)
-        b, b_ld, b_scales, b_scales_ld = _as_read(b, b_scales, n, k)
+        a, a_ld, a_scales, a_scales_ld = _as_read(a, a_scales, m, k, MAX_SUM)
+        b, b_ld, b_scales, b_scales_ld = _as_read(b, b_scales, n, k, MAX_SUM)
         _lib.launch("spr_fp8_matmul_ex", dev, a.data_ptr(), a_ld, a_scales.data_ptr(), a_scales_ld, a_square, b.data_ptr(),
                     b_ld, b_scales.data_ptr(), b_scales_ld, b_square, m, n, k, bias_at, bias_code, code, int(fast_sums),
                     out.data_ptr())

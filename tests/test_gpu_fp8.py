@@ -367,3 +367,21 @@ def test_one_row_on_more_columns_than_a_launch_of_few_rows_has(dev):
 def test_products_of_few_tiles_whose_waves_share_the_sum_are_exact(dev, m, n, k):
     """Odd and even counts of blocks between two groups of waves, more of them than a window of scales holds."""
     test_products_on_tiles_of_every_size_are_exact(dev, m, n, k)
+
+
+def test_a_sum_in_parts_that_one_call_does_not_take(dev):
+    """Columns of codes whose rows are further apart than an entry point takes: a sum of 2^22 + 272 terms as two."""
+    from sparsepr_amd.kernels.fp8 import fp8_matmul
+
+    m, n, k, half = 40, 3, 2**22 + 272, 2**21
+    g = torch.Generator(device=dev).manual_seed(5)
+    a, b = (torch.randint(-1, 2, (r, k), generator=g, device=dev).to(torch.float8_e4m3fn) for r in (m, n))
+    sa, sb = (torch.full((r, -(-k // 128)), 127, dtype=torch.uint8, device=dev) for r in (m, n))
+    parts = [fp8_matmul(a[:, p], sa[:, s], b[:, p], sb[:, s], out_dtype=torch.float32)
+             for p, s in ((slice(0, half), slice(0, half // 128)), (slice(half, k), slice(half // 128, None)))]
+    assert torch.equal(parts[0] + parts[1], a.float() @ b.float().t())  # whole numbers below 2^24
+    for last in (0, 16, 128):  # one row of them, narrow columns at the end
+        p = slice(k - 128 - last, k - last)
+        for rows in (slice(0, 1), slice(5, 8)):
+            got = fp8_matmul(a[rows, p], sa[rows, :1], b[:, p], sb[:, :1], out_dtype=torch.float32)
+            assert torch.equal(got, a[rows, p].float() @ b[:, p].float().t())
