@@ -623,7 +623,8 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Matrix a, Matrix b
 //   300 x 1536 x 8960                 45.6      29.6     22.7        19.0
 //   64 x 500 x 14,000       130       67.5      42.8     31.3        25.7      31.4
 //   1000 x 1000 x 1008     16.2        9.3       7.3      6.1         6.2
-enum Kernel { LARGE, MIDDLE, SMALL, TINY, TINY2, FEW };
+constexpr int64_t MOST_TILES = int64_t(1) << 22;  // of a launch, below: 512 threads each, and their count is 32 bits
+enum Kernel { LARGE, MIDDLE, SMALL, TINY, TINY2, FEW, NONE };
 struct Cost {
   int32_t tm, tn, full, start, all, most, some;
 };
@@ -639,11 +640,13 @@ Kernel pick_kernel(int64_t M, int64_t N, int32_t K, bool wide) {
                                     {64, 64, 512, 200, 95, 80, 45},
                                     {64, 64, 256, 300, 55, 50, 36}}};
   const int64_t blocks = spr::ceil_div(K, KB);
-  Kernel best = LARGE;
+  Kernel best = NONE;
   int64_t least = INT64_MAX;
   for (int i = 0; i < 5; ++i) {
     const Cost& c = costs[wide ? 1 : 0][i];
     const int64_t tiles = spr::ceil_div(M, c.tm) * spr::ceil_div(N, c.tn), rest = tiles % c.full;
+    // (256 x 256 for 64 rows or columns is three quarters empty, and what no other tile takes is refused)
+    if (tiles >= MOST_TILES || (i == LARGE && (M <= 64 || N <= 64))) continue;
     const int64_t cost = spr::ceil_div(tiles, c.full) * c.start +
                          blocks * (tiles / c.full * c.all + (rest == 0 ? 0 : 2 * rest > c.full ? c.most : c.some));
     if (cost < least) least = cost, best = static_cast<Kernel>(i);
@@ -663,8 +666,8 @@ template <int DT, bool WIDE>
 int launch_product(const Matrix& a, const Matrix& b, int32_t K, const Output& o, hipStream_t stream) {
   const int32_t M = a.rows, N = b.rows;
   const Kernel kernel = pick_kernel(M, N, K, WIDE);
+  SPR_REQUIRE(kernel != NONE, "spr_fp8_matmul: too many outputs");
   if (kernel == FEW) {
-    SPR_REQUIRE(N < (1 << 27), "spr_fp8_matmul: too many outputs");  // 2^32 threads of a launch
     const uint32_t grid = static_cast<uint32_t>(spr::ceil_div(N, 16));
     if (M <= 16) few_rows_kernel<DT, WIDE, 1, 8><<<grid, 512, 0, stream>>>(a, b, K, o);
     else if (M <= 32) few_rows_kernel<DT, WIDE, 2, 8><<<grid, 512, 0, stream>>>(a, b, K, o);
@@ -674,7 +677,6 @@ int launch_product(const Matrix& a, const Matrix& b, int32_t K, const Output& o,
   }
   const int64_t tm = spr::ceil_div(M, kernel == LARGE ? 256 : kernel == MIDDLE ? 128 : 64);
   const int64_t tn = spr::ceil_div(N, kernel == LARGE ? 256 : kernel >= TINY ? 64 : 128);
-  SPR_REQUIRE(tm * tn < (int64_t(1) << 22), "spr_fp8_matmul: too many outputs");
   const uint32_t grid = static_cast<uint32_t>(tm * tn);
   const int32_t rows = static_cast<int32_t>(tm), columns = static_cast<int32_t>(tn);
   if (kernel == MIDDLE) {

@@ -385,3 +385,23 @@ def test_a_sum_in_parts_that_one_call_does_not_take(dev):
         for rows in (slice(0, 1), slice(5, 8)):
             got = fp8_matmul(a[rows, p], sa[rows, :1], b[:, p], sb[:, :1], out_dtype=torch.float32)
             assert torch.equal(got, a[rows, p].float() @ b[:, p].float().t())
+
+
+@pytest.mark.parametrize("fast", [False, True])
+def test_more_rows_than_the_fastest_kernels_launch_takes(dev, fast):
+    """2^22 tiles of 128 x 128, the kernel that such a shape would get by its time: 2^21 of 256 x 256 do it."""
+    from sparsepr_amd.kernels.fp8 import fp8_matmul
+
+    m, n = 2**29, 65
+    if torch.cuda.mem_get_info()[0] < 100 * 2**30:
+        pytest.skip("needs 80 GB")
+    a = torch.zeros(m, 16, dtype=torch.uint8, device=dev)
+    a[-300:] = a[m // 2] = 0x38  # 1.0
+    b = torch.full((n, 16), 0x38, dtype=torch.uint8, device=dev)
+    scale = torch.full((1, 1), 127, dtype=torch.uint8, device=dev)
+    y = fp8_matmul(a.view(torch.float8_e4m3fn), scale.expand(m, 1), b.view(torch.float8_e4m3fn), scale.expand(n, 1), fast_sums=fast)
+    assert (y[-300:] == 16).all() and (y[m // 2] == 16).all()
+    for i in (0, m // 4, m // 2 - 5000, m // 2 + 1, m - 5300):
+        assert not y[i:i + 5000].any()
+    del a, y
+    torch.cuda.empty_cache()
