@@ -606,39 +606,42 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Matrix a, Matrix b
 
 // Which kernel: by what the whole call takes, in hundredths of a microsecond, from measured times of a block
 // of the summed dim while the chip is full of tiles (`full` of them), more than half full or less.  In us, outputs in
-// 16 bits, K = 5120 where none is given:
-//                     256 x 256  128 x 128  64 x 128  64 x 64  two groups  few rows
-//   1 x 5120                          26.7      17.9     13.2        11.5      10.1
-//   1 x 15,360                        28.4      19.0     15.1        14.8      18.2
-//   16 x 5120                         26.7      18.1     13.3        11.7      14.2
-//   64 x 15,360                       30.8      20.4     16.0        15.8      55.0
-//   512 x 5120             51.4       33.0      29.1     33.9        38.0
-//   1024 x 5120            52.1       41.9      47.3     54.6        63.8
-//   2048 x 5120            53.5       67.7      68.9     92.0
-//   4096 x 5120             116        108       139      180
-//   32,760 x 5120           643        816      1072     1413
-//   333 x 5000 x 4112      45.6       28.4      18.9     24.1        24.4
-//   100 x 2560 x 2560      27.4       15.8      11.1      8.5         7.8
-//   77 x 4096 x 4096                  21.7      15.1     11.2         9.6
-//   300 x 1536 x 8960                 45.6      29.6     22.7        19.0
-//   64 x 500 x 14,000       130       67.5      42.8     31.3        25.7      31.4
-//   1000 x 1000 x 1008     16.2        9.3       7.3      6.1         6.2
+// bf16, sums in fp32 / fast, K = 5120 where none is given; of each pair the rule's pick is marked:
+//                      256 x 256     128 x 128     64 x 128      64 x 64       two groups    few rows
+//   1 x 5120                         43   / 26     29   / 18     22   / 13     18   / 11     10*  / 10*
+//   1 x 15,360                       43   / 28     29   / 19     23   / 15*    19   / 15     19*  / 18
+//   16 x 5120                        42   / 27     29   / 18     22   / 13     18   / 12*    14*  / 14
+//   64 x 15,360        107  / 50     44   / 31     30   / 20     24   / 16*    20*  / 16     56
+//   512 x 5120         109  / 53     47*  / 33     46   / 28*    50   / 32     54   / 36
+//   1024 x 5120        108  / 53     71*  / 39*    68   / 44     77   / 50     87   / 59
+//   2048 x 5120        110  / 55*    107* / 69     110  / 69     150  / 95     175  / 116
+//   4096 x 5120        228  / 117    178* / 106*   226  / 140    294  / 181    346  / 230
+//   32,760 x 5120      1209*/ 676*   1392 / 868    1708 / 1091   2280 / 1441   2748 / 1845
+//   333 x 5000 x 4112  95   / 46     39   / 28     27*  / 18*    29   / 23     33   / 23
+//   100 x 2560 x 2560  55   / 28     24   / 16     16   / 11     13   / 8      11*  / 8*
+//   77 x 4096 x 4096   85   / 39     35   / 22     24   / 15     18   / 11     15*  / 10*
+//   300 x 1536 x 8960  183  / 86     73   / 46     48   / 30     37   / 23     30*  / 19*
+//   64 x 500 x 14,000  280  / 129    111  / 68     72   / 43     55   / 31     43   / 26*    32*
+//   1000 x 1000 x 1008 27   / 16     12   / 9      9    / 7      8    / 6*     7*   / 6
+//   4095 x 2560 x 2560 60   / 33*    57*  / 39     59   / 39     78   / 50     99   / 68
+//   2560 x 2560 x 4096 88   / 44     56*  / 31*    68   / 38     81   / 48     94   / 60
+// (fp32 outputs take up to 5 % longer than bf16 ones.)
 constexpr int64_t MOST_TILES = int64_t(1) << 22;  // of a launch, below: 512 threads each, and their count is 32 bits
 enum Kernel { LARGE, MIDDLE, SMALL, TINY, TINY2, FEW, NONE };
 struct Cost {
   int32_t tm, tn, full, start, all, most, some;
 };
 Kernel pick_kernel(int64_t M, int64_t N, int32_t K, bool wide) {
-  static const Cost costs[2][5] = {{{256, 256, 256, 600, 168, 165, 139},
+  static const Cost costs[2][5] = {{{256, 256, 256, 600, 160, 130, 120},
                                     {128, 128, 512, 300, 95, 80, 70},
                                     {64, 128, 512, 200, 71, 57, 43},
                                     {64, 64, 512, 200, 55, 50, 30},
                                     {64, 64, 256, 300, 30, 29, 21}},
-                                   {{256, 256, 256, 600, 335, 320, 306},
-                                    {128, 128, 512, 300, 184, 170, 160},
-                                    {64, 128, 512, 200, 117, 110, 84},
-                                    {64, 64, 512, 200, 95, 80, 45},
-                                    {64, 64, 256, 300, 55, 50, 36}}};
+                                   {{256, 256, 256, 600, 287, 270, 257},
+                                    {128, 128, 512, 300, 167, 169, 98},
+                                    {64, 128, 512, 200, 105, 105, 70},
+                                    {64, 64, 512, 200, 68, 80, 52},
+                                    {64, 64, 256, 300, 38, 43, 38}}};
   const int64_t blocks = spr::ceil_div(K, KB);
   Kernel best = NONE;
   int64_t least = INT64_MAX;
