@@ -5,8 +5,12 @@
     q, k, v, x = front(y, positions, residual=x)       # x + y normed to 8 bits, projected, Q and K turned by place
     out = SparsePRAttention(config)(q, k, v)
 
+The norm of the hidden rows is the root-mean-square one.  With another norm in front (a layer norm with a scale and a
+shift by time step, as Wan's blocks have it), `norm=False` takes rows as the caller has normed them.
+
 The hidden rows are read once between the residual's addition and the 8-bit product; nothing is rounded to 16
-bits in between.  All calls are kernels/rms_norm.py's, kernels/fp8.py's and kernels/axial_rope.py's, on torch's
+bits in between.  The product's outputs are rounded to x's type, Q and K again where they are normed and where they
+are turned.  All calls are kernels/rms_norm.py's, kernels/fp8.py's and kernels/axial_rope.py's, on torch's
 current stream; none waits for the GPU, and a captured graph replays what an eager call does."""
 
 from __future__ import annotations
@@ -22,18 +26,22 @@ class QKVProjection:
     def __init__(self, weight: torch.Tensor, *, heads: int, kv_heads: int | None = None, axis_dims, theta: float = 10000.0,
                  pairs: str = "interleaved", norm_weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                  q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, epsilon: float = 1e-6,
-                 fast_sums: bool = False):
+                 fast_sums: bool = False,
+                 norm: bool = True):
         """weight [(heads + 2 kv_heads) D, C]: the rows of Q, then K, then V, quantised here once (128 x 128 blocks).
         norm_weight [C] and bias as in rms_norm and fp8_matmul.  q_norm and k_norm norm Q and K before they are
         turned: [D] every head by itself, [heads * D] all channels together.  axis_dims: the rotated dims of each
-        axis of the positions (axial_frequencies).  fast_sums: the product's (fp8_matmul)."""
+        axis of the positions (axial_frequencies).  fast_sums: the product's (fp8_matmul).  norm False:
+        x has been normed, and is quantised as it is."""
         kv_heads = heads if kv_heads is None else kv_heads
         what = "QKV projection"
         if heads < 1 or kv_heads < 1 or heads % kv_heads != 0:
             raise RuntimeError(f"{what}: {heads} query heads on {kv_heads} kv heads")
         if weight.dim() != 2 or weight.shape[0] % (heads + 2 * kv_heads) != 0 or weight.numel() == 0:
             raise RuntimeError(f"{what}: weight {tuple(weight.shape)} is not [({heads} + 2 * {kv_heads}) D, C]")
-        self.heads, self.kv_heads = heads, kv_heads
+        if norm_weight is not None and not norm:
+            raise RuntimeError(f"{what}: norm_weight is for a norm of x, which norm=False leaves to the caller")
+        self.heads, self.kv_heads, self.norm = heads, kv_heads, norm
         self.head_dim = weight.shape[0] // (heads + 2 * kv_heads)
         for t, h, name in ((q_norm, heads, "q_norm"), (k_norm, kv_heads, "k_norm")):
             if t is not None and t.shape not in ((self.head_dim,), (h * self.head_dim,)):
@@ -58,8 +66,15 @@ class QKVProjection:
         and with a residual the sum x + residual as well."""
         if x.dim() != 3 or x.shape[2] != self.width:
             raise RuntimeError(f"QKV projection: x must be [B, T, {self.width}], got {tuple(x.shape)}")
-        codes, scales, *total = rms_norm_fp8(x, self.norm_weight, residual=residual, epsilon=self.epsilon)
-        y = fp8_matmul(codes.flatten(0, 1), scales.flatten(0, 1), *self.weight, bias=self.bias, out_dtype=x.dtype,
+        if not self.norm and residual is not None:
+            raise RuntimeError("QKV projection: a residual is added in front of the norm, which norm=False leaves to the caller")
+        total = []
+        if self.norm:
+            codes, scales, *total = rms_norm_fp8(x, self.norm_weight, residual=residual, epsilon=self.epsilon)
+            codes, scales = codes.flatten(0, 1), scales.flatten(0, 1)
+        else:
+            codes, scales = fp8_quantize(x.flatten(0, 1))
+        y = fp8_matmul(codes, scales, *self.weight, bias=self.bias, out_dtype=x.dtype,
                        fast_sums=self.fast_sums)
         q_dims, kv_dims = self.heads * self.head_dim, self.kv_heads * self.head_dim
         q, k, v = y.view(*x.shape[:2], q_dims + 2 * kv_dims).split((q_dims, kv_dims, kv_dims), -1)

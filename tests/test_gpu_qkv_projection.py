@@ -210,3 +210,40 @@ def test_no_batch_and_no_tokens(dev, b, t, norms):
             q, k, v, *total = front(x, places, residual=residual)
             assert q.shape == (b, h, t, d) and k.shape == v.shape == (b, hk, t, d) and v.dtype == x.dtype
             assert [s.shape for s in total] == ([] if residual is None else [(b, t, 384)])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rows_that_the_caller_has_normed(dev, dtype):
+    """A layer norm with a scale and a shift per batch in front, as the operators one by one give it, and replayed."""
+    from sparsepr_amd.kernels.axial_rope import axial_rope
+    from sparsepr_amd.kernels.fp8 import fp8_matmul, fp8_quantize
+    from sparsepr_amd.qkv_projection import QKVProjection
+
+    h, hk, d, width = 4, 2, 64, 500
+    g = torch.Generator(device=dev).manual_seed(6)
+    w = (torch.randn((h + 2 * hk) * d, width, generator=g, device=dev) / width**0.5).to(dtype)
+    x, scale, shift = (torch.randn(2, n, width, generator=g, device=dev).to(dtype) for n in (150, 1, 1))
+    x = torch.nn.functional.layer_norm(x, (width,)) * (1 + scale) + shift
+    front = QKVProjection(w, heads=h, kv_heads=hk, axis_dims=(24, 20, 20), norm=False)
+    places = torch.randint(0, 500, (150, 3), generator=g, device=dev)
+    q, k, v = front(x, places)
+    codes, scales = fp8_quantize(x.view(300, width))
+    y = fp8_matmul(codes, scales, *fp8_quantize(w, square=True), out_dtype=dtype).view(2, 150, -1)
+    want_q, want_k, want_v = (t.unflatten(-1, (-1, d)).transpose(1, 2) for t in y.split((h * d, hk * d, hk * d), -1))
+    want_q, want_k = axial_rope(want_q, want_k, places, front.freqs, front.axis)
+    assert torch.equal(q, want_q) and torch.equal(k, want_k) and torch.equal(v, want_v)
+    assert all(torch.equal(a, b) for a, b in zip(front(x.transpose(0, 1).contiguous().transpose(0, 1), places), (q, k, v)))
+    assert front(x[:0], places)[2].shape == (0, hk, 150, d) and front(x[:, :0], places[:0])[0].shape == (2, h, 0, d)
+    buffer, graph = x.clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = front(buffer, places)
+    for t in (x, 2 * x, x.flip(1)):
+        eager = front(t, places)
+        buffer.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+    with pytest.raises(RuntimeError, match="a residual is added in front of the norm"):
+        front(x, places, residual=x)
+    with pytest.raises(RuntimeError, match="norm_weight is for a norm of x"):
+        QKVProjection(w, heads=h, kv_heads=hk, axis_dims=(64,), norm=False, norm_weight=w[0])
