@@ -1,4 +1,4 @@
-"""How the 8-bit product adds, on every kernel that its rule picks.
+"""The 8-bit product on every kernel that its rule picks: how it adds, what it reads and where it writes.
 
 With sums in fp32 (the default) rows are built so that the 8-bit matrix instruction would lose every digit of the
 result: of eight neighbouring products one is 2^12, which the next eight take off again, and seven are 2^-2, 2^-14 of
@@ -18,8 +18,9 @@ pytestmark = pytest.mark.gpu
 
 DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 HALF = {t: torch.finfo(t).eps / 2 for t in DT.values()}
-# 256 x 256 tiles, 128 x 128, 64 x 128, 64 x 64, 64 x 64 with two groups of waves, few rows (16, 32, 64 of them); each
-# with a last block and last tiles that are not whole
+# Tiles of 256 x 256, 128 x 128, 64 x 128 (two sizes, the first with sums in fp32 128 x 128), 64 x 64 (two, the second
+# with sums in fp32 two groups of waves), two groups (two), few rows (16, 32 and, with sums in fp32, 64); each
+# with a last block and last tiles that are not whole.
 SIZES = [(4000, 3500, 272), (2100, 2300, 784), (500, 5000, 4240), (700, 1800, 528), (513, 260, 400), (90, 5000, 8208),
          (300, 1500, 8208), (70, 100, 4496), (1, 500, 4112), (17, 33, 5136), (60, 32, 12048)]
 
@@ -106,3 +107,79 @@ def test_values_are_multiplied_as_bf16_holds_them(dev, byte):
             assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(got.isnan(), want.isnan())
             full = fp8_dequantize(codes[r], scales[r], dtype=torch.float32)[:, 3:4].expand(-1, n)
             assert not 3 <= byte <= 246 or torch.equal(got.nan_to_num(7.0), full.nan_to_num(7.0))
+
+
+WAYS = [(out, fast) for out in DT.values() for fast in (False, True) if not (fast and out is torch.float32)]
+
+
+def _spread(scales, rows, k):
+    """The scales of every value, in 64 bits."""
+    s = torch.where(scales == 255, torch.nan, torch.exp2(scales.double() - 127))
+    s = s if len(scales) == rows else s.repeat_interleave(128, 0)[:rows]
+    return s.repeat_interleave(128, 1)[:, :k]
+
+
+@pytest.mark.parametrize("squares", [(False, True), (True, False)])
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_rows_and_scales_inside_others(dev, m, n, k, squares):
+    """Codes and scales as slices of larger tensors that hold NaN in front of, behind and between them: whole numbers up
+    to 4 at scales up to 4, whose sums are exact in any order."""
+    from sparsepr_amd.kernels.fp8 import fp8_matmul
+
+    g = torch.Generator(device=dev).manual_seed(n)
+    sides = []
+    for rows, square, gap in ((m, squares[0], 48), (n, squares[1], 16)):
+        whole = torch.full((rows + 3, k + gap + 16), 0x7F, dtype=torch.uint8, device=dev)
+        codes = torch.randint(-2, 3, (rows, k), generator=g, device=dev).to(torch.float8_e4m3fn)
+        whole[2:-1, 16:16 + k] = codes.view(torch.uint8)
+        blocks, groups = -(-k // 128), -(-rows // 128) if square else rows
+        around = torch.full((groups + 3, blocks + 5), 255, dtype=torch.uint8, device=dev)
+        around[1:-2, 3:-2] = torch.randint(126, 129, (groups, blocks), generator=g, device=dev)
+        sides.append((whole.view(torch.float8_e4m3fn)[2:-1, 16:16 + k], around[1:-2, 3:-2]))
+    (a, sa), (b, sb) = sides
+    want = (a.float() * _spread(sa, m, k).float()) @ (b.float() * _spread(sb, n, k).float()).t()
+    for out, fast in WAYS:
+        assert torch.equal(fp8_matmul(a, sa, b, sb, out_dtype=out, fast_sums=fast), want.to(out))
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_nan_and_the_ends_of_the_scales(dev, m, n, k):
+    """A NaN code or scale reaches its row or column and nothing else; scales of 2^127 and 2^-127 meet.  (Results below
+    2^-100 are flushed or not.)"""
+    from sparsepr_amd.kernels.fp8 import fp8_matmul
+
+    g = torch.Generator(device=dev).manual_seed(k)
+    blocks = -(-k // 128)
+    (a, sa), (b, sb) = ((torch.randint(0, 3, (r, k), generator=g, device=dev).to(torch.float8_e4m3fn).view(torch.uint8),
+                         torch.full((r, blocks), 127, dtype=torch.uint8, device=dev)) for r in (m, n))
+    one = 0x38
+    a[0] = b[:2] = one
+    sa[0], sb[1] = 254, 0  # 2^127 and 2^-127
+    if m > 1:
+        a[1], sa[1], sb[0] = one, 1, 253  # 2^-126 and 2^126
+    if m > 4:
+        a[m - 1, k - 1], sa[m - 2, blocks - 1], a[m // 2, 0] = 0x7F, 255, 0xFF
+    b[n - 1, k - 1], sb[n - 2, blocks - 1], b[n // 2, 17] = 0xFF, 255, 0x7F
+    a, b = a.view(torch.float8_e4m3fn), b.view(torch.float8_e4m3fn)
+    want = (a.double() * _spread(sa, m, k)) @ (b.double() * _spread(sb, n, k)).t().contiguous()
+    assert want[0, 1] == k and want.isnan().any(0).sum() == (n if m > 4 else 3)
+    low = want.abs() < 2.0**-100
+    for out, fast in WAYS:
+        got = fp8_matmul(a, sa, b, sb, out_dtype=out, fast_sums=fast)
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(torch.where(low, 0, got).nan_to_num(7.0, 9.0), torch.where(low, 0, want).to(out).nan_to_num(7.0, 9.0))
+        assert (got[low].double().abs() <= 2.0**-99).all()
+
+
+@pytest.mark.parametrize("m,n", [(32900, 4112), (32771, 4099)])
+def test_outputs_that_the_caches_do_not_hold(dev, m, n):
+    """Above 256 MB in 16 bits, every value of them, rows that start on 16 bytes or anywhere."""
+    from sparsepr_amd.kernels.fp8 import fp8_matmul
+
+    g, k = torch.Generator(device=dev).manual_seed(m), 272
+    a, b = (torch.randint(-2, 3, (r, k), generator=g, device=dev).to(torch.float8_e4m3fn) for r in (m, n))
+    sa, sb = (torch.randint(126, 129, (r, 3), generator=g, device=dev).to(torch.uint8) for r in (m, -(-n // 128)))
+    want = (a.float() * _spread(sa, m, k).float()) @ (b.float() * _spread(sb, n, k).float()).t()
+    assert m * n * 2 > 256 << 20
+    for out, fast in WAYS:
+        assert torch.equal(fp8_matmul(a, sa, b, sb, out_dtype=out, fast_sums=fast), want.to(out))

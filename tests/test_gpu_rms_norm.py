@@ -262,3 +262,22 @@ def test_gradient_of_very_small_and_large_rows(dev, width, scale):
     low = 2.0**-17 if scale < 2.0**-63 else 0.0
     assert (np.abs(_f64(dx) - want_x) <= (97 * F32 + low) * size).all()
     assert (np.abs(_f64(dw) - want_w) <= (84 * F32 + low) * np.abs(y64 * s64 * r).sum(0)).all()
+
+
+@pytest.mark.parametrize("width", [1, 16, 100, 128, 300, 512, 640, 2050, 5120, 16384])
+def test_an_output_is_rounded_once(dev, width):
+    """Whole numbers up to 8, whose squares add up exactly: the root is then 64 bits, and what is left is the rounding
+    of s r w to fp32, at most half a step of the output (2^-44 of it more, from the root's and the products' low parts)."""
+    from sparsepr_amd.kernels.rms_norm import rms_norm
+
+    rng = np.random.default_rng(width)
+    s = torch.from_numpy(rng.integers(1, 9, (60, width)) * rng.choice([-1.0, 1.0], (60, width)))
+    w = torch.from_numpy(rng.uniform(0.5, 2.0, width).astype(np.float32))
+    want = model.norm(_f64(s), _f64(w), 2.0**-20)
+    half = np.spacing(np.abs(want).astype(np.float32)).astype(np.float64) / 2
+    got = _f64(rms_norm(s.float().to(dev), w.to(dev), epsilon=2.0**-20))
+    assert (np.abs(got - want) <= half + 2.0**-44 * np.abs(want)).all()
+    # a residual of the same numbers: the sum is exact too
+    y, total = rms_norm(torch.zeros(60, width, dtype=torch.float16, device=dev), w.to(dev), residual=s.half().to(dev), epsilon=2.0**-20)
+    assert torch.equal(total.cpu(), s.half())
+    assert (np.abs(_f64(y) - want) <= (HALF[torch.float16] + F32) * np.abs(want) * (1 + 2.0**-10)).all()
