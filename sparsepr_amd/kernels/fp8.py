@@ -25,6 +25,8 @@ from .. import _lib
 BLOCK = 128
 MAX_SIZE = 1 << 30  # of a dim: the entry points count columns in 32 bits
 MAX_SUM = 1 << 22  # terms of a product, and bytes from row to row
+ROWS = (1 << 24) - 1  # that one launch quantises, with scales of their own
+GROUPS = (1 << 28) - 65  # of 128 values, the same
 CODES = torch.float8_e4m3fn
 
 
@@ -88,8 +90,8 @@ def fp8_quantize(x: torch.Tensor, *, square: bool = False, transpose: bool = Fal
     """x [R, C] in bf16, fp16 or fp32 -> (codes, scales), see the module's text.
 
     `square`: one scale for 128 x 128 values, else for 128 values of a row.  `transpose`: the 8-bit matrix
-    of x^T, codes [C, R rounded up to 16], its groups along x's columns.  R is below 2^24, with either at most
-    65535 * 128."""
+    of x^T, codes [C, R rounded up to 16], its groups along x's columns.  R and C are at most 2^30, with either R
+    at most 65535 * 128 and R C / 128 below 2^28.  Without them more than 2^24 rows take several launches."""
     what = "8-bit quantisation"
     dev = _lib.require_gpu(x, what=what)
     no_gradient(what, x)
@@ -105,8 +107,14 @@ def fp8_quantize(x: torch.Tensor, *, square: bool = False, transpose: bool = Fal
     scales = x.new_empty((-(-rows // BLOCK) if square else rows, -(-width // BLOCK)), dtype=torch.uint8)
     if height > 0 and across > 0:
         x, ld = _packed_rows(x, height, across)
-        _lib.launch("spr_fp8_quantize", dev, x.data_ptr(), ld, height, across, code, int(square), int(transpose),
-                    codes.data_ptr(), scales.data_ptr())
+        groups = -(-across // BLOCK)
+        step = height
+        if not square and not transpose and (height > ROWS or height * groups > GROUPS):
+            step = min(ROWS, GROUPS // groups)
+        for r in range(0, height, step):
+            _lib.launch("spr_fp8_quantize", dev, x.data_ptr() + r * ld * x.element_size(), ld, min(step, height - r), across,
+                        code, int(square), int(transpose), codes.data_ptr() + r * codes.shape[1],
+                        scales.data_ptr() + r * groups)
     return codes, scales
 
 

@@ -405,3 +405,20 @@ def test_more_rows_than_the_fastest_kernels_launch_takes(dev, fast):
         assert not y[i:i + 5000].any()
     del a, y
     torch.cuda.empty_cache()
+
+
+def test_more_rows_than_one_launch_quantises(dev):
+    """Rows with scales of their own: past 2^24 of them, packed and with a stride, and past 2^28 groups."""
+    from sparsepr_amd.kernels.fp8 import fp8_quantize
+
+    for rows, width, stride in ((2**24 + 1000, 16, 24), (2**24 - 1, 8, 8), (2**24, 8, 8), (2**28 + 5, 4, 0)):
+        x = torch.arange(max(1, (rows if stride else 1) * stride // 8), device=dev)[:, None] % 1021 - 500 + torch.arange(8, device=dev)
+        x = x.to(torch.bfloat16).flatten().as_strided((rows, width), (stride, 1))
+        codes, scales = fp8_quantize(x)
+        assert codes.shape == (rows, 16) and scales.shape == (rows, 1)
+        for part in (slice(0, 100), slice(2**24 - 60, min(rows, 2**24 + 60)), slice(rows - 100, rows)):
+            c, s = fp8_quantize(x[part].clone())
+            assert torch.equal(codes[part].view(torch.uint8), c.view(torch.uint8)) and torch.equal(scales[part], s)
+        if stride == 0:
+            assert (codes.view(torch.uint8) == codes[0].view(torch.uint8)).all() and (scales == scales[0]).all()
+    torch.cuda.empty_cache()
