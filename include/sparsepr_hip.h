@@ -594,7 +594,8 @@ int spr_kv4_attention(const void* q, int64_t q_b, int64_t q_h, int64_t q_t, int3
 
 /* ---------------------------------------------------------------- norm of the hidden rows
  * No counterpart in the reference: what its model blocks leave to torch in front of the QKV projection.
- * x [n0, n1, width] of dtype with strides x_s0, x_s1 (elements) and packed rows; width 1 .. 16384.
+ * x [n0, n1, width] of dtype with strides x_s0, x_s1 (elements) and packed rows; width 1 .. 16384; the threads of a
+ * launch (16 for a row to 128 channels, 64 to 512, 64 for every 1024 above) are fewer than 2^32.
  *   s = x + residual, rounded to residual_dtype (dtype or 2); s = x where residual is null
  *   y = s / sqrt(mean(s^2) + epsilon) * weight (null: ones; weight_dtype dtype or 2)
  * out: y of dtype, contiguous; where `scales` is not null, e4m3 codes [rows, width rounded up to 16] (8-byte

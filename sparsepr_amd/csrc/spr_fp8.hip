@@ -4,7 +4,7 @@
 // Bound by memory: values are read once, 8 a lane, and kept in registers while the group's maximum is
 // found.  The transposed codes go through LDS, so that both sides move whole 128-byte lines.  A bf16 weight of
 // 13,824 x 5120 to transposed codes (212 MB) takes 44 to 48 us, 4.5 TB/s where a copy has 5.1, and 34 us back;
-// 20 x 32 tiles 10 us, a workgroup's load, maximum and store behind one another.
+// 20 x 32 tiles 10 us, a workgroup's load, maximum and store behind one another with 2.5 of them a CU.
 #include "spr_fp8.h"
 
 namespace {

@@ -10,7 +10,7 @@
 // digits down to 2^-13 of the largest of the eight; the sums of the eights are fp32.  On normal rows the digits that it
 // cuts are 5e-5 of the output's norm, a thirtieth of a bf16 output's own rounding and a quarter of an fp16 one's; an
 // output whose large products cancel may lose all of it, so a caller asks for it.  32,760 x 5120 x 5120 to bf16 takes
-// 1209 us with sums in fp32 and 676 with fast ones, 333 x 5000 x 4112 29 and 18, one row by 15,360 x 5120 18 and 14.
+// 1209 us with sums in fp32 and 676 with fast ones, 333 x 5000 x 4112 27 and 18, one row by 15,360 x 5120 18 and 14.
 //
 // Either way the sum over all blocks stays in one fp32 accumulator.  b's rows are the instruction's rows and a's its
 // columns: a lane then holds four neighbours of an output row.  The order of k within a block is free as
@@ -42,8 +42,8 @@ struct Output {
   void* out;
   const void* bias;
   int32_t bias_dtype;  // -1: none
-  // Outputs that the 256 MB cache cannot hold are written past it: 335 MB 674 instead of 684 us, but 50 MB (5000 x 5000,
-  // K = 320) 42 instead of 26.
+  // Outputs that the 256 MB cache cannot hold are written past it (16 bits): 335 MB 674 instead of 684 us, but 50 MB
+  // (5000 x 5000, K = 320) 42 instead of 26, with fast sums.
   bool past_caches;
 };
 
@@ -230,9 +230,10 @@ __device__ __forceinline__ void fetch_scales(const Matrix& a, const Matrix& b, i
 //
 // KG groups of such waves share one tile's blocks: a turn takes KG of them, each group one from buffers of its own,
 // and the first adds the other's sums at the end.  For few tiles, where a block is a chain of its DMA, reads
-// and products that one group alone leaves gaps in: 64 x 500 x 14,000 takes 25.7 us with two groups and 31.3 with one, in
-// fp32 42.9 and 54.9.  Where tiles are many it loses (512 x 5120 x 5120: 38 and 34), since the groups wait for one another;
-// four groups take 23.0 us on the first, but 21.4 instead of two's 19.0 on 300 x 1536 x 8960.
+// and products that one group alone leaves gaps in: 64 x 500 x 14,000 takes 25.7 us with two groups and 31.3 with one, with
+// sums in fp32 42.6 and 54.8.  Where tiles are many it loses (512 x 5120 x 5120: 36 and 32, sums in fp32 54 and 50), since
+// the groups wait for one another; four groups take 23.0 us on the first, but 21.4 instead of two's 19.0 on
+// 300 x 1536 x 8960 (fast sums).
 template <int DT, bool WIDE, int TM, int TN, int WM, int WN, int WIN, int NBUF, int KG>
 __global__ __launch_bounds__(64 * WM * WN * KG) void product_kernel(Matrix a, Matrix b, int32_t K, int32_t tiles_m,
                                                               int32_t tiles_n, Output o) {
@@ -334,7 +335,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void product_kernel(Matrix a, Ma
       spr::lds_barrier();
     }
     // the next DMA, into the buffer that all have read: with two buffers it cannot start too early (41 instead of 37 us
-    // on 1024 x 5120 x 5120 behind the reads), with three the reads go first (19.0 instead of 20.6 us on 333 x 5000 x 4112)
+    // on 1024 x 5120 x 5120 behind the reads), with three the reads go first (19.0 instead of 20.6 us on 333 x 5000 x 4112;
+    // both with fast sums)
     if (NBUF == 2) fetch(turn + NBUF - 1, mine + next);
     read(turn, mine + now);
     if (NBUF > 2) fetch(turn + NBUF - 1, mine + next);
@@ -386,10 +388,10 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void product_kernel(Matrix a, Ma
 // The first turn has twice the third one's reads, so it ends when b's are there; a's come in while the
 // products begin.  A part of LDS is filled again as soon as both groups have read it: b's rows (kb + 2's) in the
 // third turn, a's first half in the fourth, its second half (kb + 1's) in the first.  Each DMA has four or five
-// turns to land.  (Whole blocks at once had three: 834 us instead of 703 on 32,760 x 5120 x 5120.)
-// That size takes 643 to 688 us, 2.5 to 2.7 PFLOP/s: what bounds it is the matrix units, busy for 63 % of the cycles at
-// the 1.9 GHz that real codes leave them (2.34 with constant ones).  Alone, the products take 400 us, with the
-// LDS reads 511, with the DMA 641.  One wave a SIMD with 128 x 128 outputs, half the LDS reads, takes 761.
+// turns to land.  (With three, and 32 x 32 x 64 instructions in half blocks, 32,760 x 5120 x 5120 took 834 us instead of 703.)
+// That size takes 643 to 688 us, 2.5 to 2.7 PFLOP/s.  What bounds it is feeding the matrix units: they are busy for 63 % of
+// the cycles, at the 1.9 GHz that real codes leave them (2.34 with constant ones).  Alone, the products take 400 us, with
+// the LDS reads 511, with the DMA 641.  One wave a SIMD with 128 x 128 outputs, half the LDS reads, takes 761.
 template <int DT>
 __global__ __launch_bounds__(512) void turns_product_kernel(Matrix a, Matrix b, int32_t K, int32_t tiles_m,
                                                            int32_t tiles_n, Output o) {

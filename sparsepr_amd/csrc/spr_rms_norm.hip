@@ -11,7 +11,8 @@
 // Bound by memory: every input is read once and kept in registers over the reduction, vectors of 8 channels a
 // lane.  32,760 rows of 5120 in bf16 with residual and codes (1.18 GB) take 215 us one call behind the other, 5.5 TB/s
 // where a copy has 5.1, and 241 to 265 between other kernels; the gradient of 8191 rows of 2560 (294 MB) 55 us, and
-// 6 us for the weight's partial sums.  One row of 5120 takes 4.0 us.
+// 6 us for the weight's partial sums.  Outputs in bf16 (671 MB) take 139 to 146 us, with a residual (1.34 GB) 233 to 251.
+// One row of 5120 takes 4.0 us.
 #include "spr_fp8.h"
 
 namespace {
@@ -75,8 +76,8 @@ __device__ __forceinline__ double inverse_rms(double ss, double inv_width, float
 }
 
 // s inv w with the roundings of the two products carried along, so rounded once to fp32: a value next to a border of its
-// output's type then goes where the formula in more digits sends it (of 5 M bf16 outputs 2 to 5 go elsewhere, 30 with two
-// roundings; 305 instead of 301 us on 32,760 rows of 5120).  Where a product is 0, infinite or NaN it is as it is.
+// output's type then goes where the formula in more digits sends it (of 5 M bf16 outputs 2 to 12 go elsewhere, 16 to 35
+// with two roundings; 305 instead of 301 us on 32,760 rows of 5120).  Where a product is 0, infinite or NaN it is as it is.
 __device__ __forceinline__ float normed(float s, float inv, float inv_low, float w) {
   const float a = s * inv, y = a * w;
   const float low = __builtin_fmaf(s, inv_low, __builtin_fmaf(s, inv, -a));

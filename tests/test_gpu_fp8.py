@@ -7,6 +7,8 @@ magnitudes, then half a step of the output's type.  Outputs in 16 bits come from
 instruction, which cuts the other seven of eight neighbouring products 2^-13 below the largest: 7 * 2^-13 of
 each eight's largest product more.  (Whole numbers up to 16 with scales alike in a block lose nothing there.)"""
 
+# Outputs in 16 bits come from the 8-bit instruction only where fast sums are asked for (test_gpu_fp8_sums.py); the bound
+# above holds for both ways of summing.
 import numpy as np
 import pytest
 import torch

@@ -4,6 +4,8 @@ Errors in fp32: a sum of C squares, 32 terms a lane in a chain and at most 16 jo
 steps (2^-24) of itself, its root by half of that; with the division, the root and the two products a value is off by
 at most 32 * 2^-24.  Then half a step of the output's type."""
 
+# A lane's chain is one or two squares now and the roundings of the products are carried along, so that the bound above is
+# wide; test_an_output_is_rounded_once holds what those roundings leave.
 import numpy as np
 import pytest
 import torch
